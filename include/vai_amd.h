@@ -37,7 +37,12 @@ typedef enum {
 
 /* Dtype codes: the reference's DTYPE_F32 / DTYPE_F16 / DTYPE_NONE
  * (/root/reference/vai/shaders/common/spec_constants.h:6-8). */
-enum { VAI_DTYPE_F32 = 0, VAI_DTYPE_F16 = 1, VAI_DTYPE_NONE = 2 };
+enum {
+    VAI_DTYPE_F32 = 0,
+    VAI_DTYPE_F16 = 1,
+    VAI_DTYPE_NONE = 2,
+    VAI_DTYPE_Q4 = 3,   /* a KV cache in 4 bits (vai_attention_args.cache_dtype only); not the reference's */
+};
 
 /* Epilogue codes in the order of vai::Epilogue
  * (/root/reference/vai/nodes/common.h:31-39). */
@@ -132,6 +137,53 @@ vai_status vai_linear_pack_weight(const vai_linear_args* args, void* packed, siz
 /* Which kernel vai_linear_launch picks for args (for tests and reports):
  * writes a short name ("slab", "slab_any", "tile_f16_128x128", ...). */
 vai_status vai_linear_plan(const vai_linear_args* args, char* name, size_t name_len, uint32_t* split_count);
+
+/* ---------------------------------------------------------------------------
+ * Linear over 8-bit weights. No counterpart in the reference. Rows of X are
+ * rounded to 8-bit integers in the call, each with a scale of its own, and
+ * multiplied with the weight's integers:
+ *   x_m = fp32(max_k |I[m,k]| / 127),  a[m,k] = round(I[m,k] / x_m)
+ *   A[m,n] = x_m * w_scale[n] * sum_k a[m,k] W[n,k]
+ *   O = s * epi(A + bias) + R          (residual_order AFTER)
+ *   O = s * epi(A + bias + R)          (residual_order BEFORE)
+ * round is to the nearest integer, halves to even, of the exact quotient; the
+ * sums are 32-bit integers (exact), the rest fp32, rounded once to o_dtype.
+ * I [M,K] fp32 or fp16; W [N] rows of 8-bit integers, each row starting K
+ * rounded up to 16 bytes after the one before (what lies between does not
+ * count) and the first 16-byte aligned; w_scale [N] fp32. A row of zeros
+ * (or below fp32's normal range over 127) gives 0 for A, one that holds a NaN
+ * or an infinity NaN. bias, residual, their repeats, epilogue and scalar_scale
+ * as in vai_linear_args. K <= 131072.
+ * The workspace (vai_linear_i8_workspace_size() bytes, 16-byte aligned) holds
+ * the rounded rows of X; calls that overlap in time need one each.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    void* out;
+    const void* in;
+    const void* weight;
+    const float* w_scale;
+    const void* bias;        /* NULL: no bias */
+    const void* residual;    /* NULL: no residual */
+    void* workspace;
+    size_t workspace_bytes;
+    uint32_t M, N, K;
+    int32_t o_dtype, i_dtype, b_dtype;
+    uint32_t epilogue;
+    uint32_t residual_order;
+    uint32_t bias_repeat;
+    uint32_t residual_repeat;
+    float scalar_scale;
+} vai_linear_i8_args;
+
+vai_status vai_linear_i8_launch(const vai_linear_i8_args* args, vai_stream_t stream);
+size_t vai_linear_i8_workspace_size(const vai_linear_i8_args* args);
+
+/* Rounds `rows` rows of K values (fp32 or fp16) as above: out gets rows of K
+ * rounded up to 16 bytes (zeros past K, 16-byte aligned), scale one fp32 each.
+ * Of a weight [N,K] it makes W and w_scale. K <= 131072. A row with a NaN or
+ * an infinity gets scale NaN. */
+vai_status vai_quantize_i8_launch(void* out, float* scale, const void* in, int32_t i_dtype,
+                                  uint32_t rows, uint32_t K, vai_stream_t stream);
 
 /* GatedMul alone: O[r,j] = epi(I[r,j]) * I[r,H+j], I [rows, 2H].
  * Replaces gated-mul.comp (/root/reference/vai/nodes/gated-mul.h:75-114). */
@@ -272,12 +324,26 @@ typedef struct {
      * max(i + Tkv - Tq, 0) and sees up to count + (its mask end among the
      * new keys), attention-fa.comp:137-146,470-478. K / V may be NULL with
      * Tkv = 0: the call attends the cache alone. The caller keeps count + Tkv
-     * <= cache_size without a ring, and advances the count itself. */
+     * <= cache_size without a ring, and advances the count itself.
+     * cache_dtype VAI_DTYPE_Q4 keeps the cache in 4 bits (head_dim <= 256; no
+     * counterpart in the reference): planes of vai_attention_cache_bytes()
+     * bytes, 16-byte aligned, in a layout of the library's own. A row is
+     * rounded to fp16 and cut into groups of 32 values (the last may be
+     * shorter); a group keeps m = its minimum, s = fp16((max - m) / 15) and
+     * codes n = round((x - m) / s) of 0 .. 15, and stands for s n + m (s the
+     * fp16 number below where 15 s + m would leave fp16's range). Every
+     * key and value is attended as stored, the call's own among them, so the
+     * result does not depend on how a sequence was cut into calls. A group
+     * with a value that is not finite in fp16 is stored as NaN; a query that
+     * sees a row with such a group in K or V is NaN, one it is hidden from is
+     * not touched by it. Positions past the count may hold anything. A 4-bit
+     * ring is attended as far as it holds: span counts as at most cache_size -
+     * Tkv + 1 (0 as that), and Tkv <= cache_size. */
     void* k_cache;
     void* v_cache;
     const uint32_t* cache_count;
     uint32_t cache_size;
-    int32_t cache_dtype;          /* VAI_DTYPE_F32 or VAI_DTYPE_F16 */
+    int32_t cache_dtype;          /* VAI_DTYPE_F32, VAI_DTYPE_F16 or VAI_DTYPE_Q4 */
     uint32_t cache_ring;
 } vai_attention_args;
 
@@ -287,6 +353,74 @@ vai_status vai_attention_launch(const vai_attention_args* args, vai_stream_t str
  * GPU and long key ranges are split over workgroups (partial results merged by
  * a second pass, the split-K of attention-fa-reduce.comp). */
 size_t vai_attention_workspace_size(const vai_attention_args* args);
+
+/* Bytes of one cache plane (k_cache and v_cache each): hkv * cache_size *
+ * head_dim values in an fp32 or fp16 cache; a 4-bit one keeps rows of 64, 128
+ * or 256 values (the next that holds head_dim) at 5 bits a value, positions
+ * rounded up to 32. 0: no such cache. */
+size_t vai_attention_cache_bytes(uint32_t hkv, uint32_t cache_size, uint32_t head_dim, int32_t cache_dtype);
+
+/* Rows of a cache as the values they stand for: rows first_row .. first_row +
+ * rows - 1 (past the plane's end they go on at row 0) of every head, as
+ * [hkv, rows, head_dim] in o_dtype (fp32 or fp16). For a ring, row = position
+ * % cache_size. */
+typedef struct {
+    void* k_out;
+    void* v_out;
+    const void* k_cache;
+    const void* v_cache;
+    int32_t o_dtype;
+    int32_t cache_dtype;          /* VAI_DTYPE_F32, VAI_DTYPE_F16 or VAI_DTYPE_Q4 */
+    uint32_t hkv, cache_size, head_dim;
+    uint32_t first_row, rows;
+} vai_attention_cache_read_args;
+
+vai_status vai_attention_cache_read(const vai_attention_cache_read_args* args, vai_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * From the fused query / key / value projection to the planes attention reads:
+ * the RMS norm of each query and key head, the position rotation, and token-
+ * major rows to head-major planes. No counterpart in the reference's hot path.
+ *   qkv [batch,tokens] rows of row_stride elements (0: (hq + 2 hkv) head_dim),
+ *   hq query heads, then hkv key heads, then hkv value heads, in i_dtype;
+ *   q_out [batch,hq,tokens,head_dim], k_out and v_out [batch,hkv,tokens,
+ *   head_dim] in o_dtype, disjoint from qkv. v_out NULL: values stay.
+ * norm = 1: y = x / sqrt(mean x^2 + eps) * (w + weight_offset) over each head,
+ * w = q_weight / k_weight [head_dim] in w_dtype; NULL: the factor is 1. norm =
+ * 0: y = x. Values are only moved.
+ * Rotation of the first rot_dim values (even; 0: head_dim) of a head at
+ * position p: pair i, (a, e) = (y[i], y[i + rot_dim/2]) (HALVES) or (y[2i],
+ * y[2i+1]) (NEIGHBOURS), becomes (a cos - e sin, e cos + a sin) of the angle
+ * p * f_i, f_i = inv_freq[i] (fp32, device, rot_dim/2 of them; scaled bases) or,
+ * NULL, theta^(-2i/rot_dim). Angles are taken in 64 bits, so far positions keep
+ * theirs; the rest is fp32, rounded once to o_dtype.
+ * p = positions[batch,tokens] (device uint32), or when NULL *count + token
+ * (count: a device uint32 read when the kernel runs, the KV cache's counter;
+ * NULL: 0). head_dim <= 2048.
+ * ------------------------------------------------------------------------- */
+enum { VAI_ROPE_NONE = 0, VAI_ROPE_HALVES = 1, VAI_ROPE_NEIGHBOURS = 2 };
+
+typedef struct {
+    void* q_out;
+    void* k_out;
+    void* v_out;
+    const void* qkv;
+    const void* q_weight;
+    const void* k_weight;
+    const uint32_t* positions;
+    const uint32_t* count;
+    const float* inv_freq;
+    uint32_t batch, tokens, hq, hkv, head_dim;
+    uint32_t row_stride;
+    int32_t i_dtype, o_dtype, w_dtype;
+    uint32_t norm;
+    float eps, weight_offset;
+    uint32_t rope;
+    uint32_t rot_dim;
+    float theta;
+} vai_qk_norm_rope_args;
+
+vai_status vai_qk_norm_rope_launch(const vai_qk_norm_rope_args* args, vai_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * Device memory and streams: what the host side (vai::Tensor's pooled

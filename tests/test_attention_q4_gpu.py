@@ -1,0 +1,307 @@
+"""Attention over a 4-bit KV cache against its definition in 64 bits: the codes
+exactly (through vai_attention_cache_read), the attention of the values they
+stand for within the roundings of the kernels.
+
+Tolerance of an output value sum_j p_j v_j: a score may be off by dS = 2^-11 *
+scale * sum |q k| for each operand the matrix cores take rounded to fp16 (K as
+stored always may be, an fp32 Q is), plus fp32 sums over the head dim; p then by
+a factor of e^(2 dS) (its own score and the sum's), p and v are rounded to fp16
+once each and so may be a partial result, and fp32 sums over the keys follow:
+sum p |v| * (2 max dS + 3 * 2^-11 + 2^-16)."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from helpers import draw
+
+pytestmark = pytest.mark.gpu
+F16, F32 = np.float16, np.float32
+
+
+def stored(x):
+    """The values 4-bit rows [..., D] stand for, in 64 bits: NaN where a group is not finite in fp16."""
+    with np.errstate(over="ignore"):
+        x = x.astype(F16).astype(np.float64)
+    out = np.empty_like(x)
+    for g in range(0, x.shape[-1], 32):
+        y = x[..., g:g + 32]
+        ok = np.isfinite(y).all(-1, keepdims=True)
+        y = np.where(ok, y, 0.0)
+        lo, hi = y.min(-1, keepdims=True), y.max(-1, keepdims=True)
+        s = ((hi - lo) / 15).astype(F16)
+        s = np.where(15 * s.astype(np.float64) + lo > 65504, np.nextafter(s, F16(0)), s).astype(np.float64)
+        n = np.where(s > 0, np.rint((y - lo) / np.where(s > 0, s, 1)), 0).clip(0, 15)
+        out[..., g:g + 32] = np.where(ok, n * s + lo, np.nan)
+    return out
+
+
+def attend(q, k, v, see, q_rounded):
+    """q [hq, T, D], k / v [hkv, L, D] as stored, see [T, L] -> (out [T, hq, D], tolerance before the output's)"""
+    hq, T, D = q.shape
+    grp = hq // k.shape[0]
+    out, tol = np.zeros((T, hq, D)), np.zeros((T, hq, D))
+    q = q.astype(np.float64)
+    for h in range(hq):
+        K, V = k[h // grp], v[h // grp]
+        s = np.where(see, (q[h] @ K.T) / np.sqrt(D), -np.inf)
+        ds = 2.0 ** -11 * (2 if q_rounded else 1) * (np.abs(q[h]) @ np.abs(K).T) / np.sqrt(D) * (1 + 2.0 ** -8)
+        ds = np.where(see, ds, 0).max(-1, initial=0)[:, None]
+        m = s.max(-1, keepdims=True, initial=-np.inf)
+        p = np.exp(s - np.where(np.isfinite(m), m, 0))
+        l = p.sum(-1, keepdims=True)
+        p = np.where(l > 0, p / np.where(l > 0, l, 1), 0)
+        out[:, h] = p @ V
+        tol[:, h] = (p @ np.abs(V)) * (2 * ds + 3 * 2.0 ** -11 + 2.0 ** -16) + 1e-7
+    return out, tol
+
+
+def visible(count, tq, tkv, first, span, causal=True):
+    """see [tq, positions first .. count + tkv)"""
+    key = np.arange(first, count + tkv)
+    i = np.arange(tq)
+    end = count + np.clip(i + 1 + tkv - tq if causal else np.full(tq, tkv), 0, tkv)
+    pos = count + np.maximum(i + tkv - tq, 0)
+    see = key[None] < end[:, None]
+    if span:
+        see &= key[None] > (pos - span)[:, None]
+    return see
+
+
+class Cache:
+    """Planes that start out as garbage, and the rows they should hold."""
+
+    def __init__(self, gpu, hkv, size, d, ring):
+        self.gpu, self.hkv, self.size, self.d, self.ring = gpu, hkv, size, d, ring
+        self.k, self.v = (gpu.CachePlane(hkv, size, d, gpu.Q4) for _ in range(2))
+        for p in (self.k, self.v):
+            p.buf.fill_(0xFF)
+        self.count = gpu.DeviceArray.from_numpy(np.zeros(1, np.uint32))
+        self.n = 0
+        self.rows = [np.zeros((hkv, 0, d)) for _ in range(2)]   # all positions, as stored
+
+    def set_count(self, n):
+        self.n = n
+        self.gpu.check(self.gpu.lib().vai_memcpy_h2d(self.count.ptr, np.array([n], np.uint32).ctypes.data, 4, None), "h2d")
+
+    def first(self, end):
+        return max(0, end - self.size) if self.ring else 0
+
+    def call(self, q, k, v, odt=F32, span=0, causal=True, blocks=None):
+        """One call at the current count; then the count moves on."""
+        g, D = self.gpu, self.gpu.DeviceArray.from_numpy
+        hq, tq, _ = q.shape
+        out = g.DeviceArray((1, tq, hq, self.d), odt)
+        out.fill_(0xFF)
+        g.attention(out, D(q[None]), None if k is None else D(k[None]), None if v is None else D(v[None]),
+                    causal=causal and blocks is None, span=span, blocks=blocks,
+                    cache=(self.k, self.v, self.count, self.ring))
+        if k is not None:
+            self.rows = [np.concatenate([r[:, :self.n], stored(x)], 1) for r, x in zip(self.rows, (k, v))]
+            self.set_count(self.n + k.shape[1])
+        return out.numpy()[0]
+
+    def append(self, rng, n, dt=F16, piece=None):
+        """n rows through calls of one query."""
+        while n:
+            m = min(n, piece or self.size)
+            q = draw((self.hkv, 1, self.d), rng, F16)
+            self.call(q, draw((self.hkv, m, self.d), rng, dt), draw((self.hkv, m, self.d), rng, dt), span=1)
+            n -= m
+
+    def check_rows(self):
+        end, first = self.n, self.first(self.n)
+        n = end - first
+        if n == 0:
+            return
+        outs = [self.gpu.DeviceArray((self.hkv, n, self.d), F32) for _ in range(2)]
+        self.gpu.attention_cache_read(*outs, self.k, self.v, first % self.size if self.ring else first)
+        for o, r in zip(outs, self.rows):
+            np.testing.assert_array_equal(o.numpy(), r[:, first:end].astype(F32))
+
+
+def check(got, want, tol):
+    if got.dtype == F16:
+        tol = tol + np.abs(want) * 2.0 ** -11 + 2.0 ** -25
+    err = np.abs(got.astype(np.float64) - want)
+    assert np.isfinite(got).all()
+    assert (err <= tol).all(), f"max error {err.max()}, {(err / tol).max()} of what is allowed"
+
+
+CASES = [
+    # d, hq, hkv, tq, tkv, count, size, ring, span, xdt, odt
+    (64, 1, 1, 1, 1, 0, 32, False, 0, F16, F32),          # the first token of all
+    (64, 8, 2, 1, 1, 31, 4096, False, 0, F16, F16),       # the new row ends a tile
+    (64, 8, 2, 1, 1, 32, 4096, False, 0, F16, F16),       # ... starts one
+    (128, 32, 8, 1, 1, 3000, 4096, False, 0, F16, F16),   # a decode step
+    (128, 4, 4, 1, 1, 255, 256, False, 0, F32, F32),      # the cache filled to its last row, fp32
+    (128, 8, 1, 4, 4, 1021, 2000, False, 0, F16, F16),    # 32 rows of one head, over a tile's end
+    (128, 17, 1, 1, 1, 500, 512, False, 0, F16, F32),     # 17 rows
+    (64, 4, 1, 16, 16, 700, 1024, False, 0, F16, F32),    # 64 rows
+    (64, 4, 1, 17, 17, 700, 1024, False, 0, F16, F32),    # 68 rows
+    (256, 8, 2, 5, 5, 900, 1280, False, 0, F16, F16),     # D = 256
+    (256, 16, 1, 2, 2, 3000, 4096, False, 300, F32, F16),  # ... a window, fp32
+    (32, 4, 2, 3, 3, 100, 128, False, 0, F16, F16),       # one group a row
+    (80, 10, 2, 1, 1, 333, 400, False, 0, F16, F32),      # a short last group, a size that is no whole tile
+    (96, 6, 2, 2, 2, 64, 99, False, 0, F32, F32),
+    (17, 2, 1, 3, 3, 50, 64, False, 0, F16, F32),         # odd head dim
+    (1, 2, 1, 2, 2, 5, 64, False, 0, F32, F32),
+    (200, 4, 2, 3, 3, 90, 128, False, 50, F16, F32),
+    (64, 4, 2, 8, 8, 252, 256, True, 60, F16, F16),       # the new rows wrap the ring
+    (128, 4, 2, 5, 5, 1000, 64, True, 30, F32, F32),      # the smallest ring, wrapped many times
+    (128, 8, 2, 1, 1, 700, 256, True, 0, F16, F16),       # a ring without a window: what it holds
+    (256, 4, 2, 3, 3, 130, 128, True, 126, F16, F16),     # the widest window the ring allows
+    (64, 4, 4, 2, 32, 100, 512, False, 0, F16, F16),      # more new keys than queries
+    (64, 4, 4, 9, 4, 0, 512, False, 0, F16, F32),         # more queries than keys: the first see none
+    (64, 2, 2, 200, 200, 100, 512, False, 0, F16, F16),   # a chunk of a prompt
+    (128, 8, 2, 130, 130, 1000, 2048, False, 0, F16, F16),
+    (128, 4, 1, 300, 300, 0, 300, False, 100, F32, F32),  # a whole prompt into a cache of its size, window
+    (256, 4, 2, 70, 70, 200, 320, True, 200, F16, F16),
+    (72, 4, 2, 100, 100, 30, 256, False, 0, F16, F32),
+    (20, 4, 2, 90, 90, 30, 256, False, 0, F16, F32),
+]
+
+
+@pytest.mark.parametrize("d, hq, hkv, tq, tkv, count, size, ring, span, xdt, odt", CASES)
+def test_attention_q4(gpu, d, hq, hkv, tq, tkv, count, size, ring, span, xdt, odt):
+    rng = np.random.default_rng(d + size + count)
+    c = Cache(gpu, hkv, size, d, ring)
+    print(f"q4 d={d} hq={hq} hkv={hkv} tq={tq} tkv={tkv} count={count} size={size} ring={ring} span={span}", flush=True)
+    c.append(rng, count)
+    q, k, v = draw((hq, tq, d), rng, xdt), draw((hkv, tkv, d), rng, xdt), draw((hkv, tkv, d), rng, xdt)
+    got = c.call(q, k, v, odt, span)
+    c.check_rows()
+    first = c.first(count + tkv)
+    held = size - tkv + 1
+    eff = (min(span, held) if span else held) if ring else span
+    see = visible(count, tq, tkv, first, eff)
+    want, tol = attend(q, *(r[:, first:] for r in c.rows), see, xdt == F32)
+    check(got, want, tol)
+
+
+@pytest.mark.parametrize("tq, span", [(1, 0), (4, 3), (40, 0), (130, 64)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_without_new_rows_and_without_a_mask(gpu, d, tq, span):
+    """Tkv = 0 attends the cache alone; an empty one gives zeros."""
+    rng = np.random.default_rng(tq)
+    c = Cache(gpu, 2, 200, d, False)
+    q = draw((4, tq, d), rng, F16)
+    print(f"q4 cache alone d={d} tq={tq}", flush=True)
+    assert (c.call(q, None, None, F32, span) == 0).all()
+    c.append(rng, 101)
+    got = c.call(q, None, None, F32, span, causal=False)
+    want, tol = attend(q, *c.rows, visible(101, tq, 0, 0, span, causal=False), False)
+    check(got, want, tol)
+
+
+def test_block_mask(gpu):
+    """A full prefix of 3, then causal: the reference's prefix-LM mask, over cached rows."""
+    rng = np.random.default_rng(6)
+    for tq in (8, 70):
+        c = Cache(gpu, 2, 256, 64, False)
+        c.append(rng, 40)
+        q, k, v = (draw((h, tq, 64), rng, F16) for h in (4, 2, 2))
+        got = c.call(q, k, v, F32, blocks=(1, [3]))
+        see = visible(40, tq, tq, 0, 0)
+        see[:3, 40:43] = True
+        want, tol = attend(q, *c.rows, see, False)
+        check(got, want, tol)
+
+
+@pytest.mark.parametrize("d, xdt", [(64, F16), (128, F32), (80, F16), (256, F16)])
+def test_cut_into_calls_the_cache_is_the_same(gpu, d, xdt):
+    """The same rows in one call, in pieces and one by one leave the same bytes."""
+    rng = np.random.default_rng(d)
+    n, hkv = 75, 3
+    k, v = draw((hkv, n, d), rng, xdt), draw((hkv, n, d), rng, xdt)
+    q = draw((hkv, 1, d), rng, F16)
+    planes = []
+    for pieces in ([n], [32, 33, 10], [1] * n):
+        c = Cache(gpu, hkv, 96, d, False)
+        for b in (c.k.buf, c.v.buf):
+            b.fill_(0)
+        at = 0
+        for m in pieces:
+            c.call(q, np.ascontiguousarray(k[:, at:at + m]), np.ascontiguousarray(v[:, at:at + m]))
+            at += m
+        c.check_rows()
+        planes.append((c.k.buf.numpy(), c.v.buf.numpy()))
+    for p in planes[1:]:
+        for a, b in zip(p, planes[0]):
+            np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("d", [64, 128, 80])
+def test_rows_with_nan_and_infinity(gpu, d):
+    """A group that is not finite is NaN for the queries that see its row and nothing for those it is hidden from,
+    one token or many; constant groups, halves and fp16's far ends keep their values."""
+    rng = np.random.default_rng(3)
+    for tq, count in ((1, 60), (4, 60), (70, 10)):
+        for what in ("k", "v"):
+            c = Cache(gpu, 2, 256, d, False)
+            c.append(rng, count)
+            q, k, v = draw((4, tq, d), rng, F16), draw((2, tq, d), rng, F32), draw((2, tq, d), rng, F32)
+            x = k if what == "k" else v
+            late = tq - 1
+            x[0, 0, :16] = 0.25
+            x[1, 0, :2] = (65504, -65504)
+            if what == "k":
+                x[1, 0] *= 2.0 ** -12
+            x[0, late, 3] = np.nan
+            x[1, late, d - 1] = 1e6
+            print(f"q4 nan d={d} tq={tq} in {what}", flush=True)
+            got = c.call(q, k, v, F32)
+            c.check_rows()
+            assert np.isnan(got[late]).all()
+            if tq > 1:
+                ks, vs = (r[:, :-1] for r in c.rows)
+                see = visible(count, tq, tq, 0, 0)[:late, :-1]
+                want, tol = attend(q[:, :late], ks, vs, see, False)
+                check(got[:late], want, tol)
+            # out of its window the row is as good as gone
+            c.append(rng, 5)
+            q1, k1, v1 = draw((4, 1, d), rng, F16), draw((2, 1, d), rng, F16), draw((2, 1, d), rng, F16)
+            got = c.call(q1, k1, v1, F32, span=5)
+            want, tol = attend(q1, *(r[:, -5:] for r in c.rows), np.ones((1, 5), bool), False)
+            check(got, want, tol)
+
+
+def test_cache_read_of_every_dtype(gpu):
+    rng = np.random.default_rng(12)
+    D = gpu.DeviceArray.from_numpy
+    for dt in (F16, F32):
+        k, v = draw((2, 40, 20), rng, dt), draw((2, 40, 20), rng, dt)
+        for odt in (F16, F32):
+            ko, vo = gpu.DeviceArray((2, 25, 20), odt), gpu.DeviceArray((2, 25, 20), odt)
+            gpu.attention_cache_read(ko, vo, D(k), D(v), 30)
+            rows = (30 + np.arange(25)) % 40
+            np.testing.assert_array_equal(ko.numpy(), k[:, rows].astype(odt))
+            np.testing.assert_array_equal(vo.numpy(), v[:, rows].astype(odt))
+
+
+@pytest.mark.parametrize("hq, tq, d", [(8, 1, 64), (8, 4, 128), (4, 80, 128)])
+def test_replayed_graph_follows_the_count(gpu, hq, tq, d):
+    rng = np.random.default_rng(9)
+    D, lib, hkv, size = gpu.DeviceArray.from_numpy, gpu.lib(), 2, 1024
+    c = Cache(gpu, hkv, size, d, False)
+    c.append(rng, 900)
+    hist = [r.copy() for r in c.rows]
+    q, k, v = draw((hq, tq, d), rng, F16), draw((hkv, tq, d), rng, F16), draw((hkv, tq, d), rng, F16)
+    out = gpu.DeviceArray((1, tq, hq, d), F16)
+    a = gpu.attention_args(out, D(q[None]), D(k[None]), D(v[None]), causal=True, cache=(c.k, c.v, c.count, False))
+    need = lib.vai_attention_workspace_size(ctypes.byref(a))
+    ws = gpu.DeviceArray((max(need, 1),), np.uint8)
+    a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
+    gpu.synchronize()
+    stream = gpu.Stream()
+    graph = gpu.Graph(stream, lambda: gpu.check(lib.vai_attention_launch(ctypes.byref(a), stream.ptr), "step"))
+    new = [stored(k), stored(v)]
+    for count in (0, 5, 127, 128, 600, 900, 40):
+        c.set_count(count)
+        graph.launch()
+        stream.synchronize()
+        for h, n in zip(hist, new):
+            h[:, count:count + tq] = n[:, :max(0, h.shape[1] - count)]
+        rows = [np.concatenate([h[:, :count], n], 1) for h, n in zip(hist, new)]
+        want, tol = attend(q, *rows, visible(count, tq, tq, 0, 0), False)
+        check(out.numpy()[0], want, tol)

@@ -12,7 +12,8 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libvai_amd.so")
 
-F32, F16, NONE = 0, 1, 2
+F32, F16, NONE, Q4 = 0, 1, 2, 3
+ROPE = {"NONE": 0, "HALVES": 1, "NEIGHBOURS": 2}
 EPILOGUES = {"NONE": 0, "RELU": 1, "GELU": 2, "GELU_TANH": 3, "SILU": 4, "SIGMOID": 5}
 RESIDUAL_ORDERS = {"AFTER_EPILOGUE": 0, "BEFORE_EPILOGUE": 1}
 MAX_CAUSAL_BLOCKS = 32
@@ -24,6 +25,8 @@ EXPORTS = [
     "vai_linear_packed_weight_size", "vai_linear_pack_weight",
     "vai_conv2d_launch", "vai_conv2d_workspace_size", "vai_conv2d_packed_weight_size", "vai_conv2d_pack_weight",
     "vai_attn_scores_launch", "vai_attention_launch", "vai_attention_workspace_size",
+    "vai_attention_cache_bytes", "vai_attention_cache_read",
+    "vai_linear_i8_launch", "vai_linear_i8_workspace_size", "vai_quantize_i8_launch", "vai_qk_norm_rope_launch",
     "vai_device_count", "vai_set_device", "vai_malloc", "vai_free", "vai_memcpy_h2d", "vai_memcpy_d2h",
     "vai_memcpy_d2d", "vai_memset", "vai_stream_create", "vai_stream_destroy", "vai_stream_sync",
     "vai_device_sync", "vai_status_string", "vai_event_create", "vai_event_destroy", "vai_event_record",
@@ -88,6 +91,41 @@ class AttentionArgs(ctypes.Structure):
     ]
 
 
+class LinearI8Args(ctypes.Structure):
+    _fields_ = [
+        ("out", ctypes.c_void_p), ("inp", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("w_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("M", ctypes.c_uint32), ("N", ctypes.c_uint32), ("K", ctypes.c_uint32),
+        ("o_dtype", ctypes.c_int32), ("i_dtype", ctypes.c_int32), ("b_dtype", ctypes.c_int32),
+        ("epilogue", ctypes.c_uint32), ("residual_order", ctypes.c_uint32),
+        ("bias_repeat", ctypes.c_uint32), ("residual_repeat", ctypes.c_uint32),
+        ("scalar_scale", ctypes.c_float),
+    ]
+
+
+class AttentionCacheReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("k_out", ctypes.c_void_p), ("v_out", ctypes.c_void_p), ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p),
+        ("o_dtype", ctypes.c_int32), ("cache_dtype", ctypes.c_int32),
+        ("hkv", ctypes.c_uint32), ("cache_size", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+        ("first_row", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+    ]
+
+
+class QkNormRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("v_out", ctypes.c_void_p), ("qkv", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("count", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+        ("batch", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("hq", ctypes.c_uint32), ("hkv", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32), ("row_stride", ctypes.c_uint32),
+        ("i_dtype", ctypes.c_int32), ("o_dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32),
+        ("norm", ctypes.c_uint32), ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
+        ("rope", ctypes.c_uint32), ("rot_dim", ctypes.c_uint32), ("theta", ctypes.c_float),
+    ]
+
+
 class VaiError(RuntimeError):
     pass
 
@@ -121,6 +159,14 @@ def lib():
         L.vai_attention_launch.argtypes = [ctypes.POINTER(AttentionArgs), vp]
         L.vai_attention_workspace_size.argtypes = [ctypes.POINTER(AttentionArgs)]
         L.vai_attention_workspace_size.restype = sz
+        L.vai_attention_cache_bytes.argtypes = [u32, u32, u32, i32]
+        L.vai_attention_cache_bytes.restype = sz
+        L.vai_attention_cache_read.argtypes = [ctypes.POINTER(AttentionCacheReadArgs), vp]
+        L.vai_linear_i8_launch.argtypes = [ctypes.POINTER(LinearI8Args), vp]
+        L.vai_linear_i8_workspace_size.argtypes = [ctypes.POINTER(LinearI8Args)]
+        L.vai_linear_i8_workspace_size.restype = sz
+        L.vai_quantize_i8_launch.argtypes = [vp, vp, vp, i32, u32, u32, vp]
+        L.vai_qk_norm_rope_launch.argtypes = [ctypes.POINTER(QkNormRopeArgs), vp]
         L.vai_malloc.argtypes = [ctypes.POINTER(vp), sz]
         L.vai_free.argtypes = [vp]
         L.vai_memcpy_h2d.argtypes = [vp, vp, sz, vp]
@@ -279,6 +325,93 @@ def linear(out, inp, weight, bias=None, residual=None, stream=None, packed=None,
     return out
 
 
+def i8_stride(k):
+    """Bytes from one row of 8-bit integers to the next."""
+    return (k + 15) // 16 * 16
+
+
+def quantize_i8(x, stream=None):
+    """Rows of x [..., K] as 8-bit integers: (codes [rows, i8_stride(K)] int8, scale [rows] fp32)."""
+    K = x.shape[-1]
+    rows = int(np.prod(x.shape[:-1]))
+    codes, scale = DeviceArray((rows, i8_stride(K)), np.int8), DeviceArray((rows,), np.float32)
+    check(lib().vai_quantize_i8_launch(codes.ptr, scale.ptr, x.ptr, x.code, rows, K, stream), "vai_quantize_i8_launch")
+    check(lib().vai_stream_sync(stream), "sync")   # the caller may drop x on return
+    return codes, scale
+
+
+def linear_i8_args(out, inp, weight, w_scale, bias=None, residual=None, *, epi="NONE", order="AFTER_EPILOGUE",
+                   scale=1.0, workspace=None):
+    """weight: 8-bit rows [N, i8_stride(K)] and their scales [N], as quantize_i8 makes them of [N, K]."""
+    a = LinearI8Args()
+    a.out, a.inp, a.weight, a.w_scale = out.ptr, inp.ptr, weight.ptr, w_scale.ptr
+    a.bias, a.residual = _ptr(bias), _ptr(residual)
+    a.K = inp.shape[-1]
+    a.M, a.N = int(np.prod(inp.shape[:-1])), weight.shape[0]
+    if weight.shape[-1] != i8_stride(a.K):
+        raise VaiError(f"8-bit weight rows of {weight.shape[-1]} bytes, {i8_stride(a.K)} expected for K = {a.K}")
+    a.o_dtype, a.i_dtype = out.code, inp.code
+    a.b_dtype = bias.code if bias is not None else NONE
+    a.epilogue = EPILOGUES[epi]
+    a.residual_order = RESIDUAL_ORDERS[order] if isinstance(order, str) else int(order)
+    MN = a.M * a.N
+    if bias is not None:
+        n = int(np.prod(bias.shape))
+        a.bias_repeat = 0 if n == MN else n
+    if residual is not None:
+        n = int(np.prod(residual.shape))
+        a.residual_repeat = 0 if n == MN else n
+    a.scalar_scale = scale
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.ptr, workspace.nbytes
+    a._keep = (out, inp, weight, w_scale, bias, residual, workspace)   # the buffers live as long as the args
+    return a
+
+
+def linear_i8(out, inp, weight, w_scale, bias=None, residual=None, stream=None, **kw):
+    """Launches the 8-bit Linear; allocates its workspace if needed."""
+    a = linear_i8_args(out, inp, weight, w_scale, bias, residual, **kw)
+    need = lib().vai_linear_i8_workspace_size(ctypes.byref(a))
+    ws = None
+    if need and a.workspace_bytes < need:
+        ws = DeviceArray((need,), np.uint8)
+        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
+    check(lib().vai_linear_i8_launch(ctypes.byref(a), stream), "vai_linear_i8_launch")
+    check(lib().vai_stream_sync(stream), "sync")   # the caller may drop its argument buffers on return
+    return out
+
+
+def qk_norm_rope_args(q, k, v, qkv, q_weight=None, k_weight=None, *, norm=True, eps=1e-6, weight_offset=0.0,
+                      pairs="HALVES", rot_dim=0, theta=10000.0, positions=None, count=None, inv_freq=None,
+                      row_stride=0):
+    """q [..., Hq, T, D] (its leading axes the batch), k, v [..., Hkv, T, D] out; qkv [..., T, (Hq + 2 Hkv) D] in.
+    v None: values stay. positions / count: device uint32 arrays ([..., T] / [1])."""
+    Hq, T, D = q.shape[-3:]
+    a = QkNormRopeArgs()
+    a.q_out, a.k_out, a.v_out, a.qkv = q.ptr, k.ptr, _ptr(v), qkv.ptr
+    a.q_weight, a.k_weight = _ptr(q_weight), _ptr(k_weight)
+    a.positions, a.count, a.inv_freq = _ptr(positions), _ptr(count), _ptr(inv_freq)
+    a.batch = int(np.prod(q.shape[:-3]))
+    a.tokens, a.hq, a.hkv, a.head_dim = T, Hq, k.shape[-3], D
+    a.row_stride = row_stride
+    a.i_dtype, a.o_dtype = qkv.code, q.code
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    if any(w.code != weights[0].code for w in weights) or any(x is not None and x.code != q.code for x in (k, v)):
+        raise VaiError("qk_norm_rope: the weights share a dtype, and so do the outputs")
+    a.w_dtype = weights[0].code if weights else NONE
+    a.norm, a.eps, a.weight_offset = 1 if norm else 0, eps, weight_offset
+    a.rope, a.rot_dim, a.theta = ROPE[pairs], rot_dim, theta
+    a._keep = (q, k, v, qkv, q_weight, k_weight, positions, count, inv_freq)
+    return a
+
+
+def qk_norm_rope(q, k, v, qkv, q_weight=None, k_weight=None, stream=None, **kw):
+    a = qk_norm_rope_args(q, k, v, qkv, q_weight, k_weight, **kw)
+    check(lib().vai_qk_norm_rope_launch(ctypes.byref(a), stream), "vai_qk_norm_rope_launch")
+    check(lib().vai_stream_sync(stream), "sync")   # the caller may drop its argument buffers on return
+    return q, k, v
+
+
 def gated_mul(out, inp, epi="SILU", stream=None):
     H = out.shape[-1]
     rows = int(np.prod(out.shape[:-1]))
@@ -374,7 +507,7 @@ def attn_scores(scores, q, k, stream=None, **kw):
 def attention_args(out, q, k, v, *, scale=None, causal=False, span=0, blocks=None, cache=None):
     """O token-major [..., Tq, Hq, D]; no mask unless causal / blocks ask for one.
     cache = (k_cache, v_cache, count, ring): the KV cache planes [Hkv, size, D]
-    (DeviceArrays of one dtype) and a device uint32 DeviceArray holding the
+    (DeviceArrays of one dtype, or CachePlanes) and a device uint32 DeviceArray holding the
     positions they held before the call; k / v may then be None (Tkv = 0)."""
     Hq, Tq, D = q.shape[-3:]
     a = AttentionArgs()
@@ -408,6 +541,40 @@ def attention(out, q, k, v, stream=None, **kw):
     check(lib().vai_attention_launch(ctypes.byref(a), stream), "vai_attention_launch")
     check(lib().vai_stream_sync(stream), "sync")   # the caller may drop its argument buffers on return
     return out
+
+
+def attention_cache_bytes(hkv, cache_size, head_dim, cache_dtype):
+    return lib().vai_attention_cache_bytes(hkv, cache_size, head_dim, cache_dtype)
+
+
+class CachePlane:
+    """A KV cache plane of any dtype code: shape [Hkv, size, D], opaque bytes for Q4."""
+
+    def __init__(self, hkv, size, head_dim, code):
+        self.shape, self.code = (hkv, size, head_dim), code
+        n = attention_cache_bytes(hkv, size, head_dim, code)
+        if not n:
+            raise VaiError(f"no cache of dtype code {code} for [{hkv}, {size}, {head_dim}]")
+        self.buf = DeviceArray((n,), np.uint8)
+        self.ptr, self.nbytes = self.buf.ptr, n
+
+
+def attention_cache_read_args(k_out, v_out, k_cache, v_cache, first_row=0):
+    """k_out, v_out [Hkv, rows, D]: the values of rows first_row .. of the planes."""
+    a = AttentionCacheReadArgs()
+    a.k_out, a.v_out, a.k_cache, a.v_cache = k_out.ptr, v_out.ptr, k_cache.ptr, v_cache.ptr
+    a.o_dtype, a.cache_dtype = k_out.code, k_cache.code
+    a.hkv, a.cache_size, a.head_dim = k_cache.shape
+    a.first_row, a.rows = first_row, k_out.shape[-2]
+    a._keep = (k_out, v_out, k_cache, v_cache)
+    return a
+
+
+def attention_cache_read(k_out, v_out, k_cache, v_cache, first_row=0, stream=None):
+    a = attention_cache_read_args(k_out, v_out, k_cache, v_cache, first_row)
+    check(lib().vai_attention_cache_read(ctypes.byref(a), stream), "vai_attention_cache_read")
+    check(lib().vai_stream_sync(stream), "sync")   # the caller may drop its argument buffers on return
+    return k_out, v_out
 
 
 def synchronize():

@@ -1048,7 +1048,7 @@ static hipError_t attention_launch_d(const AttnParams& p, hipStream_t s)
 
 hipError_t attention_launch(const AttnParams& p0, hipStream_t s)
 {
-    if (p0.cache_count && p0.tkv > 0 && !(p0.dec_units && p0.dec_append)) {
+    if (p0.cache_count && !p0.q4 && p0.tkv > 0 && !(p0.dec_units && p0.dec_append)) {
         const size_t n = (size_t)p0.tkv * p0.head_dim;
         const uint32_t blocks = (uint32_t)std::min<size_t>((n + 255) / 256, 1024);
         hipLaunchKernelGGL(attention_append_kernel, dim3(blocks, p0.hkv), dim3(256), 0, s, p0);

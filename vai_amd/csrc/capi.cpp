@@ -542,14 +542,14 @@ static vai_status make_mask(MaskRule& m, uint32_t tq, uint32_t tkv, uint32_t cau
 static vai_status attention_params(const vai_attention_args* a, AttnParams& p)
 {
     if (!a || !a->q) return VAI_ERR_INVALID_ARG;
-    const bool cache = a->cache_size > 0;
+    const bool cache = a->cache_size > 0, q4 = cache && a->cache_dtype == VAI_DTYPE_Q4;
     // K / V: needed unless a cache supplies every key (Tkv = 0)
     if ((a->tkv > 0 || !cache) && (!a->k || !a->v)) return VAI_ERR_INVALID_ARG;
     if (cache && (!a->k_cache || !a->v_cache || !a->cache_count)) return VAI_ERR_INVALID_ARG;
     const auto f32_or_f16 = [](int32_t d) { return d == VAI_DTYPE_F32 || d == VAI_DTYPE_F16; };
     if (!f32_or_f16(a->q_dtype) || !dtype_ok(a->o_dtype)) return VAI_ERR_DTYPE;
     if (a->tkv > 0 && !f32_or_f16(a->kv_dtype)) return VAI_ERR_DTYPE;
-    if (cache && !f32_or_f16(a->cache_dtype)) return VAI_ERR_DTYPE;
+    if (cache && !q4 && !f32_or_f16(a->cache_dtype)) return VAI_ERR_DTYPE;
     if (a->batch == 0 || a->hq == 0 || a->hkv == 0 || a->tq == 0 || (a->tkv == 0 && !cache) || a->head_dim == 0 ||
         a->hq % a->hkv != 0)
         return VAI_ERR_SHAPE;
@@ -557,13 +557,27 @@ static vai_status attention_params(const vai_attention_args* a, AttnParams& p)
     // (attention.h:1016); a ring's tiles must not wrap it; without a ring the
     // new rows must fit
     if (cache && (a->batch != 1 || (a->cache_ring && a->cache_size % 64 != 0) ||
-                  (!a->cache_ring && a->tkv > a->cache_size)))
+                  ((!a->cache_ring || q4) && a->tkv > a->cache_size)))
         return VAI_ERR_SHAPE;
+    if (q4 && q4_dp(a->head_dim) == 0) return VAI_ERR_UNSUPPORTED;
+    if (q4 && ((uintptr_t)a->k_cache % 16 != 0 || (uintptr_t)a->v_cache % 16 != 0)) return VAI_ERR_INVALID_ARG;
+    // a 4-bit ring attends what it holds: the rows the call's own overwrite are gone
+    uint32_t span = a->span;
+    if (q4 && a->cache_ring) {
+        const uint32_t held = a->cache_size - a->tkv + 1;
+        span = span ? std::min(span, held) : held;
+    }
     p = AttnParams{};
     p.out = a->out; p.q = a->q;
     p.o_dtype = a->o_dtype; p.q_dtype = a->q_dtype;
     p.batch = a->batch; p.hq = a->hq; p.hkv = a->hkv; p.tq = a->tq; p.tkv = a->tkv; p.head_dim = a->head_dim;
-    if (cache) {
+    if (q4) {
+        p.q4 = 1;
+        p.k4 = (uint8_t*)a->k_cache; p.v4 = (uint8_t*)a->v_cache;
+        p.k = p.v = (const void*)256; p.kv_dtype = VAI_DTYPE_F16;   // the copies in the workspace, aligned
+        p.cache_count = a->cache_count; p.kv_rows = a->cache_size; p.ring = a->cache_ring ? 1u : 0u;
+        p.k_new = a->k; p.v_new = a->v; p.new_dtype = a->kv_dtype;
+    } else if (cache) {
         p.k = a->k_cache; p.v = a->v_cache; p.kv_dtype = a->cache_dtype;
         p.cache_count = a->cache_count; p.kv_rows = a->cache_size; p.ring = a->cache_ring ? 1u : 0u;
         p.k_new = a->k; p.v_new = a->v; p.new_dtype = a->kv_dtype;
@@ -571,8 +585,8 @@ static vai_status attention_params(const vai_attention_args* a, AttnParams& p)
         p.k = a->k; p.v = a->v; p.kv_dtype = a->kv_dtype; p.kv_rows = a->tkv;
     }
     p.scale = a->scale != 0.f ? a->scale : 1.0f / std::sqrt((float)a->head_dim);
-    p.span = a->span;
-    if (vai_status st = make_mask(p.mask, a->tq, a->tkv, a->causal, a->span, a->mask_blocks, a->mask_bits,
+    p.span = span;
+    if (vai_status st = make_mask(p.mask, a->tq, a->tkv, a->causal, span, a->mask_blocks, a->mask_bits,
                                   a->mask_block_end); st != VAI_OK)
         return st;
     p.causal = p.mask.blocks == 1;
@@ -585,7 +599,7 @@ size_t vai_attention_workspace_size(const vai_attention_args* a)
 {
     AttnParams p;
     if (attention_params(a, p) != VAI_OK) return 0;
-    return attention_workspace_bytes(p);
+    return p.q4 ? attention_q4_workspace(p) : attention_workspace_bytes(p);
 }
 
 vai_status vai_attention_launch(const vai_attention_args* a, vai_stream_t stream)
@@ -594,12 +608,128 @@ vai_status vai_attention_launch(const vai_attention_args* a, vai_stream_t stream
     if (a && !a->out) return VAI_ERR_INVALID_ARG;
     vai_status st = attention_params(a, p);
     if (st != VAI_OK) return st;
-    const size_t need = attention_workspace_bytes(p);
+    const size_t need = p.q4 ? attention_q4_workspace(p) : attention_workspace_bytes(p);
     if (need) {
         if (!a->workspace || a->workspace_bytes < need) return VAI_ERR_WORKSPACE;
-        attention_set_workspace(p, a->workspace);
+        if (!p.q4) attention_set_workspace(p, a->workspace);
+    }
+    if (p.q4) {
+        if ((uintptr_t)a->workspace % 16 != 0) return VAI_ERR_INVALID_ARG;
+        attention_q4_set_workspace(p, a->workspace);
+        return hip_status(attention_q4_launch(p, (hipStream_t)stream));
     }
     return hip_status(attention_launch(p, (hipStream_t)stream));
+}
+
+size_t vai_attention_cache_bytes(uint32_t hkv, uint32_t cache_size, uint32_t head_dim, int32_t cache_dtype)
+{
+    if (hkv == 0 || cache_size == 0 || head_dim == 0) return 0;
+    if (cache_dtype == VAI_DTYPE_Q4) return q4_dp(head_dim) ? q4_plane_bytes(hkv, cache_size, head_dim) : 0;
+    return dtype_ok(cache_dtype) ? (size_t)hkv * cache_size * head_dim * dtype_bytes(cache_dtype) : 0;
+}
+
+vai_status vai_attention_cache_read(const vai_attention_cache_read_args* a, vai_stream_t stream)
+{
+    if (!a || !a->k_out || !a->v_out || !a->k_cache || !a->v_cache) return VAI_ERR_INVALID_ARG;
+    if (!dtype_ok(a->o_dtype) || (!dtype_ok(a->cache_dtype) && a->cache_dtype != VAI_DTYPE_Q4)) return VAI_ERR_DTYPE;
+    if (a->hkv == 0 || a->hkv > 65535 || a->cache_size == 0 || a->head_dim == 0 || a->rows == 0 ||
+        a->rows > a->cache_size || a->first_row >= a->cache_size)
+        return VAI_ERR_SHAPE;
+    const bool q4 = a->cache_dtype == VAI_DTYPE_Q4;
+    if (q4 && q4_dp(a->head_dim) == 0) return VAI_ERR_UNSUPPORTED;
+    if (q4 && ((uintptr_t)a->k_cache % 16 != 0 || (uintptr_t)a->v_cache % 16 != 0)) return VAI_ERR_INVALID_ARG;
+    CacheReadParams p{};
+    p.k_out = a->k_out; p.v_out = a->v_out; p.k = a->k_cache; p.v = a->v_cache;
+    p.o_dtype = a->o_dtype; p.cache_dtype = a->cache_dtype;
+    p.hkv = a->hkv; p.rows = a->cache_size; p.head_dim = a->head_dim; p.first = a->first_row; p.n = a->rows;
+    return hip_status(cache_read_launch(p, (hipStream_t)stream));
+}
+
+vai_status vai_qk_norm_rope_launch(const vai_qk_norm_rope_args* a, vai_stream_t stream)
+{
+    if (!a || !a->q_out || !a->k_out || !a->qkv) return VAI_ERR_INVALID_ARG;
+    if (!dtype_ok(a->i_dtype) || !dtype_ok(a->o_dtype)) return VAI_ERR_DTYPE;
+    if ((a->q_weight || a->k_weight) && !dtype_ok(a->w_dtype)) return VAI_ERR_DTYPE;
+    if (a->rope > VAI_ROPE_NEIGHBOURS || a->norm > 1) return VAI_ERR_INVALID_ARG;
+    if (a->batch == 0 || a->tokens == 0 || a->hq == 0 || a->hkv == 0 || a->head_dim == 0) return VAI_ERR_SHAPE;
+    if (a->head_dim > QkNormRopeParams::MAX_DIM || a->hq > 65535 || a->hkv > 65535) return VAI_ERR_UNSUPPORTED;
+    const uint64_t row = (uint64_t)(a->hq + 2 * a->hkv) * a->head_dim;
+    if (row > UINT32_MAX || (a->row_stride && a->row_stride < row)) return VAI_ERR_SHAPE;
+    const uint32_t rot = a->rope == VAI_ROPE_NONE ? 0u : a->rot_dim ? a->rot_dim : a->head_dim;
+    if (rot > a->head_dim || rot % 2 != 0) return VAI_ERR_SHAPE;
+    // (theta = 1 is no rotation scale but a legal base; NaN fails every comparison)
+    if (rot && !a->inv_freq && !(a->theta > 0.f && a->theta <= 3.4028235e38f)) return VAI_ERR_INVALID_ARG;
+    if (a->norm && !(a->eps >= 0.f)) return VAI_ERR_INVALID_ARG;
+    QkNormRopeParams p{};
+    p.q_out = a->q_out; p.k_out = a->k_out; p.v_out = a->v_out; p.qkv = a->qkv;
+    p.q_weight = a->norm ? a->q_weight : nullptr; p.k_weight = a->norm ? a->k_weight : nullptr;
+    p.positions = a->positions; p.count = a->count; p.inv_freq = a->inv_freq;
+    p.i_dtype = a->i_dtype; p.o_dtype = a->o_dtype; p.w_dtype = a->w_dtype;
+    p.batch = a->batch; p.tokens = a->tokens; p.hq = a->hq; p.hkv = a->hkv; p.head_dim = a->head_dim;
+    p.row_stride = a->row_stride ? a->row_stride : (uint32_t)row;
+    p.norm = a->norm; p.neighbours = a->rope == VAI_ROPE_NEIGHBOURS; p.rot_dim = rot;
+    p.eps = a->eps; p.weight_offset = a->weight_offset;
+    return hip_status(qk_norm_rope_launch(p, a->theta, (hipStream_t)stream));
+}
+
+// Rows of 8-bit integers: weights start every 16 bytes, the call's own rounding
+// of X every 128 (whole blocks of the kernels).
+static uint32_t i8_row(uint32_t K) { return (K + 15) / 16 * 16; }
+static uint32_t i8_x_row(uint32_t K) { return (K + 127) / 128 * 128; }
+static constexpr uint32_t kMaxI8K = 131072;   // 128 * 128 * K stays within 32-bit sums
+
+vai_status vai_quantize_i8_launch(void* out, float* scale, const void* in, int32_t i_dtype, uint32_t rows, uint32_t K,
+                                  vai_stream_t stream)
+{
+    if (!out || !scale || !in) return VAI_ERR_INVALID_ARG;
+    if (!dtype_ok(i_dtype)) return VAI_ERR_DTYPE;
+    if (rows == 0 || K == 0) return VAI_ERR_SHAPE;
+    if (K > kMaxI8K || rows >= 1u << 24) return VAI_ERR_UNSUPPORTED;
+    if ((uintptr_t)out % 16 != 0) return VAI_ERR_INVALID_ARG;
+    return hip_status(quantize_i8_launch(out, scale, in, i_dtype, rows, K, i8_row(K), (hipStream_t)stream));
+}
+
+static vai_status check_linear_i8(const vai_linear_i8_args* a)
+{
+    if (!a || !a->out || !a->in || !a->weight || !a->w_scale) return VAI_ERR_INVALID_ARG;
+    if (a->M == 0 || a->N == 0 || a->K == 0) return VAI_ERR_SHAPE;
+    if (a->K > kMaxI8K || a->M >= 1u << 21 || a->N >= 1u << 24) return VAI_ERR_UNSUPPORTED;
+    if (!dtype_ok(a->o_dtype) || !dtype_ok(a->i_dtype)) return VAI_ERR_DTYPE;
+    if (a->bias && !dtype_ok(a->b_dtype)) return VAI_ERR_DTYPE;
+    if (a->epilogue > VAI_EPI_SIGMOID || a->residual_order > 1) return VAI_ERR_INVALID_ARG;
+    if ((uintptr_t)a->weight % 16 != 0) return VAI_ERR_INVALID_ARG;
+    const uint64_t MN = (uint64_t)a->M * a->N;
+    if (a->bias && a->bias_repeat && (a->bias_repeat % a->N != 0 || MN % a->bias_repeat != 0)) return VAI_ERR_SHAPE;
+    if (a->residual && a->residual_repeat && (a->residual_repeat % a->N != 0 || MN % a->residual_repeat != 0))
+        return VAI_ERR_SHAPE;
+    return VAI_OK;
+}
+
+size_t vai_linear_i8_workspace_size(const vai_linear_i8_args* a)
+{
+    if (check_linear_i8(a) != VAI_OK) return 0;
+    return (size_t)a->M * i8_x_row(a->K) + (size_t)a->M * sizeof(float);
+}
+
+vai_status vai_linear_i8_launch(const vai_linear_i8_args* a, vai_stream_t stream)
+{
+    const vai_status st = check_linear_i8(a);
+    if (st != VAI_OK) return st;
+    const size_t need = vai_linear_i8_workspace_size(a);
+    if (need && (!a->workspace || a->workspace_bytes < need)) return VAI_ERR_WORKSPACE;
+    if ((uintptr_t)a->workspace % 16 != 0) return VAI_ERR_INVALID_ARG;
+    LinearI8Params p{};
+    p.out = a->out; p.bias = a->bias; p.residual = a->residual;
+    p.o_dtype = a->o_dtype; p.b_dtype = a->b_dtype;
+    p.bias_repeat = a->bias_repeat; p.residual_repeat = a->residual_repeat;
+    p.epilogue = a->epilogue; p.residual_order = a->residual_order; p.scalar_scale = a->scalar_scale;
+    p.M = a->M; p.N = a->N; p.K = a->K; p.x_stride = i8_x_row(a->K); p.w_stride = i8_row(a->K);
+    int8_t* x = (int8_t*)a->workspace;
+    float* xs = (float*)(x + (size_t)a->M * p.x_stride);
+    p.x = x; p.x_scale = xs; p.weight = (const int8_t*)a->weight; p.w_scale = a->w_scale;
+    const hipError_t e = quantize_i8_launch(x, xs, a->in, a->i_dtype, a->M, a->K, p.x_stride, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_status(e);
+    return hip_status(linear_i8_launch(p, (hipStream_t)stream));
 }
 
 vai_status vai_gated_mul_launch(void* out, int32_t o_dtype, const void* in, int32_t i_dtype, uint32_t rows,

@@ -24,7 +24,7 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 typedef float float8v __attribute__((ext_vector_type(8)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
-enum : int { DT_F32 = 0, DT_F16 = 1 };
+enum : int { DT_F32 = 0, DT_F16 = 1, DT_Q4 = 3 };   // (Q4: a KV cache's planes)
 
 __device__ __forceinline__ float ld(const void* p, int dt, size_t i)
 {

@@ -215,6 +215,12 @@ struct AttnParams {
     // unit | its chunk count << 16 (a head has at most FA_WG_TAB units, so at
     // most that many query tiles)
     uint32_t qt_tab[FA_WG_TAB];
+    // A cache in 4 bits (attention_q4.hip): its planes; k / v then point at the
+    // fp16 copies the other kernels read, and the new rows, appended first,
+    // count as cached rows like any other.
+    uint8_t* k4;
+    uint8_t* v4;
+    uint32_t q4;
     // Few query rows per KV head (attention_decode.hip): dec_units > 0 takes
     // that path, with dec_rows = tq * hq / hkv rows per KV head, dec_rpb of
     // them per workgroup; dec_append: it also appends the new rows.
@@ -254,6 +260,64 @@ void attention_plan(AttnParams& p, uint32_t cus);
 size_t attention_workspace_bytes(const AttnParams& p);
 void attention_set_workspace(AttnParams& p, void* ws);
 hipError_t attention_launch(const AttnParams& p, hipStream_t s);
+
+// The KV cache in 4 bits (attention_q4.hip). A plane holds, per KV head, tiles
+// of 32 positions of rows `dp` wide (the head dim padded to 64, 128 or 256).
+uint32_t q4_dp(uint32_t head_dim);                       // 0: head_dim > 256
+size_t q4_plane_bytes(uint32_t hkv, uint32_t rows, uint32_t head_dim);
+hipError_t attention_q4_launch(const AttnParams& p, hipStream_t s);
+size_t attention_q4_workspace(const AttnParams& p);
+void attention_q4_set_workspace(AttnParams& p, void* ws);
+
+// Rows of a cache as values: rows [first, first + n) of every head (wrapping at
+// the plane's end) to [hkv, n, head_dim].
+struct CacheReadParams {
+    void* k_out;
+    void* v_out;
+    const void* k;
+    const void* v;
+    int o_dtype, cache_dtype;     // DT_F32, DT_F16 or DT_Q4
+    uint32_t hkv, rows, head_dim, first, n;
+};
+hipError_t cache_read_launch(const CacheReadParams& p, hipStream_t s);
+
+// Head norms and the position rotation (qk_norm_rope.hip).
+struct QkNormRopeParams {
+    static constexpr uint32_t MAX_DIM = 2048;
+    void* q_out;                  // [batch, hq, tokens, head_dim]
+    void* k_out;                  // [batch, hkv, tokens, head_dim]
+    void* v_out;                  // the same, or null: values stay where they are
+    const void* qkv;              // [batch, tokens] rows of row_stride elements: hq + 2 hkv heads
+    const void* q_weight;         // [head_dim] or null: ones
+    const void* k_weight;
+    const uint32_t* positions;    // [batch, tokens], or null: count + token
+    const uint32_t* count;        // device uint32, or null: 0
+    const float* inv_freq;        // [rot_dim / 2], or null: the tables
+    int i_dtype, o_dtype, w_dtype;
+    uint32_t batch, tokens, hq, hkv, head_dim, row_stride;
+    uint32_t norm, neighbours, rot_dim;   // rot_dim 0: no rotation
+    float eps, weight_offset;
+    double turn_hi[MAX_DIM / 32], turn_lo[16];   // pair i turns turn_hi[i / 16] * turn_lo[i % 16] a position
+};
+hipError_t qk_norm_rope_launch(QkNormRopeParams p, float theta, hipStream_t s);
+
+// Linear over 8-bit weights (linear_i8.hip).
+struct LinearI8Params {
+    void* out;
+    const void* bias;
+    const void* residual;
+    int o_dtype, b_dtype;
+    uint32_t bias_repeat, residual_repeat, epilogue, residual_order;
+    float scalar_scale;
+    const int8_t* x;              // [M] rows of x_stride bytes (a multiple of 128), zeros past K
+    const float* x_scale;         // [M]
+    const int8_t* weight;         // [N] rows of w_stride bytes (K rounded up to 16)
+    const float* w_scale;         // [N]
+    uint32_t M, N, K, x_stride, w_stride;
+};
+hipError_t quantize_i8_launch(void* out, float* scale, const void* in, int in_dtype, uint32_t rows, uint32_t K,
+                              uint32_t stride, hipStream_t s);
+hipError_t linear_i8_launch(const LinearI8Params& p, hipStream_t s);
 
 // Implicit-GEMM convolution, fp16 weights packed per tap in MFMA fragment order.
 struct ConvParams {
