@@ -652,7 +652,9 @@ vai_status vai_qk_norm_rope_launch(const vai_qk_norm_rope_args* a, vai_stream_t 
     if ((a->q_weight || a->k_weight) && !dtype_ok(a->w_dtype)) return VAI_ERR_DTYPE;
     if (a->rope > VAI_ROPE_NEIGHBOURS || a->norm > 1) return VAI_ERR_INVALID_ARG;
     if (a->batch == 0 || a->tokens == 0 || a->hq == 0 || a->hkv == 0 || a->head_dim == 0) return VAI_ERR_SHAPE;
-    if (a->head_dim > QkNormRopeParams::MAX_DIM || a->hq > 65535 || a->hkv > 65535) return VAI_ERR_UNSUPPORTED;
+    if (a->head_dim > QkNormRopeParams::MAX_DIM || a->hq > 65535 || a->hkv > 65535 ||
+        (uint64_t)a->batch * a->tokens >= 1u << 31)
+        return VAI_ERR_UNSUPPORTED;
     const uint64_t row = (uint64_t)(a->hq + 2 * a->hkv) * a->head_dim;
     if (row > UINT32_MAX || (a->row_stride && a->row_stride < row)) return VAI_ERR_SHAPE;
     const uint32_t rot = a->rope == VAI_ROPE_NONE ? 0u : a->rot_dim ? a->rot_dim : a->head_dim;
