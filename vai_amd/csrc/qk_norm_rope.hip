@@ -17,12 +17,22 @@ namespace vai_dev {
 
 // cos and sin of position * f_i. The angle is taken in turns, in 64 bits (at
 // position 100000 the fastest pair has made 16000 turns, of which fp32 would
-// keep three digits), and only its fraction goes on in fp32.
+// keep three digits), and only its fraction goes on in fp32. From there the
+// nearest quarter turn is taken off and the rest, at most pi / 4, put into the
+// power series: the first term left out is below 2^-25 for the cosine (x^10 /
+// 10!) and 2^-28 of the sine (x^10 / 11!).
 __device__ __forceinline__ void turn_of(const QkNormRopeParams& p, uint32_t pos, uint32_t i, float& c, float& s)
 {
     const double f = p.inv_freq ? (double)p.inv_freq[i] * 0.15915494309189533577 : p.turn_hi[i >> 4] * p.turn_lo[i & 15];
     const double t = (double)pos * f;
-    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+    const float fr = (float)(t - rint(t)), q = rintf(4.0f * fr);
+    const float x = 6.2831853071795865f * fmaf(-0.25f, q, fr), x2 = x * x;
+    const float sx = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), x);
+    const float cx = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 1.f / 40320, -1.f / 720), 1.f / 24), -0.5f), 1.0f);
+    const int k = (int)q & 3;
+    const float a = k & 1 ? cx : sx, b = k & 1 ? sx : cx;
+    s = k & 2 ? -a : a;
+    c = k == 1 || k == 2 ? -b : b;
 }
 
 // Any head dim: a wave takes one head at a time, in LDS as fp32.
@@ -93,8 +103,11 @@ __device__ __forceinline__ float group_sum(float x)
 // so that a lane holds both values of its four pairs: with halves values 4 j ..
 // +3 and the same of the other half, else 8 neighbouring ones. A lane's four
 // angles then serve every head of the token. A wave takes a token's heads 64 / L
-// at a time, its share of them ([first, last) steps of the token), four steps'
-// loads in flight.
+// at a time, its share of them (blockIdx.y of `shares`). One step's loads at a
+// time and 44 registers: eight waves a SIMD hide the loads better than four
+// steps at a time in 72 registers do. 4096 tokens of 32 + 8 + 8 fp16 heads of
+// 128: 20.4 us (23.8 with four steps at a time), 4.9 TB/s, where a large copy
+// makes 5.2; a single token's 3.9 us are latency (the smallest kernels here take 2.3).
 __device__ __forceinline__ float4v weight4(const void* w, int dt, uint32_t d)
 {
     typedef half4 half4u __attribute__((aligned(2)));
@@ -107,7 +120,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, u
 {
     typedef TI in4 __attribute__((ext_vector_type(4)));
     typedef TO out4 __attribute__((ext_vector_type(4)));
-    constexpr int HPW = 64 / L, U = 4;
+    constexpr int HPW = 64 / L;
     const uint32_t D = p.head_dim, heads = p.hq + 2 * p.hkv, nk = p.hq + p.hkv, lane = threadIdx.x & 63;
     const uint32_t j = lane % L, sub = lane / L, half = p.rot_dim / 2;
     const bool on = 8 * j < D, turned = 8 * j < p.rot_dim, split = turned && !p.neighbours;
@@ -130,15 +143,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, u
         const TI* row = (const TI*)p.qkv + (size_t)bt * p.row_stride;
         float c[4], s[4];
         bool angles = false;
-        for (uint32_t it = s0; it < s1; it += U) {
-            in4 xa[U], xb[U];
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                if (it + k >= s1) break;
-                const uint32_t h = min((it + k) * HPW + sub, heads - 1);
-                xa[k] = *(const in4*)(row + (size_t)h * D + oa);
-                xb[k] = *(const in4*)(row + (size_t)h * D + ob);
-            }
+        for (uint32_t it = s0; it < s1; ++it) {
+            const uint32_t h = it * HPW + sub, hc = min(h, heads - 1);
+            const in4 xa = *(const in4*)(row + (size_t)hc * D + oa), xb = *(const in4*)(row + (size_t)hc * D + ob);
             if (!angles) {   // (under the first loads)
                 angles = true;
                 const uint32_t pos = p.positions ? p.positions[bt] : first_pos + t;
@@ -149,49 +156,40 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, u
                     if (turned) turn_of(p, pos, 4 * j + i, c[i], s[i]);
                 }
             }
+            float y[8], sq = 0.f;
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                if (it + k >= s1) break;
-                const uint32_t h = (it + k) * HPW + sub;
-                float y[8], sq = 0.f;
+            for (int e = 0; e < 4; ++e) {
+                y[e] = (float)xa[e];
+                y[4 + e] = (float)xb[e];
+            }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    y[e] = (float)xa[k][e];
-                    y[4 + e] = (float)xb[k][e];
-                }
+            for (int e = 0; e < 8; ++e) sq = fmaf(y[e], y[e], sq);
+            sq = group_sum<L>(on ? sq : 0.f);
+            const bool is_q = h < p.hq, is_v = h >= nk;
+            if (p.norm && !is_v) {
+                const float inv = __builtin_amdgcn_rsqf(sq * inv_d + p.eps);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sq = fmaf(y[e], y[e], sq);
-                sq = group_sum<L>(on ? sq : 0.f);
-                const bool is_q = h < p.hq, is_v = h >= nk;
-                if (p.norm && !is_v) {
-                    const float inv = __builtin_amdgcn_rsqf(sq * inv_d + p.eps);
+                for (int e = 0; e < 8; ++e) y[e] *= inv * (is_q ? wq[e >> 2][e & 3] : wk[e >> 2][e & 3]);
+            }
+            if (turned && !is_v) {
+                const auto turn = [&](float& a, float& e, int i) __attribute__((always_inline)) {
+                    const float x = a;
+                    a = x * c[i] - e * s[i];
+                    e = e * c[i] + x * s[i];
+                };
+                if (p.neighbours)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] *= inv * (is_q ? wq[e >> 2][e & 3] : wk[e >> 2][e & 3]);
-                }
-                if (turned && !is_v) {
-                    if (p.neighbours) {
+                    for (int i = 0; i < 4; ++i) turn(y[2 * i], y[2 * i + 1], i);
+                else
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float a = y[2 * i], e = y[2 * i + 1];
-                            y[2 * i] = a * c[i] - e * s[i];
-                            y[2 * i + 1] = e * c[i] + a * s[i];
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float a = y[i], e = y[4 + i];
-                            y[i] = a * c[i] - e * s[i];
-                            y[4 + i] = e * c[i] + a * s[i];
-                        }
-                    }
-                }
-                TO* out = (TO*)(is_q ? p.q_out : is_v ? p.v_out : p.k_out);
-                const uint32_t oh = is_q ? h : is_v ? h - nk : h - p.hq, nh = is_q ? p.hq : p.hkv;
-                if (on && h < heads && out) {
-                    TO* dst = out + (((size_t)b * nh + oh) * p.tokens + t) * D;
-                    *(out4*)(dst + oa) = __builtin_convertvector((float4v{y[0], y[1], y[2], y[3]}), out4);
-                    *(out4*)(dst + ob) = __builtin_convertvector((float4v{y[4], y[5], y[6], y[7]}), out4);
-                }
+                    for (int i = 0; i < 4; ++i) turn(y[i], y[4 + i], i);
+            }
+            TO* out = (TO*)(is_q ? p.q_out : is_v ? p.v_out : p.k_out);
+            const uint32_t oh = is_q ? h : is_v ? h - nk : h - p.hq, nh = is_q ? p.hq : p.hkv;
+            if (on && h < heads && out) {
+                TO* dst = out + (((size_t)b * nh + oh) * p.tokens + t) * D;
+                *(out4*)(dst + oa) = __builtin_convertvector((float4v{y[0], y[1], y[2], y[3]}), out4);
+                *(out4*)(dst + ob) = __builtin_convertvector((float4v{y[4], y[5], y[6], y[7]}), out4);
             }
         }
     }
@@ -200,9 +198,11 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, u
 template <typename TI, typename TO, int L>
 static hipError_t launch_vec(const QkNormRopeParams& p, hipStream_t s)
 {
+    // tokens whose waves alone fill the chip are not shared out: each share takes
+    // the angles again (4096 tokens: one share 20.4 us, two 22.6)
     const uint32_t steps = (p.hq + 2 * p.hkv + 64 / L - 1) / (64 / L);
     const uint32_t rows = p.batch * p.tokens;
-    const uint32_t shares = std::min(steps, std::max(1u, 8192 / rows));
+    const uint32_t shares = std::min(steps, std::max(1u, 4096 / rows));
     hipLaunchKernelGGL((qk_norm_rope_kernel<TI, TO, L>), dim3(std::min((rows + 3) / 4, 1u << 20), shares), dim3(256), 0, s,
                        p, shares, steps);
     return hipGetLastError();
