@@ -154,8 +154,9 @@ vai_status vai_linear_plan(const vai_linear_args* args, char* name, size_t name_
  * (or below fp32's normal range over 127) gives 0 for A, one that holds a NaN
  * or an infinity NaN. bias, residual, their repeats, epilogue and scalar_scale
  * as in vai_linear_args. K <= 131072.
- * The workspace (vai_linear_i8_workspace_size() bytes, 16-byte aligned) holds
- * the rounded rows of X; calls that overlap in time need one each.
+ * The workspace (vai_linear_i8_workspace_size() bytes, 16-byte aligned; 0 for
+ * one or a few short rows) holds the rounded rows of X; calls that overlap in
+ * time need one each.
  * ------------------------------------------------------------------------- */
 typedef struct {
     void* out;

@@ -709,7 +709,7 @@ static vai_status check_linear_i8(const vai_linear_i8_args* a)
 
 size_t vai_linear_i8_workspace_size(const vai_linear_i8_args* a)
 {
-    if (check_linear_i8(a) != VAI_OK) return 0;
+    if (check_linear_i8(a) != VAI_OK || linear_i8_fused(a->M, a->K)) return 0;
     return (size_t)a->M * i8_x_row(a->K) + (size_t)a->M * sizeof(float);
 }
 
@@ -719,16 +719,18 @@ vai_status vai_linear_i8_launch(const vai_linear_i8_args* a, vai_stream_t stream
     if (st != VAI_OK) return st;
     const size_t need = vai_linear_i8_workspace_size(a);
     if (need && (!a->workspace || a->workspace_bytes < need)) return VAI_ERR_WORKSPACE;
-    if ((uintptr_t)a->workspace % 16 != 0) return VAI_ERR_INVALID_ARG;
+    if (need && (uintptr_t)a->workspace % 16 != 0) return VAI_ERR_INVALID_ARG;
     LinearI8Params p{};
     p.out = a->out; p.bias = a->bias; p.residual = a->residual;
     p.o_dtype = a->o_dtype; p.b_dtype = a->b_dtype;
     p.bias_repeat = a->bias_repeat; p.residual_repeat = a->residual_repeat;
     p.epilogue = a->epilogue; p.residual_order = a->residual_order; p.scalar_scale = a->scalar_scale;
     p.M = a->M; p.N = a->N; p.K = a->K; p.x_stride = i8_x_row(a->K); p.w_stride = i8_row(a->K);
+    p.weight = (const int8_t*)a->weight; p.w_scale = a->w_scale;
+    if (!need) return hip_status(linear_i8_fused_launch(p, a->in, a->i_dtype, (hipStream_t)stream));
     int8_t* x = (int8_t*)a->workspace;
     float* xs = (float*)(x + (size_t)a->M * p.x_stride);
-    p.x = x; p.x_scale = xs; p.weight = (const int8_t*)a->weight; p.w_scale = a->w_scale;
+    p.x = x; p.x_scale = xs;
     const hipError_t e = quantize_i8_launch(x, xs, a->in, a->i_dtype, a->M, a->K, p.x_stride, (hipStream_t)stream);
     if (e != hipSuccess) return hip_status(e);
     return hip_status(linear_i8_launch(p, (hipStream_t)stream));
