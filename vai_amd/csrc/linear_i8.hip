@@ -199,8 +199,7 @@ __device__ __forceinline__ void few_wait_lds() { __builtin_amdgcn_s_waitcnt(15 |
 // flight, and no wave waits for another until the sums meet. Chunk c of slab row
 // r stands at chunk c ^ (r / 2 % 8): fragment reads hit every bank group once.
 // FUSED (MT = 1): X is rounded here, under the first copies of W, by every
-// workgroup for itself (NW / M waves share a row: each takes the whole row's
-// largest value and rounds its part); else its codes come from the workspace,
+// workgroup for itself (NW / M waves share a row); else its codes come from the workspace,
 // through the ring like W.
 template <int MT, int NT, int NW, int D, bool FUSED> struct FewCfg {
     static constexpr int BLOCK = (NT + (FUSED ? 0 : MT)) * 2048;   // a block of K in LDS: 16-row slabs
@@ -242,14 +241,15 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
                                                      (int)(slab_row * (w ? p.w_stride : p.x_stride) + ch * 16 + k), 0, 0, 0);
         }
     };
+    // FUSED: this wave's parts of its row of X, 1024 values every `share` of them
     // (X before W: loads and copies are waited for in their order)
     constexpr int KEEP = FUSED ? 4 : 1;
-    const uint32_t share = std::max<uint32_t>(NW / p.M, 1);   // FUSED: waves of a row
+    const uint32_t share = std::max<uint32_t>(NW / p.M, 1), part = wave % share;   // waves of a row
     Raw16<TX> kept[KEEP];
     if constexpr (FUSED)
 #pragma unroll
         for (int i = 0; i < KEEP; ++i)
-            kept[i].load(in + (size_t)std::min<uint32_t>(wave / share, p.M - 1) * p.K, i * 1024 + lane * 16, p.K);
+            kept[i].load(in + (size_t)std::min<uint32_t>(wave / share, p.M - 1) * p.K, (i * share + part) * 1024 + lane * 16, p.K);
     if (mine > 0)
 #pragma unroll
         for (int i = 0; i < D; ++i) copy(i);
@@ -258,11 +258,15 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
     LDS_AS int8_t* xl = (LDS_AS int8_t*)(lds + C::RING);
     LDS_AS float* sl = (LDS_AS float*)(xl + p.M * ls);
     if constexpr (FUSED) {
-        for (uint32_t m = wave / share; m < p.M; m += NW / share) {
-            const TX* x = in + (size_t)m * p.K;
-            if (m >= NW)   // (a wave's second row and on)
+        LDS_AS uint32_t* ml = (LDS_AS uint32_t*)(sl + p.M);   // largest values, a part each
+        const uint32_t step = share * 1024, rest = KEEP * step + part * 1024 + lane * 16;
+        for (uint32_t m0f = 0; m0f < p.M; m0f += NW / share) {
+            const uint32_t m = m0f + wave / share;
+            const bool on = m < p.M;
+            const TX* x = in + (size_t)(on ? m : 0u) * p.K;
+            if (m0f > 0)   // (rows past the first of each wave)
 #pragma unroll
-                for (int i = 0; i < KEEP; ++i) kept[i].load(x, i * 1024 + lane * 16, p.K);
+                for (int i = 0; i < KEEP; ++i) kept[i].load(x, (i * share + part) * 1024 + lane * 16, p.K);
             uint32_t amax = 0;
 #pragma unroll
             for (int i = 0; i < KEEP; ++i) {
@@ -270,26 +274,30 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
                 kept[i].values(y);
                 amax = abs_max16(y, amax);
             }
-            for (uint32_t k = KEEP * 1024 + lane * 16; k < p.K; k += 1024) {
+            for (uint32_t k = rest; k < p.K; k += step) {
                 float y[16];
                 row16(x, k, p.K, y);
                 amax = abs_max16(y, amax);
             }
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) amax = std::max(amax, (uint32_t)__shfl_xor((int)amax, o));
+            if (share > 1) {   // (uniform: then every row is in this one pass)
+                if (lane == 0) ml[wave] = amax;
+                __syncthreads();
+                for (uint32_t w = 0; w < share; ++w) amax = std::max(amax, (uint32_t)ml[wave / share * share + w]);
+            }
             const float s = row_scale(amax), inv = s > 0.f ? 1.0f / s : 0.f;
-            const uint32_t part = wave % share;
+            if (!on) continue;
             if (part == 0 && lane == 0) sl[m] = s;
 #pragma unroll
             for (int i = 0; i < KEEP; ++i) {
-                const uint32_t k = i * 1024 + lane * 16;
-                if (k >= p.x_stride || i % share != part) continue;
+                const uint32_t k = (i * share + part) * 1024 + lane * 16;
+                if (k >= p.x_stride) continue;
                 float y[16];
                 kept[i].values(y);
                 *(LDS_AS int4v*)(xl + m * ls + k) = inv > 0.f ? codes16(y, s, inv) : (int4v)0;
             }
-            for (uint32_t i = KEEP, k = KEEP * 1024 + lane * 16; k < p.x_stride; k += 1024, ++i) {
-                if (i % share != part) continue;
+            for (uint32_t k = rest; k < p.x_stride; k += step) {
                 float y[16];
                 row16(x, k, p.K, y);
                 *(LDS_AS int4v*)(xl + m * ls + k) = inv > 0.f ? codes16(y, s, inv) : (int4v)0;
@@ -332,15 +340,15 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
 
     // the waves' sums, then lane (c16, g) of fragment (m, j) holds row 16 m + c16, columns 16 j + 4 g ..+3
     __syncthreads();
-    LDS_AS int4v* part = (LDS_AS int4v*)lds;
+    LDS_AS int4v* sums = (LDS_AS int4v*)lds;
 #pragma unroll
-    for (int f = 0; f < MT * NT; ++f) part[(wave * MT * NT + f) * 64 + lane] = acc[f / NT][f % NT];
+    for (int f = 0; f < MT * NT; ++f) sums[(wave * MT * NT + f) * 64 + lane] = acc[f / NT][f % NT];
     __syncthreads();
     const OutputSpec q = i8_output(p);
     for (int f = wave; f < MT * NT; f += NW) {
-        int4v v = part[f * 64 + lane];
+        int4v v = sums[f * 64 + lane];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) v += part[(w * MT * NT + f) * 64 + lane];
+        for (int w = 1; w < NW; ++w) v += sums[(w * MT * NT + f) * 64 + lane];
         const uint32_t m = m0 + 16 * (f / NT) + c16, n = n0 + 16 * (f % NT) + 4 * g;
         if (m >= p.M) continue;
         const float xs = FUSED ? sl[m] : p.x_scale[m];
@@ -362,30 +370,52 @@ static hipError_t few_launch_t(const LinearI8Params& p, const void* in, hipStrea
         if (e != hipSuccess) return e;
     }
     const dim3 grid((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT));
-    const size_t lds = C::RING + (FUSED ? (size_t)p.M * (p.x_stride + 16 + sizeof(float)) : 0);
+    const size_t lds = C::RING + (FUSED ? (size_t)p.M * (p.x_stride + 16 + sizeof(float)) + NW * 4 : 0);
     hipLaunchKernelGGL(kern, grid, dim3(64 * NW), lds, s, p, (const TX*)in);
     return hipGetLastError();
 }
 
 bool linear_i8_fused(uint32_t M, uint32_t K)
 {
-    return M <= 16 && (uint64_t)M * K <= 16384 && M * ((K + 127) / 128 * 128 + 20) <= 40 * 1024;
+    return M <= 16 && (uint64_t)M * K <= 8192 && M * ((K + 127) / 128 * 128 + 20) + 64 <= 40 * 1024;
 }
 
+// Wider workgroups where there are enough of them (M = 1, K = 2048, N = 8192, us:
+// 32 columns 7.7, 16 8.5; K = N = 4096: 8.9, 8.0).
 hipError_t linear_i8_fused_launch(const LinearI8Params& p, const void* in, int in_dtype, hipStream_t s)
 {
-    return in_dtype == DT_F16 ? few_launch_t<1, 1, 4, 8, half_t, true>(p, in, s) : few_launch_t<1, 1, 4, 8, float, true>(p, in, s);
+    if (p.N <= 4096)
+        return in_dtype == DT_F16 ? few_launch_t<1, 1, 4, 8, half_t, true>(p, in, s) : few_launch_t<1, 1, 4, 8, float, true>(p, in, s);
+    return in_dtype == DT_F16 ? few_launch_t<1, 2, 4, 4, half_t, true>(p, in, s) : few_launch_t<1, 2, 4, 4, float, true>(p, in, s);
 }
 
+// Up to 64 rows over up to 8192 columns the wave rings, whose workgroups are then
+// one round (us, rings / 64-wide tiles: 32 x 4096 x 4096 7.0 / 10.2, 61 x 5003 x
+// 1999 8.2 / 9.1; 16 and 64 x 16384 x 4096 13.5 and 25 / 12.2). Past that the
+// tile whose modelled time is least: kt stages of 128 bytes of K, c tiles a CU.
+// Measured, us, 64-wide / 128-wide / 256-wide: 500 x 2048 x 2048 7.9 / 14.7 /
+// 32.7, 1000 x 4096 x 4096 28 / 25 / 57, 2048 x 4096 x 11008 137 / 90 / 135,
+// 4096^3 103 / 77 / 67.
 hipError_t linear_i8_launch(const LinearI8Params& p, hipStream_t s)
 {
-    if (p.M <= 16) return few_launch_t<1, 1, 4, 4, half_t, false>(p, nullptr, s);
-    if (p.M <= 32) return few_launch_t<2, 2, 4, 3, half_t, false>(p, nullptr, s);
-    if (p.M <= 64) return few_launch_t<4, 2, 4, 3, half_t, false>(p, nullptr, s);
-    const auto tiles = [&](uint32_t b) { return (uint64_t)((p.M + b - 1) / b) * ((p.N + b - 1) / b); };
-    if (p.M >= 128 && tiles(256) >= 128) return linear_i8_big_launch(p, 4, s);
-    if (p.M >= 64 && tiles(128) >= 128) return linear_i8_big_launch(p, 2, s);
-    return linear_i8_big_launch(p, 1, s);
+    if (p.N <= 8192) {
+        if (p.M <= 16)
+            return p.N <= 4096 ? few_launch_t<1, 1, 4, 4, half_t, false>(p, nullptr, s)
+                               : few_launch_t<1, 2, 4, 4, half_t, false>(p, nullptr, s);
+        if (p.M <= 32) return few_launch_t<2, 2, 4, 3, half_t, false>(p, nullptr, s);
+        if (p.M <= 64) return few_launch_t<4, 2, 4, 3, half_t, false>(p, nullptr, s);
+    }
+    int cus = 0;
+    const hipError_t e = device_cus(&cus);
+    if (e != hipSuccess) return e;
+    const auto per_cu = [&](uint32_t b) {
+        const uint64_t tiles = (uint64_t)((p.M + b - 1) / b) * ((p.N + b - 1) / b);
+        return (float)((tiles + cus - 1) / cus);
+    };
+    const float kt = (float)(p.x_stride / 128);
+    const float t1 = 3.f + kt * (.1f + .2f * per_cu(64)), t2 = 3.f + kt * (.2f + .5f * per_cu(128)),
+                t4 = 4.f + kt * 2.f * per_cu(256);
+    return linear_i8_big_launch(p, t4 <= t2 && t4 <= t1 ? 4 : t2 <= t1 ? 2 : 1, s);
 }
 
 }   // namespace vai_dev
