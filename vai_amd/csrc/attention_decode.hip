@@ -26,6 +26,7 @@
 // of an fp32 cache 14.8 us.
 #include <algorithm>
 
+#include "decode_range.h"
 #include "device_common.h"
 #include "kernels.h"
 #include "launch_once.h"
@@ -37,7 +38,6 @@ namespace vai_dev {
 typedef float float2v __attribute__((ext_vector_type(2)));
 
 namespace fd {
-constexpr int NW = 4, KT = 32;   // waves per workgroup; keys per wave tile
 template <int D> struct Lds {
     static constexpr int VROW = D * 2 + 32;             // bytes per V row in LDS
     static constexpr int VWAVE = KT * VROW;             // one wave's V tile
@@ -49,28 +49,6 @@ template <int D> struct Lds {
     }
 };
 
-// The launch's key range: [tb, te) are the 32-key tiles some row sees. They
-// are dealt out in turn, tile tb + i to wave i % NW of unit (i / NW) % units,
-// so that which tiles a wave reads first does not wait for the live count
-// unless a window moves tb.
-struct Range {
-    uint32_t cached, live;
-    int64_t tb, te;
-    uint32_t used;   // units with work (at least 1)
-};
-__device__ __forceinline__ Range range_of(const AttnDecodeParams& p)
-{
-    Range r;
-    r.cached = p.cache_count ? __builtin_amdgcn_readfirstlane(*p.cache_count) : 0u;
-    r.live = p.ring ? r.cached + p.tkv : std::min(r.cached + p.tkv, p.kv_rows);
-    const int64_t kend = std::min<int64_t>(p.mask.key_end_cached(p.tq - 1, r.cached), r.live);
-    const int64_t kbeg = p.mask.key_start_cached(0, r.cached);
-    r.tb = kbeg / KT;
-    r.te = kend <= kbeg ? r.tb : (kend + KT - 1) / KT;
-    const uint32_t n = __builtin_amdgcn_readfirstlane((uint32_t)(r.te - r.tb));
-    r.used = std::min(p.units, std::max<uint32_t>((n + NW - 1) / NW, 1u));
-    return r;
-}
 }
 
 __device__ __forceinline__ half4 fd_read_tr16(const LDS_AS char* a)
@@ -494,6 +472,15 @@ static hipError_t decode_launch_d(const AttnDecodeParams& p, int kv_dtype, uint3
         e = kv_dtype == DT_F16 ? decode_launch_t<D, 2, half_t>(p, grid, s) : decode_launch_t<D, 2, float>(p, grid, s);
     if (e != hipSuccess || p.units == 1) return e;
     hipLaunchKernelGGL(attention_decode_merge_kernel<D>, dim3(p.rows, p.hkv, batch), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+hipError_t attention_decode_merge_launch(const AttnDecodeParams& p, uint32_t dp, uint32_t batch, hipStream_t s)
+{
+    const dim3 grid(p.rows, p.hkv, batch);
+    if (dp == 64) hipLaunchKernelGGL(attention_decode_merge_kernel<64>, grid, dim3(256), 0, s, p);
+    else if (dp == 128) hipLaunchKernelGGL(attention_decode_merge_kernel<128>, grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(attention_decode_merge_kernel<256>, grid, dim3(256), 0, s, p);
     return hipGetLastError();
 }
 

@@ -12,58 +12,30 @@
 
 namespace vai_dev {
 
-// fp16's finite range, as the value arrives there
-__device__ __forceinline__ bool q4_finite(float x) { return __builtin_fabsf(x) <= 65504.f; }
-
 // One half wave per group: 32 lanes hold its values.
 __global__ __launch_bounds__(256) void q4_append_kernel(AttnParams p, uint32_t dp)
 {
-    const uint32_t HD = p.head_dim, groups = (HD + 31) / 32, hk = blockIdx.y, plane = blockIdx.z;
+    const uint32_t HD = p.head_dim, groups = dp / 32, hk = blockIdx.y, plane = blockIdx.z;
     const uint32_t cached = *p.cache_count, lane = threadIdx.x & 31;
     uint8_t* head = (plane ? p.v4 : p.k4) + (size_t)hk * q4::head_bytes(p.kv_rows, dp);
     const void* src = plane ? p.v_new : p.k_new;
     const uint64_t n = (uint64_t)p.tkv * groups;
-    // (a whole number of passes for every lane: the shuffles need both half waves)
+    // (a whole number of passes for every lane: the exchanges need them all)
     for (uint64_t u0 = (uint64_t)blockIdx.x * 8; u0 < n; u0 += (uint64_t)gridDim.x * 8) {
         const uint64_t u = u0 + (threadIdx.x >> 5);
         const uint32_t tok = (uint32_t)(u / groups), grp = (uint32_t)(u % groups), d = 32 * grp + lane;
         const uint32_t pos = cached + tok;
-        // positions past a plane are dropped, and of a ring's rows the call's last stand
-        const bool keep = u < n && (p.ring ? tok + p.kv_rows >= p.tkv : pos < p.kv_rows && pos >= cached);
+        // positions past a plane are dropped (a ring's rows all differ: Tkv <= its size)
+        const bool keep = u < n && (p.ring || (pos < p.kv_rows && pos >= cached));
         const bool in = keep && d < HD;
         const float x = in ? (float)(half_t)ld(src, p.new_dtype, ((size_t)hk * p.tkv + tok) * HD + d) : 0.f;
-        float lo = in ? x : __builtin_inff(), hi = in ? x : -__builtin_inff();
-        int fin = in ? (int)q4_finite(x) : 1;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor(lo, o, 32));
-            hi = fmaxf(hi, __shfl_xor(hi, o, 32));
-            fin &= __shfl_xor(fin, o, 32);
-        }
         half_t s, m;
-        q4::step_of(lo, hi, fin, s, m);
-        const uint32_t code = in && fin ? q4::code_of(x, (float)m, (float)s) : 0u;
+        const uint32_t code = q4::encode(x, in, s, m);
+        if (!keep) continue;
         const uint32_t row = p.ring ? pos % p.kv_rows : pos, j = row % q4::KT;
         uint8_t* tile = head + (size_t)(row / q4::KT) * q4::tile_bytes(dp);
-        if (plane == 0) {
-            uint32_t w = code << (4 * q4::nibble_of(d & 7));
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) w |= (uint32_t)__shfl_xor((int)w, o, 32);
-            if (keep && (lane & 7) == 0) *(uint32_t*)(tile + q4::k_word(dp, j, d)) = w;
-            if (keep && lane == 0) {
-                half_t* sm = (half_t*)(tile + q4::k_scale(dp, j, d));
-                sm[0] = s;
-                sm[1] = m;
-            }
-        } else {
-            const uint32_t w = code | (uint32_t)__shfl_xor((int)code, 1, 32) << 4;
-            if (keep && (lane & 1) == 0) tile[q4::v_byte(dp, j, d)] = (uint8_t)w;
-            if (keep && lane == 0) {
-                half_t* sm = (half_t*)(tile + q4::v_scale(dp, j, d));
-                sm[0] = s;
-                sm[8] = m;
-            }
-        }
+        if (plane == 0) q4::put_k(tile, dp, j, d, code, s, m);
+        else q4::put_v(tile, dp, j, d, code, s, m);
     }
 }
 
@@ -146,10 +118,26 @@ static size_t copy_bytes(const AttnParams& p)
     return (2 * (size_t)p.hkv * p.kv_rows * p.head_dim * sizeof(half_t) + 255) & ~(size_t)255;
 }
 
-size_t attention_q4_workspace(const AttnParams& p) { return copy_bytes(p) + attention_workspace_bytes(p); }
+void attention_q4_plan(AttnParams& p, uint32_t cus)
+{
+    if (q4_few_rows(p)) {
+        p.q4 = 2;
+        q4_decode_plan(p, cus);
+    } else {
+        p.q4 = 1;
+        attention_plan(p, cus);
+    }
+}
+
+size_t attention_q4_workspace(const AttnParams& p)
+{
+    return p.q4 == 2 ? q4_decode_workspace(p) : copy_bytes(p) + attention_workspace_bytes(p);
+}
 
 void attention_q4_set_workspace(AttnParams& p, void* ws)
 {
+    p.ws4 = ws;
+    if (p.q4 == 2) return;
     p.k = ws;
     p.v = (half_t*)ws + (size_t)p.hkv * p.kv_rows * p.head_dim;
     attention_set_workspace(p, (char*)ws + copy_bytes(p));
@@ -157,9 +145,10 @@ void attention_q4_set_workspace(AttnParams& p, void* ws)
 
 hipError_t attention_q4_launch(const AttnParams& p, hipStream_t s)
 {
+    if (p.q4 == 2) return q4_decode_launch(p, p.ws4, s);
     const uint32_t dp = q4_dp(p.head_dim);
     if (p.tkv > 0) {
-        const uint64_t units = ((uint64_t)p.tkv * ((p.head_dim + 31) / 32) + 7) / 8;
+        const uint64_t units = ((uint64_t)p.tkv * (dp / 32) + 7) / 8;
         hipLaunchKernelGGL(q4_append_kernel, dim3((uint32_t)std::min<uint64_t>(units, 2048), p.hkv, 2), dim3(256), 0, s,
                            p, dp);
         const hipError_t e = hipGetLastError();

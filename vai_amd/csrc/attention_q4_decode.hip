@@ -1,0 +1,474 @@
+// attention_q4_decode.hip -- a few query rows over a 4-bit KV cache: append and
+// attention in one launch (and a merge where the keys are split).
+//
+// What bounds it: reading the cache once, 5 bits a value. The query rows of a KV
+// head are the columns of one matrix tile (16 or 32), as in attention_decode.hip;
+// a workgroup is a share of the head's 32-position tiles, which its 4 waves take
+// in turn, each through a ring of its own in LDS: a tile's 20 dp bytes of K and of
+// V are copied there as they lie, D tiles in flight, and no wave waits for another
+// until the share ends.
+//
+// The codes enter the matrix cores as they are. An fp16 whose bits are a code n of
+// 0 .. 15 is n * 2^-24, and the cores multiply such numbers exactly, so one step
+// of 32 head-dim values (a group) gives 2^-24 sum n q from masked nibbles alone,
+// and a score is
+//   scale * sum over groups of (s * sum n q + m * sum q),
+// in fp32 from there on: K is never rounded. V enters as s n + m rounded to fp16
+// (one packed fma from the exact n), the probabilities as two fp16 numbers (the
+// second the rest that the first leaves), so that V's and the result's are the
+// only roundings to fp16: error against 64 bits 3.0e-4 of the result, of which the
+// rounding of the result is 2.1e-4 (3.6e-4 with the probabilities in one number).
+//
+// The call's own rows are rounded by the wave whose tile they are in, into that
+// tile in LDS (and into the cache): nothing waits for an append.
+#include <algorithm>
+
+#include "decode_range.h"
+#include "kernels.h"
+#include "launch_once.h"
+#include "q4_cache.h"
+
+#define LDS_AS __attribute__((address_space(3)))
+
+namespace vai_dev {
+
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+
+namespace {
+
+template <int DP> struct Q4Lds {
+    static constexpr int TILE = (int)q4::tile_bytes(DP);      // one plane's tile
+    static constexpr int COPIES = (TILE + 1023) / 1024;       // 1 KB copies, the last one partly
+    static constexpr int D = DP == 256 ? 3 : 4;               // tiles in flight a wave
+    static constexpr int WAVE = D * 2 * TILE;
+    static constexpr int OROW = DP * 4 + 16;                  // bytes of an fp32 O row in the final exchange
+    template <int NQ> static constexpr int bytes()
+    {
+        const int o = fd::NW * NQ * 16 * OROW + fd::NW * NQ * 16 * 8;   // (m, l) per wave and row after it
+        return fd::NW * WAVE > o ? fd::NW * WAVE : o;
+    }
+};
+
+template <int N>
+__device__ __forceinline__ void q4_wait()
+{
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+__device__ __forceinline__ void q4_wait_lds() { __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14)); }
+
+__device__ __forceinline__ float swap_max16(float x)
+{
+    float y = x;
+    lane_swap<16>(x, y);
+    return fmaxf(x, y);
+}
+
+}   // namespace
+
+// DP: the padded head dim; NQ: 16-row query blocks. Grid: (units, row blocks x
+// hkv). p.k / p.v are the 4-bit planes.
+template <int DP, int NQ>
+__global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q4_decode_kernel(AttnDecodeParams p)
+{
+    using namespace fd;
+    using L = Q4Lds<DP>;
+    constexpr int G = DP / 32, ND = DP / 16, D = L::D;   // groups; values of a lane's V slice
+    constexpr uint32_t NIB = 0x000f000fu;
+    extern __shared__ uint4v q4_lds[];
+    LDS_AS uint8_t* lds = (LDS_AS uint8_t*)(LDS_AS void*)q4_lds;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g = lane >> 4;
+    const uint32_t HD = p.head_dim, unit = blockIdx.x, hk = blockIdx.y % p.hkv, rb = blockIdx.y / p.hkv;
+
+    // query rows: row r of the KV head is query head hk g + r / tq, token r % tq
+    // (loaded before the first copies: both are waited for in order)
+    const uint32_t rows = p.rows, row0 = rb * p.rpb, rend = std::min(row0 + p.rpb, rows);
+    half8 qf[NQ][G];
+    uint32_t tok[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const uint32_t r = std::min(row0 + q * 16 + c16, rend - 1);
+        tok[q] = r % p.tq;
+        const size_t base = ((size_t)hk * rows + r) * HD;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            const uint32_t d = 32 * i + 8 * g;
+            half8 v = (half8)(half_t)0;   // (HD is a multiple of 8)
+            if (d < HD) v = p.q_dtype == DT_F16 ? load8((const half_t*)p.q + base + d) : load8((const float*)p.q + base + d);
+            qf[q][i] = v;
+        }
+    }
+    const Range R = range_of(p);
+    if (unit >= R.used) return;
+
+    const size_t hb = q4::head_bytes(p.kv_rows, DP);
+    uint8_t* kh = uniform_ptr((uint8_t*)p.k + hk * hb);
+    uint8_t* vh = uniform_ptr((uint8_t*)p.v + hk * hb);
+    LDS_AS uint8_t* ring = lds + wave * L::WAVE;
+    // this wave's tiles: first, first + step, ..
+    const int64_t first = R.tb + unit * NW + wave, step = (int64_t)p.units * NW;
+    const int mine = __builtin_amdgcn_readfirstlane((int)(R.te > first ? (R.te - first + step - 1) / step : 0));
+    const auto tile_of = [&](int i) __attribute__((always_inline)) {   // its place in the planes
+        const int64_t t = first + i * step;   // (a ring's size is a multiple of 64: no tile wraps)
+        return __builtin_amdgcn_readfirstlane((uint32_t)(p.ring ? t * KT % p.kv_rows / KT : t));
+    };
+    const auto copy = [&](int i) __attribute__((always_inline)) {      // past the last: it again, never read
+        const uint32_t t = tile_of(std::min(i, mine - 1));
+        LDS_AS uint8_t* dst = ring + (i % D) * 2 * L::TILE;
+#pragma unroll
+        for (int plane = 0; plane < 2; ++plane) {
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)((plane ? vh : kh) + (size_t)t * L::TILE), (short)0, L::TILE, 0x00020000);
+#pragma unroll
+            for (int c = 0; c < L::COPIES; ++c)
+                if ((c + 1) * 1024 <= L::TILE || c * 1024 + lane * 16 < L::TILE)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LDS_AS void*)(dst + plane * L::TILE + c * 1024), 16,
+                                                             c * 1024 + lane * 16, 0, 0, 0);
+        }
+    };
+    if (mine > 0)
+#pragma unroll
+        for (int i = 0; i < D; ++i) copy(i);
+
+    // 2^-24 sum q over each group, of the row as the cores take it
+    float qs[NQ][G];
+    int64_t kbeg[NQ], kend[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        kend[q] = std::min<int64_t>(p.mask.key_end_cached(tok[q], R.cached), R.live);
+        kbeg[q] = p.mask.key_start_cached(tok[q], R.cached);
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += (float)qf[q][i][e];
+            s = swap_sum<16>(s, s);
+            qs[q][i] = swap_sum<32>(s, s) * 5.9604644775390625e-8f;
+        }
+    }
+    const int64_t kfirst = p.mask.key_start_cached(0, R.cached);   // no query sees a position before it
+    const float sc = p.scale * (1.4426950408889634f * 16777216.f);   // scores in log2 units
+
+    float m[NQ], l[NQ];
+    float4v o[NQ][ND];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        m[q] = -__builtin_inff();
+        l[q] = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[q][d] = (float4v)0.f;
+    }
+
+    for (int it = 0; it < mine; ++it) {
+        q4_wait<(D - 1) * 2 * L::COPIES>();   // its copies have landed; the next tiles' may be in flight
+        const int64_t j0 = (first + it * step) * KT;
+        LDS_AS uint8_t* kt = ring + (it % D) * 2 * L::TILE;
+        LDS_AS uint8_t* vt = kt + L::TILE;
+
+        // the call's own rows in this tile
+        if (p.n_new != 0 && j0 + KT > R.cached) {
+            const uint32_t ja = R.cached > j0 ? (uint32_t)(R.cached - j0) : 0u;
+            const uint32_t je = (uint32_t)std::min<int64_t>(KT, R.live - j0);
+            const size_t at = (size_t)tile_of(it) * L::TILE;
+            for (uint32_t j = ja; j < je; ++j) {
+                const size_t src = ((size_t)hk * p.n_new + (uint32_t)(j0 + j - R.cached)) * HD;
+                static_for<DP / 64>([&](auto I) __attribute__((always_inline)) {
+                    const uint32_t d = 64 * I + lane;
+                    const bool in = d < HD;
+                    const float xk = in ? (float)(half_t)ld(p.k_new, p.new_dtype, src + d) : 0.f;
+                    const float xv = in ? (float)(half_t)ld(p.v_new, p.new_dtype, src + d) : 0.f;
+                    half_t ks, km, vs, vm;
+                    const uint32_t ck = q4::encode(xk, in, ks, km), cv = q4::encode(xv, in, vs, vm);
+                    q4::put_k(kt, DP, j, d, ck, ks, km);
+                    q4::put_v(vt, DP, j, d, cv, vs, vm);
+                    if (rb == 0) {
+                        q4::put_k(kh + at, DP, j, d, ck, ks, km);
+                        q4::put_v(vh + at, DP, j, d, cv, vs, vm);
+                    }
+                });
+            }
+            q4_wait_lds();
+        }
+
+        // this lane's share of the tile
+        uint32_t kw[2][G];
+        uint4v ksm[2][G];      // (s, m) of rows 4 g ..+3
+        uint32_t vw[ND];       // words 2 i, 2 i + 1: the two halves of the block's positions, values 2 i and 2 i + 1
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            LDS_AS const uint8_t* a = kt + ((t * 4 + g) * 16 + c16) * (G * 4);
+            if constexpr (G == 2) {
+                const uint2v w = *(LDS_AS const uint2v*)a;
+                kw[t][0] = w.x;
+                kw[t][1] = w.y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < G; i += 4) {
+                    const uint4v w = *(LDS_AS const uint4v*)(a + 4 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) kw[t][i + e] = w[e];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+                ksm[t][i] = *(LDS_AS const uint4v*)(kt + q4::scale_offset(DP) + ((i * 2 + t) * 16 + 4 * g) * 4);
+        }
+        {
+            LDS_AS const uint8_t* a = vt + g * (DP * 4) + c16 * (DP / 4);
+#pragma unroll
+            for (int i = 0; i < ND; i += 4) {
+                const uint4v w = *(LDS_AS const uint4v*)(a + 4 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) vw[i + e] = w[e];
+            }
+        }
+        LDS_AS const uint8_t* va = vt + q4::scale_offset(DP) + ((c16 * ND / 32) * 4 + g) * 32;
+        half8 vs = *(LDS_AS const half8*)va, vm = *(LDS_AS const half8*)(va + 16);
+        q4_wait_lds();         // read before the slot is copied over
+        copy(it + D);
+
+        // S^T: lane (c16, g) holds query row c16 and positions 8 g + 4 t ..+3
+        float4v x[2][NQ];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) x[t][q] = (float4v)0.f;
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t w = kw[t][i];
+                const half8 a = __builtin_bit_cast(half8, uint4v{w & NIB, (w >> 4) & NIB, (w >> 8) & NIB, (w >> 12) & NIB});
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    const float4v n = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[q][i], (float4v)0.f, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t both = ksm[t][i][r];   // (a bit cast of the element itself takes the vector's first)
+                        const half2v sm = __builtin_bit_cast(half2v, both);
+                        x[t][q][r] = fmaf((float)sm.x, n[r], x[t][q][r]);
+                        x[t][q][r] = fmaf((float)sm.y, qs[q][i], x[t][q][r]);
+                    }
+                }
+            }
+
+        // Positions that no query sees (stale rows, rows past the count) may hold
+        // anything: their V is zero here, their scores are masked below.
+        if (j0 < kfirst || j0 + KT > R.live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int64_t j = j0 + 8 * g + q4::order_of(e);
+                if (j < kfirst || j >= R.live) vs[e] = vm[e] = (half_t)0.f;
+            }
+        }
+        // A row with a NaN in V must not reach a query it is hidden from through 0 *
+        // NaN: its V is zero and its score NaN, which the mask replaces. (The sum of
+        // the minima is NaN if one is, and at worst also where they overflow.)
+        uint32_t bad = 0;
+        {
+            const half2v z = half2v{vm[0], vm[1]} + half2v{vm[2], vm[3]} + half2v{vm[4], vm[5]} + half2v{vm[6], vm[7]};
+            if (__builtin_expect(__any(z.x != z.x || z.y != z.y), 0)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (vm[e] != vm[e]) {
+                        vs[e] = vm[e] = (half_t)0.f;
+                        bad |= 1u << q4::order_of(e);
+                    }
+                bad |= q4::moved<q4::XOR1>(bad);
+                bad |= q4::moved<q4::XOR2>(bad);
+                bad |= q4::moved<q4::MIRROR8>(bad);
+                bad |= q4::moved<q4::MIRROR16>(bad);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (bad >> (4 * t + r) & 1) x[t][q][r] = __builtin_nanf("");
+            }
+        }
+
+        half8 ph[NQ], pl[NQ];   // P^T: positions 0 2 1 3 4 6 5 7 of the lane's 8, and what fp16 leaves of them
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = x[i >> 2][q][i & 3] * sc;
+            if (!__all(j0 >= kbeg[q] && j0 + KT <= kend[q])) {
+                const int lo = (int)std::min<int64_t>(std::max<int64_t>(kbeg[q] - j0, -1), KT + 1);
+                const int hi = (int)std::min<int64_t>(std::max<int64_t>(kend[q] - j0, -1), KT + 1);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (8 * g + i >= hi || 8 * g + i < lo) v[i] = -__builtin_inff();
+            }
+            float tmax = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+            tmax = swap_max32(swap_max16(tmax));
+            // the row's reference m moves only when the max exceeds it by more than 8
+            // (P stays below 2^8), for the whole wave at once
+            if (__any(tmax > m[q] + 8.f)) {
+                const float mnew = fmaxf(m[q], tmax);
+                const float alpha = __builtin_amdgcn_exp2f(m[q] - (mnew == -__builtin_inff() ? 0.f : mnew));
+                l[q] *= alpha;
+                m[q] = mnew;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[q][d] *= alpha;
+            }
+            const float mref = m[q] == -__builtin_inff() ? 0.f : m[q];
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(v[i] - mref);
+            l[q] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));   // (this lane's positions)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = e[q4::order_of(i)];
+                ph[q][i] = (half_t)f;
+                pl[q][i] = (half_t)(f - (float)ph[q][i]);
+            }
+        }
+
+        // O^T += V^T P^T: value c16 ND + 2 i + h in row c16 of the product's A
+#pragma unroll
+        for (int i = 0; i < ND / 2; ++i) {
+            const uint32_t w0 = vw[2 * i], w1 = vw[2 * i + 1];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // 1024 + n as bits, then n: exact
+                const uint4v b = uint4v{(w0 >> (4 * h)) & NIB, (w0 >> (8 + 4 * h)) & NIB, (w1 >> (4 * h)) & NIB,
+                                        (w1 >> (8 + 4 * h)) & NIB} | (uint4v)0x64006400u;
+                const half8 n = __builtin_bit_cast(half8, b) - (half8)(half_t)1024.f;
+                const half8 a = __builtin_elementwise_fma(n, vs, vm);
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    o[q][2 * i + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[q], o[q][2 * i + h], 0, 0, 0);
+                    o[q][2 * i + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[q], o[q][2 * i + h], 0, 0, 0);
+                }
+            }
+        }
+    }
+    q4_wait<0>();   // (the copies past the last tile)
+
+    // the waves' sums meet in LDS (the rings are done with); o[q][d] register r is
+    // row c16, value (4 g + r) ND + d
+    __syncthreads();
+    LDS_AS uint8_t* ml = lds + NW * NQ * 16 * L::OROW;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const int r = q * 16 + c16;
+        float s = l[q];
+        s = swap_sum<16>(s, s);
+        s = swap_sum<32>(s, s);
+        if (g == 0) *(LDS_AS float2v*)(ml + (wave * NQ * 16 + r) * 8) = float2v{m[q], s};
+        LDS_AS uint8_t* orow = lds + (wave * NQ * 16 + r) * L::OROW;
+#pragma unroll
+        for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+            for (int d = 0; d < ND; d += 4)
+                *(LDS_AS float4v*)(orow + ((4 * g + rr) * ND + d) * 4) =
+                    float4v{o[q][d][rr], o[q][d + 1][rr], o[q][d + 2][rr], o[q][d + 3][rr]};
+    }
+    __syncthreads();
+    const bool whole = R.used == 1;
+    constexpr int C4 = DP / 4;
+    for (uint32_t e = threadIdx.x; e < (rend - row0) * C4; e += 256) {
+        const uint32_t r = e / C4, c = e % C4;
+        float mw[NW], lw[NW], M = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float2v y = *(LDS_AS const float2v*)(ml + (w * NQ * 16 + r) * 8);
+            mw[w] = y.x;
+            lw[w] = y.y;
+            M = fmaxf(M, y.x);
+        }
+        const float mref = M == -__builtin_inff() ? 0.f : M;
+        float4v acc = (float4v)0.f;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float a = __builtin_amdgcn_exp2f(mw[w] - mref);
+            acc += a * *(LDS_AS const float4v*)(lds + (w * NQ * 16 + r) * L::OROW + c * 16);
+            sum += a * lw[w];
+        }
+        const uint32_t row = row0 + r;
+        if (whole) {
+            // (no key: zeros; a NaN stays one)
+            acc *= sum == 0.f ? 0.f : 1.0f / sum;
+            const uint32_t h = hk * (p.hq / p.hkv) + row / p.tq, t = row % p.tq;
+            const size_t out = ((size_t)t * p.hq + h) * HD + 4 * c;
+            if (4 * c < HD) {
+                if (p.o_dtype == DT_F16) *(half4*)((half_t*)p.out + out) = __builtin_convertvector(acc, half4);
+                else *(float4v*)((float*)p.out + out) = acc;
+            }
+        } else {
+            const size_t part = ((size_t)hk * p.units + unit) * rows + row;
+            *(float4v*)(p.ws_o + part * DP + 4 * c) = acc;
+            if (c == 0) {
+                p.ws_ml[2 * part] = M;
+                p.ws_ml[2 * part + 1] = sum;
+            }
+        }
+    }
+}
+
+template <int DP, int NQ>
+static hipError_t q4_decode_launch_t(const AttnDecodeParams& p, hipStream_t s)
+{
+    constexpr int bytes = Q4Lds<DP>::template bytes<NQ>();
+    static PerDevice lds_once;
+    if constexpr (bytes > 64 * 1024) {
+        const hipError_t e = set_max_lds(lds_once, (const void*)attention_q4_decode_kernel<DP, NQ>, bytes);
+        if (e != hipSuccess) return e;
+    }
+    const dim3 grid(p.units, (p.rows + p.rpb - 1) / p.rpb * p.hkv);
+    hipLaunchKernelGGL((attention_q4_decode_kernel<DP, NQ>), grid, dim3(256), bytes, s, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.units == 1) return e;
+    return attention_decode_merge_launch(p, DP, 1, s);
+}
+
+// Few rows: as the fp16 cache's plan, at most 16 tokens and 64 rows of a KV head,
+// and new rows that lie in what some query sees (their tiles' waves append them).
+bool q4_few_rows(const AttnParams& p)
+{
+    return p.head_dim % 8 == 0 && p.tq <= 16 && p.hq / p.hkv * p.tq <= 64 && (uint64_t)p.hq * p.tq <= 65535 && p.tkv <= 32 &&
+           (p.span == 0 || p.tkv < p.tq + p.span);
+}
+
+void q4_decode_plan(AttnParams& p, uint32_t cus)
+{
+    const uint32_t dp = q4_dp(p.head_dim);
+    p.dp = dp;
+    p.dec_rows = p.hq / p.hkv * p.tq;
+    p.dec_rpb = std::min<uint32_t>(p.dec_rows, dp == 256 ? 16 : 32);
+    const uint32_t keys = p.span ? std::min<uint64_t>(p.kv_rows, (uint64_t)p.span + p.tq + 2 * fd::KT) : p.kv_rows;
+    const uint32_t tiles = (keys + fd::KT - 1) / fd::KT, most = std::max<uint32_t>((tiles + fd::NW - 1) / fd::NW, 1);
+    const uint32_t blocks = p.hkv * ((p.dec_rows + p.dec_rpb - 1) / p.dec_rpb), wgs = dp == 256 || p.dec_rpb > 16 ? cus : 2 * cus;
+    p.dec_units = std::min(std::min(std::max((wgs + blocks - 1) / blocks, 1u), most), AttnDecodeParams::MAX_UNITS);
+}
+
+size_t q4_decode_workspace(const AttnParams& p) { return attention_decode_workspace(p, p.dec_units); }
+
+hipError_t q4_decode_launch(const AttnParams& a, void* ws, hipStream_t s)
+{
+    AttnDecodeParams p{};
+    p.out = a.out; p.q = a.q; p.k = a.k4; p.v = a.v4;
+    p.o_dtype = a.o_dtype; p.q_dtype = a.q_dtype;
+    p.hq = a.hq; p.hkv = a.hkv; p.tq = a.tq; p.tkv = a.tkv; p.head_dim = a.head_dim;
+    p.cache_count = a.cache_count; p.kv_rows = a.kv_rows; p.ring = a.ring;
+    p.k_new = a.k_new; p.v_new = a.v_new; p.n_new = a.tkv; p.new_dtype = a.new_dtype;
+    p.scale = a.scale;
+    p.mask = a.mask;
+    p.rows = a.dec_rows; p.rpb = a.dec_rpb; p.units = a.dec_units;
+    p.ws_o = (float*)ws;
+    p.ws_ml = (float*)ws + (size_t)a.hkv * a.dec_units * a.dec_rows * a.dp;
+    switch (a.dp) {
+    case 64: return p.rpb <= 16 ? q4_decode_launch_t<64, 1>(p, s) : q4_decode_launch_t<64, 2>(p, s);
+    case 128: return p.rpb <= 16 ? q4_decode_launch_t<128, 1>(p, s) : q4_decode_launch_t<128, 2>(p, s);
+    default: return q4_decode_launch_t<256, 1>(p, s);
+    }
+}
+
+}   // namespace vai_dev

@@ -591,7 +591,8 @@ static vai_status attention_params(const vai_attention_args* a, AttnParams& p)
         return st;
     p.causal = p.mask.blocks == 1;
     if (!attention_ok(p)) return VAI_ERR_UNSUPPORTED;
-    attention_plan(p, plan_cus());
+    if (p.q4) attention_q4_plan(p, plan_cus());
+    else attention_plan(p, plan_cus());
     return VAI_OK;
 }
 
@@ -614,7 +615,7 @@ vai_status vai_attention_launch(const vai_attention_args* a, vai_stream_t stream
         if (!p.q4) attention_set_workspace(p, a->workspace);
     }
     if (p.q4) {
-        if ((uintptr_t)a->workspace % 16 != 0) return VAI_ERR_INVALID_ARG;
+        if (need && (uintptr_t)a->workspace % 16 != 0) return VAI_ERR_INVALID_ARG;
         attention_q4_set_workspace(p, a->workspace);
         return hip_status(attention_q4_launch(p, (hipStream_t)stream));
     }

@@ -220,7 +220,8 @@ struct AttnParams {
     // count as cached rows like any other.
     uint8_t* k4;
     uint8_t* v4;
-    uint32_t q4;
+    void* ws4;                    // the call's workspace
+    uint32_t q4;                  // 0: none; 1: through the copies; 2: few rows, from the planes themselves
     // Few query rows per KV head (attention_decode.hip): dec_units > 0 takes
     // that path, with dec_rows = tq * hq / hkv rows per KV head, dec_rpb of
     // them per workgroup; dec_append: it also appends the new rows.
@@ -249,6 +250,7 @@ struct AttnDecodeParams {
 void attention_decode_plan(AttnParams& p, uint32_t cus, uint32_t key_rows, size_t flash_workspace);
 size_t attention_decode_workspace(const AttnParams& p, uint32_t units);
 hipError_t attention_decode_launch(const AttnParams& p, hipStream_t s);
+hipError_t attention_decode_merge_launch(const AttnDecodeParams& p, uint32_t dp, uint32_t batch, hipStream_t s);
 
 bool attention_ok(const AttnParams& p);
 // Units per head for p's shape (0 when no query tile needs splitting), and
@@ -265,9 +267,15 @@ hipError_t attention_launch(const AttnParams& p, hipStream_t s);
 // of 32 positions of rows `dp` wide (the head dim padded to 64, 128 or 256).
 uint32_t q4_dp(uint32_t head_dim);                       // 0: head_dim > 256
 size_t q4_plane_bytes(uint32_t hkv, uint32_t rows, uint32_t head_dim);
+void attention_q4_plan(AttnParams& p, uint32_t cus);
 hipError_t attention_q4_launch(const AttnParams& p, hipStream_t s);
 size_t attention_q4_workspace(const AttnParams& p);
 void attention_q4_set_workspace(AttnParams& p, void* ws);
+// its few-rows path (attention_q4_decode.hip)
+bool q4_few_rows(const AttnParams& p);
+void q4_decode_plan(AttnParams& p, uint32_t cus);
+size_t q4_decode_workspace(const AttnParams& p);
+hipError_t q4_decode_launch(const AttnParams& p, void* ws, hipStream_t s);
 
 // Rows of a cache as values: rows [first, first + n) of every head (wrapping at
 // the plane's end) to [hkv, n, head_dim].

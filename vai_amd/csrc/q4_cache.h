@@ -6,19 +6,21 @@
 // groups of 32 values. A group keeps its minimum m and its step s = (max - m) /
 // 15 as fp16, and 4-bit codes n: the values stored are s n + m. Per KV head a
 // plane is a run of tiles of 32 positions, each dp * 20 bytes: 16 dp of codes,
-// then 4 dp of (s, m). Codes and steps of a tile lie together so that a walk
-// over the keys reads one stream per plane, and inside a tile every lane of
-// the decode kernel finds its share contiguous:
-//   K: position j's row is dp / 8 words of 8 codes; the word of values 32 i +
-//      8 q ..+7 is word q * (dp / 32) + i, so that quarter q's words of a row
-//      are one load. A word's nibbles 0, 4, 1, 5, 2, 6, 3, 7 are its values in
-//      order: masking alternate nibbles gives the pairs of an fp16 operand.
-//      Then (s, m) of group i, position j: word 32 i + j.
+// then 4 dp of (s, m). A tile is copied into LDS as it lies, and there every lane
+// of the attention kernel finds its share contiguous:
+//   K: lane (r, q) of the score product takes row r of 16 and quarter q, the
+//      values 32 i + 8 q ..+7 of each group i: dp / 32 words of 8 codes. Half t
+//      of a tile's positions, quarter and row lead: [t][q][r][i]. Row r of half
+//      t is position 8 (r / 4) + 4 t + r % 4, so that the scores a lane receives,
+//      rows 4 g ..+3 of both halves, are 8 positions in a row. A word's nibbles 0,
+//      4, 1, 5, 2, 6, 3, 7 are its values in order: masking every fourth nibble
+//      gives the pairs of an fp16 operand. Then (s, m) as [i][t][r].
 //   V: 4 blocks of 8 positions, each 16 slices (dp / 16 values): byte (i, j) of
 //      a slice, 8 i + j, holds values 2 i (low) and 2 i + 1 (high) of position
 //      j: a word is 4 positions of the same two values, as the transposed
 //      operand needs it. Then for group i and block b 8 steps and 8 minima,
 //      positions in the order 0 2 1 3 4 6 5 7 (the operand's).
+// Groups past the head dim hold zeros.
 #pragma once
 #include "device_common.h"
 
@@ -37,13 +39,15 @@ __host__ __device__ constexpr uint32_t nibble_of(uint32_t v) { return (v & 1) * 
 __host__ __device__ constexpr uint32_t order_of(uint32_t j) { return (j & 4) | ((j & 1) << 1) | ((j >> 1) & 1); }
 
 // Byte offsets in a tile of position j (0 .. 31) and value d.
+__host__ __device__ constexpr uint32_t half_of(uint32_t j) { return (j >> 2) & 1; }
+__host__ __device__ constexpr uint32_t row_of(uint32_t j) { return (j >> 3) * 4 + (j & 3); }
 __host__ __device__ constexpr uint32_t k_word(uint32_t dp, uint32_t j, uint32_t d)
 {
-    return j * (dp / 2) + (((d >> 3) & 3) * (dp / 32) + (d >> 5)) * 4;
+    return (((half_of(j) * 4 + ((d >> 3) & 3)) * 16 + row_of(j)) * (dp / 32) + (d >> 5)) * 4;
 }
 __host__ __device__ constexpr uint32_t k_scale(uint32_t dp, uint32_t j, uint32_t d)
 {
-    return scale_offset(dp) + ((d >> 5) * 32 + j) * 4;
+    return scale_offset(dp) + (((d >> 5) * 2 + half_of(j)) * 16 + row_of(j)) * 4;
 }
 __host__ __device__ constexpr uint32_t v_byte(uint32_t dp, uint32_t j, uint32_t d)
 {
@@ -56,13 +60,16 @@ __host__ __device__ constexpr uint32_t v_scale(uint32_t dp, uint32_t j, uint32_t
 
 // A group's step from its extremes. Both are fp16 values, so max - min is
 // exact in fp32 but for the far ends of fp16's range. A group that holds
-// something not finite in fp16 keeps m = NaN, s = 0: all its values are NaN.
+// something not finite in fp16 keeps m = NaN, s = 0: all its values are NaN; one
+// without values (past the head dim, lo > hi) zeros.
 __device__ __forceinline__ void step_of(float lo, float hi, bool finite, half_t& s, half_t& m)
 {
-    s = finite ? (half_t)((hi - lo) / 15.0f) : (half_t)0.f;
+    const bool some = finite && lo <= hi;
+    s = some ? (half_t)((hi - lo) / 15.0f) : (half_t)0.f;
+    m = some ? (half_t)lo : finite ? (half_t)0.f : (half_t)__builtin_nanf("");
     // (s rounded up near fp16's end: one below, so that 15 s + m is an fp16 number too)
-    if (fmaf(15.0f, (float)s, lo) > 65504.f) s = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, s) - 1));
-    m = finite ? (half_t)lo : (half_t)__builtin_nanf("");
+    if (some && fmaf(15.0f, (float)s, lo) > 65504.f)
+        s = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, s) - 1));
 }
 
 // (x - m) / s to the nearest integer, halves to even, from the exact remainder;
@@ -77,6 +84,63 @@ __device__ __forceinline__ uint32_t code_of(float x, float m, float s)
     if (r > s || (r == s && odd)) n += 1.f;
     else if (r < -s || (r == -s && odd)) n -= 1.f;
     return (uint32_t)fminf(n, 15.f);
+}
+
+// What lane ^ 1, ^ 2, and the mirror image in 8 and in 16 lanes hold: with an
+// associative operation after each, every lane gets its 2, 4, 8, 16 lanes' result.
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true); }
+template <int CTRL>
+__device__ __forceinline__ float moved(float x) { return __builtin_bit_cast(float, moved<CTRL>(__builtin_bit_cast(uint32_t, x))); }
+constexpr int XOR1 = 0xB1, XOR2 = 0x4E, MIRROR8 = 0x141, MIRROR16 = 0x140;
+
+// 32 lanes hold a group's values x (in: the value exists), already rounded to
+// fp16: its step and minimum, and this lane's code.
+__device__ __forceinline__ uint32_t encode(float x, bool in, half_t& s, half_t& m)
+{
+    float lo = in ? x : __builtin_inff(), hi = in ? x : -__builtin_inff();
+    uint32_t top = in ? __builtin_bit_cast(uint32_t, x) & 0x7fffffffu : 0u;   // NaN and infinity above all
+    const auto step = [&](float l, float h, uint32_t t) __attribute__((always_inline)) {
+        lo = fminf(lo, l);
+        hi = fmaxf(hi, h);
+        top = t > top ? t : top;
+    };
+    step(moved<XOR1>(lo), moved<XOR1>(hi), moved<XOR1>(top));
+    step(moved<XOR2>(lo), moved<XOR2>(hi), moved<XOR2>(top));
+    step(moved<MIRROR8>(lo), moved<MIRROR8>(hi), moved<MIRROR8>(top));
+    step(moved<MIRROR16>(lo), moved<MIRROR16>(hi), moved<MIRROR16>(top));
+    step(__shfl_xor(lo, 16), __shfl_xor(hi, 16), (uint32_t)__shfl_xor((int)top, 16));
+    const bool finite = top < 0x7f800000u;
+    step_of(lo, hi, finite, s, m);
+    return in && finite ? code_of(x, (float)m, (float)s) : 0u;
+}
+
+template <class T>
+__device__ __forceinline__ void store(uint8_t* p, T v) { *(T*)p = v; }
+template <class T>
+__device__ __forceinline__ void store(__attribute__((address_space(3))) uint8_t* p, T v) { *(__attribute__((address_space(3))) T*)p = v; }
+
+// Writes position j's value d (code; every lane of its group calls) into a tile.
+template <class P>   // a byte pointer, global or LDS
+__device__ __forceinline__ void put_k(P tile, uint32_t dp, uint32_t j, uint32_t d, uint32_t code, half_t s, half_t m)
+{
+    uint32_t w = code << (4 * nibble_of(d & 7));
+    w |= moved<XOR1>(w);
+    w |= moved<XOR2>(w);
+    w |= moved<MIRROR8>(w);
+    if ((d & 7) == 0) store<uint32_t>(tile + k_word(dp, j, d), w);
+    if ((d & 31) == 0)
+        store<uint32_t>(tile + k_scale(dp, j, d), (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16);
+}
+template <class P>
+__device__ __forceinline__ void put_v(P tile, uint32_t dp, uint32_t j, uint32_t d, uint32_t code, half_t s, half_t m)
+{
+    const uint32_t w = code | moved<XOR1>(code) << 4;
+    if ((d & 1) == 0) store<uint8_t>(tile + v_byte(dp, j, d), (uint8_t)w);
+    if ((d & 31) == 0) {
+        store<uint16_t>(tile + v_scale(dp, j, d), __builtin_bit_cast(uint16_t, s));
+        store<uint16_t>(tile + v_scale(dp, j, d) + 16, __builtin_bit_cast(uint16_t, m));
+    }
 }
 
 }   // namespace q4
