@@ -109,26 +109,32 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
     uint8_t* kh = uniform_ptr((uint8_t*)p.k + hk * hb);
     uint8_t* vh = uniform_ptr((uint8_t*)p.v + hk * hb);
     LDS_AS uint8_t* ring = lds + wave * L::WAVE;
-    // this wave's tiles: first, first + step, ..
-    const int64_t first = R.tb + unit * NW + wave, step = (int64_t)p.units * NW;
-    const int mine = __builtin_amdgcn_readfirstlane((int)(R.te > first ? (R.te - first + step - 1) / step : 0));
-    const auto tile_of = [&](int i) __attribute__((always_inline)) {   // its place in the planes
-        const int64_t t = first + i * step;   // (a ring's size is a multiple of 64: no tile wraps)
-        return __builtin_amdgcn_readfirstlane((uint32_t)(p.ring ? t * KT % p.kv_rows / KT : t));
+    // this wave's tiles: first, first + step, .., and their places in the planes
+    // (a ring's size is a multiple of 64: no tile wraps)
+    const int64_t first = R.tb + unit * NW + wave;
+    const uint32_t step = p.units * NW, wrap = p.ring ? p.kv_rows / KT : 0xffffffffu;
+    const int mine = __builtin_amdgcn_readfirstlane((int)(R.te > first ? ((uint32_t)(R.te - first) + step - 1) / step : 0));
+    const uint32_t place0 = __builtin_amdgcn_readfirstlane((uint32_t)(p.ring ? first % wrap : first));
+    const uint32_t hop = __builtin_amdgcn_readfirstlane(p.ring ? step % wrap : step);
+    const auto next_place = [&](uint32_t t) __attribute__((always_inline)) {
+        t += hop;
+        return t >= wrap ? t - wrap : t;
     };
-    const auto copy = [&](int i) __attribute__((always_inline)) {      // past the last: it again, never read
-        const uint32_t t = tile_of(std::min(i, mine - 1));
-        LDS_AS uint8_t* dst = ring + (i % D) * 2 * L::TILE;
+    uint32_t ahead = place0;   // the next copy's place, and how many were made
+    int copied = 0;
+    const auto copy = [&](int slot) __attribute__((always_inline)) {   // past the last: it again, never read
+        LDS_AS uint8_t* dst = ring + slot * 2 * L::TILE;
 #pragma unroll
         for (int plane = 0; plane < 2; ++plane) {
             const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                (void*)((plane ? vh : kh) + (size_t)t * L::TILE), (short)0, L::TILE, 0x00020000);
+                (void*)((plane ? vh : kh) + (size_t)ahead * L::TILE), (short)0, L::TILE, 0x00020000);
 #pragma unroll
             for (int c = 0; c < L::COPIES; ++c)
                 if ((c + 1) * 1024 <= L::TILE || c * 1024 + lane * 16 < L::TILE)
                     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LDS_AS void*)(dst + plane * L::TILE + c * 1024), 16,
                                                              c * 1024 + lane * 16, 0, 0, 0);
         }
+        if (++copied < mine) ahead = next_place(ahead);
     };
     if (mine > 0)
 #pragma unroll
@@ -151,6 +157,10 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
         }
     }
     const int64_t kfirst = p.mask.key_start_cached(0, R.cached);   // no query sees a position before it
+    // what every row of this wave sees: tiles inside need no mask
+    // (both bounds grow with the token)
+    const int64_t all_beg = p.mask.key_start_cached(p.tq - 1, R.cached);
+    const int64_t all_end = std::min<int64_t>(p.mask.key_end_cached(0, R.cached), R.live);
     const float sc = p.scale * (1.4426950408889634f * 16777216.f);   // scores in log2 units
 
     float m[NQ], l[NQ];
@@ -163,36 +173,63 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
         for (int d = 0; d < ND; ++d) o[q][d] = (float4v)0.f;
     }
 
+    uint32_t place = place0;
+    int slot = 0;
     for (int it = 0; it < mine; ++it) {
         q4_wait<(D - 1) * 2 * L::COPIES>();   // its copies have landed; the next tiles' may be in flight
-        const int64_t j0 = (first + it * step) * KT;
-        LDS_AS uint8_t* kt = ring + (it % D) * 2 * L::TILE;
+        const int64_t j0 = (first + (int64_t)it * step) * KT;
+        LDS_AS uint8_t* kt = ring + slot * 2 * L::TILE;
         LDS_AS uint8_t* vt = kt + L::TILE;
 
-        // the call's own rows in this tile
+        // the call's own rows in this tile, each read while the one before is rounded
         if (p.n_new != 0 && j0 + KT > R.cached) {
             const uint32_t ja = R.cached > j0 ? (uint32_t)(R.cached - j0) : 0u;
             const uint32_t je = (uint32_t)std::min<int64_t>(KT, R.live - j0);
-            const size_t at = (size_t)tile_of(it) * L::TILE;
+            const size_t at = (size_t)place * L::TILE;
+            const size_t src = ((size_t)hk * p.n_new + (uint32_t)(j0 + ja - R.cached)) * HD;
+            float xk[DP / 64], xv[DP / 64];
+            const auto load = [&](size_t row) __attribute__((always_inline)) {
+                if (p.new_dtype == DT_F16) {
+#pragma unroll
+                    for (int i = 0; i < DP / 64; ++i) {
+                        const uint32_t d = std::min<uint32_t>(64 * i + lane, HD - 1);
+                        xk[i] = (float)((const half_t*)p.k_new)[row + d];
+                        xv[i] = (float)((const half_t*)p.v_new)[row + d];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < DP / 64; ++i) {
+                        const uint32_t d = std::min<uint32_t>(64 * i + lane, HD - 1);
+                        xk[i] = ((const float*)p.k_new)[row + d];
+                        xv[i] = ((const float*)p.v_new)[row + d];
+                    }
+                }
+            };
+            if (ja < je) load(src);
             for (uint32_t j = ja; j < je; ++j) {
-                const size_t src = ((size_t)hk * p.n_new + (uint32_t)(j0 + j - R.cached)) * HD;
-                static_for<DP / 64>([&](auto I) __attribute__((always_inline)) {
-                    const uint32_t d = 64 * I + lane;
-                    const bool in = d < HD;
-                    const float xk = in ? (float)(half_t)ld(p.k_new, p.new_dtype, src + d) : 0.f;
-                    const float xv = in ? (float)(half_t)ld(p.v_new, p.new_dtype, src + d) : 0.f;
+                float yk[DP / 64], yv[DP / 64];
+#pragma unroll
+                for (int i = 0; i < DP / 64; ++i) {
+                    yk[i] = (float)(half_t)xk[i];
+                    yv[i] = (float)(half_t)xv[i];
+                }
+                if (j + 1 < je) load(src + (size_t)(j + 1 - ja) * HD);
+#pragma unroll
+                for (int i = 0; i < DP / 64; ++i) {
+                    const uint32_t d = 64 * i + lane;
                     half_t ks, km, vs, vm;
-                    const uint32_t ck = q4::encode(xk, in, ks, km), cv = q4::encode(xv, in, vs, vm);
+                    const uint32_t ck = q4::encode(yk[i], d < HD, ks, km), cv = q4::encode(yv[i], d < HD, vs, vm);
                     q4::put_k(kt, DP, j, d, ck, ks, km);
                     q4::put_v(vt, DP, j, d, cv, vs, vm);
                     if (rb == 0) {
                         q4::put_k(kh + at, DP, j, d, ck, ks, km);
                         q4::put_v(vh + at, DP, j, d, cv, vs, vm);
                     }
-                });
+                }
             }
             q4_wait_lds();
         }
+        place = next_place(place);
 
         // this lane's share of the tile
         uint32_t kw[2][G];
@@ -229,7 +266,8 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
         LDS_AS const uint8_t* va = vt + q4::scale_offset(DP) + ((c16 * ND / 32) * 4 + g) * 32;
         half8 vs = *(LDS_AS const half8*)va, vm = *(LDS_AS const half8*)(va + 16);
         q4_wait_lds();         // read before the slot is copied over
-        copy(it + D);
+        copy(slot);
+        slot = slot + 1 == D ? 0 : slot + 1;
 
         // S^T: lane (c16, g) holds query row c16 and positions 8 g + 4 t ..+3
         float4v x[2][NQ];
@@ -298,7 +336,7 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = x[i >> 2][q][i & 3] * sc;
-            if (!__all(j0 >= kbeg[q] && j0 + KT <= kend[q])) {
+            if (j0 < all_beg || j0 + KT > all_end) {
                 const int lo = (int)std::min<int64_t>(std::max<int64_t>(kbeg[q] - j0, -1), KT + 1);
                 const int hi = (int)std::min<int64_t>(std::max<int64_t>(kend[q] - j0, -1), KT + 1);
 #pragma unroll
@@ -322,12 +360,9 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
 #pragma unroll
             for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(v[i] - mref);
             l[q] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));   // (this lane's positions)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float f = e[q4::order_of(i)];
-                ph[q][i] = (half_t)f;
-                pl[q][i] = (half_t)(f - (float)ph[q][i]);
-            }
+            const float8v f = {e[0], e[2], e[1], e[3], e[4], e[6], e[5], e[7]};
+            ph[q] = __builtin_convertvector(f, half8);
+            pl[q] = __builtin_convertvector(f - __builtin_convertvector(ph[q], float8v), half8);
         }
 
         // O^T += V^T P^T: value c16 ND + 2 i + h in row c16 of the product's A
@@ -336,10 +371,12 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
             const uint32_t w0 = vw[2 * i], w1 = vw[2 * i + 1];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                // 1024 + n as bits, then n: exact
-                const uint4v b = uint4v{(w0 >> (4 * h)) & NIB, (w0 >> (8 + 4 * h)) & NIB, (w1 >> (4 * h)) & NIB,
-                                        (w1 >> (8 + 4 * h)) & NIB} | (uint4v)0x64006400u;
-                const half8 n = __builtin_bit_cast(half8, b) - (half8)(half_t)1024.f;
+                // 1024 + n or (high nibbles where they stand) 1024 + 16 n as bits, then n: exact
+                const uint32_t mask = h ? 0x00f000f0u : NIB;
+                const uint4v b = uint4v{w0 & mask, (w0 >> 8) & mask, w1 & mask, (w1 >> 8) & mask} | (uint4v)0x64006400u;
+                const half8 k = __builtin_bit_cast(half8, b);
+                const half8 n = h ? __builtin_elementwise_fma(k, (half8)(half_t)0.0625f, (half8)(half_t)-64.f)
+                                  : k - (half8)(half_t)1024.f;
                 const half8 a = __builtin_elementwise_fma(n, vs, vm);
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {

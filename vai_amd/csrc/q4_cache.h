@@ -78,7 +78,7 @@ __device__ __forceinline__ uint32_t code_of(float x, float m, float s)
 {
     if (!(s > 0.f)) return 0;
     const float t = x - m;
-    float n = rintf(t / s);
+    float n = rintf(t * __builtin_amdgcn_rcpf(s));   // (at most one off, next to a half)
     const float r = 2.0f * fmaf(-n, s, t);
     const bool odd = (int)n & 1;
     if (r > s || (r == s && odd)) n += 1.f;
