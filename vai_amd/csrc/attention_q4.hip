@@ -12,30 +12,28 @@
 
 namespace vai_dev {
 
-// One half wave per group: 32 lanes hold its values.
+// dp / 8 lanes to a row of one plane, 8 values each; a workgroup takes 2048 / dp
+// rows of K and of V at a time.
 __global__ __launch_bounds__(256) void q4_append_kernel(AttnParams p, uint32_t dp)
 {
-    const uint32_t HD = p.head_dim, groups = dp / 32, hk = blockIdx.y, plane = blockIdx.z;
-    const uint32_t cached = *p.cache_count, lane = threadIdx.x & 31;
+    const uint32_t HD = p.head_dim, hk = blockIdx.y, lanes = dp / 8, c = threadIdx.x % lanes, plane = blockIdx.z;
+    const uint32_t cached = *p.cache_count, step = 256 / lanes;
     uint8_t* head = (plane ? p.v4 : p.k4) + (size_t)hk * q4::head_bytes(p.kv_rows, dp);
     const void* src = plane ? p.v_new : p.k_new;
-    const uint64_t n = (uint64_t)p.tkv * groups;
-    // (a whole number of passes for every lane: the exchanges need them all)
-    for (uint64_t u0 = (uint64_t)blockIdx.x * 8; u0 < n; u0 += (uint64_t)gridDim.x * 8) {
-        const uint64_t u = u0 + (threadIdx.x >> 5);
-        const uint32_t tok = (uint32_t)(u / groups), grp = (uint32_t)(u % groups), d = 32 * grp + lane;
-        const uint32_t pos = cached + tok;
-        // positions past a plane are dropped (a ring's rows all differ: Tkv <= its size)
-        const bool keep = u < n && (p.ring || (pos < p.kv_rows && pos >= cached));
-        const bool in = keep && d < HD;
-        const float x = in ? (float)(half_t)ld(src, p.new_dtype, ((size_t)hk * p.tkv + tok) * HD + d) : 0.f;
+    // (whole workgroups of rows: the exchanges between a group's lanes need them all)
+    for (uint64_t t0 = (uint64_t)blockIdx.x * step; t0 < p.tkv; t0 += (uint64_t)gridDim.x * step) {
+        const uint64_t t = t0 + threadIdx.x / lanes;
+        const uint32_t tok = (uint32_t)std::min<uint64_t>(t, p.tkv - 1), pos = cached + tok;
         half_t s, m;
-        const uint32_t code = q4::encode(x, in, s, m);
-        if (!keep) continue;
+        const uint32_t values = 8 * c < HD ? HD - 8 * c : 0u;
+        const half8 h = q4::row8(src, p.new_dtype, ((size_t)hk * p.tkv + tok) * HD, 8 * c, HD);
+        const uint32_t codes = q4::encode8(h, values, s, m);
+        // positions past a plane are dropped (a ring's rows all differ: Tkv <= its size)
+        if (t >= p.tkv || !(p.ring || (pos < p.kv_rows && pos >= cached))) continue;
         const uint32_t row = p.ring ? pos % p.kv_rows : pos, j = row % q4::KT;
         uint8_t* tile = head + (size_t)(row / q4::KT) * q4::tile_bytes(dp);
-        if (plane == 0) q4::put_k(tile, dp, j, d, code, s, m);
-        else q4::put_v(tile, dp, j, d, code, s, m);
+        if (plane == 0) q4::put_k(tile, dp, j, c, codes, s, m);
+        else q4::put_v(tile, dp, j, c, codes, s, m);
     }
 }
 
@@ -148,9 +146,8 @@ hipError_t attention_q4_launch(const AttnParams& p, hipStream_t s)
     if (p.q4 == 2) return q4_decode_launch(p, p.ws4, s);
     const uint32_t dp = q4_dp(p.head_dim);
     if (p.tkv > 0) {
-        const uint64_t units = ((uint64_t)p.tkv * (dp / 32) + 7) / 8;
-        hipLaunchKernelGGL(q4_append_kernel, dim3((uint32_t)std::min<uint64_t>(units, 2048), p.hkv, 2), dim3(256), 0, s,
-                           p, dp);
+        const uint32_t blocks = (p.tkv + 2048 / dp - 1) / (2048 / dp);
+        hipLaunchKernelGGL(q4_append_kernel, dim3(std::min(blocks, 4096u), p.hkv, 2), dim3(256), 0, s, p, dp);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -181,49 +181,27 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
         LDS_AS uint8_t* kt = ring + slot * 2 * L::TILE;
         LDS_AS uint8_t* vt = kt + L::TILE;
 
-        // the call's own rows in this tile, each read while the one before is rounded
+        // the call's own rows in this tile, 256 / DP at a time: DP / 8 lanes to a row of
+        // K, as many to V's, 8 values each
         if (p.n_new != 0 && j0 + KT > R.cached) {
+            constexpr uint32_t LR = DP / 8, RP = 32 / LR;
             const uint32_t ja = R.cached > j0 ? (uint32_t)(R.cached - j0) : 0u;
             const uint32_t je = (uint32_t)std::min<int64_t>(KT, R.live - j0);
+            const uint32_t c = lane % LR, jr = lane / LR % RP, values = 8 * c < HD ? HD - 8 * c : 0u;
+            const bool is_v = lane >= 32;
+            const void* rows_new = is_v ? p.v_new : p.k_new;
             const size_t at = (size_t)place * L::TILE;
-            const size_t src = ((size_t)hk * p.n_new + (uint32_t)(j0 + ja - R.cached)) * HD;
-            float xk[DP / 64], xv[DP / 64];
-            const auto load = [&](size_t row) __attribute__((always_inline)) {
-                if (p.new_dtype == DT_F16) {
-#pragma unroll
-                    for (int i = 0; i < DP / 64; ++i) {
-                        const uint32_t d = std::min<uint32_t>(64 * i + lane, HD - 1);
-                        xk[i] = (float)((const half_t*)p.k_new)[row + d];
-                        xv[i] = (float)((const half_t*)p.v_new)[row + d];
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < DP / 64; ++i) {
-                        const uint32_t d = std::min<uint32_t>(64 * i + lane, HD - 1);
-                        xk[i] = ((const float*)p.k_new)[row + d];
-                        xv[i] = ((const float*)p.v_new)[row + d];
-                    }
-                }
-            };
-            if (ja < je) load(src);
-            for (uint32_t j = ja; j < je; ++j) {
-                float yk[DP / 64], yv[DP / 64];
-#pragma unroll
-                for (int i = 0; i < DP / 64; ++i) {
-                    yk[i] = (float)(half_t)xk[i];
-                    yv[i] = (float)(half_t)xv[i];
-                }
-                if (j + 1 < je) load(src + (size_t)(j + 1 - ja) * HD);
-#pragma unroll
-                for (int i = 0; i < DP / 64; ++i) {
-                    const uint32_t d = 64 * i + lane;
-                    half_t ks, km, vs, vm;
-                    const uint32_t ck = q4::encode(yk[i], d < HD, ks, km), cv = q4::encode(yv[i], d < HD, vs, vm);
-                    q4::put_k(kt, DP, j, d, ck, ks, km);
-                    q4::put_v(vt, DP, j, d, cv, vs, vm);
+            for (uint32_t ju = ja; ju < je; ju += RP) {
+                const uint32_t j = ju + jr, jc = std::min(j, je - 1);
+                const size_t row = ((size_t)hk * p.n_new + (uint32_t)(j0 + jc - R.cached)) * HD;
+                half_t s, m;
+                const uint32_t codes = q4::encode8(q4::row8(rows_new, p.new_dtype, row, 8 * c, HD), values, s, m);
+                if (j < je) {
+                    if (is_v) q4::put_v(vt, DP, j, c, codes, s, m);
+                    else q4::put_k(kt, DP, j, c, codes, s, m);
                     if (rb == 0) {
-                        q4::put_k(kh + at, DP, j, d, ck, ks, km);
-                        q4::put_v(vh + at, DP, j, d, cv, vs, vm);
+                        if (is_v) q4::put_v(vh + at, DP, j, c, codes, s, m);
+                        else q4::put_k(kh + at, DP, j, c, codes, s, m);
                     }
                 }
             }
@@ -231,29 +209,46 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
         }
         place = next_place(place);
 
-        // this lane's share of the tile
-        uint32_t kw[2][G];
-        uint4v ksm[2][G];      // (s, m) of rows 4 g ..+3
-        uint32_t vw[ND];       // words 2 i, 2 i + 1: the two halves of the block's positions, values 2 i and 2 i + 1
+        // S^T: lane (c16, g) holds query row c16 and positions 8 g + 4 t ..+3
+        float4v x[2][NQ];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            uint32_t kw[G];
             LDS_AS const uint8_t* a = kt + ((t * 4 + g) * 16 + c16) * (G * 4);
             if constexpr (G == 2) {
                 const uint2v w = *(LDS_AS const uint2v*)a;
-                kw[t][0] = w.x;
-                kw[t][1] = w.y;
+                kw[0] = w.x;
+                kw[1] = w.y;
             } else {
 #pragma unroll
                 for (int i = 0; i < G; i += 4) {
                     const uint4v w = *(LDS_AS const uint4v*)(a + 4 * i);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) kw[t][i + e] = w[e];
+                    for (int e = 0; e < 4; ++e) kw[i + e] = w[e];
                 }
             }
 #pragma unroll
-            for (int i = 0; i < G; ++i)
-                ksm[t][i] = *(LDS_AS const uint4v*)(kt + q4::scale_offset(DP) + ((i * 2 + t) * 16 + 4 * g) * 4);
+            for (int q = 0; q < NQ; ++q) x[t][q] = (float4v)0.f;
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                // (s, m) of rows 4 g ..+3
+                const uint4v ksm = *(LDS_AS const uint4v*)(kt + q4::scale_offset(DP) + ((i * 2 + t) * 16 + 4 * g) * 4);
+                const uint32_t w = kw[i];
+                const half8 n8 = __builtin_bit_cast(half8, uint4v{w & NIB, (w >> 4) & NIB, (w >> 8) & NIB, (w >> 12) & NIB});
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    const float4v n = __builtin_amdgcn_mfma_f32_16x16x32_f16(n8, qf[q][i], (float4v)0.f, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t both = ksm[r];   // (a bit cast of the element itself takes the vector's first)
+                        const half2v sm = __builtin_bit_cast(half2v, both);
+                        x[t][q][r] = fmaf((float)sm.x, n[r], x[t][q][r]);
+                        x[t][q][r] = fmaf((float)sm.y, qs[q][i], x[t][q][r]);
+                    }
+                }
+            }
         }
+        uint32_t vw[ND];       // words 2 i, 2 i + 1: the two halves of the block's positions, values 2 i and 2 i + 1
         {
             LDS_AS const uint8_t* a = vt + g * (DP * 4) + c16 * (DP / 4);
 #pragma unroll
@@ -268,31 +263,6 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
         q4_wait_lds();         // read before the slot is copied over
         copy(slot);
         slot = slot + 1 == D ? 0 : slot + 1;
-
-        // S^T: lane (c16, g) holds query row c16 and positions 8 g + 4 t ..+3
-        float4v x[2][NQ];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) x[t][q] = (float4v)0.f;
-#pragma unroll
-        for (int i = 0; i < G; ++i)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint32_t w = kw[t][i];
-                const half8 a = __builtin_bit_cast(half8, uint4v{w & NIB, (w >> 4) & NIB, (w >> 8) & NIB, (w >> 12) & NIB});
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) {
-                    const float4v n = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[q][i], (float4v)0.f, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t both = ksm[t][i][r];   // (a bit cast of the element itself takes the vector's first)
-                        const half2v sm = __builtin_bit_cast(half2v, both);
-                        x[t][q][r] = fmaf((float)sm.x, n[r], x[t][q][r]);
-                        x[t][q][r] = fmaf((float)sm.y, qs[q][i], x[t][q][r]);
-                    }
-                }
-            }
 
         // Positions that no query sees (stale rows, rows past the count) may hold
         // anything: their V is zero here, their scores are masked below.

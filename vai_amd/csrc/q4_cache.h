@@ -72,18 +72,16 @@ __device__ __forceinline__ void step_of(float lo, float hi, bool finite, half_t&
         s = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, s) - 1));
 }
 
-// (x - m) / s to the nearest integer, halves to even, from the exact remainder;
-// s = 0 gives 0. x >= m, and s is rounded: the last code is 15 all the same.
-__device__ __forceinline__ uint32_t code_of(float x, float m, float s)
+// (x - m) / s to the nearest integer, halves to even, from the exact remainder
+// (inv: 1 / s or next to it: the first guess is at most one off); s = 0 gives 0.
+// x >= m, and s is rounded: the last code is 15 all the same.
+__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv)
 {
-    if (!(s > 0.f)) return 0;
-    const float t = x - m;
-    float n = rintf(t * __builtin_amdgcn_rcpf(s));   // (at most one off, next to a half)
-    const float r = 2.0f * fmaf(-n, s, t);
-    const bool odd = (int)n & 1;
-    if (r > s || (r == s && odd)) n += 1.f;
-    else if (r < -s || (r == -s && odd)) n -= 1.f;
-    return (uint32_t)fminf(n, 15.f);
+    const float t = x - m, q = rintf(t * inv), r = 2.0f * fmaf(-q, s, t);
+    const int n = (int)q;
+    const bool odd = n & 1, up = r > s || (r == s && odd), down = r < -s || (r == -s && odd);
+    const int c = n + (int)up - (int)down;
+    return s > 0.f ? (uint32_t)(c < 15 ? c : 15) : 0u;
 }
 
 // What lane ^ 1, ^ 2, and the mirror image in 8 and in 16 lanes hold: with an
@@ -94,53 +92,77 @@ template <int CTRL>
 __device__ __forceinline__ float moved(float x) { return __builtin_bit_cast(float, moved<CTRL>(__builtin_bit_cast(uint32_t, x))); }
 constexpr int XOR1 = 0xB1, XOR2 = 0x4E, MIRROR8 = 0x141, MIRROR16 = 0x140;
 
-// 32 lanes hold a group's values x (in: the value exists), already rounded to
-// fp16: its step and minimum, and this lane's code.
-__device__ __forceinline__ uint32_t encode(float x, bool in, half_t& s, half_t& m)
-{
-    float lo = in ? x : __builtin_inff(), hi = in ? x : -__builtin_inff();
-    uint32_t top = in ? __builtin_bit_cast(uint32_t, x) & 0x7fffffffu : 0u;   // NaN and infinity above all
-    const auto step = [&](float l, float h, uint32_t t) __attribute__((always_inline)) {
-        lo = fminf(lo, l);
-        hi = fmaxf(hi, h);
-        top = t > top ? t : top;
-    };
-    step(moved<XOR1>(lo), moved<XOR1>(hi), moved<XOR1>(top));
-    step(moved<XOR2>(lo), moved<XOR2>(hi), moved<XOR2>(top));
-    step(moved<MIRROR8>(lo), moved<MIRROR8>(hi), moved<MIRROR8>(top));
-    step(moved<MIRROR16>(lo), moved<MIRROR16>(hi), moved<MIRROR16>(top));
-    step(__shfl_xor(lo, 16), __shfl_xor(hi, 16), (uint32_t)__shfl_xor((int)top, 16));
-    const bool finite = top < 0x7f800000u;
-    step_of(lo, hi, finite, s, m);
-    return in && finite ? code_of(x, (float)m, (float)s) : 0u;
-}
-
 template <class T>
 __device__ __forceinline__ void store(uint8_t* p, T v) { *(T*)p = v; }
 template <class T>
 __device__ __forceinline__ void store(__attribute__((address_space(3))) uint8_t* p, T v) { *(__attribute__((address_space(3))) T*)p = v; }
 
-// Writes position j's value d (code; every lane of its group calls) into a tile.
-template <class P>   // a byte pointer, global or LDS
-__device__ __forceinline__ void put_k(P tile, uint32_t dp, uint32_t j, uint32_t d, uint32_t code, half_t s, half_t m)
+// 8 values of a row, from value 8 c on (c: the lane's place, 4 neighbouring lanes
+// hold a group), already rounded to fp16; those from `values` on do not exist.
+// Its group's step and minimum, and the codes, value e in nibble e.
+__device__ __forceinline__ uint32_t encode8(const half8 h, uint32_t values, half_t& s, half_t& m)
 {
-    uint32_t w = code << (4 * nibble_of(d & 7));
-    w |= moved<XOR1>(w);
-    w |= moved<XOR2>(w);
-    w |= moved<MIRROR8>(w);
-    if ((d & 7) == 0) store<uint32_t>(tile + k_word(dp, j, d), w);
-    if ((d & 31) == 0)
-        store<uint32_t>(tile + k_scale(dp, j, d), (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16);
+    float x[8], lo = __builtin_inff(), hi = -__builtin_inff();
+    uint32_t top = 0;   // the largest |x| as bits: NaN and infinity above all
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] = (float)h[e];
+        if ((uint32_t)e < values) {
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+            const uint32_t b = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu;
+            top = b > top ? b : top;
+        }
+    }
+    const auto step = [&](float l, float u, uint32_t t) __attribute__((always_inline)) {
+        lo = fminf(lo, l);
+        hi = fmaxf(hi, u);
+        top = t > top ? t : top;
+    };
+    step(moved<XOR1>(lo), moved<XOR1>(hi), moved<XOR1>(top));
+    step(moved<XOR2>(lo), moved<XOR2>(hi), moved<XOR2>(top));
+    const bool finite = top < 0x7f800000u;
+    step_of(lo, hi, finite, s, m);
+    const float fs = (float)s, fm = (float)m, inv = fs > 0.f ? __builtin_amdgcn_rcpf(fs) : 0.f;
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (finite && (uint32_t)e < values) w |= code_of(x[e], fm, fs, inv) << (4 * e);
+    return w;
+}
+
+// Writes the 8 values from 8 c on of position j into a tile.
+template <class P>   // a byte pointer, global or LDS
+__device__ __forceinline__ void put_k(P tile, uint32_t dp, uint32_t j, uint32_t c, uint32_t codes, half_t s, half_t m)
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) w |= (codes >> (4 * e) & 15u) << (4 * nibble_of(e));
+    store<uint32_t>(tile + k_word(dp, j, 8 * c), w);
+    if ((c & 3) == 0)
+        store<uint32_t>(tile + k_scale(dp, j, 8 * c), (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16);
 }
 template <class P>
-__device__ __forceinline__ void put_v(P tile, uint32_t dp, uint32_t j, uint32_t d, uint32_t code, half_t s, half_t m)
+__device__ __forceinline__ void put_v(P tile, uint32_t dp, uint32_t j, uint32_t c, uint32_t codes, half_t s, half_t m)
 {
-    const uint32_t w = code | moved<XOR1>(code) << 4;
-    if ((d & 1) == 0) store<uint8_t>(tile + v_byte(dp, j, d), (uint8_t)w);
-    if ((d & 31) == 0) {
-        store<uint16_t>(tile + v_scale(dp, j, d), __builtin_bit_cast(uint16_t, s));
-        store<uint16_t>(tile + v_scale(dp, j, d) + 16, __builtin_bit_cast(uint16_t, m));
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) store<uint8_t>(tile + v_byte(dp, j, 8 * c + 2 * i), (uint8_t)(codes >> (8 * i)));
+    if ((c & 3) == 0) {
+        store<uint16_t>(tile + v_scale(dp, j, 8 * c), __builtin_bit_cast(uint16_t, s));
+        store<uint16_t>(tile + v_scale(dp, j, 8 * c) + 16, __builtin_bit_cast(uint16_t, m));
     }
+}
+
+// 8 values of a new row from value d on, as fp16
+__device__ __forceinline__ half8 row8(const void* rows, int dt, size_t row, uint32_t d, uint32_t HD)
+{
+    half8 h = (half8)(half_t)0;
+    if (d + 8 <= HD) h = dt == DT_F16 ? load8((const half_t*)rows + row + d) : load8((const float*)rows + row + d);
+    else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (d + e < HD) h[e] = (half_t)ld(rows, dt, row + d + e);
+    return h;
 }
 
 }   // namespace q4
