@@ -37,62 +37,143 @@ __global__ __launch_bounds__(256) void q4_append_kernel(AttnParams p, uint32_t d
     }
 }
 
-// The value stored at position row, value d of a head's plane.
-__device__ __forceinline__ float q4_value(const uint8_t* head, uint32_t dp, uint32_t row, uint32_t d, bool is_v)
+// 8 values of a row from value 8 c on, in fp32
+__device__ __forceinline__ void q4_values8(const uint8_t* head, uint32_t dp, uint32_t row, uint32_t c, bool is_v, float (&x)[8])
 {
-    const uint32_t j = row % q4::KT;
+    const uint32_t j = row % q4::KT, d = 8 * c;
     const uint8_t* tile = head + (size_t)(row / q4::KT) * q4::tile_bytes(dp);
     const half_t* sm = (const half_t*)(tile + (is_v ? q4::v_scale(dp, j, d) : q4::k_scale(dp, j, d)));
-    const uint32_t n = is_v ? (tile[q4::v_byte(dp, j, d)] >> (4 * (d & 1))) & 15u
-                            : (*(const uint32_t*)(tile + q4::k_word(dp, j, d)) >> (4 * q4::nibble_of(d & 7))) & 15u;
-    return fmaf((float)sm[0], (float)n, (float)sm[is_v ? 8 : 1]);
+    const float s = (float)sm[0], m = (float)sm[is_v ? 8 : 1];
+    uint32_t w = 0;
+    if (is_v) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) w |= (uint32_t)tile[q4::v_byte(dp, j, d + 2 * i)] << (8 * i);
+    } else {
+        w = *(const uint32_t*)(tile + q4::k_word(dp, j, d));
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) x[e] = fmaf(s, (float)(w >> (4 * (is_v ? e : q4::nibble_of(e))) & 15u), m);
 }
 
 // The live rows of the cache as fp16 copies for the kernels that read fp16:
-// from the 64-position tile the first query's window starts in. Each wave takes
-// a row of one head. A hidden position must not reach a query through a NaN
-// (0 * NaN in P V), so a row with a NaN in V is copied as V = 0 and K = NaN:
-// the score is masked where the position is hidden and NaN where it is not.
-__global__ __launch_bounds__(256) void q4_copy_kernel(AttnParams p, uint32_t dp, half_t* k16, half_t* v16)
+// from the 64-position tile the first query's window starts in. A workgroup
+// takes a 32-position tile of one head at a time: half its threads V (a slice of
+// 4 positions each, so that a row's values leave in wide stores), half K (a word
+// of 8 values each). A hidden position must not reach a query through a NaN (0 *
+// NaN in P V), so a row with a NaN in V is copied as V = 0 and K = NaN: the score
+// is masked where the position is hidden and NaN where it is not.
+// 7513 positions of 8 heads of 128: 25 us with a wave to a row.
+template <int DP>
+__global__ __launch_bounds__(256) void q4_copy_kernel(AttnParams p, half_t* k16, half_t* v16)
 {
-    const uint32_t HD = p.head_dim, hk = blockIdx.y, lane = threadIdx.x & 63;
+    constexpr int G = DP / 32, ND = DP / 16;
+    __shared__ uint32_t bad[2][q4::KT];
+    const uint32_t HD = p.head_dim, hk = blockIdx.y, t = threadIdx.x;
     const uint32_t cached = *p.cache_count;
     const uint64_t end = (uint64_t)cached + p.tkv;
     uint64_t beg = (uint64_t)p.mask.key_start_cached(0, cached) / 64 * 64;
     // (a ring holds the last kv_rows positions)
     if (p.ring && end > p.kv_rows && beg < end - p.kv_rows) beg = end - p.kv_rows;
     const uint64_t live = p.ring ? end : std::min<uint64_t>(end, p.kv_rows);
-    const size_t hb = q4::head_bytes(p.kv_rows, dp);
+    const size_t hb = q4::head_bytes(p.kv_rows, DP);
     const uint8_t* kh = p.k4 + hk * hb;
     const uint8_t* vh = p.v4 + hk * hb;
-    for (uint64_t pos = beg + blockIdx.x * 4 + (threadIdx.x >> 6); pos < live; pos += (uint64_t)gridDim.x * 4) {
-        const uint32_t row = p.ring ? (uint32_t)(pos % p.kv_rows) : (uint32_t)pos;
-        const size_t dst = ((size_t)hk * p.kv_rows + row) * HD;
-        bool bad = false;
-        for (uint32_t d = lane; d < HD; d += 64) {
-            const float v = q4_value(vh, dp, row, d, true);
-            bad |= v != v;
-            v16[dst + d] = v != v ? (half_t)0.f : (half_t)v;
+    const uint32_t wrap = p.ring ? p.kv_rows / q4::KT : 0xffffffffu;
+    if (t < 2 * q4::KT) bad[t / q4::KT][t % q4::KT] = 0;
+    __syncthreads();
+    uint32_t round = 0;
+    for (uint64_t T = beg / q4::KT + blockIdx.x; T * q4::KT < live; T += gridDim.x, round ^= 1) {
+        const uint32_t place = (uint32_t)(p.ring ? T % wrap : T), row0 = place * q4::KT;
+        const uint8_t* kt = kh + (size_t)place * q4::tile_bytes(DP);
+        const uint8_t* vt = vh + (size_t)place * q4::tile_bytes(DP);
+        const size_t dst = ((size_t)hk * p.kv_rows + row0) * HD;
+        // rows of this tile that are copied (of a ring also those a full turn older: not before beg)
+        const auto copied = [&](uint32_t j) { return T * q4::KT + j >= beg && T * q4::KT + j < live; };
+        for (uint32_t e = t; e < q4::KT * G; e += 256) {
+            const uint32_t j = e % q4::KT;
+            const half_t m = *(const half_t*)(vt + q4::v_scale(DP, j, e / q4::KT * 32) + 16);
+            if (m != m) bad[round][j] = 1;
         }
-        bad = __any(bad);
-        for (uint32_t d = lane; d < HD; d += 64)
-            k16[dst + d] = bad ? (half_t)__builtin_nanf("") : (half_t)q4_value(kh, dp, row, d, false);
+        __syncthreads();
+        if (t < 128) {
+            const uint32_t slice = t % 16, b = t / 32, h = t / 16 % 2, d0 = slice * ND;   // positions 8 b + 4 h ..+3
+            uint32_t w[ND / 2];
+#pragma unroll
+            for (int i = 0; i < ND / 2; ++i)
+                w[i] = *(const uint32_t*)(vt + b * (DP * 4) + slice * (DP / 4) + i * 8 + h * 4);
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                const uint32_t j = 8 * b + 4 * h + r;
+                const half_t* sm = (const half_t*)(vt + q4::v_scale(DP, j, d0));
+                const float s = (float)sm[0], m = (float)sm[8];
+                typedef half_t out_t __attribute__((ext_vector_type(ND)));
+                typedef out_t out_u __attribute__((aligned(2)));
+                out_t x;
+#pragma unroll
+                for (int i = 0; i < ND; ++i) {
+                    const float v = fmaf(s, (float)(w[i / 2] >> (8 * r + 4 * (i & 1)) & 15u), m);
+                    x[i] = v != v ? (half_t)0.f : (half_t)v;
+                }
+                half_t* o = v16 + dst + (size_t)j * HD + d0;
+                if (!copied(j)) continue;
+                if (d0 + ND <= HD) *(out_u*)o = x;
+                else
+#pragma unroll
+                    for (int i = 0; i < ND; ++i)
+                        if (d0 + i < HD) o[i] = x[i];
+            }
+        } else {
+            for (uint32_t e = t - 128; e < q4::KT * DP / 8; e += 128) {
+                const uint32_t j = e / (DP / 8), c = e % (DP / 8);
+                const uint32_t w = *(const uint32_t*)(kt + q4::k_word(DP, j, 8 * c));
+                const half_t* sm = (const half_t*)(kt + q4::k_scale(DP, j, 8 * c));
+                const float s = bad[round][j] ? __builtin_nanf("") : (float)sm[0], m = (float)sm[1];
+                typedef half8 half8u __attribute__((aligned(2)));
+                half8 x;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) x[i] = (half_t)fmaf(s, (float)(w >> (4 * q4::nibble_of(i)) & 15u), m);
+                half_t* o = k16 + dst + (size_t)j * HD + 8 * c;
+                if (!copied(j)) continue;
+                if (8 * c + 8 <= HD) *(half8u*)o = x;
+                else
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        if (8 * c + i < HD) o[i] = x[i];
+            }
+        }
+        // (the other round's flags, which every thread is done with)
+        if (t < q4::KT) bad[round ^ 1][t] = 0;
+        __syncthreads();
     }
 }
 
+// 8 values a thread
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheReadParams p, uint32_t dp)
 {
-    const uint32_t hk = blockIdx.y, plane = blockIdx.z, HD = p.head_dim;
-    const size_t total = (size_t)p.n * HD;
+    const uint32_t hk = blockIdx.y, plane = blockIdx.z, HD = p.head_dim, C = (HD + 7) / 8;
+    const uint64_t total = (uint64_t)p.n * C;
     void* out = plane ? p.v_out : p.k_out;
     const void* src = plane ? p.v : p.k;
-    for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (size_t)gridDim.x * 256) {
-        const uint32_t i = (uint32_t)(e / HD), d = (uint32_t)(e % HD);
+    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
+        const uint32_t i = (uint32_t)(e / C), c = (uint32_t)(e % C);
         const uint32_t row = (uint32_t)(((uint64_t)p.first + i) % p.rows);
-        const float v = p.cache_dtype == DT_Q4
-                            ? q4_value((const uint8_t*)src + hk * q4::head_bytes(p.rows, dp), dp, row, d, plane != 0)
-                            : ld(src, p.cache_dtype, ((size_t)hk * p.rows + row) * HD + d);
-        st(out, p.o_dtype, (size_t)hk * total + e, v);
+        float x[8];
+        if (p.cache_dtype == DT_Q4)
+            q4_values8((const uint8_t*)src + hk * q4::head_bytes(p.rows, dp), dp, row, c, plane != 0, x);
+        else
+#pragma unroll
+            for (uint32_t d = 0; d < 8; ++d)
+                x[d] = 8 * c + d < HD ? ld(src, p.cache_dtype, ((size_t)hk * p.rows + row) * HD + 8 * c + d) : 0.f;
+        const size_t o = ((size_t)hk * p.n + i) * HD + 8 * c;
+        if (8 * c + 8 <= HD && p.o_dtype == DT_F32) {
+            typedef float4v float4u __attribute__((aligned(4)));
+            *(float4u*)((float*)out + o) = float4v{x[0], x[1], x[2], x[3]};
+            *(float4u*)((float*)out + o + 4) = float4v{x[4], x[5], x[6], x[7]};
+        } else {
+#pragma unroll
+            for (uint32_t d = 0; d < 8; ++d)
+                if (8 * c + d < HD) st(out, p.o_dtype, o + d, x[d]);
+        }
     }
 }
 
@@ -105,7 +186,7 @@ size_t q4_plane_bytes(uint32_t hkv, uint32_t rows, uint32_t head_dim)
 
 hipError_t cache_read_launch(const CacheReadParams& p, hipStream_t s)
 {
-    const size_t blocks = ((size_t)p.n * p.head_dim + 255) / 256;
+    const size_t blocks = ((size_t)p.n * ((p.head_dim + 7) / 8) + 255) / 256;
     hipLaunchKernelGGL(cache_read_kernel, dim3((uint32_t)std::min<size_t>(blocks, 4096), p.hkv, 2), dim3(256), 0, s, p,
                        q4_dp(p.head_dim));
     return hipGetLastError();
@@ -151,8 +232,11 @@ hipError_t attention_q4_launch(const AttnParams& p, hipStream_t s)
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(q4_copy_kernel, dim3(std::min<uint32_t>((p.kv_rows + 3) / 4, 2048), p.hkv), dim3(256), 0, s, p, dp,
-                       (half_t*)p.k, (half_t*)p.v);
+    const dim3 grid(std::min<uint32_t>((p.kv_rows + q4::KT - 1) / q4::KT, 1024), p.hkv);
+    half_t *k16 = (half_t*)p.k, *v16 = (half_t*)p.v;
+    if (dp == 64) hipLaunchKernelGGL(q4_copy_kernel<64>, grid, dim3(256), 0, s, p, k16, v16);
+    else if (dp == 128) hipLaunchKernelGGL(q4_copy_kernel<128>, grid, dim3(256), 0, s, p, k16, v16);
+    else hipLaunchKernelGGL(q4_copy_kernel<256>, grid, dim3(256), 0, s, p, k16, v16);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     return attention_launch(p, s);
