@@ -62,6 +62,7 @@ void OutputNode::prepare() {}
 
 NeuralNet::NeuralNet(const NeuralNetConfig& config) : config_(config)
 {
+    require(config_.wDefaultDtype != Dtype::Q4 && config_.oDefaultDtype != Dtype::Q4, "Q4 is a KV cache's dtype alone");
     require(config_.wDefaultDtype != Dtype::None && config_.oDefaultDtype != Dtype::None,
             "NeuralNetConfig: default dtypes must not be None");
     currentNet_ = this;

@@ -12,6 +12,7 @@ static int32_t code(Dtype d)
     switch (d) {
     case Dtype::Fp32: return VAI_DTYPE_F32;
     case Dtype::Fp16: return VAI_DTYPE_F16;
+    case Dtype::Q4: return VAI_DTYPE_Q4;
     default: return VAI_DTYPE_NONE;
     }
 }
@@ -43,6 +44,7 @@ Linear::Linear(Config config) : config_(config)
 {
     require(config_.inDim > 0 && config_.outDim > 0, "Linear: inDim and outDim must be positive");
     require(config_.epilogue < Epilogue::Max, "Linear: bad epilogue");
+    require(!config_.int8Weights || config_.splitSize == 0, "Linear: splitSize does not apply to int8Weights");
     addSlot("out0", NodeSlot::output);
     addSlot("in0", NodeSlot::input);
     addSlot("weight", NodeSlot::persistent);
@@ -103,7 +105,7 @@ bool Linear::canFuseGate(const GatedMul& gm) const
 {
     (void)gm;
     const bool biasRow = !hasBias() || (*this)["bias"].numElements() == config_.outDim;
-    return !config_.acceptResidual && config_.epilogue == Epilogue::None && config_.scalarScale == 1.0f &&
+    return !config_.int8Weights && !config_.acceptResidual && config_.epilogue == Epilogue::None && config_.scalarScale == 1.0f &&
            config_.outDim % 2 == 0 && biasRow;
 }
 
@@ -133,6 +135,7 @@ void Linear::prepare()
     std::vector<uint32_t> shape = in.shape();
     shape.back() = N;
     (*this)["out0"] = Tensor(shape, outputDtype());
+    if (config_.int8Weights) return prepareI8();
 
     vai_linear_args a = args(false);
     // Prefill shapes and decode GEMVs of 3-8 rows stream a fragment-major copy
@@ -163,8 +166,67 @@ void Linear::prepare()
     (*this)["partial"] = ws ? Tensor({uint32_t((ws + 3) / 4)}, Dtype::Fp32) : Tensor();
 }
 
+vai_linear_i8_args Linear::i8Args(bool withPointers) const
+{
+    vai_linear_i8_args a{};
+    const Tensor& in = (*this)["in0"];
+    a.M = M_;
+    a.N = config_.outDim;
+    a.K = config_.inDim;
+    a.i_dtype = code(in.dtype());
+    a.o_dtype = code(outputDtype());
+    a.b_dtype = hasBias() ? code((*this)["bias"].dtype()) : VAI_DTYPE_NONE;
+    a.epilogue = uint32_t(config_.epilogue);
+    a.residual_order = uint32_t(config_.residualOrder);
+    a.bias_repeat = biasRepeat_;
+    a.residual_repeat = residualRepeat_;
+    a.scalar_scale = config_.scalarScale;
+    // (placeholders for the size query's checks)
+    a.in = a.out = reinterpret_cast<void*>(256);
+    a.weight = reinterpret_cast<void*>(256);
+    a.w_scale = reinterpret_cast<const float*>(256);
+    if (withPointers) {
+        a.in = in.devicePtr();
+        a.out = (*this)["out0"].devicePtr();
+        a.weight = codes_.ptr();
+        a.w_scale = static_cast<const float*>(scales_.ptr());
+        a.bias = hasBias() ? (*this)["bias"].devicePtr() : nullptr;
+        a.residual = config_.acceptResidual ? ptrOrNull((*this)["residual"]) : nullptr;
+        const Tensor& part = (*this)["partial"];
+        a.workspace = ptrOrNull(part);
+        a.workspace_bytes = part.validShape() ? part.numBytes() : 0;
+    }
+    return a;
+}
+
+// The weight's integers and scales are made once per upload, as a packed weight is.
+void Linear::prepareI8()
+{
+    const Tensor& w = (*this)["weight"];
+    const size_t row = (size_t(config_.inDim) + 15) / 16 * 16;
+    if (!codes_ || packedFrom_ != w.uploadId()) {
+        codes_ = bufferPool().requestBuffer(row * config_.outDim);
+        scales_ = bufferPool().requestBuffer(sizeof(float) * config_.outDim);
+        const vai_stream_t stream = (vai_stream_t)net().stream();
+        check(vai_quantize_i8_launch(codes_.ptr(), static_cast<float*>(scales_.ptr()), w.devicePtr(), code(w.dtype()),
+                                     config_.outDim, config_.inDim, stream), "Linear");
+        check(vai_stream_sync(stream), "Linear");
+        packedFrom_ = w.uploadId();
+    }
+    plan_ = "i8";
+    splitCount_ = 1;
+    const vai_linear_i8_args a = i8Args(false);
+    const size_t ws = vai_linear_i8_workspace_size(&a);
+    (*this)["partial"] = ws ? Tensor({uint32_t((ws + 3) / 4)}, Dtype::Fp32) : Tensor();
+}
+
 void Linear::run(CommandStream& cmd)
 {
+    if (config_.int8Weights) {
+        const vai_linear_i8_args a = i8Args(true);
+        check(vai_linear_i8_launch(&a, (vai_stream_t)cmd.stream()), "Linear");
+        return;
+    }
     vai_linear_args a = args(true);
     check(vai_linear_launch(&a, (vai_stream_t)cmd.stream()), "Linear");
 }
@@ -383,8 +445,11 @@ Attention::Attention(Config config) : config_(config)
     if (config_.numKVHeads == 0) config_.numKVHeads = config_.numQHeads;
     require(config_.numQHeads > 0 && config_.headDim > 0, "Attention: heads and headDim must be positive");
     require(config_.numQHeads % config_.numKVHeads == 0, "Attention: numQHeads must be a multiple of numKVHeads");
-    require(config_.kvCacheSize == 0 || config_.kvCacheDtype == Dtype::Fp16 || config_.kvCacheDtype == Dtype::Fp32,
-            "Attention: a KV cache needs kvCacheDtype fp16 or fp32 (attention.h:959)");
+    require(config_.kvCacheSize == 0 || config_.kvCacheDtype == Dtype::Fp16 || config_.kvCacheDtype == Dtype::Fp32 ||
+                config_.kvCacheDtype == Dtype::Q4,
+            "Attention: a KV cache needs kvCacheDtype fp16 or fp32 (attention.h:959), or Q4");
+    require(config_.kvCacheSize == 0 || config_.kvCacheDtype != Dtype::Q4 || config_.headDim <= 256,
+            "Attention: a Q4 cache needs headDim <= 256");
     require(!config_.kvCacheRing || config_.kvCacheSize > 0, "Attention: a ring needs kvCacheSize (attention.h:960)");
     if (config_.kvCacheRing)
         config_.kvCacheSize = (config_.kvCacheSize + kvRingAlign - 1) / kvRingAlign * kvRingAlign;
@@ -396,8 +461,11 @@ Attention::Attention(Config config) : config_(config)
     if (config_.kvCacheSize > 0) {
         addSlot("K_cache", NodeSlot::persistent);
         addSlot("V_cache", NodeSlot::persistent);
-        (*this)["K_cache"] = Tensor({config_.numKVHeads, config_.kvCacheSize, config_.headDim}, config_.kvCacheDtype);
-        (*this)["V_cache"] = Tensor({config_.numKVHeads, config_.kvCacheSize, config_.headDim}, config_.kvCacheDtype);
+        const size_t words = vai_attention_cache_bytes(1, config_.kvCacheSize, config_.headDim, VAI_DTYPE_Q4) / sizeof(float);
+        for (const char* name : {"K_cache", "V_cache"})
+            (*this)[name] = config_.kvCacheDtype == Dtype::Q4
+                                ? Tensor({config_.numKVHeads, uint32_t(words)}, Dtype::Fp32)
+                                : Tensor({config_.numKVHeads, config_.kvCacheSize, config_.headDim}, config_.kvCacheDtype);
     }
 }
 
@@ -493,6 +561,87 @@ void Attention::run(CommandStream& cmd)
 {
     const vai_attention_args a = args(true);
     check(vai_attention_launch(&a, (vai_stream_t)cmd.stream()), "Attention");
+}
+
+// ------------------------------------------------------------ QkNormRope ----
+
+QkNormRope::QkNormRope(Config config) : config_(config)
+{
+    if (config_.numKVHeads == 0) config_.numKVHeads = config_.numQHeads;
+    require(config_.numQHeads > 0 && config_.headDim > 0, "QkNormRope: heads and headDim must be positive");
+    if (config_.rotDim == 0) config_.rotDim = config_.headDim;
+    require(config_.pairs == Pairs::None || (config_.rotDim <= config_.headDim && config_.rotDim % 2 == 0),
+            "QkNormRope: rotDim must be even and at most headDim");
+    addSlot("in0", NodeSlot::input);
+    addSlot("Q", NodeSlot::output);
+    addSlot("K", NodeSlot::output);
+    addSlot("V", NodeSlot::output);
+    addSlot("q_weight", NodeSlot::persistent);
+    addSlot("k_weight", NodeSlot::persistent);
+    addSlot("inv_freq", NodeSlot::persistent);
+}
+
+void QkNormRope::setPositionCounter(const uint32_t* counter)
+{
+    counter_ = counter;
+    if (ownedNet_) ownedNet_->invalidateCommandBuffer();
+}
+
+void QkNormRope::prepare()
+{
+    const Tensor& in = (*this)["in0"];
+    const auto& s = in.shape();
+    const uint32_t hq = config_.numQHeads, hkv = config_.numKVHeads, d = config_.headDim;
+    require(s.size() >= 2 && s.back() == (hq + 2 * hkv) * d,
+            "QkNormRope: in0 must be [..., T, (numQHeads + 2 numKVHeads) headDim]");
+    Dtype weights = Dtype::None;
+    for (const char* name : {"q_weight", "k_weight"}) {
+        const Tensor& w = (*this)[name];
+        if (!w.validShape()) continue;
+        require(config_.norm, "QkNormRope: weights without norm");
+        require(w.isShapeOf({d}), "QkNormRope: weights must be [headDim]");
+        require(weights == Dtype::None || weights == w.dtype(), "QkNormRope: the weights must share a dtype");
+        weights = w.dtype();
+    }
+    const Tensor& f = (*this)["inv_freq"];
+    require(!f.validShape() || (f.isShapeOf({config_.rotDim / 2}) && f.dtype() == Dtype::Fp32),
+            "QkNormRope: inv_freq must be [rotDim / 2] fp32");
+    batch_ = outerSize(s, 2);
+    tokens_ = s[s.size() - 2];
+    for (const char* name : {"Q", "K", "V"}) {
+        std::vector<uint32_t> os(s.begin(), s.end() - 2);
+        os.insert(os.end(), {name[0] == 'Q' ? hq : hkv, tokens_, d});
+        (*this)[name] = Tensor(os, outputDtype());
+    }
+}
+
+void QkNormRope::run(CommandStream& cmd)
+{
+    vai_qk_norm_rope_args a{};
+    const Tensor &qw = (*this)["q_weight"], &kw = (*this)["k_weight"];
+    a.qkv = (*this)["in0"].devicePtr();
+    a.q_out = (*this)["Q"].devicePtr();
+    a.k_out = (*this)["K"].devicePtr();
+    a.v_out = (*this)["V"].devicePtr();
+    a.q_weight = ptrOrNull(qw);
+    a.k_weight = ptrOrNull(kw);
+    a.inv_freq = static_cast<const float*>(ptrOrNull((*this)["inv_freq"]));
+    a.count = counter_;
+    a.batch = batch_;
+    a.tokens = tokens_;
+    a.hq = config_.numQHeads;
+    a.hkv = config_.numKVHeads;
+    a.head_dim = config_.headDim;
+    a.i_dtype = code((*this)["in0"].dtype());
+    a.o_dtype = code(outputDtype());
+    a.w_dtype = qw.validShape() ? code(qw.dtype()) : code(kw.dtype());
+    a.norm = config_.norm ? 1 : 0;
+    a.eps = config_.eps;
+    a.weight_offset = config_.weightOffset;
+    a.rope = uint32_t(config_.pairs);
+    a.rot_dim = config_.rotDim;
+    a.theta = config_.theta;
+    check(vai_qk_norm_rope_launch(&a, (vai_stream_t)cmd.stream()), "QkNormRope");
 }
 
 }   // namespace vai::node

@@ -44,6 +44,11 @@ public:
         Epilogue epilogue = Epilogue::None;
         float scalarScale = 1.0f;
         uint32_t splitSize = 0;   // split-K span; 0 lets the library choose per shape
+        // The product in 8-bit integers (vai_linear_i8_launch; not the reference's):
+        // the weight is rounded once per upload, with a scale per output channel,
+        // rows of the input in each forward. The weight slot takes fp32 or fp16 as
+        // ever; splitSize and an accumulator dtype do not apply.
+        bool int8Weights = false;
     } config_;
 
     explicit Linear(Config config);
@@ -81,7 +86,10 @@ private:
     uint32_t M_ = 0, biasRepeat_ = 0, residualRepeat_ = 0;
     std::string plan_;
     uint32_t splitCount_ = 1;
+    PooledBuffer codes_, scales_;      // int8Weights: the rounded weight
     vai_linear_args args(bool withPointers) const;
+    vai_linear_i8_args i8Args(bool withPointers) const;
+    void prepareI8();
     bool packedMatches(const vai_linear_args& a) const;
 };
 
@@ -188,6 +196,8 @@ private:
 // the kernels run, so a recorded forward follows it). Each forward appends
 // its Tkv new K / V rows after the cached ones and attends both; K / V may
 // stay unwired (Tkv = 0) to attend the cache alone. One sequence only.
+// A Q4 cache's slots hold the library's own layout, [numKVHeads, 4-byte words];
+// vai_attention_cache_read gives its values.
 // "partialO" holds the workspace (fp16 K / V copies, key-split partials)
 // when a launch needs one.
 class Attention : public Node
@@ -198,7 +208,7 @@ public:
         uint32_t numQHeads;
         uint32_t numKVHeads = 0;              // for GQA (Hkv < numQHeads); 0: numQHeads
         uint32_t kvCacheSize = 0;             // tokens the cache holds; 0: no cache at all
-        Dtype kvCacheDtype = Dtype::None;     // required with a cache
+        Dtype kvCacheDtype = Dtype::None;     // required with a cache: Fp32, Fp16 or Q4 (4 bits, headDim <= 256)
         bool kvCacheRing = false;             // keep the last kvCacheSize positions (rounded up to kvRingAlign)
     } config_;
     static constexpr uint32_t kvRingAlign = 256;
@@ -221,6 +231,43 @@ private:
     const uint32_t* kvCacheCounter_ = nullptr;
     uint32_t batch_ = 1, tq_ = 0, tkv_ = 0;
     CausalMask mask_;
+};
+
+// From a fused query / key / value projection to what Attention takes: the RMS
+// norm of each query and key head, the position rotation, and token-major rows
+// to head-major planes, in one pass (vai_qk_norm_rope_launch; not the
+// reference's). in0 [..., T, (numQHeads + 2 numKVHeads) headDim] fp32 or fp16;
+// "Q" [..., numQHeads, T, headDim], "K" and "V" [..., numKVHeads, T, headDim] in
+// the node's output dtype. "q_weight" / "k_weight" [headDim] (one dtype; left
+// unset: no factor) and "inv_freq" [rotDim / 2] fp32 (left unset: theta's powers)
+// are optional. Token t of each sequence is at position *counter + t: the counter
+// is a device-readable uint32, read when the kernel runs (the one that
+// Attention::setKvCacheCounter takes serves both); never set, it counts from 0.
+class QkNormRope : public Node
+{
+public:
+    enum class Pairs : uint32_t { None = VAI_ROPE_NONE, Halves = VAI_ROPE_HALVES, Neighbours = VAI_ROPE_NEIGHBOURS };
+    struct Config {
+        uint32_t headDim;
+        uint32_t numQHeads;
+        uint32_t numKVHeads = 0;              // 0: numQHeads
+        bool norm = true;
+        float eps = 1e-6f;
+        float weightOffset = 0.0f;            // added to the weights
+        Pairs pairs = Pairs::Halves;          // which values a rotation pairs; None: no rotation
+        uint32_t rotDim = 0;                  // rotated values of a head; 0: headDim
+        float theta = 10000.0f;
+    } config_;
+
+    explicit QkNormRope(Config config);
+    void prepare() override;
+    void run(CommandStream& cmd) override;
+    const char* kind() const override { return "QkNormRope"; }
+    void setPositionCounter(const uint32_t* counter);
+
+private:
+    const uint32_t* counter_ = nullptr;
+    uint32_t batch_ = 1, tokens_ = 0;
 };
 
 }   // namespace node

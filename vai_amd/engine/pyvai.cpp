@@ -96,7 +96,7 @@ PYBIND11_MODULE(_pyvai, m)
 {
     m.doc() = "vai_amd engine: NeuralNet / Tensor / nodes on MI355X kernels";
 
-    py::enum_<Dtype>(m, "Dtype").value("F32", Dtype::Fp32).value("F16", Dtype::Fp16);
+    py::enum_<Dtype>(m, "Dtype").value("F32", Dtype::Fp32).value("F16", Dtype::Fp16).value("Q4", Dtype::Q4);
     py::enum_<Epilogue>(m, "Epilogue")
         .value("NONE", Epilogue::None).value("RELU", Epilogue::Relu).value("GELU", Epilogue::Gelu)
         .value("GELU_TANH", Epilogue::GeluTanh).value("SILU", Epilogue::Silu).value("SIGMOID", Epilogue::Sigmoid);
@@ -163,8 +163,9 @@ PYBIND11_MODULE(_pyvai, m)
     auto nodes = m.def_submodule("nodes");
     py::class_<node::Linear, Node>(nodes, "LinearNode")
         .def(py::init([](uint32_t in_dim, uint32_t out_dim, bool accept_residual, ResidualOrder residual_order,
-                         Epilogue epilogue, float scalar_scale, uint32_t split_size) {
+                         Epilogue epilogue, float scalar_scale, uint32_t split_size, bool int8_weights) {
                  node::Linear::Config c{in_dim, out_dim};
+                 c.int8Weights = int8_weights;
                  c.acceptResidual = accept_residual;
                  c.residualOrder = residual_order;
                  c.epilogue = epilogue;
@@ -174,11 +175,28 @@ PYBIND11_MODULE(_pyvai, m)
              }),
              py::arg("in_dim"), py::arg("out_dim"), py::arg("accept_residual") = false,
              py::arg("residual_order") = ResidualOrder::AfterEpilogue, py::arg("epilogue") = Epilogue::None,
-             py::arg("scalar_scale") = 1.0f, py::arg("split_size") = 0)
+             py::arg("scalar_scale") = 1.0f, py::arg("split_size") = 0, py::arg("int8_weights") = false)
         .def_property_readonly("plan", &node::Linear::plan)
         .def_property_readonly("split_count", &node::Linear::splitCount)
         .def_property_readonly("fused", [](node::Linear& l) { return l.fusedGate() != nullptr; })
         .def("has_bias", &node::Linear::hasBias);
+    py::enum_<node::QkNormRope::Pairs>(nodes, "RopePairs")
+        .value("NONE", node::QkNormRope::Pairs::None).value("HALVES", node::QkNormRope::Pairs::Halves)
+        .value("NEIGHBOURS", node::QkNormRope::Pairs::Neighbours);
+    py::class_<node::QkNormRope, Node>(nodes, "QkNormRopeNode")
+        .def(py::init([](uint32_t num_q_heads, uint32_t head_dim, uint32_t num_kv_heads, bool norm, float eps,
+                         float weight_offset, node::QkNormRope::Pairs pairs, uint32_t rot_dim, float theta) {
+                 node::QkNormRope::Config c{.headDim = head_dim, .numQHeads = num_q_heads, .numKVHeads = num_kv_heads,
+                                            .norm = norm, .eps = eps, .weightOffset = weight_offset, .pairs = pairs,
+                                            .rotDim = rot_dim, .theta = theta};
+                 return std::make_unique<node::QkNormRope>(c);
+             }),
+             py::arg("num_q_heads"), py::arg("head_dim"), py::arg("num_kv_heads") = 0, py::arg("norm") = true,
+             py::arg("eps") = 1e-6f, py::arg("weight_offset") = 0.0f, py::arg("pairs") = node::QkNormRope::Pairs::Halves,
+             py::arg("rot_dim") = 0, py::arg("theta") = 10000.0f)
+        .def("set_position_counter", [](node::QkNormRope& n, uintptr_t ptr) {
+                 n.setPositionCounter(reinterpret_cast<const uint32_t*>(ptr));
+             }, py::arg("device_ptr"));
     py::class_<node::GatedMul, Node>(nodes, "GatedMulNode")
         .def(py::init([](Epilogue activation) {
                  return std::make_unique<node::GatedMul>(node::GatedMul::Config{activation});

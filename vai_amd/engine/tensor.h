@@ -20,7 +20,8 @@ namespace vai {
 class NeuralNet;
 
 // /root/reference/vai/engine/tensor.h:19
-enum class Dtype { Fp32, Fp16, None };
+// (Q4, a KV cache in 4 bits, is a cache's alone: Attention::Config::kvCacheDtype)
+enum class Dtype { Fp32, Fp16, None, Q4 };
 
 constexpr size_t bytesPerElement(Dtype dt) noexcept
 {
@@ -28,6 +29,7 @@ constexpr size_t bytesPerElement(Dtype dt) noexcept
     case Dtype::Fp16: return 2;
     case Dtype::Fp32: return 4;
     case Dtype::None: return 0;
+    case Dtype::Q4: return 0;
     }
     return 4;
 }
@@ -52,7 +54,11 @@ class TensorData
     std::pair<NeuralNet*, uint64_t> lastSubmission_{nullptr, 0};
 
 public:
-    explicit TensorData(Dtype dt = Dtype::Fp32) : dtype_(dt) { VAI_ASSERT(dt != Dtype::None); }
+    explicit TensorData(Dtype dt = Dtype::Fp32) : dtype_(dt)
+    {
+        VAI_ASSERT(dt != Dtype::None);
+        require(dt != Dtype::Q4, "a tensor has no 4-bit dtype (a KV cache has: Attention::Config::kvCacheDtype)");
+    }
 };
 
 class Tensor
