@@ -185,3 +185,20 @@ def test_replayed_graph_follows_the_counter(gpu):
         graph.launch()
         stream.synchronize()
         check((q.numpy(), k.numpy(), v.numpy()), *want64(qkv, hq, hkv, d, pos=np.array([[c]])))
+
+
+@pytest.mark.parametrize("d", [1, 2, 7, 18, 33, 66, 100, 127, 250, 495, 497])
+@pytest.mark.parametrize("pairs", ["HALVES", "NEIGHBOURS"])
+def test_odd_head_dims_and_rotated_parts(gpu, d, pairs):
+    """Parts of a lane's eight values: every remainder of the rotated part, and of what follows it."""
+    rng = np.random.default_rng(d)
+    T, hq, hkv = 3, 3, 2
+    qkv = draw((2, T, (hq + 2 * hkv) * d), rng, F16)
+    qw, kw = (draw((d,), rng, F16) for _ in range(2))
+    pos = rng.integers(0, 5000, (2, T)).astype(np.uint32)
+    for rot in sorted({2, 4, 6, 10, 12, 14, 16, d // 2 * 2, d // 4 * 2, d // 3 * 2} & set(range(2, d + 1, 2))):
+        print(f"norm_rope odd d={d} rot={rot} {pairs}", flush=True)
+        got = run(gpu, qkv, hq, hkv, d, F16, q_weight=qw, k_weight=kw, pairs=pairs, rot_dim=rot, positions=pos)
+        check(got, *want64(qkv, hq, hkv, d, qw, kw, pairs=pairs, rot=rot, pos=pos))
+    got = run(gpu, qkv, hq, hkv, d, F16, q_weight=qw, k_weight=kw, pairs="NONE", positions=pos)
+    check(got, *want64(qkv, hq, hkv, d, qw, kw, pairs="NONE", pos=pos))

@@ -35,7 +35,7 @@ __device__ __forceinline__ void turn_of(const QkNormRopeParams& p, uint32_t pos,
     c = k == 1 || k == 2 ? -b : b;
 }
 
-// Any head dim: a wave takes one head at a time, in LDS as fp32.
+// Larger head dims: a wave takes one head at a time, in LDS as fp32.
 __global__ __launch_bounds__(64) void qk_norm_rope_any_kernel(QkNormRopeParams p)
 {
     __shared__ float y[QkNormRopeParams::MAX_DIM];
@@ -98,43 +98,69 @@ __device__ __forceinline__ float group_sum(float x)
     return x;
 }
 
-// Head dims that are a multiple of 8, up to 512, rotated in whole groups of 8:
-// L lanes (D / 8 rounded up to a power of two) share a head, 8 values each, cut
-// so that a lane holds both values of its four pairs: with halves values 4 j ..
-// +3 and the same of the other half, else 8 neighbouring ones. A lane's four
-// angles then serve every head of the token. A wave takes a token's heads 64 / L
-// at a time, its share of them (blockIdx.y of `shares`). One step's loads at a
-// time and 44 registers: eight waves a SIMD hide the loads better than four
-// steps at a time in 72 registers do. 4096 tokens of 32 + 8 + 8 fp16 heads of
-// 128: 20.4 us (23.8 with four steps at a time), 4.9 TB/s, where a large copy
-// makes 5.2; a single token's 3.9 us are latency (the smallest kernels here take 2.3).
-__device__ __forceinline__ float4v weight4(const void* w, int dt, uint32_t d)
+// Head dims up to 512: L lanes share a head, 8 values each, cut so that a lane
+// holds both values of its four pairs: with halves values 4 j ..+3 and the same of
+// the other half, else (and past the rotated values) 8 neighbouring ones. Where a
+// half is no multiple of 4, or what is left none of 8, a lane's last values do not
+// exist (na, nb of its two groups of four do; FULL: all). A lane's four angles serve every
+// head of the token. A wave takes a token's heads 64 / L at a time, its share of
+// them (blockIdx.y of `shares`). One step's loads at a time and 44 registers:
+// eight waves a SIMD hide the loads better than four steps at a time in 72
+// registers do. 4096 tokens of 32 + 8 + 8 fp16 heads of 128: 20.4 us (23.8 with
+// four steps at a time), 4.9 TB/s, where a large copy makes 5.2; a single token's
+// 3.9 us are latency (the smallest kernels here take 2.3).
+// n of 4 values at any alignment of their type, zeros for the rest (FULL: 4)
+template <bool FULL, typename T>
+__device__ __forceinline__ float4v some4(const T* p, uint32_t n)
 {
-    typedef half4 half4u __attribute__((aligned(2)));
-    if (dt == DT_F16) return __builtin_convertvector(*(const half4u*)((const half_t*)w + d), float4v);
-    return load4f((const float*)w + d);
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    typedef t4 t4u __attribute__((aligned(sizeof(T))));
+    if (FULL || n == 4) return __builtin_convertvector(*(const t4u*)p, float4v);
+    float4v v = (float4v)0.f;
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if ((uint32_t)e < n) v[e] = (float)p[e];
+    return v;
+}
+template <bool FULL, typename T>
+__device__ __forceinline__ void put4(T* p, uint32_t n, float4v v)
+{
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    typedef t4 t4u __attribute__((aligned(sizeof(T))));
+    if (FULL || n == 4) *(t4u*)p = __builtin_convertvector(v, t4);
+    else
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if ((uint32_t)e < n) p[e] = (T)v[e];
+}
+__device__ __forceinline__ float4v weight4(const void* w, int dt, uint32_t d, uint32_t n)
+{
+    return dt == DT_F16 ? some4<false>((const half_t*)w + d, n) : some4<false>((const float*)w + d, n);
 }
 
-template <typename TI, typename TO, int L>
+template <typename TI, typename TO, int L, bool FULL>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, uint32_t shares, uint32_t steps)
 {
-    typedef TI in4 __attribute__((ext_vector_type(4)));
-    typedef TO out4 __attribute__((ext_vector_type(4)));
     constexpr int HPW = 64 / L;
     const uint32_t D = p.head_dim, heads = p.hq + 2 * p.hkv, nk = p.hq + p.hkv, lane = threadIdx.x & 63;
     const uint32_t j = lane % L, sub = lane / L, half = p.rot_dim / 2;
-    const bool on = 8 * j < D, turned = 8 * j < p.rot_dim, split = turned && !p.neighbours;
-    const uint32_t oa = !on ? 0u : split ? 4 * j : 8 * j, ob = split ? oa + half : on ? oa + 4 : 0u;
+    const uint32_t turners = (p.neighbours ? p.rot_dim + 7 : 2 * half + 6) / 8;   // lanes with pairs
+    const bool turned = j < turners, split = turned && !p.neighbours;
+    // (neighbours: 8 values a lane throughout, pairs past rot_dim stay)
+    const uint32_t base = p.neighbours || turned ? 8 * j : p.rot_dim + 8 * (j - turners);
+    const uint32_t oa = split ? 4 * j : base, ob = split ? oa + half : base + 4, lim = split ? half : D;
+    const uint32_t na = oa < lim ? min(4u, lim - oa) : 0u, nb = split ? na : ob < D ? min(4u, D - ob) : 0u;
+    const bool on = na != 0;   // (a lane past the head's last value loads its first ones where FULL, and drops them)
     const uint32_t first_pos = p.count ? *p.count : 0u, rows = p.batch * p.tokens;
     const float inv_d = 1.0f / (float)D;
     float4v wq[2] = {(float4v)1.0f, (float4v)1.0f}, wk[2] = {(float4v)1.0f, (float4v)1.0f};
     if (p.q_weight) {
-        wq[0] = weight4(p.q_weight, p.w_dtype, oa) + p.weight_offset;
-        wq[1] = weight4(p.q_weight, p.w_dtype, ob) + p.weight_offset;
+        wq[0] = weight4(p.q_weight, p.w_dtype, oa, na) + p.weight_offset;
+        wq[1] = weight4(p.q_weight, p.w_dtype, ob, nb) + p.weight_offset;
     }
     if (p.k_weight) {
-        wk[0] = weight4(p.k_weight, p.w_dtype, oa) + p.weight_offset;
-        wk[1] = weight4(p.k_weight, p.w_dtype, ob) + p.weight_offset;
+        wk[0] = weight4(p.k_weight, p.w_dtype, oa, na) + p.weight_offset;
+        wk[1] = weight4(p.k_weight, p.w_dtype, ob, nb) + p.weight_offset;
     }
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t s0 = steps * blockIdx.y / shares, s1 = steps * (blockIdx.y + 1) / shares;
@@ -145,7 +171,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, u
         bool angles = false;
         for (uint32_t it = s0; it < s1; ++it) {
             const uint32_t h = it * HPW + sub, hc = min(h, heads - 1);
-            const in4 xa = *(const in4*)(row + (size_t)hc * D + oa), xb = *(const in4*)(row + (size_t)hc * D + ob);
+            const float4v xa = some4<FULL>(row + (size_t)hc * D + (FULL && !on ? 0u : oa), na);
+            const float4v xb = some4<FULL>(row + (size_t)hc * D + (FULL && !on ? 0u : ob), nb);
             if (!angles) {   // (under the first loads)
                 angles = true;
                 const uint32_t pos = p.positions ? p.positions[bt] : first_pos + t;
@@ -153,18 +180,18 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, u
                 for (int i = 0; i < 4; ++i) {
                     c[i] = 1.f;
                     s[i] = 0.f;
-                    if (turned) turn_of(p, pos, 4 * j + i, c[i], s[i]);
+                    if (2 * (4 * j + i) < p.rot_dim) turn_of(p, pos, 4 * j + i, c[i], s[i]);
                 }
             }
             float y[8], sq = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                y[e] = (float)xa[e];
-                y[4 + e] = (float)xb[e];
+                y[e] = xa[e];
+                y[4 + e] = xb[e];
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) sq = fmaf(y[e], y[e], sq);
-            sq = group_sum<L>(on ? sq : 0.f);
+            sq = group_sum<L>(FULL && !on ? 0.f : sq);
             const bool is_q = h < p.hq, is_v = h >= nk;
             if (p.norm && !is_v) {
                 const float inv = __builtin_amdgcn_rsqf(sq * inv_d + p.eps);
@@ -188,14 +215,14 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, u
             const uint32_t oh = is_q ? h : is_v ? h - nk : h - p.hq, nh = is_q ? p.hq : p.hkv;
             if (on && h < heads && out) {
                 TO* dst = out + (((size_t)b * nh + oh) * p.tokens + t) * D;
-                *(out4*)(dst + oa) = __builtin_convertvector((float4v{y[0], y[1], y[2], y[3]}), out4);
-                *(out4*)(dst + ob) = __builtin_convertvector((float4v{y[4], y[5], y[6], y[7]}), out4);
+                put4<FULL>(dst + oa, na, float4v{y[0], y[1], y[2], y[3]});
+                put4<FULL>(dst + ob, nb, float4v{y[4], y[5], y[6], y[7]});
             }
         }
     }
 }
 
-template <typename TI, typename TO, int L>
+template <typename TI, typename TO, int L, bool FULL>
 static hipError_t launch_vec(const QkNormRopeParams& p, hipStream_t s)
 {
     // tokens whose waves alone fill the chip are not shared out: each share takes
@@ -203,20 +230,21 @@ static hipError_t launch_vec(const QkNormRopeParams& p, hipStream_t s)
     const uint32_t steps = (p.hq + 2 * p.hkv + 64 / L - 1) / (64 / L);
     const uint32_t rows = p.batch * p.tokens;
     const uint32_t shares = std::min(steps, std::max(1u, 4096 / rows));
-    hipLaunchKernelGGL((qk_norm_rope_kernel<TI, TO, L>), dim3(std::min((rows + 3) / 4, 1u << 20), shares), dim3(256), 0, s,
+    hipLaunchKernelGGL((qk_norm_rope_kernel<TI, TO, L, FULL>), dim3(std::min((rows + 3) / 4, 1u << 20), shares), dim3(256), 0, s,
                        p, shares, steps);
     return hipGetLastError();
 }
 
-template <typename TI, typename TO>
+template <typename TI, typename TO, bool FULL>
 static hipError_t launch_lanes(const QkNormRopeParams& p, hipStream_t s)
 {
-    const uint32_t l = p.head_dim / 8;
-    if (l <= 4) return launch_vec<TI, TO, 4>(p, s);
-    if (l <= 8) return launch_vec<TI, TO, 8>(p, s);
-    if (l <= 16) return launch_vec<TI, TO, 16>(p, s);
-    if (l <= 32) return launch_vec<TI, TO, 32>(p, s);
-    return launch_vec<TI, TO, 64>(p, s);
+    const uint32_t l = p.neighbours || !p.rot_dim ? (p.head_dim + 7) / 8
+                                                  : (p.rot_dim + 6) / 8 + (p.head_dim - p.rot_dim + 7) / 8;
+    if (l <= 4) return launch_vec<TI, TO, 4, FULL>(p, s);
+    if (l <= 8) return launch_vec<TI, TO, 8, FULL>(p, s);
+    if (l <= 16) return launch_vec<TI, TO, 16, FULL>(p, s);
+    if (l <= 32) return launch_vec<TI, TO, 32, FULL>(p, s);
+    return launch_vec<TI, TO, 64, FULL>(p, s);
 }
 
 hipError_t qk_norm_rope_launch(QkNormRopeParams p, float theta, hipStream_t s)
@@ -228,14 +256,17 @@ hipError_t qk_norm_rope_launch(QkNormRopeParams p, float theta, hipStream_t s)
         for (uint32_t a = 0; 16 * a < p.rot_dim / 2; ++a) p.turn_hi[a] = std::exp2(16.0 * a * step);
         for (uint32_t b = 0; b < 16; ++b) p.turn_lo[b] = std::exp2(b * step) * 0.15915494309189533577;
     }
-    // four values at a time from every row of every plane
-    const size_t isz = p.i_dtype == DT_F16 ? 8 : 16, osz = p.o_dtype == DT_F16 ? 8 : 16;
-    const uintptr_t outs = (uintptr_t)p.q_out | (uintptr_t)p.k_out | (uintptr_t)p.v_out;
-    if (p.head_dim % 8 == 0 && p.head_dim <= 512 && p.rot_dim % 8 == 0 && p.row_stride % 4 == 0 &&
-        (uintptr_t)p.qkv % isz == 0 && outs % osz == 0) {
-        if (p.i_dtype == DT_F16)
-            return p.o_dtype == DT_F16 ? launch_lanes<half_t, half_t>(p, s) : launch_lanes<half_t, float>(p, s);
-        return p.o_dtype == DT_F16 ? launch_lanes<float, half_t>(p, s) : launch_lanes<float, float>(p, s);
+    // whole groups of four values everywhere (the tests for others cost a third:
+    // 4096 tokens 33.7 us with them, 23.3 without)
+    const bool full = p.head_dim % 8 == 0 && p.rot_dim % 8 == 0;
+    if (p.head_dim <= (full ? 512 : 496)) {   // 64 lanes hold a head (with one more where both parts are odd)
+        const auto go = [&](auto in, auto out) {
+            typedef decltype(in) TI;
+            typedef decltype(out) TO;
+            return full ? launch_lanes<TI, TO, true>(p, s) : launch_lanes<TI, TO, false>(p, s);
+        };
+        if (p.i_dtype == DT_F16) return p.o_dtype == DT_F16 ? go(half_t{}, half_t{}) : go(half_t{}, float{});
+        return p.o_dtype == DT_F16 ? go(float{}, half_t{}) : go(float{}, float{});
     }
     const uint64_t units = (uint64_t)p.batch * p.tokens * (p.hq + 2 * p.hkv);
     hipLaunchKernelGGL(qk_norm_rope_any_kernel, dim3((uint32_t)std::min<uint64_t>(units, 65536)), dim3(64), 0, s, p);
