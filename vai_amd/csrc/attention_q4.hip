@@ -42,8 +42,8 @@ __device__ __forceinline__ void q4_values8(const uint8_t* head, uint32_t dp, uin
 {
     const uint32_t j = row % q4::KT, d = 8 * c;
     const uint8_t* tile = head + (size_t)(row / q4::KT) * q4::tile_bytes(dp);
-    const half_t* sm = (const half_t*)(tile + (is_v ? q4::v_scale(dp, j, d) : q4::k_scale(dp, j, d)));
-    const float s = (float)sm[0], m = (float)sm[is_v ? 8 : 1];
+    const float s = (float)*(const half_t*)(tile + (is_v ? q4::v_scale(dp, j, d) : q4::k_step(dp, j, d)));
+    const float m = (float)*(const half_t*)(tile + (is_v ? q4::v_scale(dp, j, d) + 16 : q4::k_min(dp, j, d)));
     uint32_t w = 0;
     if (is_v) {
 #pragma unroll
@@ -126,8 +126,8 @@ __global__ __launch_bounds__(256) void q4_copy_kernel(AttnParams p, half_t* k16,
             for (uint32_t e = t - 128; e < q4::KT * DP / 8; e += 128) {
                 const uint32_t j = e / (DP / 8), c = e % (DP / 8);
                 const uint32_t w = *(const uint32_t*)(kt + q4::k_word(DP, j, 8 * c));
-                const half_t* sm = (const half_t*)(kt + q4::k_scale(DP, j, 8 * c));
-                const float s = bad[round][j] ? __builtin_nanf("") : (float)sm[0], m = (float)sm[1];
+                const float s = bad[round][j] ? __builtin_nanf("") : (float)*(const half_t*)(kt + q4::k_step(DP, j, 8 * c));
+                const float m = (float)*(const half_t*)(kt + q4::k_min(DP, j, 8 * c));
                 typedef half8 half8u __attribute__((aligned(2)));
                 half8 x;
 #pragma unroll

@@ -12,16 +12,22 @@
 // 0 .. 15 is n * 2^-24, and the cores multiply such numbers exactly, so one step
 // of 32 head-dim values (a group) gives 2^-24 sum n q from masked nibbles alone,
 // and a score is
-//   scale * sum over groups of (s * sum n q + m * sum q),
-// in fp32 from there on: K is never rounded. V enters as s n + m rounded to fp16
-// (one packed fma from the exact n), the probabilities as two fp16 numbers (the
-// second the rest that the first leaves), so that V's and the result's are the
-// only roundings to fp16: error against 64 bits 3.0e-4 of the result, of which the
-// rounding of the result is 2.1e-4 (3.6e-4 with the probabilities in one number).
+//   scale * (sum over groups of s * sum n q + sum over groups of m * sum q):
+// the first sum in fp32, the second a product of its own of the minima with the
+// groups' sums of q (as two fp16 numbers each): K is never rounded. Nibbles that
+// stand 4 bits up are 16 n; their q is taken as q / 16. For that every row of q is
+// scaled by a power of two, so that its largest value lies in [512, 1024) and none
+// that counts is lost (fp16 holds what is 2^-25 of it). An fp32 q enters as two
+// fp16 numbers. V enters as s n + m rounded to fp16 (one packed fma from the exact
+// n), the probabilities as two fp16 numbers (the second the rest that the first
+// leaves), so that V's and the result's are the only roundings to fp16: error
+// against 64 bits 2.9e-4 of the result, of which the rounding of the result is
+// 2.1e-4 (3.6e-4 with the probabilities in one number).
 //
 // The call's own rows are rounded by the wave whose tile they are in, into that
 // tile in LDS (and into the cache): nothing waits for an append.
 #include <algorithm>
+#include <type_traits>
 
 #include "decode_range.h"
 #include "kernels.h"
@@ -71,13 +77,13 @@ __device__ __forceinline__ float swap_max16(float x)
 
 // DP: the padded head dim; NQ: 16-row query blocks. Grid: (units, row blocks x
 // hkv). p.k / p.v are the 4-bit planes.
-template <int DP, int NQ>
+template <int DP, int NQ, bool Q32>
 __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q4_decode_kernel(AttnDecodeParams p)
 {
     using namespace fd;
     using L = Q4Lds<DP>;
     constexpr int G = DP / 32, ND = DP / 16, D = L::D;   // groups; values of a lane's V slice
-    constexpr uint32_t NIB = 0x000f000fu;
+    constexpr uint32_t NIB = 0x000f000fu, NIB16 = 0x00f000f0u;
     extern __shared__ uint4v q4_lds[];
     LDS_AS uint8_t* lds = (LDS_AS uint8_t*)(LDS_AS void*)q4_lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -87,7 +93,8 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
     // query rows: row r of the KV head is query head hk g + r / tq, token r % tq
     // (loaded before the first copies: both are waited for in order)
     const uint32_t rows = p.rows, row0 = rb * p.rpb, rend = std::min(row0 + p.rpb, rows);
-    half8 qf[NQ][G];
+    typedef typename std::conditional<Q32, float8v, half8>::type q8;
+    q8 qraw[NQ][G];
     uint32_t tok[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
@@ -96,10 +103,10 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
         const size_t base = ((size_t)hk * rows + r) * HD;
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            const uint32_t d = 32 * i + 8 * g;
-            half8 v = (half8)(half_t)0;   // (HD is a multiple of 8)
-            if (d < HD) v = p.q_dtype == DT_F16 ? load8((const half_t*)p.q + base + d) : load8((const float*)p.q + base + d);
-            qf[q][i] = v;
+            const uint32_t d = 32 * i + 8 * g;   // (HD is a multiple of 8)
+            typedef q8 q8u __attribute__((aligned(sizeof(qraw[0][0][0]))));
+            qraw[q][i] = 0;
+            if (d < HD) qraw[q][i] = *(const q8u*)((const typename std::conditional<Q32, float, half_t>::type*)p.q + base + d);
         }
     }
     const Range R = range_of(p);
@@ -140,20 +147,43 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
 #pragma unroll
         for (int i = 0; i < D; ++i) copy(i);
 
-    // 2^-24 sum q over each group, of the row as the cores take it
-    float qs[NQ][G];
+    // the rows as the cores take them: qf (and ql, what fp16 leaves of an fp32 q),
+    // and the groups' sums in two numbers (quarter 0 the first, quarter 1 the second)
+    half8 qf[NQ][G], ql[Q32 ? NQ : 1][Q32 ? G : 1], qsum[NQ];
+    float down[NQ];   // undoes the row's power of two
     int64_t kbeg[NQ], kend[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
         kend[q] = std::min<int64_t>(p.mask.key_end_cached(tok[q], R.cached), R.live);
         kbeg[q] = p.mask.key_start_cached(tok[q], R.cached);
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf((float)qraw[q][i][e]));
+        top = swap_max32(swap_max16(top));
+        const int ex = top > 0.f && top < __builtin_inff() ? 10 - __builtin_amdgcn_frexp_expf(top) : 0;
+        down[q] = ldexpf(1.f, -ex);
+        qsum[q] = (half8)(half_t)0;
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            float s = 0.f;
+            float8v x = __builtin_convertvector(qraw[q][i], float8v);
+            float sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s += (float)qf[q][i][e];
-            s = swap_sum<16>(s, s);
-            qs[q][i] = swap_sum<32>(s, s) * 5.9604644775390625e-8f;
+            for (int e = 0; e < 8; ++e) {
+                x[e] = ldexpf(x[e], ex);
+                sum += x[e];
+            }
+            const float8v part = {1.f, 1.f, .0625f, .0625f, 1.f, 1.f, .0625f, .0625f};
+            qf[q][i] = __builtin_convertvector(x * part, half8);
+            if constexpr (Q32) {
+                const float8v rest = x * part - __builtin_convertvector(qf[q][i], float8v);
+                ql[q][i] = __builtin_convertvector(rest, half8);
+            }
+            sum = swap_sum<16>(sum, sum);
+            sum = swap_sum<32>(sum, sum);
+            const half_t hi = (half_t)sum;
+            qsum[q][i] = g == 0 ? hi : g == 1 ? (half_t)(sum - (float)hi) : (half_t)0.f;
         }
     }
     const int64_t kfirst = p.mask.key_start_cached(0, R.cached);   // no query sees a position before it
@@ -161,7 +191,7 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
     // (both bounds grow with the token)
     const int64_t all_beg = p.mask.key_start_cached(p.tq - 1, R.cached);
     const int64_t all_end = std::min<int64_t>(p.mask.key_end_cached(0, R.cached), R.live);
-    const float sc = p.scale * (1.4426950408889634f * 16777216.f);   // scores in log2 units
+    const float sl2 = p.scale * 1.4426950408889634f;   // scores in log2 units
 
     float m[NQ], l[NQ];
     float4v o[NQ][ND];
@@ -210,7 +240,7 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
         place = next_place(place);
 
         // S^T: lane (c16, g) holds query row c16 and positions 8 g + 4 t ..+3
-        float4v x[2][NQ];
+        float4v x[2][NQ], y[2][NQ];   // 2^-24 sum s sum n q, sum m sum q
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             uint32_t kw[G];
@@ -227,24 +257,27 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
                     for (int e = 0; e < 4; ++e) kw[i + e] = w[e];
                 }
             }
+            typedef half_t halfg __attribute__((ext_vector_type(G)));
+            const halfg mg = *(LDS_AS const halfg*)(kt + q4::k_min_offset(DP) + (t * 16 + c16) * (G * 2));
+            half8 ma = (half8)(half_t)0;
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) x[t][q] = (float4v)0.f;
+            for (int i = 0; i < G; ++i) ma[i] = mg[i];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                x[t][q] = (float4v)0.f;
+                y[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ma, qsum[q], (float4v)0.f, 0, 0, 0);
+            }
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                // (s, m) of rows 4 g ..+3
-                const uint4v ksm = *(LDS_AS const uint4v*)(kt + q4::scale_offset(DP) + ((i * 2 + t) * 16 + 4 * g) * 4);
-                const uint32_t w = kw[i];
-                const half8 n8 = __builtin_bit_cast(half8, uint4v{w & NIB, (w >> 4) & NIB, (w >> 8) & NIB, (w >> 12) & NIB});
+                const half4 ks = *(LDS_AS const half4*)(kt + q4::scale_offset(DP) + ((i * 2 + t) * 16 + 4 * g) * 2);   // rows 4 g ..+3
+                const uint32_t w = kw[i], u = w >> 8;
+                const half8 n8 = __builtin_bit_cast(half8, uint4v{w & NIB, w & NIB16, u & NIB, u & NIB16});
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {
-                    const float4v n = __builtin_amdgcn_mfma_f32_16x16x32_f16(n8, qf[q][i], (float4v)0.f, 0, 0, 0);
+                    float4v n = __builtin_amdgcn_mfma_f32_16x16x32_f16(n8, qf[q][i], (float4v)0.f, 0, 0, 0);
+                    if constexpr (Q32) n = __builtin_amdgcn_mfma_f32_16x16x32_f16(n8, ql[q][i], n, 0, 0, 0);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t both = ksm[r];   // (a bit cast of the element itself takes the vector's first)
-                        const half2v sm = __builtin_bit_cast(half2v, both);
-                        x[t][q][r] = fmaf((float)sm.x, n[r], x[t][q][r]);
-                        x[t][q][r] = fmaf((float)sm.y, qs[q][i], x[t][q][r]);
-                    }
+                    for (int r = 0; r < 4; ++r) x[t][q][r] = fmaf((float)ks[r], n[r], x[t][q][r]);
                 }
             }
         }
@@ -304,8 +337,9 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
             float v[8];
+            const float sc = sl2 * down[q];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = x[i >> 2][q][i & 3] * sc;
+            for (int i = 0; i < 8; ++i) v[i] = fmaf(x[i >> 2][q][i & 3], 16777216.f, y[i >> 2][q][i & 3]) * sc;
             if (j0 < all_beg || j0 + KT > all_end) {
                 const int lo = (int)std::min<int64_t>(std::max<int64_t>(kbeg[q] - j0, -1), KT + 1);
                 const int hi = (int)std::min<int64_t>(std::max<int64_t>(kend[q] - j0, -1), KT + 1);
@@ -342,7 +376,7 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 // 1024 + n or (high nibbles where they stand) 1024 + 16 n as bits, then n: exact
-                const uint32_t mask = h ? 0x00f000f0u : NIB;
+                const uint32_t mask = h ? NIB16 : NIB;
                 const uint4v b = uint4v{w0 & mask, (w0 >> 8) & mask, w1 & mask, (w1 >> 8) & mask} | (uint4v)0x64006400u;
                 const half8 k = __builtin_bit_cast(half8, b);
                 const half8 n = h ? __builtin_elementwise_fma(k, (half8)(half_t)0.0625f, (half8)(half_t)-64.f)
@@ -420,17 +454,17 @@ __global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q
     }
 }
 
-template <int DP, int NQ>
+template <int DP, int NQ, bool Q32>
 static hipError_t q4_decode_launch_t(const AttnDecodeParams& p, hipStream_t s)
 {
     constexpr int bytes = Q4Lds<DP>::template bytes<NQ>();
     static PerDevice lds_once;
     if constexpr (bytes > 64 * 1024) {
-        const hipError_t e = set_max_lds(lds_once, (const void*)attention_q4_decode_kernel<DP, NQ>, bytes);
+        const hipError_t e = set_max_lds(lds_once, (const void*)attention_q4_decode_kernel<DP, NQ, Q32>, bytes);
         if (e != hipSuccess) return e;
     }
     const dim3 grid(p.units, (p.rows + p.rpb - 1) / p.rpb * p.hkv);
-    hipLaunchKernelGGL((attention_q4_decode_kernel<DP, NQ>), grid, dim3(256), bytes, s, p);
+    hipLaunchKernelGGL((attention_q4_decode_kernel<DP, NQ, Q32>), grid, dim3(256), bytes, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.units == 1) return e;
     return attention_decode_merge_launch(p, DP, 1, s);
@@ -471,10 +505,18 @@ hipError_t q4_decode_launch(const AttnParams& a, void* ws, hipStream_t s)
     p.rows = a.dec_rows; p.rpb = a.dec_rpb; p.units = a.dec_units;
     p.ws_o = (float*)ws;
     p.ws_ml = (float*)ws + (size_t)a.hkv * a.dec_units * a.dec_rows * a.dp;
+    const bool one = p.rpb <= 16;
+    if (a.q_dtype == DT_F32) {
+        switch (a.dp) {
+        case 64: return one ? q4_decode_launch_t<64, 1, true>(p, s) : q4_decode_launch_t<64, 2, true>(p, s);
+        case 128: return one ? q4_decode_launch_t<128, 1, true>(p, s) : q4_decode_launch_t<128, 2, true>(p, s);
+        default: return q4_decode_launch_t<256, 1, true>(p, s);
+        }
+    }
     switch (a.dp) {
-    case 64: return p.rpb <= 16 ? q4_decode_launch_t<64, 1>(p, s) : q4_decode_launch_t<64, 2>(p, s);
-    case 128: return p.rpb <= 16 ? q4_decode_launch_t<128, 1>(p, s) : q4_decode_launch_t<128, 2>(p, s);
-    default: return q4_decode_launch_t<256, 1>(p, s);
+    case 64: return one ? q4_decode_launch_t<64, 1, false>(p, s) : q4_decode_launch_t<64, 2, false>(p, s);
+    case 128: return one ? q4_decode_launch_t<128, 1, false>(p, s) : q4_decode_launch_t<128, 2, false>(p, s);
+    default: return q4_decode_launch_t<256, 1, false>(p, s);
     }
 }
 

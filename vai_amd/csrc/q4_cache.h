@@ -14,7 +14,9 @@
 //      t is position 8 (r / 4) + 4 t + r % 4, so that the scores a lane receives,
 //      rows 4 g ..+3 of both halves, are 8 positions in a row. A word's nibbles 0,
 //      4, 1, 5, 2, 6, 3, 7 are its values in order: masking every fourth nibble
-//      gives the pairs of an fp16 operand. Then (s, m) as [i][t][r].
+//      gives the pairs of an fp16 operand. Then the steps as [i][t][r], as the
+//      lanes that hold the product's results take them, and the minima as
+//      [t][r][i], an operand of their own.
 //   V: 4 blocks of 8 positions, each 16 slices (dp / 16 values): byte (i, j) of
 //      a slice, 8 i + j, holds values 2 i (low) and 2 i + 1 (high) of position
 //      j: a word is 4 positions of the same two values, as the transposed
@@ -45,9 +47,14 @@ __host__ __device__ constexpr uint32_t k_word(uint32_t dp, uint32_t j, uint32_t 
 {
     return (((half_of(j) * 4 + ((d >> 3) & 3)) * 16 + row_of(j)) * (dp / 32) + (d >> 5)) * 4;
 }
-__host__ __device__ constexpr uint32_t k_scale(uint32_t dp, uint32_t j, uint32_t d)
+__host__ __device__ constexpr uint32_t k_step(uint32_t dp, uint32_t j, uint32_t d)
 {
-    return scale_offset(dp) + (((d >> 5) * 2 + half_of(j)) * 16 + row_of(j)) * 4;
+    return scale_offset(dp) + (((d >> 5) * 2 + half_of(j)) * 16 + row_of(j)) * 2;
+}
+__host__ __device__ constexpr uint32_t k_min_offset(uint32_t dp) { return scale_offset(dp) + dp * 2; }
+__host__ __device__ constexpr uint32_t k_min(uint32_t dp, uint32_t j, uint32_t d)
+{
+    return k_min_offset(dp) + ((half_of(j) * 16 + row_of(j)) * (dp / 32) + (d >> 5)) * 2;
 }
 __host__ __device__ constexpr uint32_t v_byte(uint32_t dp, uint32_t j, uint32_t d)
 {
@@ -139,8 +146,10 @@ __device__ __forceinline__ void put_k(P tile, uint32_t dp, uint32_t j, uint32_t 
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) w |= (codes >> (4 * e) & 15u) << (4 * nibble_of(e));
     store<uint32_t>(tile + k_word(dp, j, 8 * c), w);
-    if ((c & 3) == 0)
-        store<uint32_t>(tile + k_scale(dp, j, 8 * c), (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16);
+    if ((c & 3) == 0) {
+        store<uint16_t>(tile + k_step(dp, j, 8 * c), __builtin_bit_cast(uint16_t, s));
+        store<uint16_t>(tile + k_min(dp, j, 8 * c), __builtin_bit_cast(uint16_t, m));
+    }
 }
 template <class P>
 __device__ __forceinline__ void put_v(P tile, uint32_t dp, uint32_t j, uint32_t c, uint32_t codes, half_t s, half_t m)
