@@ -48,7 +48,11 @@ namespace {
 template <int DP> struct Q4Lds {
     static constexpr int TILE = (int)q4::tile_bytes(DP);      // one plane's tile
     static constexpr int COPIES = (TILE + 1023) / 1024;       // 1 KB copies, the last one partly
-    static constexpr int D = DP == 256 ? 3 : 4;               // tiles in flight a wave
+    // tiles in flight a wave: what a CU's waves have in flight together hides the
+    // latency. 128: two tiles and three workgroups a CU, 38.0 + 6.0 us (the merge
+    // of more shares) over 131072 positions, 32 heads over 8; four tiles and two
+    // workgroups 41.9 + 5.0
+    static constexpr int D = DP == 256 ? 3 : DP == 128 ? 2 : 4;
     static constexpr int WAVE = D * 2 * TILE;
     static constexpr int OROW = DP * 4 + 16;                  // bytes of an fp32 O row in the final exchange
     template <int NQ> static constexpr int bytes()
@@ -75,10 +79,16 @@ __device__ __forceinline__ float swap_max16(float x)
 
 }   // namespace
 
+// workgroups a CU, as registers allow
+constexpr int q4_resident(uint32_t dp, uint32_t nq, bool q32)
+{
+    return dp == 256 || nq == 2 ? 1 : dp == 128 && !q32 ? 3 : 2;
+}
+
 // DP: the padded head dim; NQ: 16-row query blocks. Grid: (units, row blocks x
 // hkv). p.k / p.v are the 4-bit planes.
 template <int DP, int NQ, bool Q32>
-__global__ __launch_bounds__(256, DP == 256 || NQ == 2 ? 1 : 2) void attention_q4_decode_kernel(AttnDecodeParams p)
+__global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_decode_kernel(AttnDecodeParams p)
 {
     using namespace fd;
     using L = Q4Lds<DP>;
@@ -486,7 +496,8 @@ void q4_decode_plan(AttnParams& p, uint32_t cus)
     p.dec_rpb = std::min<uint32_t>(p.dec_rows, dp == 256 ? 16 : 32);
     const uint32_t keys = p.span ? std::min<uint64_t>(p.kv_rows, (uint64_t)p.span + p.tq + 2 * fd::KT) : p.kv_rows;
     const uint32_t tiles = (keys + fd::KT - 1) / fd::KT, most = std::max<uint32_t>((tiles + fd::NW - 1) / fd::NW, 1);
-    const uint32_t blocks = p.hkv * ((p.dec_rows + p.dec_rpb - 1) / p.dec_rpb), wgs = dp == 256 || p.dec_rpb > 16 ? cus : 2 * cus;
+    const uint32_t blocks = p.hkv * ((p.dec_rows + p.dec_rpb - 1) / p.dec_rpb),
+                   wgs = cus * q4_resident(dp, p.dec_rpb > 16 ? 2 : 1, p.q_dtype == DT_F32);
     p.dec_units = std::min(std::min(std::max((wgs + blocks - 1) / blocks, 1u), most), AttnDecodeParams::MAX_UNITS);
 }
 
