@@ -305,3 +305,55 @@ def test_replayed_graph_follows_the_count(gpu, hq, tq, d):
         rows = [np.concatenate([h[:, :count], n], 1) for h, n in zip(hist, new)]
         want, tol = attend(q, *rows, visible(count, tq, tq, 0, 0), False)
         check(out.numpy()[0], want, tol)
+
+
+@pytest.mark.parametrize("d, hq, hkv, tq, xdt", [(64, 8, 2, 1, F16), (128, 8, 2, 3, F16), (128, 4, 4, 1, F32),
+                                                 (96, 16, 1, 2, F32), (256, 4, 2, 2, F16), (256, 4, 2, 1, F32)])
+def test_queries_of_any_magnitude(gpu, d, hq, hkv, tq, xdt):
+    """A query times a power of two under a scale divided by it: the same result bit
+    for bit (nothing under- or overflows: |q| >= 2^-6 or 0). A query of zeros: the mean of V."""
+    rng = np.random.default_rng(d + hq)
+    c = Cache(gpu, hkv, 320, d, False)
+    c.append(rng, 300)
+    q = draw((hq, tq, d), rng, xdt)
+    q = np.where(np.abs(q) < 2.0 ** -6, 0, q).astype(xdt)
+    q[1, 0] = 0
+    print(f"q4 magnitudes d={d} hq={hq} tq={tq} {xdt.__name__}", flush=True)
+    D = gpu.DeviceArray.from_numpy
+
+    def run(e):
+        out = gpu.DeviceArray((1, tq, hq, d), F32)
+        gpu.attention(out, D((q * xdt(2.0 ** e))[None]), None, None, causal=True, scale=2.0 ** -e / np.sqrt(d),
+                      cache=(c.k, c.v, c.count, False))
+        return out.numpy()[0]
+
+    got = run(0)
+    check(got, *attend(q, *c.rows, visible(300, tq, 0, 0, 0), xdt == F32))
+    for e in (-4, 8) if xdt == F16 else (-60, -20, 30, 100):
+        np.testing.assert_array_equal(run(e), got)
+
+
+@pytest.mark.parametrize("tq", [1, 40])
+def test_planes_past_32_bit_offsets(gpu, tq):
+    """The last rows of planes of 5 GB, behind a window."""
+    rng = np.random.default_rng(tq)
+    size, d, hkv = (1 << 26) + 64, 32, 2
+    c = Cache(gpu, hkv, size, d, False)
+    assert c.k.nbytes > 1 << 32
+    n0 = size - 300
+    c.set_count(n0)
+    print(f"q4 far rows tq={tq}", flush=True)
+    for m in (1, 200):   # appended by the attention itself, and by the append of a longer call
+        k, v = (draw((hkv, m, d), rng, F16) for _ in range(2))
+        c.call(draw((2, 1 if m == 1 else 20, d), rng, F16), k, v, span=1)
+    q, k, v = draw((4, tq, d), rng, F16), draw((hkv, tq, d), rng, F16), draw((hkv, tq, d), rng, F16)
+    got = c.call(q, k, v, F32, span=100)
+    n = 201 + tq
+    assert c.n == n0 + n
+    see = visible(201, tq, tq, 0, 100)
+    want, tol = attend(q, *c.rows, see, False)
+    check(got, want, tol)
+    outs = [gpu.DeviceArray((hkv, n, d), F32) for _ in range(2)]
+    gpu.attention_cache_read(*outs, c.k, c.v, n0)
+    for o, r in zip(outs, c.rows):
+        np.testing.assert_array_equal(o.numpy(), r.astype(F32))

@@ -62,7 +62,7 @@ __device__ __forceinline__ void q4_values8(const uint8_t* head, uint32_t dp, uin
 // of 8 values each). A hidden position must not reach a query through a NaN (0 *
 // NaN in P V), so a row with a NaN in V is copied as V = 0 and K = NaN: the score
 // is masked where the position is hidden and NaN where it is not.
-// 7513 positions of 8 heads of 128: 25 us with a wave to a row.
+// 7513 positions of 8 heads of 128: 16 us (25 with a wave to a row).
 template <int DP>
 __global__ __launch_bounds__(256) void q4_copy_kernel(AttnParams p, half_t* k16, half_t* v16)
 {

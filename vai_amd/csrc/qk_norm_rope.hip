@@ -98,17 +98,6 @@ __device__ __forceinline__ float group_sum(float x)
     return x;
 }
 
-// Head dims up to 512: L lanes share a head, 8 values each, cut so that a lane
-// holds both values of its four pairs: with halves values 4 j ..+3 and the same of
-// the other half, else (and past the rotated values) 8 neighbouring ones. Where a
-// half is no multiple of 4, or what is left none of 8, a lane's last values do not
-// exist (na, nb of its two groups of four do; FULL: all). A lane's four angles serve every
-// head of the token. A wave takes a token's heads 64 / L at a time, its share of
-// them (blockIdx.y of `shares`). One step's loads at a time and 44 registers:
-// eight waves a SIMD hide the loads better than four steps at a time in 72
-// registers do. 4096 tokens of 32 + 8 + 8 fp16 heads of 128: 20.4 us (23.8 with
-// four steps at a time), 4.9 TB/s, where a large copy makes 5.2; a single token's
-// 3.9 us are latency (the smallest kernels here take 2.3).
 // n of 4 values at any alignment of their type, zeros for the rest (FULL: 4)
 template <bool FULL, typename T>
 __device__ __forceinline__ float4v some4(const T* p, uint32_t n)
@@ -138,6 +127,17 @@ __device__ __forceinline__ float4v weight4(const void* w, int dt, uint32_t d, ui
     return dt == DT_F16 ? some4<false>((const half_t*)w + d, n) : some4<false>((const float*)w + d, n);
 }
 
+// Head dims up to 512: L lanes share a head, 8 values each, cut so that a lane
+// holds both values of its four pairs: with halves values 4 j ..+3 and the same of
+// the other half, else (and past the rotated values) 8 neighbouring ones. Where a
+// half is no multiple of 4, or what is left none of 8, a lane's last values do not
+// exist (na, nb of its two groups of four do; FULL: all). A lane's four angles
+// serve every head of the token. A wave takes a token's heads 64 / L at a time,
+// its share of them (blockIdx.y of `shares`). One step's loads at a time and 44
+// registers: eight waves a SIMD hide the loads better than four steps at a time in
+// 72 registers do. 4096 tokens of 32 + 8 + 8 fp16 heads of 128: 20.4 us (23.8 with
+// four steps at a time), 4.9 TB/s, where a large copy makes 5.2; a single token's
+// 3.9 us are latency (the smallest kernels here take 2.3).
 template <typename TI, typename TO, int L, bool FULL>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, uint32_t shares, uint32_t steps)
 {
