@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
     };
     uint32_t ahead = place0;   // the next copy's place, and how many were made
     int copied = 0;
-    const auto copy = [&](int slot) __attribute__((always_inline)) {   // past the last: it again, never read
+    const auto copy = [&](int slot) __attribute__((always_inline)) {
         LDS_AS uint8_t* dst = ring + slot * 2 * L::TILE;
 #pragma unroll
         for (int plane = 0; plane < 2; ++plane) {
@@ -152,11 +152,12 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
                     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LDS_AS void*)(dst + plane * L::TILE + c * 1024), 16,
                                                              c * 1024 + lane * 16, 0, 0, 0);
         }
-        if (++copied < mine) ahead = next_place(ahead);
+        ++copied;
+        ahead = next_place(ahead);
     };
-    if (mine > 0)
 #pragma unroll
-        for (int i = 0; i < D; ++i) copy(i);
+    for (int i = 0; i < D; ++i)
+        if (i < mine) copy(i);
 
     // the rows as the cores take them: qf (and ql, what fp16 leaves of an fp32 q),
     // and the groups' sums in two numbers (quarter 0 the first, quarter 1 the second)
@@ -217,7 +218,9 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
     uint32_t place = place0;
     int slot = 0;
     for (int it = 0; it < mine; ++it) {
-        q4_wait<(D - 1) * 2 * L::COPIES>();   // its copies have landed; the next tiles' may be in flight
+        // its copies have landed; the next tiles' may be in flight
+        if (it + D <= mine) q4_wait<(D - 1) * 2 * L::COPIES>();
+        else q4_wait<0>();
         const int64_t j0 = (first + (int64_t)it * step) * KT;
         LDS_AS uint8_t* kt = ring + slot * 2 * L::TILE;
         LDS_AS uint8_t* vt = kt + L::TILE;
@@ -305,7 +308,7 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
         LDS_AS const uint8_t* va = vt + q4::scale_offset(DP) + ((c16 * ND / 32) * 4 + g) * 32;
         half8 vs = *(LDS_AS const half8*)va, vm = *(LDS_AS const half8*)(va + 16);
         q4_wait_lds();         // read before the slot is copied over
-        copy(slot);
+        if (copied < mine) copy(slot);
         slot = slot + 1 == D ? 0 : slot + 1;
 
         // Positions that no query sees (stale rows, rows past the count) may hold
@@ -401,7 +404,6 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
             }
         }
     }
-    q4_wait<0>();   // (the copies past the last tile)
 
     // the waves' sums meet in LDS (the rings are done with); o[q][d] register r is
     // row c16, value (4 g + r) ND + d
