@@ -333,8 +333,10 @@ typedef struct {
      * shorter); a group keeps m = its minimum, s = fp16((max - m) / 15) and
      * codes n = round((x - m) / s) of 0 .. 15, and stands for s n + m (s the
      * fp16 number below where 15 s + m would leave fp16's range). Every
-     * key and value is attended as stored, the call's own among them, so the
-     * result does not depend on how a sequence was cut into calls. A group
+     * key and value is attended as stored, the call's own among them: what the
+     * cache holds does not depend on how a sequence was cut into calls. (More
+     * than 16 queries, 64 query rows of a KV head or 32 new keys, and head dims
+     * that are no multiple of 8, go over copies rounded to fp16.) A group
      * with a value that is not finite in fp16 is stored as NaN; a query that
      * sees a row with such a group in K or V is NaN, one it is hidden from is
      * not touched by it. Positions past the count may hold anything. A 4-bit
@@ -350,8 +352,8 @@ typedef struct {
 
 vai_status vai_attention_launch(const vai_attention_args* args, vai_stream_t stream);
 /* Bytes of workspace a launch needs: nonzero when fp32 K / V take the flash
- * kernel (their fp16 copies), or when the query tiles alone do not fill the
- * GPU and long key ranges are split over workgroups (partial results merged by
+ * kernel (their fp16 copies; those of a 4-bit cache where a call takes them),
+ * or when the query tiles alone do not fill the GPU and long key ranges are split over workgroups (partial results merged by
  * a second pass, the split-K of attention-fa-reduce.comp). */
 size_t vai_attention_workspace_size(const vai_attention_args* args);
 

@@ -229,3 +229,25 @@ def test_quantized_weight_serves_linear(gpu):
     # |ab - a'b'| <= |a| hb + |b| ha + ha hb, ha, hb half a step each
     bound = np.abs(x64).sum(1)[:, None] * hw.T + hx * np.abs(w64).sum(1)[None, :] + k * hx * hw.T
     assert (np.abs(got - x64 @ w64.T) <= 1.001 * bound).all()
+
+
+@pytest.mark.parametrize("n, k, xdt", [(300, 2048, F16), (300, 2049, F16), (515, 2730, F32), (16384, 96, F16),
+                                       (16400, 96, F16), (77, 8192, F32)])
+def test_rows_do_not_depend_on_their_number(gpu, n, k, xdt):
+    """The sums are integers, so a row's outputs are the same bits in calls of 1 to 200
+    rows: one launch or two, split over waves or in tiles."""
+    rng = np.random.default_rng(n + k)
+    x, (w, ws) = draw((200, k), rng, xdt), weight(rng, n, k)
+    D, lib = gpu.DeviceArray.from_numpy, gpu.lib()
+    dw, dws, outs = on_gpu(gpu, w), D(ws), {}
+    for m in (1, 2, 3, 4, 5, 16, 17, 40, 64, 70, 200):
+        out = gpu.DeviceArray((m, n), F32)
+        out.fill_(0xFF)
+        dx = D(x[:m])
+        need = lib.vai_linear_i8_workspace_size(ctypes.byref(gpu.linear_i8_args(out, dx, dw, dws)))
+        assert (need == 0) == (m <= 4 and m * k <= 8192 and n <= 16384 and n * k <= 1 << 26)
+        print(f"linear_i8 rows {m} x {n} x {k}", flush=True)
+        outs[m] = gpu.linear_i8(out, dx, dw, dws).numpy()
+    check(outs[200], *want64(x, w, ws), "NONE")
+    for m, o in outs.items():
+        np.testing.assert_array_equal(o, outs[200][:m])

@@ -710,7 +710,7 @@ static vai_status check_linear_i8(const vai_linear_i8_args* a)
 
 size_t vai_linear_i8_workspace_size(const vai_linear_i8_args* a)
 {
-    if (check_linear_i8(a) != VAI_OK || linear_i8_fused(a->M, a->K)) return 0;
+    if (check_linear_i8(a) != VAI_OK || linear_i8_fused(a->M, a->N, a->K)) return 0;
     return (size_t)a->M * i8_x_row(a->K) + (size_t)a->M * sizeof(float);
 }
 

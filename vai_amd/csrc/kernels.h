@@ -327,7 +327,7 @@ hipError_t quantize_i8_launch(void* out, float* scale, const void* in, int in_dt
                               uint32_t stride, hipStream_t s);
 hipError_t linear_i8_launch(const LinearI8Params& p, hipStream_t s);
 // Few rows and values of X: rounded in the product's own launch, no workspace.
-bool linear_i8_fused(uint32_t M, uint32_t K);
+bool linear_i8_fused(uint32_t M, uint32_t N, uint32_t K);
 hipError_t linear_i8_fused_launch(const LinearI8Params& p, const void* in, int in_dtype, hipStream_t s);
 // 256 x 256 (f = 4) or 128 x 128 (f = 2) tiles, for sizes where the matrix cores are the bound
 hipError_t linear_i8_big_launch(const LinearI8Params& p, int f, hipStream_t s);

@@ -199,8 +199,8 @@ __device__ __forceinline__ void few_wait_lds() { __builtin_amdgcn_s_waitcnt(15 |
 // flight, and no wave waits for another until the sums meet. Chunk c of slab row
 // r stands at chunk c ^ (r / 2 % 8): fragment reads hit every bank group once.
 // FUSED (MT = 1): X is rounded here, under the first copies of W, by every
-// workgroup for itself (NW / M waves share a row); else its codes come from the workspace,
-// through the ring like W.
+// workgroup for itself; else its codes come from the workspace, through the ring
+// like W.
 template <int MT, int NT, int NW, int D, bool FUSED> struct FewCfg {
     static constexpr int BLOCK = (NT + (FUSED ? 0 : MT)) * 2048;   // a block of K in LDS: 16-row slabs
     static constexpr int COPIES = BLOCK / 1024;
@@ -241,15 +241,16 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
                                                      (int)(slab_row * (w ? p.w_stride : p.x_stride) + ch * 16 + k), 0, 0, 0);
         }
     };
-    // FUSED: this wave's parts of its row of X, 1024 values every `share` of them
-    // (X before W: loads and copies are waited for in their order)
-    constexpr int KEEP = FUSED ? 4 : 1;
-    const uint32_t share = std::max<uint32_t>(NW / p.M, 1), part = wave % share;   // waves of a row
+    // FUSED (M <= 4, M K <= 8192): NW / M waves share a row of X, 1024 values at a
+    // time each, 3 times at most (X before W: loads and copies are waited for in
+    // their order)
+    constexpr int KEEP = FUSED ? 3 : 1;
+    const uint32_t share = std::max<uint32_t>(NW / p.M, 1), part = wave % share, row = wave / share;
     Raw16<TX> kept[KEEP];
     if constexpr (FUSED)
 #pragma unroll
         for (int i = 0; i < KEEP; ++i)
-            kept[i].load(in + (size_t)std::min<uint32_t>(wave / share, p.M - 1) * p.K, (i * share + part) * 1024 + lane * 16, p.K);
+            kept[i].load(in + (size_t)std::min<uint32_t>(row, p.M - 1) * p.K, (i * share + part) * 1024 + lane * 16, p.K);
     if (mine > 0)
 #pragma unroll
         for (int i = 0; i < D; ++i) copy(i);
@@ -259,48 +260,28 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
     LDS_AS float* sl = (LDS_AS float*)(xl + p.M * ls);
     if constexpr (FUSED) {
         LDS_AS uint32_t* ml = (LDS_AS uint32_t*)(sl + p.M);   // largest values, a part each
-        const uint32_t step = share * 1024, rest = KEEP * step + part * 1024 + lane * 16;
-        for (uint32_t m0f = 0; m0f < p.M; m0f += NW / share) {
-            const uint32_t m = m0f + wave / share;
-            const bool on = m < p.M;
-            const TX* x = in + (size_t)(on ? m : 0u) * p.K;
-            if (m0f > 0)   // (rows past the first of each wave)
+        uint32_t amax = 0;
 #pragma unroll
-                for (int i = 0; i < KEEP; ++i) kept[i].load(x, (i * share + part) * 1024 + lane * 16, p.K);
-            uint32_t amax = 0;
+        for (int i = 0; i < KEEP; ++i) {
+            float y[16];
+            kept[i].values(y);
+            amax = abs_max16(y, amax);
+        }
 #pragma unroll
-            for (int i = 0; i < KEEP; ++i) {
-                float y[16];
-                kept[i].values(y);
-                amax = abs_max16(y, amax);
-            }
-            for (uint32_t k = rest; k < p.K; k += step) {
-                float y[16];
-                row16(x, k, p.K, y);
-                amax = abs_max16(y, amax);
-            }
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) amax = std::max(amax, (uint32_t)__shfl_xor((int)amax, o));
-            if (share > 1) {   // (uniform: then every row is in this one pass)
-                if (lane == 0) ml[wave] = amax;
-                __syncthreads();
-                for (uint32_t w = 0; w < share; ++w) amax = std::max(amax, (uint32_t)ml[wave / share * share + w]);
-            }
+        for (int o = 32; o > 0; o >>= 1) amax = std::max(amax, (uint32_t)__shfl_xor((int)amax, o));
+        if (lane == 0) ml[wave] = amax;
+        __syncthreads();
+        for (uint32_t w = 0; w < share; ++w) amax = std::max(amax, (uint32_t)ml[wave / share * share + w]);
+        if (row < p.M) {
             const float s = row_scale(amax), inv = s > 0.f ? 1.0f / s : 0.f;
-            if (!on) continue;
-            if (part == 0 && lane == 0) sl[m] = s;
+            if (part == 0 && lane == 0) sl[row] = s;
 #pragma unroll
             for (int i = 0; i < KEEP; ++i) {
                 const uint32_t k = (i * share + part) * 1024 + lane * 16;
                 if (k >= p.x_stride) continue;
                 float y[16];
                 kept[i].values(y);
-                *(LDS_AS int4v*)(xl + m * ls + k) = inv > 0.f ? codes16(y, s, inv) : (int4v)0;
-            }
-            for (uint32_t k = rest; k < p.x_stride; k += step) {
-                float y[16];
-                row16(x, k, p.K, y);
-                *(LDS_AS int4v*)(xl + m * ls + k) = inv > 0.f ? codes16(y, s, inv) : (int4v)0;
+                *(LDS_AS int4v*)(xl + row * ls + k) = inv > 0.f ? codes16(y, s, inv) : (int4v)0;
             }
         }
         __syncthreads();
@@ -364,7 +345,7 @@ static hipError_t few_launch_t(const LinearI8Params& p, const void* in, hipStrea
     typedef FewCfg<MT, NT, NW, D, FUSED> C;
     static PerDevice once;
     auto kern = linear_i8_few_kernel<MT, NT, NW, D, TX, FUSED>;
-    constexpr int xmax = FUSED ? 40 * 1024 : 0;   // what linear_i8_fused allows
+    constexpr int xmax = FUSED ? 9 * 1024 : 0;   // more than linear_i8_fused allows
     if constexpr (C::RING + xmax > 64 * 1024) {
         const hipError_t e = set_max_lds(once, (const void*)kern, C::RING + xmax);
         if (e != hipSuccess) return e;
@@ -375,9 +356,17 @@ static hipError_t few_launch_t(const LinearI8Params& p, const void* in, hipStrea
     return hipGetLastError();
 }
 
-bool linear_i8_fused(uint32_t M, uint32_t K)
+// One launch in place of two where every workgroup can round X for itself at no
+// cost: the kernels' times are then alike and a launch's host time is saved
+// (one / two launches, us: 1 x 8192 x 2048 8.2 / 8.2, 1 x 16384 x 2048 8.8 / 9.3,
+// 4 x 16384 x 2048 8.2 / 10.0). Not with a wave for more than one row (8 x 4096 x
+// 1024 8.8 / 6.9, 16 x 4096 x 512 10.7 / 7.6), longer rows (4 x 4096 x 8192 13.6 /
+// 10.8), more workgroups than one round of the chip (1 x 32768 x 2048 19 / 16) or
+// weights of more than 64 MB, whose read the tiles' deeper copies carry better (1 x
+// 16384 x 8192 33 / 27, 1 x 8192 x 8192 22.9 / 24.4).
+bool linear_i8_fused(uint32_t M, uint32_t N, uint32_t K)
 {
-    return M <= 16 && (uint64_t)M * K <= 8192 && M * ((K + 127) / 128 * 128 + 20) + 64 <= 40 * 1024;
+    return M <= 4 && (uint64_t)M * K <= 8192 && N <= 16384 && (uint64_t)N * K <= 1u << 26;
 }
 
 // Wider workgroups where there are enough of them (M = 1, K = 2048, N = 8192, us:
