@@ -362,11 +362,11 @@ static hipError_t few_launch_t(const LinearI8Params& p, const void* in, hipStrea
 // 4 x 16384 x 2048 8.2 / 10.0). Not with a wave for more than one row (8 x 4096 x
 // 1024 8.8 / 6.9, 16 x 4096 x 512 10.7 / 7.6), longer rows (4 x 4096 x 8192 13.6 /
 // 10.8), more workgroups than one round of the chip (1 x 32768 x 2048 19 / 16) or
-// weights of more than 64 MB, whose read the tiles' deeper copies carry better (1 x
-// 16384 x 8192 33 / 27, 1 x 8192 x 8192 22.9 / 24.4).
+// weights from 64 MB on, which the 64-wide tiles read faster (below; 1 x 16384 x
+// 8192 33 / 27, 1 x 8192 x 8192 22.9 / 21.2).
 bool linear_i8_fused(uint32_t M, uint32_t N, uint32_t K)
 {
-    return M <= 4 && (uint64_t)M * K <= 8192 && N <= 16384 && (uint64_t)N * K <= 1u << 26;
+    return M <= 4 && (uint64_t)M * K <= 8192 && N <= 16384 && (uint64_t)N * K < 1u << 26;
 }
 
 // Wider workgroups where there are enough of them (M = 1, K = 2048, N = 8192, us:
@@ -378,21 +378,24 @@ hipError_t linear_i8_fused_launch(const LinearI8Params& p, const void* in, int i
     return in_dtype == DT_F16 ? few_launch_t<1, 2, 4, 4, half_t, true>(p, in, s) : few_launch_t<1, 2, 4, 4, float, true>(p, in, s);
 }
 
-// Up to 64 rows over up to 8192 columns the wave rings, whose workgroups are then
-// one round (us, rings / 64-wide tiles: 32 x 4096 x 4096 7.0 / 10.2, 61 x 5003 x
-// 1999 8.2 / 9.1; 16 and 64 x 16384 x 4096 13.5 and 25 / 12.2). Past that the
+// Up to 32 rows over up to 8192 columns, and 64 over 5120, the wave rings, whose
+// workgroups are then one round (us, rings / 64-wide tiles: 8 x 4096 x 8192 6.5 / 16,
+// 16 x 8192 x 4096 7.2 / 10.5, 32 x 4096 x 4096 7.0 / 10.2, 61 x 5003 x 1999 8.2 /
+// 9.1, 64 x 8192 x 2048 9.1 / 7.1; 16 and 64 x 16384 x 4096 13.5 and 25 / 12.2), and
+// weights that the L2s hold or nearly (16 x 6144 x 8192 16.2 / 15.9, 8 x 8192 x 8192
+// 20.0 / 16.5, 64 x 8192 x 8192 24.6 / 17.0). Past that the
 // tile whose modelled time is least: kt stages of 128 bytes of K, c tiles a CU.
 // Measured, us, 64-wide / 128-wide / 256-wide: 500 x 2048 x 2048 7.9 / 14.7 /
 // 32.7, 1000 x 4096 x 4096 28 / 25 / 57, 2048 x 4096 x 11008 137 / 90 / 135,
 // 4096^3 103 / 77 / 67.
 hipError_t linear_i8_launch(const LinearI8Params& p, hipStream_t s)
 {
-    if (p.N <= 8192) {
+    if (p.N <= 8192 && (uint64_t)p.N * p.K < 1u << 26) {
         if (p.M <= 16)
             return p.N <= 4096 ? few_launch_t<1, 1, 4, 4, half_t, false>(p, nullptr, s)
                                : few_launch_t<1, 2, 4, 4, half_t, false>(p, nullptr, s);
         if (p.M <= 32) return few_launch_t<2, 2, 4, 3, half_t, false>(p, nullptr, s);
-        if (p.M <= 64) return few_launch_t<4, 2, 4, 3, half_t, false>(p, nullptr, s);
+        if (p.M <= 64 && p.N <= 5120) return few_launch_t<4, 2, 4, 3, half_t, false>(p, nullptr, s);
     }
     int cus = 0;
     const hipError_t e = device_cus(&cus);
