@@ -7,7 +7,8 @@
 // in turn, each through a ring of its own in LDS: a tile's 20 dp bytes of K and of
 // V are copied there as they lie, D tiles in flight, and no wave waits for another
 // until the share ends. 131072 positions, 32 heads over 8 of 128: 38 us, 4.4 TB/s,
-// where a large copy makes 5.2; the VALU, which unpacks the codes, is busy for 60%.
+// where a large copy makes 5.2; waves wait for memory a quarter of their time, and
+// for an issue slot, the unpacking of each other's codes, a third.
 //
 // The codes enter the matrix cores as they are. An fp16 whose bits are a code n of
 // 0 .. 15 is n * 2^-24, and the cores multiply such numbers exactly, so one step
