@@ -357,3 +357,51 @@ def test_planes_past_32_bit_offsets(gpu, tq):
     gpu.attention_cache_read(*outs, c.k, c.v, n0)
     for o, r in zip(outs, c.rows):
         np.testing.assert_array_equal(o.numpy(), r.astype(F32))
+
+
+@pytest.mark.parametrize("d, tq", [(64, 1), (128, 5), (256, 2)])
+def test_ring_at_far_positions(gpu, d, tq):
+    """Positions past 2^31 in a ring of 256."""
+    rng = np.random.default_rng(d)
+    n0, hkv = 3_000_000_019, 2
+    c = Cache(gpu, hkv, 256, d, True)
+    c.set_count(n0)
+    print(f"q4 far ring d={d} tq={tq}", flush=True)
+    for _ in range(30):
+        k, v = (draw((hkv, 10, d), rng, F16) for _ in range(2))
+        c.call(draw((4, 1, d), rng, F16), k, v, span=1)   # (one query sees the last of them)
+    q, k, v = draw((4, tq, d), rng, F16), draw((hkv, tq, d), rng, F16), draw((hkv, tq, d), rng, F16)
+    got = c.call(q, k, v, F32, span=200)
+    assert c.n == n0 + 300 + tq
+    want, tol = attend(q, *c.rows, visible(300, tq, tq, 0, 200), False)
+    check(got, want, tol)
+
+
+def test_two_streams(gpu):
+    """Decode steps of two sequences, each on a stream of its own, in turn."""
+    rng = np.random.default_rng(3)
+    D, lib, d, hkv = gpu.DeviceArray.from_numpy, gpu.lib(), 128, 2
+    caches, calls, outs = [], [], []
+    for n in (2000, 77):
+        c = Cache(gpu, hkv, 2048, d, False)
+        c.append(rng, n)
+        q, k, v = (draw((h, 1, d), rng, F16) for h in (8, hkv, hkv))
+        out = gpu.DeviceArray((1, 1, 8, d), F32)
+        a = gpu.attention_args(out, D(q[None]), D(k[None]), D(v[None]), causal=True, cache=(c.k, c.v, c.count, False))
+        ws = gpu.DeviceArray((max(lib.vai_attention_workspace_size(ctypes.byref(a)), 1),), np.uint8)
+        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
+        caches.append((c, q, k, v, ws))
+        calls.append(a)
+        outs.append(out)
+    streams = [gpu.Stream(), gpu.Stream()]
+    gpu.synchronize()
+    print("q4 two streams", flush=True)
+    for _ in range(20):   # (the count stands: the same step each time)
+        for a, s in zip(calls, streams):
+            gpu.check(lib.vai_attention_launch(ctypes.byref(a), s.ptr), "step")
+    for s in streams:
+        s.synchronize()
+    for (c, q, k, v, _), out in zip(caches, outs):
+        rows = [np.concatenate([r, stored(x)], 1) for r, x in zip(c.rows, (k, v))]
+        want, tol = attend(q, *rows, visible(c.n, 1, 1, 0, 0), False)
+        check(out.numpy()[0], want, tol)
