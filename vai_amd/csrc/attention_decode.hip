@@ -395,7 +395,17 @@ __global__ __launch_bounds__(256) void attention_decode_merge_kernel(AttnDecodeP
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
         if (ug + i * UG < R.used) acc += wgt[ug + i * UG] * v[i];
-    for (uint32_t u = ug + AHEAD * UG; u < R.used; u += UG) acc += wgt[u] * *(const float4v*)(op + u * ustride);
+    // (many units: MORE loads in flight; one at a time 256 units of one head of 256
+    // take 21.6 us, 4 at a time 15.0, 8 11.7)
+    constexpr int MORE = 8;
+    for (uint32_t u = ug + AHEAD * UG; u < R.used; u += MORE * UG) {
+        float4v y[MORE];
+#pragma unroll
+        for (int i = 0; i < MORE; ++i) y[i] = *(const float4v*)(op + std::min(u + i * UG, R.used - 1) * ustride);
+#pragma unroll
+        for (int i = 0; i < MORE; ++i)
+            if (u + i * UG < R.used) acc += wgt[u + i * UG] * y[i];
+    }
     part[t] = acc;
     __syncthreads();
     if (t >= C4 || 4 * c >= HD) return;

@@ -51,9 +51,9 @@ template <int DP> struct Q4Lds {
     static constexpr int TILE = (int)q4::tile_bytes(DP);      // one plane's tile
     static constexpr int COPIES = (TILE + 1023) / 1024;       // 1 KB copies, the last one partly
     // tiles in flight a wave: what a CU's waves have in flight together hides the
-    // latency. 128: two tiles and three workgroups a CU, 38.0 + 6.0 us (the merge
+    // latency. 128: two tiles and three workgroups a CU, 38.0 + 4.9 us (the merge
     // of more shares) over 131072 positions, 32 heads over 8; four tiles and two
-    // workgroups 41.9 + 5.0
+    // workgroups 41.9 + 4.7
     static constexpr int D = DP == 256 ? 3 : DP == 128 ? 2 : 4;
     static constexpr int WAVE = D * 2 * TILE;
     static constexpr int OROW = DP * 4 + 16;                  // bytes of an fp32 O row in the final exchange
