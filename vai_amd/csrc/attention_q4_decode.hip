@@ -70,6 +70,14 @@ __device__ __forceinline__ void q4_wait()
     static_assert(N >= 0 && N < 64, "vmcnt range");
     __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
 }
+// all but the copies of the tiles behind this one (`behind` of them, N counted) have landed
+template <int N, int COPIES>
+__device__ __forceinline__ void q4_wait_behind(int behind)
+{
+    if constexpr (N == 0) q4_wait<0>();
+    else if (behind >= N) q4_wait<N * COPIES>();
+    else q4_wait_behind<N - 1, COPIES>(behind);
+}
 __device__ __forceinline__ void q4_wait_lds() { __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14)); }
 
 __device__ __forceinline__ float swap_max16(float x)
@@ -220,8 +228,7 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
     int slot = 0;
     for (int it = 0; it < mine; ++it) {
         // its copies have landed; the next tiles' may be in flight
-        if (it + D <= mine) q4_wait<(D - 1) * 2 * L::COPIES>();
-        else q4_wait<0>();
+        q4_wait_behind<D - 1, 2 * L::COPIES>(mine - 1 - it);
         const int64_t j0 = (first + (int64_t)it * step) * KT;
         LDS_AS uint8_t* kt = ring + slot * 2 * L::TILE;
         LDS_AS uint8_t* vt = kt + L::TILE;

@@ -190,6 +190,14 @@ __device__ __forceinline__ void few_wait()
     static_assert(N >= 0 && N < 64, "vmcnt range");
     __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
 }
+// all but the copies of the blocks behind this one (`behind` of them, N counted) have landed
+template <int N, int COPIES>
+__device__ __forceinline__ void few_wait_behind(int behind)
+{
+    if constexpr (N == 0) few_wait<0>();
+    else if (behind >= N) few_wait<N * COPIES>();
+    else few_wait_behind<N - 1, COPIES>(behind);
+}
 __device__ __forceinline__ void few_wait_lds() { __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14)); }
 
 // Few rows of X (16 MT at most): bound by reading W once. A workgroup takes 16 NT
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
         (void*)(FUSED ? nullptr : p.x + (size_t)m0 * p.x_stride), (short)0, FUSED ? 0 : (int)(rows_x * p.x_stride), 0x00020000);
     const uint32_t cr = lane >> 3;
     const auto copy = [&](int i) __attribute__((always_inline)) {   // the wave's i-th block
-        const uint32_t k = (wave + NW * (uint32_t)std::min(i, mine - 1)) * 128;   // past the last: again, never read
+        const uint32_t k = (wave + NW * (uint32_t)i) * 128;
         LDS_AS char* dst = ring + (i % D) * C::BLOCK;
 #pragma unroll
         for (int c = 0; c < C::COPIES; ++c) {
@@ -251,9 +259,9 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
 #pragma unroll
         for (int i = 0; i < KEEP; ++i)
             kept[i].load(in + (size_t)std::min<uint32_t>(row, p.M - 1) * p.K, (i * share + part) * 1024 + lane * 16, p.K);
-    if (mine > 0)
 #pragma unroll
-        for (int i = 0; i < D; ++i) copy(i);
+    for (int i = 0; i < D; ++i)
+        if (i < mine) copy(i);
 
     const uint32_t ls = p.x_stride + 16;   // a row of codes in LDS (16 more: rows start in different banks)
     LDS_AS int8_t* xl = (LDS_AS int8_t*)(lds + C::RING);
@@ -294,7 +302,7 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
         for (int j = 0; j < NT; ++j) acc[i][j] = (int4v)0;
     const int swz = c16 / 2 % 8;
     for (int i = 0; i < mine; ++i) {
-        few_wait<(D - 1) * C::COPIES>();   // block i has landed; the D - 1 after it may be in flight
+        few_wait_behind<D - 1, C::COPIES>(mine - 1 - i);   // block i has landed; those after it may be in flight
         LDS_AS const char* src = ring + (i % D) * C::BLOCK + c16 * 128;
         int4v a[2][NT], b[2][MT];
 #pragma unroll
@@ -308,7 +316,7 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
                                 : *(LDS_AS const int4v*)(src + (NT + m) * 2048 + at);
         }
         few_wait_lds();                    // read before the block is copied over
-        copy(i + D);
+        if (i + D < mine) copy(i + D);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -317,7 +325,6 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
                 for (int j = 0; j < NT; ++j)
                     acc[m][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[h][j], b[h][m], acc[m][j], 0, 0, 0);
     }
-    few_wait<0>();   // (the copies past the last block)
 
     // the waves' sums, then lane (c16, g) of fragment (m, j) holds row 16 m + c16, columns 16 j + 4 g ..+3
     __syncthreads();
