@@ -202,3 +202,32 @@ def test_odd_head_dims_and_rotated_parts(gpu, d, pairs):
         check(got, *want64(qkv, hq, hkv, d, qw, kw, pairs=pairs, rot=rot, pos=pos))
     got = run(gpu, qkv, hq, hkv, d, F16, q_weight=qw, k_weight=kw, pairs="NONE", positions=pos)
     check(got, *want64(qkv, hq, hkv, d, qw, kw, pairs="NONE", pos=pos))
+
+
+@pytest.mark.parametrize("d", [32, 64, 72, 128, 17, 250, 640])
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-30, 1e-5, 1e38])
+def test_heads_of_any_magnitude(gpu, d, eps):
+    """Heads whose squares leave fp32's range, alone or beside eps: the norm of what they hold, not 0 or infinity.
+    (Below 2^-126 the inputs themselves are subnormal; the formula takes them as they stand.)"""
+    rng = np.random.default_rng(d)
+    scales = [-147, -140, -126, -100, -75, -66, -63, -62, -40, -20, 0, 40, 62, 63, 64, 100, 124]
+    T, hq, hkv = len(scales), 3, 1
+    x = draw((1, T, hq + 2 * hkv, d), rng, F32)
+    x = np.clip(x, -7, 7)
+    x[:, :, 1] = np.where(rng.uniform(size=(1, T, d)) < 0.5, 0, x[:, :, 1])   # a head with zeros in it
+    x[:, :, 1, 0] = 2.0                                                      # (not of zeros: 0 / 0 where eps is 0)
+    for t, e in enumerate(scales):
+        x[:, t] = np.ldexp(x[:, t], e)
+        x[:, t, :, 0] = np.where(x[:, t, :, 0] == 0, F32(np.ldexp(1.0, e)), x[:, t, :, 0])
+    qkv = np.ascontiguousarray(x.reshape(1, T, -1))
+    qw, kw = (draw((d,), rng, F32) for _ in range(2))
+    pairs = "HALVES" if d % 2 == 0 else "NONE"
+    pos = rng.integers(0, 1000, (1, T)).astype(np.uint32)
+    print(f"norm_rope magnitudes d={d} eps={eps}", flush=True)
+    got = run(gpu, qkv, hq, hkv, d, F32, q_weight=qw, k_weight=kw, eps=eps, pairs=pairs, positions=pos)
+    want, mag = want64(qkv, hq, hkv, d, qw, kw, True, float(F32(eps)), 0.0, pairs, 0, 10000.0, pos)
+    # (a result below fp32's normal range is rounded to a step of 2^-149, and so is each of its three parts)
+    for g, w, m in zip(got[:2], want, mag):
+        assert np.isfinite(g).all()
+        assert (np.abs(g.astype(np.float64) - w) <= 40 * U * m + 2.0 ** -147).all()
+    np.testing.assert_array_equal(got[2], x.transpose(0, 2, 1, 3)[:, hq + hkv:])

@@ -35,6 +35,24 @@ __device__ __forceinline__ void turn_of(const QkNormRopeParams& p, uint32_t pos,
     c = k == 1 || k == 2 ? -b : b;
 }
 
+// 1 / sqrt(sq / D + eps) of a head, from the sum of its squares: as far as that
+// number lies well inside fp32's range (no square that counts has then under- or
+// overflowed).
+__device__ __forceinline__ bool rms_in_range(float v) { return v > 0x1p-80f && v < 0x1p100f; }
+__device__ __forceinline__ float inv_root(float v) { return 1.0f / sqrtf(v); }
+
+// Else the head is taken in units of 2^e, 2^e the larger of its largest |x|
+// and sqrt(eps), rounded up: the squares then lie in range, and x and the root
+// lose the same factor. (A head with an infinity or a NaN stays as it is; one of
+// zeros with eps = 0 is 0 / 0.)
+__device__ __forceinline__ int rms_unit(float amax, float eps)
+{
+    if (!(amax < __builtin_inff())) return 0;
+    const int a = amax > 0.f ? __builtin_amdgcn_frexp_expf(amax) : -200;
+    const int b = eps > 0.f ? (__builtin_amdgcn_frexp_expf(eps) + 1) >> 1 : -200;
+    return a > b ? a : b;
+}
+
 // Larger head dims: a wave takes one head at a time, in LDS as fp32.
 __global__ __launch_bounds__(64) void qk_norm_rope_any_kernel(QkNormRopeParams p)
 {
@@ -58,10 +76,24 @@ __global__ __launch_bounds__(64) void qk_norm_rope_any_kernel(QkNormRopeParams p
         const uint32_t oh = is_q ? h : is_v ? h - p.hq - p.hkv : h - p.hq, nh = is_q ? p.hq : p.hkv;
         const size_t dst = (((size_t)b * nh + oh) * p.tokens + t) * D;
         if (p.norm && !is_v) {
-            const float inv = 1.0f / sqrtf(wave_sum(sq) / (float)D + p.eps);
+            float v = wave_sum(sq) / (float)D + p.eps;
+            int e = 0;
+            if (!rms_in_range(v)) {   // (the same in every lane)
+                float amax = 0.f, sum = 0.f;
+                for (uint32_t d = lane; d < D; d += 64) amax = fmaxf(amax, __builtin_fabsf(y[d]));
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+                e = rms_unit(amax, p.eps);
+                for (uint32_t d = lane; d < D; d += 64) {
+                    const float x = ldexpf(y[d], -e);
+                    sum += x * x;
+                }
+                v = wave_sum(sum) / (float)D + ldexpf(p.eps, -2 * e);
+            }
+            const float inv = inv_root(v);
             const void* w = is_q ? p.q_weight : p.k_weight;
             for (uint32_t d = lane; d < D; d += 64)
-                y[d] = y[d] * inv * (w ? ld(w, p.w_dtype, d) + p.weight_offset : 1.0f);
+                y[d] = ldexpf(y[d], -e) * inv * (w ? ld(w, p.w_dtype, d) + p.weight_offset : 1.0f);
         }
         __syncthreads();
         const uint32_t rot = is_v ? 0u : p.rot_dim, half = rot / 2;
@@ -82,21 +114,25 @@ __global__ __launch_bounds__(64) void qk_norm_rope_any_kernel(QkNormRopeParams p
     }
 }
 
-// x summed over each group of L lanes (a power of two), in every lane
-template <int L>
-__device__ __forceinline__ float group_sum(float x)
+// op(x, what another lane holds) until every lane of a group of L (a power of two) has the group's result
+template <int L, class Op>
+__device__ __forceinline__ float group_reduce(float x, Op op)
 {
     const auto moved = [](float v, auto ctrl) __attribute__((always_inline)) {
         return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, true));
     };
-    if constexpr (L >= 2) x += moved(x, std::integral_constant<int, 0xB1>{});    // lane ^ 1
-    if constexpr (L >= 4) x += moved(x, std::integral_constant<int, 0x4E>{});    // lane ^ 2
-    if constexpr (L >= 8) x += moved(x, std::integral_constant<int, 0x141>{});   // the other 4 of 8 (mirrored)
-    if constexpr (L >= 16) x += moved(x, std::integral_constant<int, 0x140>{});  // the other 8 of 16
-    if constexpr (L >= 32) x += __shfl_xor(x, 16);
-    if constexpr (L >= 64) x += __shfl_xor(x, 32);
+    if constexpr (L >= 2) x = op(x, moved(x, std::integral_constant<int, 0xB1>{}));    // lane ^ 1
+    if constexpr (L >= 4) x = op(x, moved(x, std::integral_constant<int, 0x4E>{}));    // lane ^ 2
+    if constexpr (L >= 8) x = op(x, moved(x, std::integral_constant<int, 0x141>{}));   // the other 4 of 8 (mirrored)
+    if constexpr (L >= 16) x = op(x, moved(x, std::integral_constant<int, 0x140>{}));  // the other 8 of 16
+    if constexpr (L >= 32) x = op(x, __shfl_xor(x, 16));
+    if constexpr (L >= 64) x = op(x, __shfl_xor(x, 32));
     return x;
 }
+template <int L>
+__device__ __forceinline__ float group_sum(float x) { return group_reduce<L>(x, [](float a, float b) { return a + b; }); }
+template <int L>
+__device__ __forceinline__ float group_max(float x) { return group_reduce<L>(x, [](float a, float b) { return fmaxf(a, b); }); }
 
 // n of 4 values at any alignment of their type, zeros for the rest (FULL: 4)
 template <bool FULL, typename T>
@@ -194,7 +230,23 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, u
             sq = group_sum<L>(FULL && !on ? 0.f : sq);
             const bool is_q = h < p.hq, is_v = h >= nk;
             if (p.norm && !is_v) {
-                const float inv = __builtin_amdgcn_rsqf(sq * inv_d + p.eps);
+                float v = sq * inv_d + p.eps;
+                if (__builtin_expect(__any(!rms_in_range(v)), 0)) {   // (whole groups of lanes hold the same v)
+                    float amax = 0.f, sum = 0.f;
+                    if (!FULL || on)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, __builtin_fabsf(y[e]));
+                    amax = group_max<L>(amax);
+                    const int e2 = rms_in_range(v) ? 0 : rms_unit(amax, p.eps);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        y[e] = ldexpf(y[e], -e2);
+                        sum = fmaf(y[e], y[e], sum);
+                    }
+                    sum = group_sum<L>(FULL && !on ? 0.f : sum);
+                    v = sum * inv_d + ldexpf(p.eps, -2 * e2);
+                }
+                const float inv = inv_root(v);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[e] *= inv * (is_q ? wq[e >> 2][e & 3] : wk[e >> 2][e & 3]);
             }
