@@ -231,3 +231,27 @@ def test_heads_of_any_magnitude(gpu, d, eps):
         assert np.isfinite(g).all()
         assert (np.abs(g.astype(np.float64) - w) <= 40 * U * m + 2.0 ** -147).all()
     np.testing.assert_array_equal(got[2], x.transpose(0, 2, 1, 3)[:, hq + hkv:])
+
+
+@pytest.mark.parametrize("d, rot", [(32, 6), (64, 10), (64, 20), (17, 10), (80, 36), (250, 12), (640, 6)])
+@pytest.mark.parametrize("pairs", ["HALVES", "NEIGHBOURS"])
+@pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
+def test_what_is_not_rotated_stays(gpu, d, rot, pairs, what):
+    """Values past rot_dim are only moved: one that is not finite leaves its neighbours alone."""
+    rng = np.random.default_rng(d)
+    T, hq, hkv = 3, 2, 1
+    qkv = draw((1, T, (hq + 2 * hkv) * d), rng, F16)
+    h = qkv.reshape(T, hq + 2 * hkv, d)
+    clean = qkv.copy()
+    for t in range(T):
+        h[t, :hq + hkv, min(rot + t, d - 1)] = what
+    pos = rng.integers(1, 1000, (1, T)).astype(np.uint32)
+    print(f"norm_rope not rotated d={d} rot={rot} {pairs}", flush=True)
+    q, k, v = run(gpu, qkv, hq, hkv, d, F32, norm=False, pairs=pairs, rot_dim=rot, positions=pos)
+    want, mag = want64(clean, hq, hkv, d, norm=False, pairs=pairs, rot=rot, pos=pos)
+    for o, w in ((q, want[0]), (k, want[1])):
+        for t in range(T):
+            at = o[0, :, t, min(rot + t, d - 1)]
+            np.testing.assert_array_equal(at, np.full_like(at, what))
+            o[0, :, t, min(rot + t, d - 1)] = w[0, :, t, min(rot + t, d - 1)]
+    check((q, k, v), want, mag)

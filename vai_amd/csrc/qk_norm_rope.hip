@@ -258,7 +258,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, u
                 };
                 if (p.neighbours)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) turn(y[2 * i], y[2 * i + 1], i);
+                    for (int i = 0; i < 4; ++i) {
+                        // (pairs past rot_dim are not turned by 0: an infinity times its sine would reach the other value)
+                        if (FULL || 2 * (4 * j + i) < p.rot_dim) turn(y[2 * i], y[2 * i + 1], i);
+                    }
                 else
 #pragma unroll
                     for (int i = 0; i < 4; ++i) turn(y[i], y[4 + i], i);
