@@ -251,3 +251,23 @@ def test_rows_do_not_depend_on_their_number(gpu, n, k, xdt):
     check(outs[200], *want64(x, w, ws), "NONE")
     for m, o in outs.items():
         np.testing.assert_array_equal(o, outs[200][:m])
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 70, 1000), (5, 70, 1000), (20, 600, 300), (64, 70, 1000), (100, 300, 700),
+                                     (1000, 4096, 700), (3900, 4020, 900)])
+def test_linear_i8_far_scales(gpu, m, n, k):
+    """Scales of row and channel that only together lie in fp32's range: neither half of the product overflows."""
+    rng = np.random.default_rng(m)
+    large = np.arange(m) % 2 == 0       # rows from either end of the range in turn
+    x = np.ldexp(np.clip(draw((m, k), rng, F32), -7, 7), np.where(large, 120, -110)[:, None])
+    w, ws = weight(rng, n, k)
+    D = gpu.DeviceArray.from_numpy
+    print(f"linear_i8 far scales {m} x {n} x {k}", flush=True)
+    dx, dw = D(x), on_gpu(gpu, w)
+    for rows, e in ((large, -110), (~large, 100)):
+        s = np.ldexp(ws, e)
+        got = gpu.linear_i8(gpu.DeviceArray((m, n), F32), dx, dw, D(s)).numpy()
+        codes, xs = codes64(x[rows])
+        sums = codes.astype(np.float64) @ w.astype(np.float64).T      # exact: far below 2^53
+        want = sums * xs.astype(np.float64)[:, None] * s.astype(np.float64)
+        assert (np.abs(got[rows] - want) <= 4 * U * np.abs(want)).all()

@@ -342,7 +342,7 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
         const float xs = FUSED ? sl[m] : p.x_scale[m];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (n + e < p.N) store_output(q, (size_t)m * p.N + n + e, (float)v[e] * xs * p.w_scale[n + e]);
+            if (n + e < p.N) store_output(q, (size_t)m * p.N + n + e, i8_scaled(v[e], xs, p.w_scale[n + e]));
     }
 }
 

@@ -139,7 +139,7 @@ __device__ __forceinline__ void i8_store_fast(const LinearI8Params& p, int16v (&
             float v[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                v[r] = sc * activate<EPI>((float)acc_read(acc[i][j][r]) * xs[r >> 2][r & 3] * ws[j] + cb[j], p.epilogue);
+                v[r] = sc * activate<EPI>(i8_scaled(acc_read(acc[i][j][r]), xs[r >> 2][r & 3], ws[j]) + cb[j], p.epilogue);
             if constexpr (HALF) {
 #pragma unroll
                 for (int r = 0; r < 16; r += 2)
@@ -197,7 +197,7 @@ __device__ __forceinline__ void i8_store_any(const LinearI8Params& p, int16v (&a
             if (p.residual) rows16(p.residual, p.o_dtype, p.residual_repeat, p.N, rows, cc, res);
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                res[r] = finish((float)acc_read(acc[i][j][r]) * xs[r] * ws[j] + bias[r], res[r], p.epilogue,
+                res[r] = finish(i8_scaled(acc_read(acc[i][j][r]), xs[r], ws[j]) + bias[r], res[r], p.epilogue,
                                 p.residual_order, p.scalar_scale);
             if (col < p.N) {
                 if (p.o_dtype == DT_F16) {
