@@ -405,3 +405,40 @@ def test_two_streams(gpu):
         rows = [np.concatenate([r, stored(x)], 1) for r, x in zip(c.rows, (k, v))]
         want, tol = attend(q, *rows, visible(c.n, 1, 1, 0, 0), False)
         check(out.numpy()[0], want, tol)
+
+
+# Groups whose step or codes lie next to a rounding's border: fp32 alone, rounding max - min, the quotient or the
+# difference x - m on the way, would land on the border itself. (low, values between, high)
+BORDERS = [
+    (3.045797348022461e-05, (0.5,), 1.00390625), (6.091594696044922e-05, (), 2.0078125), (9.161233901977539e-05, (), 1.0048828125),
+    (6.097555160522461e-05, (), 1.8759765625), (0.00012183189392089844, (), 4.015625), (0.00012195110321044922, (1.0,), 3.751953125),
+    (0.0009746551513671875, (), 32.125), (0.0077972412109375, (100.0,), 257.0), (0.015594482421875, (), 514.0),
+    (-10.015625, (-3.0,), 0.00024366378784179688), (-17.703125, (), -0.00048732757568359375),
+    (2.0 ** -24, (1.5, 3.5, 2.5, 14.5, 0.5), 15.0), (-2.0 ** -24, (2.5, 4.5, 1.5, 0.5, 8.5), 15.0),
+    (3 * 2.0 ** -24, (1.5, 5.5, 13.5), 15.0), (2.0 ** -14, (48.0, 80.0, 112.0), 480.0), (-2.0 ** -20, (5.0, 9.0, 29.0), 30.0),
+    (-65504.0, (2.0 ** -24, 0.0, -2.0 ** -24), 65504.0), (65472.0, (), 65504.0), (0.0, (2.0 ** -24,), 2.0 ** -24),
+    (0.0, (7 * 2.0 ** -24, 8 * 2.0 ** -24), 22 * 2.0 ** -24),
+]
+
+
+@pytest.mark.parametrize("d", [64, 40, 20])
+@pytest.mark.parametrize("together", [True, False])
+def test_steps_and_codes_next_to_a_border(gpu, d, together):
+    """Step and codes as the definition's exact arithmetic rounds them: rows appended with few queries, and a prompt's."""
+    rows = np.zeros((1, len(BORDERS), d), F16)
+    for i, (lo, between, hi) in enumerate(BORDERS):
+        row = np.full(d, lo, F16)
+        row[1:1 + len(between)] = between
+        row[1 + len(between)] = hi
+        row[32:] = row[:max(d - 32, 0)]
+        rows[0, i] = row
+    c = Cache(gpu, 1, 64, d, False)
+    q = np.ones((1, 1, d), F16)
+    print(f"q4 borders d={d} {together}", flush=True)
+    if together:
+        rows = np.concatenate([rows, rows[:, :20]], 1)      # more than 32 rows: the append of a longer call
+        c.call(q, rows, np.ascontiguousarray(rows[:, ::-1]))
+    else:
+        for i in range(rows.shape[1]):
+            c.call(q, rows[:, i:i + 1], -rows[:, i:i + 1])
+    c.check_rows()

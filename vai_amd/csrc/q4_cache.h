@@ -65,28 +65,38 @@ __host__ __device__ constexpr uint32_t v_scale(uint32_t dp, uint32_t j, uint32_t
     return scale_offset(dp) + ((d >> 5) * 4 + (j >> 3)) * 32 + order_of(j & 7) * 2;
 }
 
-// A group's step from its extremes. Both are fp16 values, so max - min is
-// exact in fp32 but for the far ends of fp16's range. A group that holds
-// something not finite in fp16 keeps m = NaN, s = 0: all its values are NaN; one
-// without values (past the head dim, lo > hi) zeros.
+// A group's step from its extremes: (max - min) / 15 rounded to fp16 once. The
+// fp32 quotient rounded again is next to it; the remainder, exact in 64 bits,
+// against half the distance to the neighbours says which fp16 number it is. A
+// group that holds something not finite in fp16 keeps m = NaN, s = 0: all its
+// values are NaN; one without values (past the head dim, lo > hi) zeros.
 __device__ __forceinline__ void step_of(float lo, float hi, bool finite, half_t& s, half_t& m)
 {
     const bool some = finite && lo <= hi;
-    s = some ? (half_t)((hi - lo) / 15.0f) : (half_t)0.f;
-    m = some ? (half_t)lo : finite ? (half_t)0.f : (half_t)__builtin_nanf("");
+    const double d = (double)hi - (double)lo;
+    uint16_t b = __builtin_bit_cast(uint16_t, (half_t)((float)d / 15.0f));
+    const auto value = [](uint16_t x) { return (double)(float)__builtin_bit_cast(half_t, x); };
+    const double r = fma(-15.0, value(b), d);
+    const double up = 7.5 * (value(b + 1) - value(b)), down = 7.5 * (value(b - 1) - value(b));   // (b = 0: down is NaN)
+    if (r > up || (r == up && (b & 1))) ++b;
+    else if (r < down || (r == down && (b & 1))) --b;
     // (s rounded up near fp16's end: one below, so that 15 s + m is an fp16 number too)
-    if (some && fmaf(15.0f, (float)s, lo) > 65504.f)
-        s = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, s) - 1));
+    if (fma(15.0, value(b), (double)lo) > 65504.0) --b;
+    s = some ? __builtin_bit_cast(half_t, b) : (half_t)0.f;
+    m = some ? (half_t)lo : finite ? (half_t)0.f : (half_t)__builtin_nanf("");
 }
 
 // (x - m) / s to the nearest integer, halves to even, from the exact remainder
 // (inv: 1 / s or next to it: the first guess is at most one off); s = 0 gives 0.
-// x >= m, and s is rounded: the last code is 15 all the same.
+// x >= m, and s is rounded: the last code is 15 all the same. x - m = t + te (te
+// what fp32 leaves of it); where te is not 0, s and 2 (t - q s) are multiples of
+// t's last place, so that their difference is exact too.
 __device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv)
 {
-    const float t = x - m, q = rintf(t * inv), r = 2.0f * fmaf(-q, s, t);
+    const float t = x - m, z = t - x, te = (x - (t - z)) - (m + z);
+    const float q = rintf(t * inv), r = 2.0f * fmaf(-q, s, t), e = -2.0f * te, above = r - s, below = r + s;
     const int n = (int)q;
-    const bool odd = n & 1, up = r > s || (r == s && odd), down = r < -s || (r == -s && odd);
+    const bool odd = n & 1, up = above > e || (above == e && odd), down = below < e || (below == e && odd);
     const int c = n + (int)up - (int)down;
     return s > 0.f ? (uint32_t)(c < 15 ? c : 15) : 0u;
 }
