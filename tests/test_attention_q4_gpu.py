@@ -442,3 +442,23 @@ def test_steps_and_codes_next_to_a_border(gpu, d, together):
         for i in range(rows.shape[1]):
             c.call(q, rows[:, i:i + 1], -rows[:, i:i + 1])
     c.check_rows()
+
+
+@pytest.mark.parametrize("d, tq, xdt, n", [(64, 1, F16, 8000), (128, 4, F32, 3000), (256, 2, F16, 3000)])
+@pytest.mark.parametrize("down", [4, 20, 26, 30])
+def test_many_keys_of_little_weight(gpu, d, tq, xdt, n, down):
+    """One key in twenty outweighs the others by 2^down, but its value is zero: the result is what the others bring."""
+    rng = np.random.default_rng(d + down)
+    c = Cache(gpu, 1, 8192, d, False)
+    k, v = np.zeros((1, n, d), F16), np.full((1, n, d), 64, F16)
+    v[0, :, 1::3] = -32
+    k[0, ::20, 0] = 15.0
+    v[0, ::20] = 0
+    q = np.zeros((4, tq, d), xdt)
+    q[:, :, 0] = down * np.log(2.0) * np.sqrt(d) / 15
+    q[1, :, 0] *= 0.75
+    for a in range(0, n, 1000):
+        c.call(np.zeros((1, 1, d), F16), np.ascontiguousarray(k[:, a:a + 1000]), np.ascontiguousarray(v[:, a:a + 1000]), span=1)
+    print(f"q4 little weight d={d} tq={tq} down={down}", flush=True)
+    got = c.call(q, None, None, F32)
+    check(got, *attend(q, *c.rows, visible(n, tq, 0, 0, 0), xdt == F32))

@@ -22,9 +22,11 @@
 // that counts is lost (fp16 holds what is 2^-25 of it). An fp32 q enters as two
 // fp16 numbers. V enters as s n + m rounded to fp16 (one packed fma from the exact
 // n), the probabilities as two fp16 numbers (the second the rest that the first
-// leaves), so that V's and the result's are the only roundings to fp16: error
-// against 64 bits 2.9e-4 of the result, of which the rounding of the result is
-// 2.1e-4 (3.6e-4 with the probabilities in one number).
+// leaves) and times 2^14, so that those far below the row's largest keep their
+// bits too (fp16 holds 2^-38 of it; unscaled, a key of 2^-25 was lost, and with
+// thousands of them what they bring): V's and the result's are then the only
+// roundings to fp16: error against 64 bits 2.9e-4 of the result, of which the
+// rounding of the result is 2.1e-4 (3.6e-4 with the probabilities in one number).
 //
 // The call's own rows are rounded by the wave whose tile they are in, into that
 // tile in LDS (and into the cache): nothing waits for an append.
@@ -104,6 +106,7 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
     using L = Q4Lds<DP>;
     constexpr int G = DP / 32, ND = DP / 16, D = L::D;   // groups; values of a lane's V slice
     constexpr uint32_t NIB = 0x000f000fu, NIB16 = 0x00f000f0u;
+    constexpr float LIFT = 14.f, SLACK = 1.f;
     extern __shared__ uint4v q4_lds[];
     LDS_AS uint8_t* lds = (LDS_AS uint8_t*)(LDS_AS void*)q4_lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -371,9 +374,10 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
             }
             float tmax = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
             tmax = swap_max32(swap_max16(tmax));
-            // the row's reference m moves only when the max exceeds it by more than 8
-            // (P stays below 2^8), for the whole wave at once
-            if (__any(tmax > m[q] + 8.f)) {
+            // the row's reference m moves only when the max exceeds it by more than
+            // SLACK (P stays below 2^(SLACK + LIFT), in fp16's range), for the whole
+            // wave at once
+            if (__any(tmax > m[q] + SLACK)) {
                 const float mnew = fmaxf(m[q], tmax);
                 const float alpha = __builtin_amdgcn_exp2f(m[q] - (mnew == -__builtin_inff() ? 0.f : mnew));
                 l[q] *= alpha;
@@ -381,7 +385,7 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[q][d] *= alpha;
             }
-            const float mref = m[q] == -__builtin_inff() ? 0.f : m[q];
+            const float mref = (m[q] == -__builtin_inff() ? 0.f : m[q]) - LIFT;   // (l and o carry 2^LIFT alike)
             float e[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(v[i] - mref);
