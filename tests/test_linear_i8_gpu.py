@@ -271,3 +271,55 @@ def test_linear_i8_far_scales(gpu, m, n, k):
         sums = codes.astype(np.float64) @ w.astype(np.float64).T      # exact: far below 2^53
         want = sums * xs.astype(np.float64)[:, None] * s.astype(np.float64)
         assert (np.abs(got[rows] - want) <= 4 * U * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("m, n, k, xdt, odt, biased, residual, epi", [
+    # wave rings over rounded rows: 16 columns a workgroup, 32, then 32 and 64 rows
+    (7, 4095, 2999, F32, F16, True, False, "NONE"), (3, 5003, 4096, F16, F32, False, True, "NONE"),
+    (7, 5120, 4096, F32, F32, True, False, "NONE"), (16, 8190, 1500, F16, F16, True, True, "SILU"),
+    (20, 8000, 700, F16, F32, True, True, "NONE"), (32, 4999, 2100, F32, F16, False, False, "GELU_TANH"),
+    (61, 5003, 1999, F16, F16, True, False, "GELU_TANH"), (64, 4100, 1300, F32, F32, True, True, "NONE"),
+    # tiles of 64
+    (500, 2048, 2048, F32, F32, False, True, "NONE"), (333, 1999, 900, F16, F16, True, False, "SILU"),
+    (70, 8191, 1100, F16, F32, True, True, "NONE"), (1, 16500, 2100, F16, F16, True, False, "NONE"),
+    # of 128: one tile a workgroup, then two
+    (1000, 4096, 700, F16, F16, True, False, "NONE"), (1000, 4091, 1100, F32, F32, True, True, "SILU"),
+    (2000, 8190, 300, F16, F16, False, False, "NONE"), (1999, 8190, 290, F16, F32, True, False, "NONE"),
+    # of 256: one tile a workgroup, then two; whole tiles, and rows, columns and K that end inside one
+    (4096, 4096, 1024, F16, F16, False, False, "NONE"), (3900, 4020, 900, F16, F16, True, False, "GELU_TANH"),
+    (3900, 4019, 1001, F32, F32, True, False, "NONE"), (3841, 3843, 900, F16, F16, True, True, "NONE"),
+    (3900, 8192, 1100, F16, F32, True, False, "NONE"), (4000, 8000, 1100, F32, F16, True, True, "SILU"),
+])
+def test_every_kernel_over_several_stages_of_k(gpu, m, n, k, xdt, odt, biased, residual, epi):
+    """Each of the kernels and epilogues the sizes choose between, over more than two 128-byte stages of K."""
+    rng = np.random.default_rng(m + n + k)
+    x, (w, ws) = draw((m, k), rng, xdt), weight(rng, n, k)
+    bias = draw((n,), rng, F16) if biased else None
+    res = draw((m, n), rng, odt) if residual else None
+    D = gpu.DeviceArray.from_numpy
+    out = gpu.DeviceArray((m + 1, n), odt)
+    out.fill_(0xFF)
+    a = gpu.linear_i8_args(gpu.DeviceArray((1, n), odt), D(x), on_gpu(gpu, w), D(ws), None if bias is None else D(bias),
+                           None if res is None else D(res), epi=epi)
+    a.out = out.ptr
+    if biased:
+        a.bias_repeat = n
+    need = gpu.lib().vai_linear_i8_workspace_size(ctypes.byref(a))
+    wsp = gpu.DeviceArray((max(need, 1),), np.uint8)
+    wsp.fill_(0xFF)                     # (NaN scales, codes of -1, were any of it read unwritten)
+    a.workspace, a.workspace_bytes = wsp.ptr, wsp.nbytes
+    print(f"linear_i8 stages {m} x {n} x {k} {xdt.__name__} {odt.__name__} {epi}", flush=True)
+    gpu.check(gpu.lib().vai_linear_i8_launch(ctypes.byref(a), None), "linear_i8")
+    gpu.synchronize()
+    got = out.numpy()
+    assert (got[m].view(np.uint8) == 0xFF).all()
+    codes, xs = codes64(x)
+    sums = codes.astype(np.float64) @ w.astype(np.float64).T          # exact: far below 2^53
+    y = sums * xs.astype(np.float64)[:, None] * ws.astype(np.float64)
+    mag = np.abs(y)
+    if biased:
+        y, mag = y + bias.astype(np.float64), mag + np.abs(bias.astype(np.float64))
+    y = np_epilogue(epi, y)
+    if residual:
+        y, mag = y + res.astype(np.float64), mag + np.abs(res.astype(np.float64))
+    check(got[:m], y, mag, epi)
