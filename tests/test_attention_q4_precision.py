@@ -220,3 +220,35 @@ def test_error_by_the_norm(gpu, case):
     whole, worst = norms(got, dense(q, k, v, see))
     print(f"error {whole:.3g}, worst row {worst:.3g}", flush=True)
     assert whole <= bounds(case)[0] and worst <= bounds(case)[1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d, hq, hkv, tq, count, size, ring, span, xdt", [
+    (20, 4, 2, 3, 30, 64, False, 0, F32), (17, 4, 1, 1, 60, 64, False, 0, F16), (250, 4, 2, 2, 30, 64, False, 0, F32),
+    (100, 2, 2, 20, 9, 64, False, 0, F16), (1, 2, 1, 5, 40, 64, False, 0, F32), (65, 4, 2, 20, 400, 128, True, 20, F32),
+    (8, 4, 2, 20, 20, 64, False, 0, F16), (30, 2, 1, 300, 500, 1024, False, 9, F16)])
+def test_other_head_dims_are_exact(gpu, d, hq, hkv, tq, count, size, ring, span, xdt):
+    """Head dims the matrix cores do not take: every value in fp32 as it is stored, so a result is off by what fp32
+    leaves of the scores (the head dim's chain of sums and the scale: (d + 4) 2^-24 of scale * sum |q k|, twice), of the
+    powers (2^-21) and of the sum over the keys (a chain of each, 2 n 2^-24)."""
+    rng = np.random.default_rng(d + tq)
+    n = count + tq
+    q, k, v = draw((hq, tq, d), rng, xdt), draw((hkv, n, d), rng, xdt), draw((hkv, n, d), rng, xdt)
+    c = Cache(gpu, hkv, size, d, ring)
+    print(f"q4 exact d={d} tq={tq}", flush=True)
+    for a in range(0, count, size):
+        b = min(count, a + size)
+        c.call(np.ones((hkv, 1, d), F16), np.ascontiguousarray(k[:, a:b]), np.ascontiguousarray(v[:, a:b]), span=1)
+    got = c.call(q, np.ascontiguousarray(k[:, count:]), np.ascontiguousarray(v[:, count:]), F32, span)
+    c.check_rows()
+    first = max(0, n - size) if ring else 0
+    see = visible(count, tq, tq, first, min(span, size - tq + 1) if ring and span else span)
+    K, V = stored(k[:, first:]), stored(v[:, first:])
+    for h in range(hq):
+        Kh, Vh, x = K[h * hkv // hq], V[h * hkv // hq], q[h].astype(np.float64)
+        s = np.where(see, x @ Kh.T / np.sqrt(d), -np.inf)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        ds = np.where(see, np.abs(x) @ np.abs(Kh).T / np.sqrt(d), 0).max(-1, keepdims=True) * (d + 4) * 2.0 ** -24
+        tol = p @ np.abs(Vh) * (4 * ds + 2.0 ** -21 + 4 * see.sum(1).max() * 2.0 ** -24)
+        assert (np.abs(got[:, h] - p @ Vh) <= tol).all()

@@ -55,16 +55,16 @@ __device__ __forceinline__ void q4_values8(const uint8_t* head, uint32_t dp, uin
     for (uint32_t e = 0; e < 8; ++e) x[e] = fmaf(s, (float)(w >> (4 * (is_v ? e : q4::nibble_of(e))) & 15u), m);
 }
 
-// The live rows of the cache as fp16 copies for the kernels that read fp16:
-// from the 64-position tile the first query's window starts in. A workgroup
+// The live rows of the cache as copies for the kernels that read rows of values
+// (T: fp16 for the flash kernel, fp32, exact, for the plain one): from the 64-position tile the first query's window starts in. A workgroup
 // takes a 32-position tile of one head at a time: half its threads V (a slice of
 // 4 positions each, so that a row's values leave in wide stores), half K (a word
 // of 8 values each). A hidden position must not reach a query through a NaN (0 *
 // NaN in P V), so a row with a NaN in V is copied as V = 0 and K = NaN: the score
 // is masked where the position is hidden and NaN where it is not.
 // 7513 positions of 8 heads of 128: 16 us (25 with a wave to a row).
-template <int DP>
-__global__ __launch_bounds__(256) void q4_copy_kernel(AttnParams p, half_t* k16, half_t* v16)
+template <int DP, typename T>
+__global__ __launch_bounds__(256) void q4_copy_kernel(AttnParams p, T* k_out, T* v_out)
 {
     constexpr int G = DP / 32, ND = DP / 16;
     __shared__ uint32_t bad[2][q4::KT];
@@ -82,13 +82,13 @@ __global__ __launch_bounds__(256) void q4_copy_kernel(AttnParams p, half_t* k16,
     if (t < 2 * q4::KT) bad[t / q4::KT][t % q4::KT] = 0;
     __syncthreads();
     uint32_t round = 0;
-    for (uint64_t T = beg / q4::KT + blockIdx.x; T * q4::KT < live; T += gridDim.x, round ^= 1) {
-        const uint32_t place = (uint32_t)(p.ring ? T % wrap : T), row0 = place * q4::KT;
+    for (uint64_t tile = beg / q4::KT + blockIdx.x; tile * q4::KT < live; tile += gridDim.x, round ^= 1) {
+        const uint32_t place = (uint32_t)(p.ring ? tile % wrap : tile), row0 = place * q4::KT;
         const uint8_t* kt = kh + (size_t)place * q4::tile_bytes(DP);
         const uint8_t* vt = vh + (size_t)place * q4::tile_bytes(DP);
         const size_t dst = ((size_t)hk * p.kv_rows + row0) * HD;
         // rows of this tile that are copied (of a ring also those a full turn older: not before beg)
-        const auto copied = [&](uint32_t j) { return T * q4::KT + j >= beg && T * q4::KT + j < live; };
+        const auto copied = [&](uint32_t j) { return tile * q4::KT + j >= beg && tile * q4::KT + j < live; };
         for (uint32_t e = t; e < q4::KT * G; e += 256) {
             const uint32_t j = e % q4::KT;
             const half_t m = *(const half_t*)(vt + q4::v_scale(DP, j, e / q4::KT * 32) + 16);
@@ -106,15 +106,15 @@ __global__ __launch_bounds__(256) void q4_copy_kernel(AttnParams p, half_t* k16,
                 const uint32_t j = 8 * b + 4 * h + r;
                 const half_t* sm = (const half_t*)(vt + q4::v_scale(DP, j, d0));
                 const float s = (float)sm[0], m = (float)sm[8];
-                typedef half_t out_t __attribute__((ext_vector_type(ND)));
-                typedef out_t out_u __attribute__((aligned(2)));
+                typedef T out_t __attribute__((ext_vector_type(ND)));
+                typedef out_t out_u __attribute__((aligned(sizeof(T))));
                 out_t x;
 #pragma unroll
                 for (int i = 0; i < ND; ++i) {
                     const float v = fmaf(s, (float)(w[i / 2] >> (8 * r + 4 * (i & 1)) & 15u), m);
-                    x[i] = v != v ? (half_t)0.f : (half_t)v;
+                    x[i] = v != v ? (T)0.f : (T)v;
                 }
-                half_t* o = v16 + dst + (size_t)j * HD + d0;
+                T* o = v_out + dst + (size_t)j * HD + d0;
                 if (!copied(j)) continue;
                 if (d0 + ND <= HD) *(out_u*)o = x;
                 else
@@ -128,13 +128,14 @@ __global__ __launch_bounds__(256) void q4_copy_kernel(AttnParams p, half_t* k16,
                 const uint32_t w = *(const uint32_t*)(kt + q4::k_word(DP, j, 8 * c));
                 const float s = bad[round][j] ? __builtin_nanf("") : (float)*(const half_t*)(kt + q4::k_step(DP, j, 8 * c));
                 const float m = (float)*(const half_t*)(kt + q4::k_min(DP, j, 8 * c));
-                typedef half8 half8u __attribute__((aligned(2)));
-                half8 x;
+                typedef T out8 __attribute__((ext_vector_type(8)));
+                typedef out8 out8u __attribute__((aligned(sizeof(T))));
+                out8 x;
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) x[i] = (half_t)fmaf(s, (float)(w >> (4 * q4::nibble_of(i)) & 15u), m);
-                half_t* o = k16 + dst + (size_t)j * HD + 8 * c;
+                for (uint32_t i = 0; i < 8; ++i) x[i] = (T)fmaf(s, (float)(w >> (4 * q4::nibble_of(i)) & 15u), m);
+                T* o = k_out + dst + (size_t)j * HD + 8 * c;
                 if (!copied(j)) continue;
-                if (8 * c + 8 <= HD) *(half8u*)o = x;
+                if (8 * c + 8 <= HD) *(out8u*)o = x;
                 else
 #pragma unroll
                     for (uint32_t i = 0; i < 8; ++i)
@@ -194,7 +195,8 @@ hipError_t cache_read_launch(const CacheReadParams& p, hipStream_t s)
 
 static size_t copy_bytes(const AttnParams& p)
 {
-    return (2 * (size_t)p.hkv * p.kv_rows * p.head_dim * sizeof(half_t) + 255) & ~(size_t)255;
+    const size_t value = p.kv_dtype == DT_F32 ? sizeof(float) : sizeof(half_t);
+    return (2 * (size_t)p.hkv * p.kv_rows * p.head_dim * value + 255) & ~(size_t)255;
 }
 
 void attention_q4_plan(AttnParams& p, uint32_t cus)
@@ -205,6 +207,7 @@ void attention_q4_plan(AttnParams& p, uint32_t cus)
     } else {
         p.q4 = 1;
         attention_plan(p, cus);
+        if (!p.dp) p.kv_dtype = DT_F32;   // the plain kernel takes values as they are
     }
 }
 
@@ -218,7 +221,8 @@ void attention_q4_set_workspace(AttnParams& p, void* ws)
     p.ws4 = ws;
     if (p.q4 == 2) return;
     p.k = ws;
-    p.v = (half_t*)ws + (size_t)p.hkv * p.kv_rows * p.head_dim;
+    const size_t n = (size_t)p.hkv * p.kv_rows * p.head_dim;
+    p.v = p.kv_dtype == DT_F32 ? (void*)((float*)ws + n) : (void*)((half_t*)ws + n);
     attention_set_workspace(p, (char*)ws + copy_bytes(p));
 }
 
@@ -233,10 +237,15 @@ hipError_t attention_q4_launch(const AttnParams& p, hipStream_t s)
         if (e != hipSuccess) return e;
     }
     const dim3 grid(std::min<uint32_t>((p.kv_rows + q4::KT - 1) / q4::KT, 1024), p.hkv);
-    half_t *k16 = (half_t*)p.k, *v16 = (half_t*)p.v;
-    if (dp == 64) hipLaunchKernelGGL(q4_copy_kernel<64>, grid, dim3(256), 0, s, p, k16, v16);
-    else if (dp == 128) hipLaunchKernelGGL(q4_copy_kernel<128>, grid, dim3(256), 0, s, p, k16, v16);
-    else hipLaunchKernelGGL(q4_copy_kernel<256>, grid, dim3(256), 0, s, p, k16, v16);
+    const auto copy = [&](auto value) {
+        typedef decltype(value) T;
+        T *k = (T*)p.k, *v = (T*)p.v;
+        if (dp == 64) hipLaunchKernelGGL((q4_copy_kernel<64, T>), grid, dim3(256), 0, s, p, k, v);
+        else if (dp == 128) hipLaunchKernelGGL((q4_copy_kernel<128, T>), grid, dim3(256), 0, s, p, k, v);
+        else hipLaunchKernelGGL((q4_copy_kernel<256, T>), grid, dim3(256), 0, s, p, k, v);
+    };
+    if (p.kv_dtype == DT_F32) copy(float{});
+    else copy(half_t{});
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     return attention_launch(p, s);
