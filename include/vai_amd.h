@@ -334,9 +334,15 @@ typedef struct {
      * codes n = round((x - m) / s) of 0 .. 15, and stands for s n + m (s the
      * fp16 number below where 15 s + m would leave fp16's range). Every
      * key and value is attended as stored, the call's own among them: what the
-     * cache holds does not depend on how a sequence was cut into calls. (More
-     * than 16 queries, 64 query rows of a KV head or 32 new keys, and head dims
-     * that are no multiple of 8, go over copies rounded to fp16.) A group
+     * cache holds does not depend on how a sequence was cut into calls. Calls of
+     * up to 128 query rows of a KV head (hq / hkv * tq; 256 with cache_size >=
+     * 4096, and hq * tq <= 65535) attend the codes themselves, where only V is
+     * rounded to fp16: an fp32 result is off by 2e-4 of its norm. Calls of more
+     * rows go over copies of the cache whose K and V are rounded to fp16, with a
+     * probability as one fp16 number, as an fp16 cache is attended: 4e-4, more
+     * where channels of K stand out; the workspace holds two such planes of the
+     * cache's size. Head dims that are no multiple of 8 go over fp32 copies, where
+     * nothing is rounded. A group
      * with a value that is not finite in fp16 is stored as NaN; a query that
      * sees a row with such a group in K or V is NaN, one it is hidden from is
      * not touched by it. Positions past the count may hold anything. A 4-bit

@@ -462,3 +462,118 @@ def test_many_keys_of_little_weight(gpu, d, tq, xdt, n, down):
     print(f"q4 little weight d={d} tq={tq} down={down}", flush=True)
     got = c.call(q, None, None, F32)
     check(got, *attend(q, *c.rows, visible(n, tq, 0, 0, 0), xdt == F32))
+
+
+MANY = [
+    # d, hq, hkv, tq, tkv, count, size, ring, span, xdt, odt: up to 128 rows of a KV head, 256 over 4096 positions, from the codes
+    (128, 4, 4, 33, 33, 1000, 2048, False, 0, F16, F32),     # 33 rows: the second block has one
+    (64, 4, 4, 200, 200, 100, 4096, False, 0, F16, F16),     # blocks that see different tiles
+    (64, 8, 2, 64, 64, 0, 4096, False, 0, F32, F32),         # a prompt
+    (64, 4, 4, 128, 128, 0, 128, False, 0, F16, F32),        # ... into a cache of its size
+    (128, 8, 1, 32, 32, 3000, 4096, False, 0, F32, F16),
+    (128, 4, 2, 100, 100, 1000, 4100, False, 40, F16, F16),  # a window that moves with the blocks
+    (128, 2, 2, 200, 200, 500, 5000, False, 7, F32, F32),    # ... of which the first blocks' is over before the last's
+    (64, 4, 2, 60, 60, 1000, 256, True, 100, F16, F32),      # in a ring
+    (128, 4, 2, 50, 250, 1000, 256, True, 0, F16, F16),      # nearly the whole ring anew
+    (128, 8, 2, 50, 50, 5000, 4096, True, 0, F16, F16),
+    (256, 4, 2, 60, 60, 700, 1024, False, 0, F32, F32),
+    (256, 4, 2, 3, 3, 700, 1024, False, 0, F16, F32),        # appended apart, few rows
+    (64, 4, 4, 2, 17, 100, 512, False, 0, F16, F16),         # ... and more new keys than queries
+    (64, 4, 4, 90, 20, 0, 512, False, 0, F16, F32),          # more queries than keys: the first blocks see none
+    (80, 6, 2, 40, 40, 333, 400, False, 0, F16, F32),
+    (200, 4, 2, 70, 70, 90, 4500, False, 50, F16, F32),
+    # past them: over the copies
+    (64, 8, 2, 65, 65, 700, 4096, False, 0, F16, F32),
+    (256, 8, 2, 40, 40, 200, 320, True, 200, F16, F16),
+    (128, 4, 2, 129, 129, 1000, 2048, False, 40, F32, F16),
+    (72, 8, 2, 100, 100, 30, 256, False, 0, F16, F32),
+    (64, 8, 1, 40, 10, 300, 512, False, 0, F16, F32),
+]
+
+
+@pytest.mark.parametrize("d, hq, hkv, tq, tkv, count, size, ring, span, xdt, odt", MANY)
+def test_many_rows(gpu, d, hq, hkv, tq, tkv, count, size, ring, span, xdt, odt):
+    test_attention_q4(gpu, d, hq, hkv, tq, tkv, count, size, ring, span, xdt, odt)
+
+
+@pytest.mark.parametrize("tq", [20, 100, 200])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_many_rows_of_a_block_mask(gpu, d, tq):
+    """A full prefix that ends inside a block of rows, then causal; a full block after it."""
+    rng = np.random.default_rng(tq)
+    c = Cache(gpu, 2, 512 if tq < 200 else 4096, d, False)
+    c.append(rng, 70)
+    q, k, v = (draw((h, tq, d), rng, F16) for h in (2, 2, 2))
+    print(f"q4 block mask d={d} tq={tq}", flush=True)
+    got = c.call(q, k, v, F32, blocks=(0b010, [7, 15]))
+    see = visible(70, tq, tq, 0, 0)
+    see[:7, 70:77] = True
+    see[15:, 85:] = True
+    want, tol = attend(q, *c.rows, see, False)
+    check(got, want, tol)
+
+
+@pytest.mark.parametrize("hq, tq, d", [(2, 40, 64), (2, 100, 128), (4, 60, 256), (2, 150, 64), (4, 150, 128), (4, 150, 256)])
+def test_rows_with_nan_among_many(gpu, hq, tq, d):
+    """As for few rows: a row that is not finite reaches the queries that see it alone, from the codes and over the copies."""
+    rng = np.random.default_rng(tq)
+    for what in ("k", "v"):
+        c = Cache(gpu, 2, 512, d, False)
+        c.append(rng, 100)
+        q, k, v = draw((hq, tq, d), rng, F16), draw((2, tq, d), rng, F32), draw((2, tq, d), rng, F32)
+        late = tq - 7
+        (k if what == "k" else v)[0, late, 3] = np.nan
+        (k if what == "k" else v)[1, late, d - 1] = -np.inf
+        print(f"q4 nan among many d={d} tq={tq} in {what}", flush=True)
+        got = c.call(q, k, v, F32)
+        c.check_rows()
+        assert np.isnan(got[late:]).all()
+        want, tol = attend(q[:, :late], *(r[:, :100 + late] for r in c.rows), visible(100, tq, tq, 0, 0)[:late, :100 + late], False)
+        check(got[:late], want, tol)
+
+
+@pytest.mark.parametrize("hq, tq, d, xdt", [(8, 80, 128, F16), (4, 60, 64, F32), (4, 100, 64, F16), (8, 5, 256, F16)])
+def test_replayed_graph_of_many_rows(gpu, hq, tq, d, xdt):
+    """Recorded once, replayed at other counts: an append and attention from the codes, or the copies."""
+    rng = np.random.default_rng(tq)
+    D, lib, hkv, size = gpu.DeviceArray.from_numpy, gpu.lib(), 2, 1024
+    c = Cache(gpu, hkv, size, d, False)
+    c.append(rng, 900)
+    hist = [r.copy() for r in c.rows]
+    q, k, v = draw((hq, tq, d), rng, xdt), draw((hkv, tq, d), rng, xdt), draw((hkv, tq, d), rng, xdt)
+    out = gpu.DeviceArray((1, tq, hq, d), F32)
+    a = gpu.attention_args(out, D(q[None]), D(k[None]), D(v[None]), causal=True, cache=(c.k, c.v, c.count, False))
+    ws = gpu.DeviceArray((max(lib.vai_attention_workspace_size(ctypes.byref(a)), 1),), np.uint8)
+    ws.fill_(0xFF)
+    a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
+    gpu.synchronize()
+    stream = gpu.Stream()
+    graph = gpu.Graph(stream, lambda: gpu.check(lib.vai_attention_launch(ctypes.byref(a), stream.ptr), "step"))
+    new = [stored(k), stored(v)]
+    print(f"q4 graph of many rows d={d} tq={tq}", flush=True)
+    for count in (0, 33, 900, 127):
+        c.set_count(count)
+        graph.launch()
+        stream.synchronize()
+        for h, n in zip(hist, new):
+            h[:, count:count + tq] = n[:, :max(0, h.shape[1] - count)]
+        rows = [np.concatenate([h[:, :count], n], 1) for h, n in zip(hist, new)]
+        want, tol = attend(q, *rows, visible(count, tq, tq, 0, 0), xdt == F32)
+        check(out.numpy()[0], want, tol)
+
+
+def test_planes_past_32_bit_offsets_over_copies(gpu):
+    """260 rows of a KV head at the end of planes of 5 GB: rows of fp32 copies of 17 GB each."""
+    rng = np.random.default_rng(1)
+    size, d, hkv, tq = (1 << 26) + 64, 32, 2, 130
+    c = Cache(gpu, hkv, size, d, False)
+    n0 = size - 400
+    c.set_count(n0)
+    print("q4 far rows over copies", flush=True)
+    k, v = (draw((hkv, 200, d), rng, F16) for _ in range(2))
+    c.call(draw((2, 20, d), rng, F16), k, v, span=1)
+    q, k, v = draw((4, tq, d), rng, F16), draw((hkv, tq, d), rng, F16), draw((hkv, tq, d), rng, F16)
+    got = c.call(q, k, v, F32, span=100)
+    assert c.n == n0 + 200 + tq
+    want, tol = attend(q, *c.rows, visible(200, tq, tq, 0, 100), False)
+    check(got, want, tol)

@@ -2,8 +2,9 @@
 // rows, reading rows back, and attention over the values as stored.
 //
 // A call's new rows are rounded into the cache first and then attended like
-// every other cached row, so the result does not depend on how a sequence was
-// cut into calls.
+// every other cached row, so what the cache holds does not depend on how a sequence
+// was cut into calls. Results do in their last places: calls of many rows
+// (q4_few_rows is false) read the cache as fp16 copies.
 #include <algorithm>
 
 #include "kernels.h"
@@ -56,10 +57,16 @@ __device__ __forceinline__ void q4_values8(const uint8_t* head, uint32_t dp, uin
 }
 
 // The live rows of the cache as copies for the kernels that read rows of values
-// (T: fp16 for the flash kernel, fp32, exact, for the plain one): from the 64-position tile the first query's window starts in. A workgroup
-// takes a 32-position tile of one head at a time: half its threads V (a slice of
-// 4 positions each, so that a row's values leave in wide stores), half K (a word
-// of 8 values each). A hidden position must not reach a query through a NaN (0 *
+// (T: fp16 for the flash kernel, fp32, exact, for the plain one): from the
+// 64-position tile the first query's window starts in. K and V rounded to fp16 are
+// what the flash kernel's matrix products take, as of an fp16 cache: a result is
+// then off by 3.4e-4 to 4.1e-4 of its norm (1.9e-4 from the codes; with fp16 output
+// and channels of K that stand out 5.8e-4), and a prompt of 512 tokens over 7001
+// cached positions takes 98 us where the codes, unpacked for every 32 rows, take 173.
+//
+// A workgroup takes a 32-position tile of one head at a time: half its threads V
+// (a slice of 4 positions each, so that a row's values leave in wide stores), half
+// K (a word of 8 values each). A hidden position must not reach a query through a NaN (0 *
 // NaN in P V), so a row with a NaN in V is copied as V = 0 and K = NaN: the score
 // is masked where the position is hidden and NaN where it is not.
 // 7513 positions of 8 heads of 128: 16 us (25 with a wave to a row).
@@ -228,14 +235,14 @@ void attention_q4_set_workspace(AttnParams& p, void* ws)
 
 hipError_t attention_q4_launch(const AttnParams& p, hipStream_t s)
 {
-    if (p.q4 == 2) return q4_decode_launch(p, p.ws4, s);
     const uint32_t dp = q4_dp(p.head_dim);
-    if (p.tkv > 0) {
+    if (p.tkv > 0 && (p.q4 == 1 || q4_append_apart(p))) {
         const uint32_t blocks = (p.tkv + 2048 / dp - 1) / (2048 / dp);
         hipLaunchKernelGGL(q4_append_kernel, dim3(std::min(blocks, 4096u), p.hkv, 2), dim3(256), 0, s, p, dp);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
+    if (p.q4 == 2) return q4_decode_launch(p, p.ws4, s);
     const dim3 grid(std::min<uint32_t>((p.kv_rows + q4::KT - 1) / q4::KT, 1024), p.hkv);
     const auto copy = [&](auto value) {
         typedef decltype(value) T;

@@ -1,13 +1,14 @@
-// attention_q4_decode.hip -- a few query rows over a 4-bit KV cache: append and
-// attention in one launch (and a merge where the keys are split).
+// attention_q4_decode.hip -- up to 128 or 256 query rows of a KV head over a 4-bit
+// cache: append and attention in one launch (and a merge where the keys are split;
+// an append before it where the call brings many rows).
 //
 // What bounds it: reading the cache once, 5 bits a value. The query rows of a KV
 // head are the columns of one matrix tile (16 or 32), as in attention_decode.hip;
 // a workgroup is a share of the head's 32-position tiles, which its 4 waves take
 // in turn, each through a ring of its own in LDS: a tile's 20 dp bytes of K and of
 // V are copied there as they lie, D tiles in flight, and no wave waits for another
-// until the share ends. 131072 positions, 32 heads over 8 of 128: 38 us, 4.4 TB/s,
-// where a large copy makes 5.2; waves wait for memory a quarter of their time, and
+// until the share ends. 120001 positions, 32 heads over 8 of 128: 37.5 us, 4.1 TB/s,
+// where a large copy makes 5.2 (fp32 queries: 1.5 us more a pass); waves wait for memory a quarter of their time, and
 // for an issue slot, the unpacking of each other's codes, a third.
 //
 // The codes enter the matrix cores as they are. An fp16 whose bits are a code n of
@@ -28,8 +29,8 @@
 // roundings to fp16: error against 64 bits 2.9e-4 of the result, of which the
 // rounding of the result is 2.1e-4 (3.6e-4 with the probabilities in one number).
 //
-// The call's own rows are rounded by the wave whose tile they are in, into that
-// tile in LDS (and into the cache): nothing waits for an append.
+// A few rows that the call brings are rounded by the wave whose tile they are in,
+// into that tile in LDS (and into the cache): nothing waits for an append.
 #include <algorithm>
 #include <type_traits>
 
@@ -53,9 +54,10 @@ template <int DP> struct Q4Lds {
     static constexpr int TILE = (int)q4::tile_bytes(DP);      // one plane's tile
     static constexpr int COPIES = (TILE + 1023) / 1024;       // 1 KB copies, the last one partly
     // tiles in flight a wave: what a CU's waves have in flight together hides the
-    // latency. 128: two tiles and three workgroups a CU, 38.0 + 4.9 us (the merge
-    // of more shares) over 131072 positions, 32 heads over 8; four tiles and two
-    // workgroups 41.9 + 4.7
+    // latency. A pass over 120000 positions, us, two / three / four tiles: 128, 32 heads
+    // over 8, one token 38.3 / 44.1 / 45.2 (three workgroups a CU with two tiles, two
+    // with four), fp32 queries 40.3 / 41.2 / 42.2, 8 tokens in blocks of 32 rows 74.3 /
+    // 75.1 / 76.2; 64, three / four tiles 29.3 / 30.0; 256, two / three 36.7 / 37.9
     static constexpr int D = DP == 256 ? 3 : DP == 128 ? 2 : 4;
     static constexpr int WAVE = D * 2 * TILE;
     static constexpr int OROW = DP * 4 + 16;                  // bytes of an fp32 O row in the final exchange
@@ -94,7 +96,7 @@ __device__ __forceinline__ float swap_max16(float x)
 // workgroups a CU, as registers allow
 constexpr int q4_resident(uint32_t dp, uint32_t nq, bool q32)
 {
-    return dp == 256 || nq == 2 ? 1 : dp == 128 && !q32 ? 3 : 2;
+    return dp == 256 ? 1 : dp == 128 && nq == 1 && !q32 ? 3 : 2;
 }
 
 // DP: the padded head dim; NQ: 16-row query blocks. Grid: (units, row blocks x
@@ -139,11 +141,19 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
     uint8_t* kh = uniform_ptr((uint8_t*)p.k + hk * hb);
     uint8_t* vh = uniform_ptr((uint8_t*)p.v + hk * hb);
     LDS_AS uint8_t* ring = lds + wave * L::WAVE;
+    // the tokens of the block's rows (all of them where it goes over a head's end)
+    const bool over = (rend - 1) / p.tq != row0 / p.tq;
+    const uint32_t tok0 = over ? 0u : row0 % p.tq, tok1 = over ? p.tq - 1 : (rend - 1) % p.tq;
     // this wave's tiles: first, first + step, .., and their places in the planes
     // (a ring's size is a multiple of 64: no tile wraps)
-    const int64_t first = R.tb + unit * NW + wave;
     const uint32_t step = p.units * NW, wrap = p.ring ? p.kv_rows / KT : 0xffffffffu;
-    const int mine = __builtin_amdgcn_readfirstlane((int)(R.te > first ? ((uint32_t)(R.te - first) + step - 1) / step : 0));
+    int64_t first = R.tb + unit * NW + wave, last = R.te;
+    if (p.n_new == 0) {   // only tiles that some row of the block sees (both bounds grow with the token)
+        const int64_t beg = p.mask.key_start_cached(tok0, R.cached) / KT;
+        last = std::min<int64_t>(last, (p.mask.key_end_cached(tok1, R.cached) + KT - 1) / KT);
+        if (beg > first) first += ((uint32_t)(beg - first) + step - 1) / step * step;
+    }
+    const int mine = __builtin_amdgcn_readfirstlane((int)(last > first ? ((uint32_t)(last - first) + step - 1) / step : 0));
     const uint32_t place0 = __builtin_amdgcn_readfirstlane((uint32_t)(p.ring ? first % wrap : first));
     const uint32_t hop = __builtin_amdgcn_readfirstlane(p.ring ? step % wrap : step);
     const auto next_place = [&](uint32_t t) __attribute__((always_inline)) {
@@ -212,9 +222,8 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
     }
     const int64_t kfirst = p.mask.key_start_cached(0, R.cached);   // no query sees a position before it
     // what every row of this wave sees: tiles inside need no mask
-    // (both bounds grow with the token)
-    const int64_t all_beg = p.mask.key_start_cached(p.tq - 1, R.cached);
-    const int64_t all_end = std::min<int64_t>(p.mask.key_end_cached(0, R.cached), R.live);
+    const int64_t all_beg = p.mask.key_start_cached(tok1, R.cached);
+    const int64_t all_end = std::min<int64_t>(p.mask.key_end_cached(tok0, R.cached), R.live);
     const float sl2 = p.scale * 1.4426950408889634f;   // scores in log2 units
 
     float m[NQ], l[NQ];
@@ -264,107 +273,109 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
         }
         place = next_place(place);
 
-        // S^T: lane (c16, g) holds query row c16 and positions 8 g + 4 t ..+3
-        float4v x[2][NQ], y[2][NQ];   // 2^-24 sum s sum n q, sum m sum q
+        // what the score product reads of the tile: codes, steps and minima
+        uint32_t kw[2][G];
+        half8 ma[2];
+        half4 ks[2][G];        // rows 4 g ..+3
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            uint32_t kw[G];
             LDS_AS const uint8_t* a = kt + ((t * 4 + g) * 16 + c16) * (G * 4);
             if constexpr (G == 2) {
                 const uint2v w = *(LDS_AS const uint2v*)a;
-                kw[0] = w.x;
-                kw[1] = w.y;
+                kw[t][0] = w.x;
+                kw[t][1] = w.y;
             } else {
 #pragma unroll
                 for (int i = 0; i < G; i += 4) {
                     const uint4v w = *(LDS_AS const uint4v*)(a + 4 * i);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) kw[i + e] = w[e];
+                    for (int e = 0; e < 4; ++e) kw[t][i + e] = w[e];
                 }
             }
             typedef half_t halfg __attribute__((ext_vector_type(G)));
             const halfg mg = *(LDS_AS const halfg*)(kt + q4::k_min_offset(DP) + (t * 16 + c16) * (G * 2));
-            half8 ma = (half8)(half_t)0;
-#pragma unroll
-            for (int i = 0; i < G; ++i) ma[i] = mg[i];
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                x[t][q] = (float4v)0.f;
-                y[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ma, qsum[q], (float4v)0.f, 0, 0, 0);
-            }
+            ma[t] = (half8)(half_t)0;
 #pragma unroll
             for (int i = 0; i < G; ++i) {
-                const half4 ks = *(LDS_AS const half4*)(kt + q4::scale_offset(DP) + ((i * 2 + t) * 16 + 4 * g) * 2);   // rows 4 g ..+3
-                const uint32_t w = kw[i], u = w >> 8;
-                const half8 n8 = __builtin_bit_cast(half8, uint4v{w & NIB, w & NIB16, u & NIB, u & NIB16});
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) {
-                    float4v n = __builtin_amdgcn_mfma_f32_16x16x32_f16(n8, qf[q][i], (float4v)0.f, 0, 0, 0);
-                    if constexpr (Q32) n = __builtin_amdgcn_mfma_f32_16x16x32_f16(n8, ql[q][i], n, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[t][q][r] = fmaf((float)ks[r], n[r], x[t][q][r]);
-                }
+                ma[t][i] = mg[i];
+                ks[t][i] = *(LDS_AS const half4*)(kt + q4::scale_offset(DP) + ((i * 2 + t) * 16 + 4 * g) * 2);
             }
         }
-        uint32_t vw[ND];       // words 2 i, 2 i + 1: the two halves of the block's positions, values 2 i and 2 i + 1
-        {
-            LDS_AS const uint8_t* a = vt + g * (DP * 4) + c16 * (DP / 4);
-#pragma unroll
-            for (int i = 0; i < ND; i += 4) {
-                const uint4v w = *(LDS_AS const uint4v*)(a + 4 * i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) vw[i + e] = w[e];
-            }
-        }
-        LDS_AS const uint8_t* va = vt + q4::scale_offset(DP) + ((c16 * ND / 32) * 4 + g) * 32;
-        half8 vs = *(LDS_AS const half8*)va, vm = *(LDS_AS const half8*)(va + 16);
-        q4_wait_lds();         // read before the slot is copied over
-        if (copied < mine) copy(slot);
-        slot = slot + 1 == D ? 0 : slot + 1;
-
-        // Positions that no query sees (stale rows, rows past the count) may hold
-        // anything: their V is zero here, their scores are masked below.
-        if (j0 < kfirst || j0 + KT > R.live) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int64_t j = j0 + 8 * g + q4::order_of(e);
-                if (j < kfirst || j >= R.live) vs[e] = vm[e] = (half_t)0.f;
-            }
-        }
-        // A row with a NaN in V must not reach a query it is hidden from through 0 *
-        // NaN: its V is zero and its score NaN, which the mask replaces. (The sum of
-        // the minima is NaN if one is, and at worst also where they overflow.)
-        uint32_t bad = 0;
-        {
-            const half2v z = half2v{vm[0], vm[1]} + half2v{vm[2], vm[3]} + half2v{vm[4], vm[5]} + half2v{vm[6], vm[7]};
-            if (__builtin_expect(__any(z.x != z.x || z.y != z.y), 0)) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (vm[e] != vm[e]) {
-                        vs[e] = vm[e] = (half_t)0.f;
-                        bad |= 1u << q4::order_of(e);
-                    }
-                bad |= q4::moved<q4::XOR1>(bad);
-                bad |= q4::moved<q4::XOR2>(bad);
-                bad |= q4::moved<q4::MIRROR8>(bad);
-                bad |= q4::moved<q4::MIRROR16>(bad);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (bad >> (4 * t + r) & 1) x[t][q][r] = __builtin_nanf("");
-            }
-        }
-
+        uint32_t vw[ND];       // V's words 2 i, 2 i + 1: the two halves of the block's positions, values 2 i and 2 i + 1
+        half8 vs, vm;
+        uint32_t bad = 0;      // of the lane's 8 positions, those whose V holds a NaN
+        bool any_bad = false;  // (of the wave's)
         half8 ph[NQ], pl[NQ];   // P^T: positions 0 2 1 3 4 6 5 7 of the lane's 8, and what fp16 leaves of them
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
+            // S^T: lane (c16, g) holds query row c16 and positions 8 g + 4 t ..+3
+            float4v x[2], y[2];   // 2^-24 sum s sum n q, sum m sum q
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                x[t] = (float4v)0.f;
+                y[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ma[t], qsum[q], (float4v)0.f, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    const uint32_t w = kw[t][i], u = w >> 8;
+                    const half8 n8 = __builtin_bit_cast(half8, uint4v{w & NIB, w & NIB16, u & NIB, u & NIB16});
+                    float4v n = __builtin_amdgcn_mfma_f32_16x16x32_f16(n8, qf[q][i], (float4v)0.f, 0, 0, 0);
+                    if constexpr (Q32) n = __builtin_amdgcn_mfma_f32_16x16x32_f16(n8, ql[q][i], n, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[t][r] = fmaf((float)ks[t][i][r], n[r], x[t][r]);
+                }
+            }
+            if (q == 0) {   // V's share of the tile, under the first rows' products
+                LDS_AS const uint8_t* a = vt + g * (DP * 4) + c16 * (DP / 4);
+#pragma unroll
+                for (int i = 0; i < ND; i += 4) {
+                    const uint4v w = *(LDS_AS const uint4v*)(a + 4 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) vw[i + e] = w[e];
+                }
+                LDS_AS const uint8_t* va = vt + q4::scale_offset(DP) + ((c16 * ND / 32) * 4 + g) * 32;
+                vs = *(LDS_AS const half8*)va;
+                vm = *(LDS_AS const half8*)(va + 16);
+                q4_wait_lds();         // read before the slot is copied over
+                if (copied < mine) copy(slot);
+                slot = slot + 1 == D ? 0 : slot + 1;
+
+                // Positions that no query sees (stale rows, rows past the count) may hold
+                // anything: their V is zero here, their scores are masked below.
+                if (j0 < kfirst || j0 + KT > R.live) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int64_t j = j0 + 8 * g + q4::order_of(e);
+                        if (j < kfirst || j >= R.live) vs[e] = vm[e] = (half_t)0.f;
+                    }
+                }
+                // A row with a NaN in V must not reach a query it is hidden from through 0 *
+                // NaN: its V is zero and its score NaN, which the mask replaces. (The sum of
+                // the minima is NaN if one is, and at worst also where they overflow.)
+                const half2v z = half2v{vm[0], vm[1]} + half2v{vm[2], vm[3]} + half2v{vm[4], vm[5]} + half2v{vm[6], vm[7]};
+                if (__builtin_expect(__any(z.x != z.x || z.y != z.y), 0)) {
+                    any_bad = true;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (vm[e] != vm[e]) {
+                            vs[e] = vm[e] = (half_t)0.f;
+                            bad |= 1u << q4::order_of(e);
+                        }
+                    bad |= q4::moved<q4::XOR1>(bad);
+                    bad |= q4::moved<q4::XOR2>(bad);
+                    bad |= q4::moved<q4::MIRROR8>(bad);
+                    bad |= q4::moved<q4::MIRROR16>(bad);
+                }
+            }
+            if (__builtin_expect(any_bad, 0))
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (bad >> (4 * t + r) & 1) x[t][r] = __builtin_nanf("");
             float v[8];
             const float sc = sl2 * down[q];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fmaf(x[i >> 2][q][i & 3], 16777216.f, y[i >> 2][q][i & 3]) * sc;
+            for (int i = 0; i < 8; ++i) v[i] = fmaf(x[i >> 2][i & 3], 16777216.f, y[i >> 2][i & 3]) * sc;
             if (j0 < all_beg || j0 + KT > all_end) {
                 const int lo = (int)std::min<int64_t>(std::max<int64_t>(kbeg[q] - j0, -1), KT + 1);
                 const int hi = (int)std::min<int64_t>(std::max<int64_t>(kend[q] - j0, -1), KT + 1);
@@ -465,8 +476,10 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
             const uint32_t h = hk * (p.hq / p.hkv) + row / p.tq, t = row % p.tq;
             const size_t out = ((size_t)t * p.hq + h) * HD + 4 * c;
             if (4 * c < HD) {
-                if (p.o_dtype == DT_F16) *(half4*)((half_t*)p.out + out) = __builtin_convertvector(acc, half4);
-                else *(float4v*)((float*)p.out + out) = acc;
+                typedef half4 half4u __attribute__((aligned(2)));
+                typedef float4v float4u __attribute__((aligned(4)));
+                if (p.o_dtype == DT_F16) *(half4u*)((half_t*)p.out + out) = __builtin_convertvector(acc, half4);
+                else *(float4u*)((float*)p.out + out) = acc;
             }
         } else {
             const size_t part = ((size_t)hk * p.units + unit) * rows + row;
@@ -495,25 +508,54 @@ static hipError_t q4_decode_launch_t(const AttnDecodeParams& p, hipStream_t s)
     return attention_decode_merge_launch(p, DP, 1, s);
 }
 
-// Few rows: as the fp16 cache's plan, at most 16 tokens and 64 rows of a KV head,
-// and new rows that lie in what some query sees (their tiles' waves append them).
+// Up to 128 query rows of a KV head, 256 over a cache of 4096 positions and more:
+// past them the copies for the flash kernel cost less than unpacking the codes for
+// 16 or 32 rows at a time. One pass, us, this way / over the copies, at 1000, 8000
+// and 120000 positions (8 KV heads, fp16 queries):
+//   D = 128, 68 rows   16.9 / 20.3   27.1 / 46.5   134 / 426
+//           128        21.3 / 21.9   31.8 / 46.5   171 / 426
+//           192        23.0 / 22.4   37.2 / 46.0   261 / 427
+//           256        24.2 / 22.0   41.2 / 45.8   322 / 427
+//           384        27.4 / 26.3   55.4 / 46.1   498 / 429
+//   D = 64, 128        17.1 / 17.4   23.3 / 37.8   122 / 255
+//           256        19.5 / 17.5   30.9 / 38.0   227 / 255
+//   D = 256, 128       21.7 / 33.8   48.2 / 75.7   474 / 989
+//           256        27.6 / 34.6   79.2 / 75.4   927 / 989
+// fp32 queries: D = 128, 256 rows 20.9 / 22.9, 43.9 / 47.0, 420 / 428. One or two
+// KV heads: faster this way at 256 rows throughout (2 of 128, 120000: 95.4 / 116).
 bool q4_few_rows(const AttnParams& p)
 {
-    return p.head_dim % 8 == 0 && p.tq <= 16 && p.hq / p.hkv * p.tq <= 64 && (uint64_t)p.hq * p.tq <= 65535 && p.tkv <= 32 &&
-           (p.span == 0 || p.tkv < p.tq + p.span);
+    return p.head_dim % 8 == 0 && (uint64_t)(p.hq / p.hkv) * p.tq <= (p.kv_rows < 4096 ? 128 : 256) &&
+           (uint64_t)p.hq * p.tq <= 65535;
+}
+
+// The call's rows are rounded where their tiles are attended, 256 / DP of them
+// at a time and by every row block, or before, by a launch of their own: its 2 us
+// against 0.4-1.4 a step. 3000 positions, us, in the walk / apart: D = 64, 8 rows
+// 13.4 / 14.0, 16 15.4 / 16.7 (in four row blocks 16.1 / 13.4), 32 22.4 / 19.5; D =
+// 128, 4 12.7 / 13.4, 5 17.0 / 15.9, 8 18.9 / 16.7; D = 256, 2 15.7 / 16.2, 4 19.3 /
+// 16.9. (And apart where a window leaves rows of the call out of every query's sight.)
+bool q4_append_apart(const AttnParams& p)
+{
+    return p.tkv > 512 / q4_dp(p.head_dim) || (p.span != 0 && p.tkv >= p.tq + p.span);
 }
 
 void q4_decode_plan(AttnParams& p, uint32_t cus)
 {
     const uint32_t dp = q4_dp(p.head_dim);
+    const bool q32 = p.q_dtype == DT_F32;
     p.dp = dp;
     p.dec_rows = p.hq / p.hkv * p.tq;
-    p.dec_rpb = std::min<uint32_t>(p.dec_rows, dp == 256 ? 16 : 32);
+    // 32 rows a workgroup where the registers hold them for two workgroups a CU (fp32
+    // queries at D = 128, 32 and 16 rows: 128 rows over 120000 positions 252, 223 us)
+    p.dec_rpb = std::min<uint32_t>(p.dec_rows, dp == 256 || (dp == 128 && q32) ? 16 : 32);
     const uint32_t keys = p.span ? std::min<uint64_t>(p.kv_rows, (uint64_t)p.span + p.tq + 2 * fd::KT) : p.kv_rows;
     const uint32_t tiles = (keys + fd::KT - 1) / fd::KT, most = std::max<uint32_t>((tiles + fd::NW - 1) / fd::NW, 1);
     const uint32_t blocks = p.hkv * ((p.dec_rows + p.dec_rpb - 1) / p.dec_rpb),
-                   wgs = cus * q4_resident(dp, p.dec_rpb > 16 ? 2 : 1, p.q_dtype == DT_F32);
-    p.dec_units = std::min(std::min(std::max((wgs + blocks - 1) / blocks, 1u), most), AttnDecodeParams::MAX_UNITS);
+                   wgs = cus * q4_resident(dp, p.dec_rpb > 16 ? 2 : 1, q32);
+    // (one round of the chip: a share more and its last workgroups run alone, 68 rows
+    // over 120000 positions 141 us instead of 132)
+    p.dec_units = std::min(std::min(std::max(wgs / blocks, 1u), most), AttnDecodeParams::MAX_UNITS);
 }
 
 size_t q4_decode_workspace(const AttnParams& p) { return attention_decode_workspace(p, p.dec_units); }
@@ -525,7 +567,7 @@ hipError_t q4_decode_launch(const AttnParams& a, void* ws, hipStream_t s)
     p.o_dtype = a.o_dtype; p.q_dtype = a.q_dtype;
     p.hq = a.hq; p.hkv = a.hkv; p.tq = a.tq; p.tkv = a.tkv; p.head_dim = a.head_dim;
     p.cache_count = a.cache_count; p.kv_rows = a.kv_rows; p.ring = a.ring;
-    p.k_new = a.k_new; p.v_new = a.v_new; p.n_new = a.tkv; p.new_dtype = a.new_dtype;
+    p.k_new = a.k_new; p.v_new = a.v_new; p.n_new = q4_append_apart(a) ? 0u : a.tkv; p.new_dtype = a.new_dtype;
     p.scale = a.scale;
     p.mask = a.mask;
     p.rows = a.dec_rows; p.rpb = a.dec_rpb; p.units = a.dec_units;
@@ -535,7 +577,7 @@ hipError_t q4_decode_launch(const AttnParams& a, void* ws, hipStream_t s)
     if (a.q_dtype == DT_F32) {
         switch (a.dp) {
         case 64: return one ? q4_decode_launch_t<64, 1, true>(p, s) : q4_decode_launch_t<64, 2, true>(p, s);
-        case 128: return one ? q4_decode_launch_t<128, 1, true>(p, s) : q4_decode_launch_t<128, 2, true>(p, s);
+        case 128: return q4_decode_launch_t<128, 1, true>(p, s);
         default: return q4_decode_launch_t<256, 1, true>(p, s);
         }
     }

@@ -221,7 +221,7 @@ struct AttnParams {
     uint8_t* k4;
     uint8_t* v4;
     void* ws4;                    // the call's workspace
-    uint32_t q4;                  // 0: none; 1: through the copies; 2: few rows, from the planes themselves
+    uint32_t q4;                  // 0: none; 1: through the copies; 2: from the codes themselves
     // Few query rows per KV head (attention_decode.hip): dec_units > 0 takes
     // that path, with dec_rows = tq * hq / hkv rows per KV head, dec_rpb of
     // them per workgroup; dec_append: it also appends the new rows.
@@ -271,8 +271,10 @@ void attention_q4_plan(AttnParams& p, uint32_t cus);
 hipError_t attention_q4_launch(const AttnParams& p, hipStream_t s);
 size_t attention_q4_workspace(const AttnParams& p);
 void attention_q4_set_workspace(AttnParams& p, void* ws);
-// its few-rows path (attention_q4_decode.hip)
+// its path from the codes themselves (attention_q4_decode.hip), and whether the
+// call's rows are appended before it
 bool q4_few_rows(const AttnParams& p);
+bool q4_append_apart(const AttnParams& p);
 void q4_decode_plan(AttnParams& p, uint32_t cus);
 size_t q4_decode_workspace(const AttnParams& p);
 hipError_t q4_decode_launch(const AttnParams& p, void* ws, hipStream_t s);
