@@ -436,7 +436,7 @@ void attention_decode_plan(AttnParams& p, uint32_t cus, uint32_t key_rows, size_
     const uint32_t group = p.hq / p.hkv;
     if (p.tq > 16 || group * p.tq > 64 || (uint64_t)p.hq * p.tq > 65535) return;
     const auto at16 = [](const void* x) { return ((uintptr_t)x % 16) == 0; };
-    p.dec_append = p.cache_count && !p.q4 && p.tkv > 0 && p.tkv <= 32 && at16(p.k_new) && at16(p.v_new) ? 1u : 0u;
+    p.dec_append = p.cache_count && p.tkv > 0 && p.tkv <= 32 && at16(p.k_new) && at16(p.v_new) ? 1u : 0u;
     p.dec_rows = group * p.tq;
     p.dec_rpb = std::min<uint32_t>(p.dec_rows, p.dp == 256 ? 16 : 32);   // (32 rows at D = 256 would spill)
     const uint32_t keys = p.span ? std::min<uint64_t>(key_rows, (uint64_t)p.span + p.tq + 2 * fd::KT) : key_rows;

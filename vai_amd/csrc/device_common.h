@@ -107,15 +107,6 @@ struct OutputSpec {
     float scale;
 };
 
-// The 8-bit Linear's sum times the scales of its row and column, in the order in
-// which nothing leaves fp32's range that the result does not: a sum (below 2^31)
-// times a row's scale up to 2^64 cannot, and past that the column's comes first.
-__device__ __forceinline__ float i8_scaled(int sum, float row, float col)
-{
-    const bool far = row > 0x1p64f;
-    return (float)sum * (far ? col : row) * (far ? row : col);
-}
-
 __device__ __forceinline__ void store_output_general(const OutputSpec& q, size_t o, float v)
 {
     const float b = q.bias ? ld(q.bias, q.b_dtype, q.bias_repeat ? o % q.bias_repeat : o) : 0.f;

@@ -88,7 +88,7 @@ __device__ __forceinline__ uint32_t abs_max16(const float (&x)[16], uint32_t m)
 // N codes as bytes. x / s is taken as x * inv, and the sum with 1.5 * 2^23
 // leaves its nearest integer in the low bits (one fma); that quotient is off by
 // 127 * 2^-23 at most, so only where it comes within 2^-13 of a half are the
-// codes taken from the exact remainder (one wave of 1024 values in ten).
+// codes taken from the exact remainder (one wave of 1024 values in five).
 template <int N>
 __device__ __forceinline__ void codes_of(const float (&x)[N], float s, float inv, uint32_t (&w)[N / 4])
 {
@@ -339,10 +339,13 @@ __global__ __launch_bounds__(64 * NW) void linear_i8_few_kernel(LinearI8Params p
         for (int w = 1; w < NW; ++w) v += sums[(w * MT * NT + f) * 64 + lane];
         const uint32_t m = m0 + 16 * (f / NT) + c16, n = n0 + 16 * (f % NT) + 4 * g;
         if (m >= p.M) continue;
+        // (a sum, below 2^31, times a row's scale up to 2^64 stays within fp32; what a larger
+        // scale has above it follows the column's)
         const float xs = FUSED ? sl[m] : p.x_scale[m];
+        const float lift = xs > 0x1p64f ? 0x1p64f : 1.0f, xr = xs > 0x1p64f ? xs * 0x1p-64f : xs;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (n + e < p.N) store_output(q, (size_t)m * p.N + n + e, i8_scaled(v[e], xs, p.w_scale[n + e]));
+            if (n + e < p.N) store_output(q, (size_t)m * p.N + n + e, (float)v[e] * xr * p.w_scale[n + e] * lift);
     }
 }
 

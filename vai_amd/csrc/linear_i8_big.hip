@@ -16,8 +16,10 @@
 //    b % 8), and goes down groups of 8 row tiles column by column, so that an
 //    L2 holds the rows of X and W its workgroups share.
 //
-// 2048 x 4096 x 16384 (fp16 in and out, F = 4): 137 us, 2.0 POP/s, where a plain
-// library product of the integers takes 131; 500 x 2048 x 2048 (F = 1): 7.7 us.
+// 2048 x 4096 x 16384 (fp16 in and out, F = 4): 160 us in the middle of a run, 1.7
+// POP/s at the clock under load (the fastest launch 138), where a plain library
+// product of the integers takes 131; 500 x 2048 x 2048 (F = 1): 7.7 us to fp16, 10.6
+// with fp32 output and residual.
 #include <algorithm>
 
 #include "device_common.h"
@@ -82,6 +84,15 @@ __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(15 | (7 
 
 template <uint32_t EPI>
 __device__ __forceinline__ float activate(float x, uint32_t epi) { return epilogue(x, EPI == 6 ? epi : EPI); }
+
+// A sum times the scales of its row and column, in the order in
+// which nothing leaves fp32's range that the result does not: a sum (below 2^31)
+// times a row's scale up to 2^64 cannot, and past that the column's comes first.
+__device__ __forceinline__ float i8_scaled(int sum, float row, float col)
+{
+    const bool far = row > 0x1p64f;
+    return (float)sum * (far ? col : row) * (far ? row : col);
+}
 
 // The accumulators are read through this so that the register allocator keeps
 // them in accumulation registers across the tile loop (a plain use of an MFMA
