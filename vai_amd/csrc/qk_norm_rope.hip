@@ -169,11 +169,12 @@ __device__ __forceinline__ float4v weight4(const void* w, int dt, uint32_t d, ui
 // half is no multiple of 4, or what is left none of 8, a lane's last values do not
 // exist (na, nb of its two groups of four do; FULL: all). A lane's four angles
 // serve every head of the token. A wave takes a token's heads 64 / L at a time,
-// its share of them (blockIdx.y of `shares`). One step's loads at a time and 44
-// registers: eight waves a SIMD hide the loads better than four steps at a time in
-// 72 registers do. 4096 tokens of 32 + 8 + 8 fp16 heads of 128: 20.4 us (23.8 with
-// four steps at a time), 4.9 TB/s, where a large copy makes 5.2; a single token's
-// 3.9 us are latency (the smallest kernels here take 2.3).
+// its share of them (blockIdx.y of `shares`). One step's loads at a time: 94
+// registers, five waves a SIMD, which hide the loads better than the three that
+// four steps at a time leave (143 registers). 4096 tokens of 32 + 8 + 8 fp16 heads
+// of 128: 21.3 us (23.8 with four steps at a time), 4.7 TB/s, where a large copy
+// makes 5.2; a single token's 4.1 us are latency (the smallest kernels here take
+// 2.3).
 template <typename TI, typename TO, int L, bool FULL>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeParams p, uint32_t shares, uint32_t steps)
 {

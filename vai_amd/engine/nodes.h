@@ -47,7 +47,8 @@ public:
         // The product in 8-bit integers (vai_linear_i8_launch; not the reference's):
         // the weight is rounded once per upload, with a scale per output channel,
         // rows of the input in each forward. The weight slot takes fp32 or fp16 as
-        // ever; splitSize and an accumulator dtype do not apply.
+        // ever and keeps its device buffer beside the integers (a byte a value and 4 a
+        // channel more); splitSize and an accumulator dtype do not apply.
         bool int8Weights = false;
     } config_;
 
