@@ -577,3 +577,55 @@ def test_planes_past_32_bit_offsets_over_copies(gpu):
     assert c.n == n0 + 200 + tq
     want, tol = attend(q, *c.rows, visible(200, tq, tq, 0, 100), False)
     check(got, want, tol)
+
+
+@pytest.mark.parametrize("d, hq, tq, xdt, odt", [(64, 8, 1, F16, F16), (128, 4, 3, F32, F32), (128, 4, 30, F16, F16), (256, 4, 20, F32, F16),
+                                                 (64, 4, 50, F16, F32), (128, 4, 140, F16, F16), (20, 4, 5, F16, F16)])
+def test_operands_anywhere(gpu, d, hq, tq, xdt, odt):
+    """Q, K, V and the output one element off any boundary; what lies before and behind the output stays. The same
+    call gives the same bits again; a scale below zero is the query's sign turned."""
+    rng = np.random.default_rng(d + tq)
+    hkv, count = 2, 333
+    D = gpu.DeviceArray.from_numpy
+    c = Cache(gpu, hkv, 1024, d, False)
+    c.append(rng, count)
+    q, k, v = draw((hq, tq, d), rng, xdt), draw((hkv, tq, d), rng, xdt), draw((hkv, tq, d), rng, xdt)
+    off = lambda t: D(np.concatenate([np.full(1, np.nan, t.dtype), t.ravel()]))  # noqa: E731
+    rows = [np.concatenate([r, stored(x)], 1) for r, x in zip(c.rows, (k, v))]
+    want, tol = attend(q, *rows, visible(count, tq, tq, 0, 0), xdt == F32)
+    outs = []
+    for sign in (1, 1, -1):
+        dq, dk, dv = off(q * xdt(sign)), off(k), off(v)
+        do = D(np.full(1 + want.size + 32, 3.0, odt))
+        a = gpu.attention_args(gpu.DeviceArray((1, tq, hq, d), odt), D(q[None]), D(k[None]), D(v[None]), causal=True,
+                               scale=sign / np.sqrt(d), cache=(c.k, c.v, c.count, False))
+        for name, x in (("q", dq), ("k", dk), ("v", dv), ("out", do)):
+            setattr(a, name, x.ptr + np.dtype(odt if name == "out" else xdt).itemsize)
+        ws = gpu.DeviceArray((max(gpu.lib().vai_attention_workspace_size(ctypes.byref(a)), 1),), np.uint8)
+        ws.fill_(0xFF)
+        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
+        print(f"q4 anywhere d={d} tq={tq} sign={sign}", flush=True)
+        gpu.check(gpu.lib().vai_attention_launch(ctypes.byref(a), None), "attention")
+        gpu.synchronize()
+        got = do.numpy()
+        assert got[0] == 3.0 and (got[1 + want.size:] == 3.0).all()
+        outs.append(got[1:1 + want.size].reshape(tq, hq, d))
+        check(outs[-1], want, tol)
+    np.testing.assert_array_equal(*outs[:2])
+
+
+@pytest.mark.parametrize("d, hq, tq", [(64, 2, 60), (128, 4, 50), (128, 4, 140)])
+def test_many_rows_of_a_ring_at_far_positions(gpu, d, hq, tq):
+    """Positions past 2^31 in a ring of 512, from the codes and over the copies."""
+    rng = np.random.default_rng(d)
+    n0, hkv = 3_000_000_019, 2
+    c = Cache(gpu, hkv, 512, d, True)
+    c.set_count(n0)
+    print(f"q4 far ring of many rows d={d} tq={tq}", flush=True)
+    for _ in range(6):
+        k, v = (draw((hkv, 100, d), rng, F16) for _ in range(2))
+        c.call(draw((2, 1, d), rng, F16), k, v, span=1)
+    q, k, v = draw((hq, tq, d), rng, F16), draw((hkv, tq, d), rng, F16), draw((hkv, tq, d), rng, F16)
+    got = c.call(q, k, v, F32, span=300)
+    want, tol = attend(q, *c.rows, visible(600, tq, tq, 0, 300), False)
+    check(got, want, tol)

@@ -22,7 +22,8 @@
 // scaled by a power of two, so that its largest value lies in [512, 1024) and none
 // that counts is lost (fp16 holds what is 2^-25 of it). An fp32 q enters as two
 // fp16 numbers. V enters as s n + m rounded to fp16 (one packed fma from the exact
-// n), the probabilities as two fp16 numbers (the second the rest that the first
+// n; as two numbers it would double both the unpacking, which the waves wait for,
+// and the products), the probabilities as two fp16 numbers (the second the rest that the first
 // leaves) and times 2^14, so that those far below the row's largest keep their
 // bits too (fp16 holds 2^-38 of it; unscaled, a key of 2^-25 was lost, and with
 // thousands of them what they bring): V's and the result's are then the only
