@@ -23,11 +23,11 @@
 // that counts is lost (fp16 holds what is 2^-25 of it). An fp32 q enters as two
 // fp16 numbers. V enters as s n + m rounded to fp16 (one packed fma from the exact
 // n; as two numbers it would double both the unpacking, which the waves wait for,
-// and the products), the probabilities as two fp16 numbers (the second the rest that the first
-// leaves) and times 2^14, so that those far below the row's largest keep their
-// bits too (fp16 holds 2^-38 of it; unscaled, a key of 2^-25 was lost, and with
-// thousands of them what they bring): V's and the result's are then the only
-// roundings to fp16: error against 64 bits 2.9e-4 of the result, of which the
+// and the products), the probabilities as two fp16 numbers (the second the rest
+// that the first leaves) and times 2^14, so that those far below the row's largest
+// keep their bits too (fp16 holds 2^-38 of it; unscaled, a key of 2^-25 was lost,
+// and with thousands of them what they bring): V's and the result's are then the
+// only roundings to fp16: error against 64 bits 2.9e-4 of the result, of which the
 // rounding of the result is 2.1e-4 (3.6e-4 with the probabilities in one number).
 //
 // A few rows that the call brings are rounded by the wave whose tile they are in,

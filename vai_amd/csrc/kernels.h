@@ -216,8 +216,8 @@ struct AttnParams {
     // most that many query tiles)
     uint32_t qt_tab[FA_WG_TAB];
     // A cache in 4 bits (attention_q4.hip): its planes; k / v then point at the
-    // fp16 copies the other kernels read, and the new rows, appended first,
-    // count as cached rows like any other.
+    // copies the other kernels read (fp16, or fp32 for the plain one), and the new
+    // rows, appended first, count as cached rows like any other.
     uint8_t* k4;
     uint8_t* v4;
     void* ws4;                    // the call's workspace
