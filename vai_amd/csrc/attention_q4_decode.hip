@@ -142,14 +142,17 @@ __global__ __launch_bounds__(256, q4_resident(DP, NQ, Q32)) void attention_q4_de
     uint8_t* kh = uniform_ptr((uint8_t*)p.k + hk * hb);
     uint8_t* vh = uniform_ptr((uint8_t*)p.v + hk * hb);
     LDS_AS uint8_t* ring = lds + wave * L::WAVE;
-    // the tokens of the block's rows (all of them where it goes over a head's end)
-    const bool over = (rend - 1) / p.tq != row0 / p.tq;
-    const uint32_t tok0 = over ? 0u : row0 % p.tq, tok1 = over ? p.tq - 1 : (rend - 1) % p.tq;
+    // the tokens of the block's rows (all of them where it is the only one or goes over a head's end)
+    uint32_t tok0 = 0, tok1 = p.tq - 1;
+    if (rows > p.rpb && (rend - 1) / p.tq == row0 / p.tq) {
+        tok0 = row0 % p.tq;
+        tok1 = (rend - 1) % p.tq;
+    }
     // this wave's tiles: first, first + step, .., and their places in the planes
     // (a ring's size is a multiple of 64: no tile wraps)
     const uint32_t step = p.units * NW, wrap = p.ring ? p.kv_rows / KT : 0xffffffffu;
     int64_t first = R.tb + unit * NW + wave, last = R.te;
-    if (p.n_new == 0) {   // only tiles that some row of the block sees (both bounds grow with the token)
+    if (p.n_new == 0 && rows > p.rpb) {   // only tiles that some row of the block sees (both bounds grow with the token)
         const int64_t beg = p.mask.key_start_cached(tok0, R.cached) / KT;
         last = std::min<int64_t>(last, (p.mask.key_end_cached(tok1, R.cached) + KT - 1) / KT);
         if (beg > first) first += ((uint32_t)(beg - first) + step - 1) / step * step;
@@ -513,17 +516,17 @@ static hipError_t q4_decode_launch_t(const AttnDecodeParams& p, hipStream_t s)
 // past them the copies for the flash kernel cost less than unpacking the codes for
 // 16 or 32 rows at a time. One pass, us, this way / over the copies, at 1000, 8000
 // and 120000 positions (8 KV heads, fp16 queries):
-//   D = 128, 68 rows   16.9 / 20.3   27.1 / 46.5   134 / 426
-//           128        21.3 / 21.9   31.8 / 46.5   171 / 426
-//           192        23.0 / 22.4   37.2 / 46.0   261 / 427
-//           256        24.2 / 22.0   41.2 / 45.8   322 / 427
+//   D = 128, 68 rows   16.8 / 20.3   27.3 / 46.5   133 / 426
+//           128        18.9 / 21.9   31.4 / 46.5   170 / 426
+//           192        23.0 / 22.4   37.4 / 46.0   260 / 427
+//           256        24.2 / 22.0   41.0 / 45.8   321 / 427
 //           384        27.4 / 26.3   55.4 / 46.1   498 / 429
-//   D = 64, 128        17.1 / 17.4   23.3 / 37.8   122 / 255
-//           256        19.5 / 17.5   30.9 / 38.0   227 / 255
-//   D = 256, 128       21.7 / 33.8   48.2 / 75.7   474 / 989
-//           256        27.6 / 34.6   79.2 / 75.4   927 / 989
-// fp32 queries: D = 128, 256 rows 20.9 / 22.9, 43.9 / 47.0, 420 / 428. One or two
-// KV heads: faster this way at 256 rows throughout (2 of 128, 120000: 95.4 / 116).
+//   D = 64, 128        16.1 / 17.4   23.2 / 37.8   122 / 255
+//           256        19.5 / 17.5   30.8 / 38.0   228 / 255
+//   D = 256, 128       21.6 / 33.8   48.1 / 75.7   471 / 989
+//           256        27.6 / 34.6   78.9 / 75.4   920 / 989
+// fp32 queries: D = 128, 256 rows 20.9 / 22.9, 43.7 / 47.0, 428 / 428. One or two
+// KV heads: faster this way at 256 rows throughout (2 of 128, 120000: 95.3 / 116).
 bool q4_few_rows(const AttnParams& p)
 {
     return p.head_dim % 8 == 0 && (uint64_t)(p.hq / p.hkv) * p.tq <= (p.kv_rows < 4096 ? 128 : 256) &&
@@ -552,11 +555,16 @@ void q4_decode_plan(AttnParams& p, uint32_t cus)
     p.dec_rpb = std::min<uint32_t>(p.dec_rows, dp == 256 || (dp == 128 && q32) ? 16 : 32);
     const uint32_t keys = p.span ? std::min<uint64_t>(p.kv_rows, (uint64_t)p.span + p.tq + 2 * fd::KT) : p.kv_rows;
     const uint32_t tiles = (keys + fd::KT - 1) / fd::KT, most = std::max<uint32_t>((tiles + fd::NW - 1) / fd::NW, 1);
-    const uint32_t blocks = p.hkv * ((p.dec_rows + p.dec_rpb - 1) / p.dec_rpb),
-                   wgs = cus * q4_resident(dp, p.dec_rpb > 16 ? 2 : 1, q32);
-    // (one round of the chip: a share more and its last workgroups run alone, 68 rows
-    // over 120000 positions 141 us instead of 132)
-    p.dec_units = std::min(std::min(std::max(wgs / blocks, 1u), most), AttnDecodeParams::MAX_UNITS);
+    const uint32_t blocks = p.hkv * ((p.dec_rows + p.dec_rpb - 1) / p.dec_rpb);
+    // shares in one round of the chip: one more and its last workgroups run alone, 68
+    // rows over 120000 positions 141 us instead of 132
+    const uint32_t chip = cus * q4_resident(dp, p.dec_rpb > 16 ? 2 : 1, q32);
+    uint32_t units = std::max(chip / blocks, 1u);
+    // 17 to 32 rows: a second workgroup a CU only where each wave still has four tiles
+    // (32 rows of D = 128, one / two: 8000 positions 18.3 / 20.3 us, 16000 22.7 / 24.4,
+    // 30000 31.0 / 30.5, 120000 74 / 58)
+    if (p.dec_rpb > 16) units = std::min(units, std::max(std::max(cus / blocks, 1u), tiles / (4 * fd::NW)));
+    p.dec_units = std::min(std::min(units, most), AttnDecodeParams::MAX_UNITS);
 }
 
 size_t q4_decode_workspace(const AttnParams& p) { return attention_decode_workspace(p, p.dec_units); }
