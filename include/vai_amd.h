@@ -432,6 +432,152 @@ typedef struct {
 vai_status vai_qk_norm_rope_launch(const vai_qk_norm_rope_args* args, vai_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Many sequences in one forward, over a KV cache in pages. No counterpart in the
+ * reference, whose cache holds one sequence.
+ *
+ * A batch is ragged: the new tokens of sequence s are rows seq_start[s] ..
+ * seq_start[s + 1] - 1 of the token-major arrays (increasing; a sequence may
+ * bring none). Rows before seq_start[0] or from seq_start[sequences] on are no
+ * sequence's: what they hold is not read, and what outputs hold there stays.
+ * Before the call sequence s held counts[s] positions; its new token t is at
+ * position counts[s] + t.
+ * Position p of sequence s lies in page page_table[s][p / page_size], slot p %
+ * page_size. A page holds [hkv, page_size, head_dim] values; pages start
+ * page_stride elements apart (0: packed; more lets K and V share an allocation).
+ * Any page_size; whole 16s (and head dims of whole 8s, 16-byte aligned fp16
+ * pages) take the fast kernels. Sequences may share pages that none of them
+ * appends to. An entry that is no page (>= num_pages; unused entries hold what
+ * they like), and positions past max_pages * page_size, hold nothing: rows
+ * appended there are dropped, queries do not see them.
+ * seq_start, counts and page_table are device uint32 arrays, read when the
+ * kernels run: a recorded graph follows them. Neither call writes them.
+ * sequences <= 4096, max_pages * page_size <= 2^30.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    void* k_pages;
+    void* v_pages;
+    const uint32_t* page_table;   /* [sequences, max_pages] */
+    const uint32_t* seq_start;    /* [sequences + 1] */
+    const uint32_t* counts;       /* [sequences] */
+    uint64_t page_stride;         /* elements from one page to the next; 0: hkv * page_size * head_dim */
+    uint32_t sequences, num_pages, page_size, max_pages;
+    int32_t page_dtype;           /* VAI_DTYPE_F32 or VAI_DTYPE_F16, K and V alike */
+} vai_kv_pages;
+
+/* From the fused query / key / value projection to the pages: the RMS norm of
+ * each query and key head and the position rotation as in vai_qk_norm_rope_args
+ * (norm, eps, weights, weight_offset, rope, rot_dim, theta, inv_freq), at the
+ * tokens' positions; keys and values go to their pages, queries to q_out.
+ *   qkv [tokens] rows of row_stride elements (0: (hq + 2 hkv) head_dim): hq query
+ *   heads, then hkv key heads, then hkv value heads, in i_dtype; q_out [tokens,
+ *   hq, head_dim] in o_dtype, disjoint from qkv, or NULL: queries stay.
+ *   head_dim <= 2048. fp32 until each value's one rounding.
+ * Two tokens of a call that land in one slot (a page twice in the table) leave
+ * one of the two there. */
+typedef struct {
+    void* q_out;
+    const void* qkv;
+    const void* q_weight;
+    const void* k_weight;
+    const float* inv_freq;
+    vai_kv_pages pages;
+    uint32_t tokens, hq, hkv, head_dim;
+    uint32_t row_stride;
+    int32_t i_dtype, o_dtype, w_dtype;
+    uint32_t norm;
+    float eps, weight_offset;
+    uint32_t rope;
+    uint32_t rot_dim;
+    float theta;
+} vai_paged_append_args;
+
+vai_status vai_paged_append_launch(const vai_paged_append_args* args, vai_stream_t stream);
+
+/* Attention of a ragged batch over the pages, its own rows appended before:
+ *   O[i,h,:] = sum_j softmax_j(scale * Q[i,h,:].K[j,h/g,:]) V[j,h/g,:], g = hq/hkv,
+ * over positions 0 .. counts[s] + n_s - 1 of row i's sequence. causal hides the
+ * positions after the query's own; span > 0 those up to its own - span. A query
+ * that sees none (or only scores of -infinity) gives zeros.
+ *   q [tokens] rows of q_stride elements (0: hq * head_dim) of hq heads in
+ *   q_dtype; out [tokens, hq, head_dim] in o_dtype. head_dim <= 256.
+ *   max_new: no sequence brings more tokens (0: tokens). It only chooses kernels
+ *   and their workspace: sequences that bring more are attended too.
+ *   Statistics and sums are fp32. Over fp16 pages an fp32 q enters the matrix
+ *   cores as two fp16 numbers, and so do the probabilities where out is fp32;
+ *   for fp16 out they are rounded to one. fp32 pages, head dims of no whole 8s
+ *   and pages of no whole 16s are attended in fp32 throughout.
+ *   What hidden positions hold does not matter. A value of V that is not finite
+ *   makes its column NaN for the queries that see it.
+ * Calls that overlap in time need a workspace each (vai_paged_attention_
+ * workspace_size() bytes, 16-byte aligned). The result does not depend on what
+ * it held. */
+typedef struct {
+    void* out;
+    const void* q;
+    void* workspace;
+    size_t workspace_bytes;
+    vai_kv_pages pages;
+    uint32_t tokens, max_new, hq, hkv, head_dim;
+    uint32_t q_stride;
+    int32_t o_dtype, q_dtype;
+    float scale;                  /* 0: 1/sqrt(head_dim) */
+    uint32_t causal;
+    uint32_t span;
+} vai_paged_attention_args;
+
+vai_status vai_paged_attention_launch(const vai_paged_attention_args* args, vai_stream_t stream);
+size_t vai_paged_attention_workspace_size(const vai_paged_attention_args* args);
+
+/* ---------------------------------------------------------------------------
+ * Drafted tokens against the target model's probabilities (speculative
+ * sampling). No counterpart in the reference. Sequence s feeds rows seq_start[s]
+ * .. seq_start[s + 1] - 1: its pending token, then its drafts; row r's logits
+ * are those of the token after row r. For r from the sequence's first row on, with
+ * x = tokens[r + 1], p_r = softmax(target[r] / T), q_r = softmax(draft[r] / T), or
+ * 1 at x alone where draft is NULL:
+ *   x is kept if uniform[r] * q_r(x) < p_r(x); the first that is not ends the
+ *   sequence, and its place takes the lowest j with
+ *     sum_{i <= j} w_i > uniform[last row] * sum_i w_i,  w = max(p_r - q_r, 0)
+ *   (w = p_r if that is 0 everywhere); where all are kept, the token after the
+ *   last row is drawn so with w = p of the last row.
+ * T = temperature[s] (NULL: 1). T = 0: p and q are 1 at the lowest index of the
+ * largest logit. Everything is computed in 64 bits. Logits of -infinity have no
+ * probability. A row that is needed and holds a NaN or +infinity, or nothing
+ * above -infinity, ends its sequence with the token VAI_NO_TOKEN.
+ *   target, draft: [rows] rows of target_stride / draft_stride elements (0:
+ *   vocab); draft's row of a sequence's last token is not read. tokens [rows]
+ *   uint32, uniform [rows] fp32 in [0, 1); a token >= vocab has no probability.
+ *   out_tokens [rows]: row seq_start[s] + i the token at place i, VAI_NO_TOKEN
+ *   past the last; accepted [sequences]: drafts kept. new_counts (may be NULL, or
+ *   counts itself): counts[s] + accepted + 1, the positions of the cache that
+ *   hold. A sequence without rows: accepted 0, its count unchanged. The arrays are
+ *   read when the kernels run. sequences <= 4096, rows and vocab < 2^24.
+ * The workspace (16-byte aligned) as for vai_paged_attention_launch.
+ * ------------------------------------------------------------------------- */
+#define VAI_NO_TOKEN 0xffffffffu
+
+typedef struct {
+    uint32_t* out_tokens;
+    uint32_t* accepted;
+    uint32_t* new_counts;
+    const void* target;
+    const void* draft;            /* NULL: drafts without probabilities of their own */
+    const uint32_t* tokens;
+    const float* uniform;
+    const float* temperature;
+    const uint32_t* seq_start;    /* [sequences + 1], as in vai_kv_pages */
+    const uint32_t* counts;       /* [sequences]; needed with new_counts */
+    void* workspace;
+    size_t workspace_bytes;
+    uint32_t sequences, rows, vocab;
+    uint32_t target_stride, draft_stride;
+    int32_t target_dtype, draft_dtype;
+} vai_verify_drafts_args;
+
+vai_status vai_verify_drafts_launch(const vai_verify_drafts_args* args, vai_stream_t stream);
+size_t vai_verify_drafts_workspace_size(const vai_verify_drafts_args* args);
+
+/* ---------------------------------------------------------------------------
  * Device memory and streams: what the host side (vai::Tensor's pooled
  * buffers, the reference's eva::Buffer role) and the tests use.
  * ------------------------------------------------------------------------- */

@@ -17,6 +17,7 @@ ROPE = {"NONE": 0, "HALVES": 1, "NEIGHBOURS": 2}
 EPILOGUES = {"NONE": 0, "RELU": 1, "GELU": 2, "GELU_TANH": 3, "SILU": 4, "SIGMOID": 5}
 RESIDUAL_ORDERS = {"AFTER_EPILOGUE": 0, "BEFORE_EPILOGUE": 1}
 MAX_CAUSAL_BLOCKS = 32
+NO_TOKEN = 0xffffffff
 
 # Every symbol include/vai_amd.h declares (checked by tests/test_capi_symbols.py).
 EXPORTS = [
@@ -27,6 +28,8 @@ EXPORTS = [
     "vai_attn_scores_launch", "vai_attention_launch", "vai_attention_workspace_size",
     "vai_attention_cache_bytes", "vai_attention_cache_read",
     "vai_linear_i8_launch", "vai_linear_i8_workspace_size", "vai_quantize_i8_launch", "vai_qk_norm_rope_launch",
+    "vai_paged_append_launch", "vai_paged_attention_launch", "vai_paged_attention_workspace_size",
+    "vai_verify_drafts_launch", "vai_verify_drafts_workspace_size",
     "vai_device_count", "vai_set_device", "vai_malloc", "vai_free", "vai_memcpy_h2d", "vai_memcpy_d2h",
     "vai_memcpy_d2d", "vai_memset", "vai_stream_create", "vai_stream_destroy", "vai_stream_sync",
     "vai_device_sync", "vai_status_string", "vai_event_create", "vai_event_destroy", "vai_event_record",
@@ -126,6 +129,50 @@ class QkNormRopeArgs(ctypes.Structure):
     ]
 
 
+class KvPages(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+        ("seq_start", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("page_stride", ctypes.c_uint64),
+        ("sequences", ctypes.c_uint32), ("num_pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+        ("max_pages", ctypes.c_uint32), ("page_dtype", ctypes.c_int32),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("q_out", ctypes.c_void_p), ("qkv", ctypes.c_void_p), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+        ("inv_freq", ctypes.c_void_p), ("pages", KvPages),
+        ("tokens", ctypes.c_uint32), ("hq", ctypes.c_uint32), ("hkv", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+        ("row_stride", ctypes.c_uint32),
+        ("i_dtype", ctypes.c_int32), ("o_dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32),
+        ("norm", ctypes.c_uint32), ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
+        ("rope", ctypes.c_uint32), ("rot_dim", ctypes.c_uint32), ("theta", ctypes.c_float),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("out", ctypes.c_void_p), ("q", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t), ("pages", KvPages),
+        ("tokens", ctypes.c_uint32), ("max_new", ctypes.c_uint32), ("hq", ctypes.c_uint32), ("hkv", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32), ("q_stride", ctypes.c_uint32),
+        ("o_dtype", ctypes.c_int32), ("q_dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("causal", ctypes.c_uint32), ("span", ctypes.c_uint32),
+    ]
+
+
+class VerifyDraftsArgs(ctypes.Structure):
+    _fields_ = [
+        ("out_tokens", ctypes.c_void_p), ("accepted", ctypes.c_void_p), ("new_counts", ctypes.c_void_p),
+        ("target", ctypes.c_void_p), ("draft", ctypes.c_void_p), ("tokens", ctypes.c_void_p),
+        ("uniform", ctypes.c_void_p), ("temperature", ctypes.c_void_p), ("seq_start", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("sequences", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("vocab", ctypes.c_uint32),
+        ("target_stride", ctypes.c_uint32), ("draft_stride", ctypes.c_uint32),
+        ("target_dtype", ctypes.c_int32), ("draft_dtype", ctypes.c_int32),
+    ]
+
+
 class VaiError(RuntimeError):
     pass
 
@@ -167,6 +214,13 @@ def lib():
         L.vai_linear_i8_workspace_size.restype = sz
         L.vai_quantize_i8_launch.argtypes = [vp, vp, vp, i32, u32, u32, vp]
         L.vai_qk_norm_rope_launch.argtypes = [ctypes.POINTER(QkNormRopeArgs), vp]
+        L.vai_paged_append_launch.argtypes = [ctypes.POINTER(PagedAppendArgs), vp]
+        L.vai_paged_attention_launch.argtypes = [ctypes.POINTER(PagedAttentionArgs), vp]
+        L.vai_paged_attention_workspace_size.argtypes = [ctypes.POINTER(PagedAttentionArgs)]
+        L.vai_paged_attention_workspace_size.restype = sz
+        L.vai_verify_drafts_launch.argtypes = [ctypes.POINTER(VerifyDraftsArgs), vp]
+        L.vai_verify_drafts_workspace_size.argtypes = [ctypes.POINTER(VerifyDraftsArgs)]
+        L.vai_verify_drafts_workspace_size.restype = sz
         L.vai_malloc.argtypes = [ctypes.POINTER(vp), sz]
         L.vai_free.argtypes = [vp]
         L.vai_memcpy_h2d.argtypes = [vp, vp, sz, vp]
@@ -575,6 +629,111 @@ def attention_cache_read(k_out, v_out, k_cache, v_cache, first_row=0, stream=Non
     check(lib().vai_attention_cache_read(ctypes.byref(a), stream), "vai_attention_cache_read")
     check(lib().vai_stream_sync(stream), "sync")   # the caller may drop its argument buffers on return
     return k_out, v_out
+
+
+def kv_pages(k_pages, v_pages, page_table, seq_start, counts, *, page_stride=0):
+    """k_pages, v_pages [num_pages, Hkv, page_size, D] of one dtype; page_table [sequences, max_pages], seq_start
+    [sequences + 1] and counts [sequences]: device 32-bit integers."""
+    p = KvPages()
+    p.k_pages, p.v_pages, p.page_table = k_pages.ptr, v_pages.ptr, page_table.ptr
+    p.seq_start, p.counts = seq_start.ptr, counts.ptr
+    p.sequences, p.max_pages = page_table.shape
+    p.num_pages, p.page_size = k_pages.shape[0], k_pages.shape[2]
+    if k_pages.code != v_pages.code or tuple(k_pages.shape) != tuple(v_pages.shape):
+        raise VaiError("kv_pages: K's and V's pages share a dtype and a shape")
+    if tuple(seq_start.shape) != (p.sequences + 1,) or tuple(counts.shape) != (p.sequences,):
+        raise VaiError(f"kv_pages: seq_start [{p.sequences + 1}] and counts [{p.sequences}] expected")
+    p.page_dtype, p.page_stride = k_pages.code, page_stride
+    p._keep = (k_pages, v_pages, page_table, seq_start, counts)
+    p._heads, p._dim = k_pages.shape[1], k_pages.shape[3]
+    return p
+
+
+def paged_append_args(q, qkv, pages, q_weight=None, k_weight=None, *, norm=True, eps=1e-6, weight_offset=0.0,
+                      pairs="HALVES", rot_dim=0, theta=10000.0, inv_freq=None, row_stride=0):
+    """q [tokens, Hq, D] out; qkv [tokens, (Hq + 2 Hkv) D] in; pages: a kv_pages()."""
+    T, Hq, D = q.shape
+    if D != pages._dim:
+        raise VaiError(f"paged_append: heads of {D} values, pages of {pages._dim}")
+    a = PagedAppendArgs()
+    a.q_out, a.qkv, a.inv_freq = q.ptr, qkv.ptr, _ptr(inv_freq)
+    a.q_weight, a.k_weight = _ptr(q_weight), _ptr(k_weight)
+    a.pages = pages
+    a.tokens, a.hq, a.hkv, a.head_dim, a.row_stride = T, Hq, pages._heads, D, row_stride
+    a.i_dtype, a.o_dtype = qkv.code, q.code
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    if any(w.code != weights[0].code for w in weights):
+        raise VaiError("paged_append: the weights share a dtype")
+    a.w_dtype = weights[0].code if weights else NONE
+    a.norm, a.eps, a.weight_offset = 1 if norm else 0, eps, weight_offset
+    a.rope, a.rot_dim, a.theta = ROPE[pairs], rot_dim, theta
+    a._keep = (q, qkv, pages, q_weight, k_weight, inv_freq)
+    return a
+
+
+def paged_append(q, qkv, pages, q_weight=None, k_weight=None, stream=None, **kw):
+    a = paged_append_args(q, qkv, pages, q_weight, k_weight, **kw)
+    check(lib().vai_paged_append_launch(ctypes.byref(a), stream), "vai_paged_append_launch")
+    check(lib().vai_stream_sync(stream), "sync")   # the caller may drop its argument buffers on return
+    return q
+
+
+def paged_attention_args(out, q, pages, *, scale=None, causal=True, span=0, max_new=0, q_stride=0):
+    """out, q [tokens, Hq, D]; pages: a kv_pages() that holds the tokens' rows already."""
+    T, Hq, D = out.shape
+    if D != pages._dim:
+        raise VaiError(f"paged_attention: heads of {D} values, pages of {pages._dim}")
+    a = PagedAttentionArgs()
+    a.out, a.q, a.pages = out.ptr, q.ptr, pages
+    a.tokens, a.max_new, a.hq, a.hkv, a.head_dim, a.q_stride = T, max_new, Hq, pages._heads, D, q_stride
+    a.o_dtype, a.q_dtype = out.code, q.code
+    a.scale = 0.0 if scale is None else float(scale)
+    a.causal, a.span = 1 if causal else 0, span
+    a._keep = (out, q, pages)
+    return a
+
+
+def paged_attention(out, q, pages, stream=None, **kw):
+    a = paged_attention_args(out, q, pages, **kw)
+    need = lib().vai_paged_attention_workspace_size(ctypes.byref(a))
+    ws = DeviceArray((need,), np.uint8) if need else None
+    if ws is not None:
+        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
+    check(lib().vai_paged_attention_launch(ctypes.byref(a), stream), "vai_paged_attention_launch")
+    check(lib().vai_stream_sync(stream), "sync")   # the caller may drop its argument buffers on return
+    return out
+
+
+def verify_drafts_args(out_tokens, accepted, target, tokens, uniform, seq_start, *, draft=None, temperature=None,
+                       counts=None, new_counts=None):
+    """out_tokens, tokens, uniform [rows]; target, draft [rows, vocab]; accepted, temperature, counts, new_counts
+    [sequences]; seq_start [sequences + 1]. Tokens and counts are device 32-bit integers."""
+    rows, vocab = target.shape
+    n = seq_start.shape[0] - 1
+    if any(x.shape[0] != rows for x in (out_tokens, tokens, uniform)) or (draft is not None and tuple(draft.shape) != (rows, vocab)):
+        raise VaiError(f"verify_drafts: {rows} rows expected")
+    if any(x is not None and x.shape[0] != n for x in (accepted, temperature, counts, new_counts)):
+        raise VaiError(f"verify_drafts: {n} sequences expected")
+    a = VerifyDraftsArgs()
+    a.out_tokens, a.accepted, a.target, a.draft = out_tokens.ptr, accepted.ptr, target.ptr, _ptr(draft)
+    a.tokens, a.uniform, a.temperature, a.seq_start = tokens.ptr, uniform.ptr, _ptr(temperature), seq_start.ptr
+    a.counts, a.new_counts = _ptr(counts), _ptr(new_counts)
+    a.sequences, a.rows, a.vocab = n, rows, vocab
+    a.target_dtype = target.code
+    a.draft_dtype = draft.code if draft is not None else NONE
+    a._keep = (out_tokens, accepted, target, tokens, uniform, seq_start, draft, temperature, counts, new_counts)
+    return a
+
+
+def verify_drafts(out_tokens, accepted, target, tokens, uniform, seq_start, stream=None, **kw):
+    a = verify_drafts_args(out_tokens, accepted, target, tokens, uniform, seq_start, **kw)
+    need = lib().vai_verify_drafts_workspace_size(ctypes.byref(a))
+    ws = DeviceArray((need,), np.uint8) if need else None
+    if ws is not None:
+        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
+    check(lib().vai_verify_drafts_launch(ctypes.byref(a), stream), "vai_verify_drafts_launch")
+    check(lib().vai_stream_sync(stream), "sync")   # the caller may drop its argument buffers on return
+    return out_tokens, accepted
 
 
 def synchronize():

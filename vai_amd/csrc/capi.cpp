@@ -675,6 +675,127 @@ vai_status vai_qk_norm_rope_launch(const vai_qk_norm_rope_args* a, vai_stream_t 
     return hip_status(qk_norm_rope_launch(p, a->theta, (hipStream_t)stream));
 }
 
+// The pages of a ragged batch (vai_kv_pages).
+static vai_status kv_pages_params(const vai_kv_pages& a, uint32_t hkv, uint32_t head_dim, KvPages& g)
+{
+    if (!a.k_pages || !a.v_pages || !a.page_table || !a.seq_start || !a.counts) return VAI_ERR_INVALID_ARG;
+    if (!dtype_ok(a.page_dtype)) return VAI_ERR_DTYPE;
+    if (a.sequences == 0 || a.num_pages == 0 || a.page_size == 0 || a.max_pages == 0) return VAI_ERR_SHAPE;
+    if (a.sequences > KvPages::MAX_SEQUENCES || (uint64_t)a.max_pages * a.page_size > KvPages::MAX_POSITIONS ||
+        hkv > 65535 || head_dim > 2048)
+        return VAI_ERR_UNSUPPORTED;
+    const uint64_t page = (uint64_t)hkv * head_dim * a.page_size, stride = a.page_stride ? a.page_stride : page;
+    if (stride < page) return VAI_ERR_SHAPE;
+    if (stride > (1ull << 60) / a.num_pages) return VAI_ERR_UNSUPPORTED;   // elements' addresses stay in 64 bits
+    g = KvPages{};
+    g.k = a.k_pages; g.v = a.v_pages; g.table = a.page_table; g.start = a.seq_start; g.counts = a.counts;
+    g.stride = stride;
+    g.sequences = a.sequences; g.num_pages = a.num_pages; g.page_size = a.page_size; g.max_pages = a.max_pages;
+    g.dtype = a.page_dtype;
+    return VAI_OK;
+}
+
+vai_status vai_paged_append_launch(const vai_paged_append_args* a, vai_stream_t stream)
+{
+    if (!a || !a->qkv) return VAI_ERR_INVALID_ARG;
+    if (!dtype_ok(a->i_dtype) || (a->q_out && !dtype_ok(a->o_dtype))) return VAI_ERR_DTYPE;
+    if ((a->q_weight || a->k_weight) && !dtype_ok(a->w_dtype)) return VAI_ERR_DTYPE;
+    if (a->rope > VAI_ROPE_NEIGHBOURS || a->norm > 1) return VAI_ERR_INVALID_ARG;
+    if (a->tokens == 0 || a->hq == 0 || a->hkv == 0 || a->head_dim == 0) return VAI_ERR_SHAPE;
+    if (a->head_dim > PagedAppendParams::MAX_DIM || a->hq > 65535 || a->tokens >= 1u << 31) return VAI_ERR_UNSUPPORTED;
+    PagedAppendParams p{};
+    if (vai_status st = kv_pages_params(a->pages, a->hkv, a->head_dim, p.pages); st != VAI_OK) return st;
+    const uint64_t row = (uint64_t)(a->hq + 2 * a->hkv) * a->head_dim;
+    if (row > UINT32_MAX || (a->row_stride && a->row_stride < row)) return VAI_ERR_SHAPE;
+    const uint32_t rot = a->rope == VAI_ROPE_NONE ? 0u : a->rot_dim ? a->rot_dim : a->head_dim;
+    if (rot > a->head_dim || rot % 2 != 0) return VAI_ERR_SHAPE;
+    if (rot && !a->inv_freq && !(a->theta > 0.f && a->theta <= 3.4028235e38f)) return VAI_ERR_INVALID_ARG;
+    if (a->norm && !(a->eps >= 0.f)) return VAI_ERR_INVALID_ARG;
+    p.q_out = a->q_out; p.qkv = a->qkv;
+    p.q_weight = a->norm ? a->q_weight : nullptr; p.k_weight = a->norm ? a->k_weight : nullptr;
+    p.inv_freq = a->inv_freq;
+    p.i_dtype = a->i_dtype; p.o_dtype = a->o_dtype; p.w_dtype = a->w_dtype;
+    p.tokens = a->tokens; p.hq = a->hq; p.hkv = a->hkv; p.head_dim = a->head_dim;
+    p.row_stride = a->row_stride ? a->row_stride : (uint32_t)row;
+    p.norm = a->norm; p.neighbours = a->rope == VAI_ROPE_NEIGHBOURS; p.rot_dim = rot;
+    p.eps = a->eps; p.weight_offset = a->weight_offset;
+    return hip_status(paged_append_launch(p, a->theta, (hipStream_t)stream));
+}
+
+static vai_status paged_attention_params(const vai_paged_attention_args* a, PagedAttnParams& p)
+{
+    if (!a || !a->out || !a->q) return VAI_ERR_INVALID_ARG;
+    if (!dtype_ok(a->q_dtype) || !dtype_ok(a->o_dtype)) return VAI_ERR_DTYPE;
+    if (a->tokens == 0 || a->hq == 0 || a->hkv == 0 || a->head_dim == 0 || a->hq % a->hkv != 0) return VAI_ERR_SHAPE;
+    if (a->head_dim > 256 || (uint64_t)a->tokens * a->hq >= 1ull << 31) return VAI_ERR_UNSUPPORTED;
+    p = PagedAttnParams{};
+    if (vai_status st = kv_pages_params(a->pages, a->hkv, a->head_dim, p.pages); st != VAI_OK) return st;
+    if ((uint64_t)a->hq * a->head_dim > UINT32_MAX || (a->q_stride && a->q_stride < a->hq * a->head_dim)) return VAI_ERR_SHAPE;
+    if (a->causal > 1 || a->scale != a->scale) return VAI_ERR_INVALID_ARG;
+    p.out = a->out; p.q = a->q;
+    p.o_dtype = a->o_dtype; p.q_dtype = a->q_dtype;
+    p.tokens = a->tokens; p.max_new = a->max_new ? std::min(a->max_new, a->tokens) : a->tokens;
+    p.hq = a->hq; p.hkv = a->hkv; p.head_dim = a->head_dim;
+    p.q_stride = a->q_stride ? a->q_stride : a->hq * a->head_dim;
+    p.scale = a->scale != 0.f ? a->scale : 1.0f / std::sqrt((float)a->head_dim);
+    p.causal = a->causal; p.span = a->span;
+    return paged_attention_plan(p, plan_cus()) ? VAI_OK : VAI_ERR_UNSUPPORTED;
+}
+
+size_t vai_paged_attention_workspace_size(const vai_paged_attention_args* a)
+{
+    PagedAttnParams p;
+    return paged_attention_params(a, p) == VAI_OK ? paged_attention_workspace(p) : 0;
+}
+
+vai_status vai_paged_attention_launch(const vai_paged_attention_args* a, vai_stream_t stream)
+{
+    PagedAttnParams p;
+    if (vai_status st = paged_attention_params(a, p); st != VAI_OK) return st;
+    if (!a->workspace || a->workspace_bytes < paged_attention_workspace(p)) return VAI_ERR_WORKSPACE;
+    if ((uintptr_t)a->workspace % 16 != 0) return VAI_ERR_INVALID_ARG;
+    paged_attention_set_workspace(p, a->workspace);
+    return hip_status(paged_attention_launch(p, (hipStream_t)stream));
+}
+
+static vai_status verify_params(const vai_verify_drafts_args* a, VerifyParams& p)
+{
+    if (!a || !a->out_tokens || !a->accepted || !a->target || !a->tokens || !a->uniform || !a->seq_start)
+        return VAI_ERR_INVALID_ARG;
+    if (a->new_counts && !a->counts) return VAI_ERR_INVALID_ARG;
+    if (!dtype_ok(a->target_dtype) || (a->draft && !dtype_ok(a->draft_dtype))) return VAI_ERR_DTYPE;
+    if (a->sequences == 0 || a->rows == 0 || a->vocab == 0) return VAI_ERR_SHAPE;
+    if ((a->target_stride && a->target_stride < a->vocab) || (a->draft && a->draft_stride && a->draft_stride < a->vocab))
+        return VAI_ERR_SHAPE;
+    if (a->sequences > KvPages::MAX_SEQUENCES || a->rows >= 1u << 24 || a->vocab >= 1u << 24) return VAI_ERR_UNSUPPORTED;
+    if ((uint64_t)a->rows * ((a->vocab + 4095) / 4096) >= 1u << 31) return VAI_ERR_UNSUPPORTED;   // (the grid)
+    p = VerifyParams{};
+    p.out_tokens = a->out_tokens; p.accepted = a->accepted; p.new_counts = a->new_counts;
+    p.target = a->target; p.draft = a->draft; p.tokens = a->tokens; p.uniform = a->uniform;
+    p.temperature = a->temperature; p.start = a->seq_start; p.counts = a->counts;
+    p.sequences = a->sequences; p.rows = a->rows; p.vocab = a->vocab;
+    p.target_stride = a->target_stride ? a->target_stride : a->vocab;
+    p.draft_stride = a->draft_stride ? a->draft_stride : a->vocab;
+    p.target_dtype = a->target_dtype; p.draft_dtype = a->draft_dtype;
+    return VAI_OK;
+}
+
+size_t vai_verify_drafts_workspace_size(const vai_verify_drafts_args* a)
+{
+    VerifyParams p;
+    return verify_params(a, p) == VAI_OK ? verify_workspace(p) : 0;
+}
+
+vai_status vai_verify_drafts_launch(const vai_verify_drafts_args* a, vai_stream_t stream)
+{
+    VerifyParams p;
+    if (vai_status st = verify_params(a, p); st != VAI_OK) return st;
+    if (!a->workspace || a->workspace_bytes < verify_workspace(p)) return VAI_ERR_WORKSPACE;
+    if ((uintptr_t)a->workspace % 16 != 0) return VAI_ERR_INVALID_ARG;
+    p.workspace = a->workspace;
+    return hip_status(verify_launch(p, (hipStream_t)stream));
+}
+
 // Rows of 8-bit integers: weights start every 16 bytes, the call's own rounding
 // of X every 128 (whole blocks of the kernels).
 static uint32_t i8_row(uint32_t K) { return (K + 15) / 16 * 16; }

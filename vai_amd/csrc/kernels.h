@@ -311,6 +311,76 @@ struct QkNormRopeParams {
 };
 hipError_t qk_norm_rope_launch(QkNormRopeParams p, float theta, hipStream_t s);
 
+// A ragged batch over a KV cache in pages: as vai_kv_pages.
+struct KvPages {
+    void* k;
+    void* v;
+    const uint32_t* table;        // [sequences, max_pages]
+    const uint32_t* start;        // [sequences + 1]
+    const uint32_t* counts;       // [sequences]
+    uint64_t stride;              // elements from one page to the next
+    uint32_t sequences, num_pages, page_size, max_pages;
+    int dtype;
+    static constexpr uint32_t MAX_SEQUENCES = 4096;
+    static constexpr uint64_t MAX_POSITIONS = 1u << 30;
+};
+
+// Head norms and the position rotation into pages (paged_append.hip).
+struct PagedAppendParams {
+    static constexpr uint32_t MAX_DIM = QkNormRopeParams::MAX_DIM;
+    void* q_out;                  // [tokens, hq, head_dim], or null: queries stay
+    const void* qkv;              // [tokens] rows of row_stride elements: hq + 2 hkv heads
+    const void* q_weight;         // [head_dim] or null: ones
+    const void* k_weight;
+    const float* inv_freq;        // [rot_dim / 2], or null: the tables
+    KvPages pages;
+    int i_dtype, o_dtype, w_dtype;
+    uint32_t tokens, hq, hkv, head_dim, row_stride;
+    uint32_t norm, neighbours, rot_dim;   // rot_dim 0: no rotation
+    float eps, weight_offset;
+    double turn_hi[MAX_DIM / 32], turn_lo[16];
+};
+hipError_t paged_append_launch(PagedAppendParams p, float theta, hipStream_t s);
+
+// Attention of a ragged batch over pages (paged_attention.hip).
+struct PagedAttnParams {
+    void* out;                    // [tokens, hq, head_dim]
+    const void* q;                // [tokens] rows of q_stride elements
+    KvPages pages;
+    int o_dtype, q_dtype;
+    uint32_t tokens, max_new, hq, hkv, head_dim, q_stride;
+    float scale;
+    uint32_t causal, span;
+    // set by the plan: workgroups, and their partial results in the workspace
+    uint32_t dp, wgs;
+    uint32_t* ws_plan;            // [sequences + 2]
+    float* ws_o;                  // [2 wgs][rows of a unit][dp]
+    float* ws_ml;                 // [2 wgs][rows of a unit][2]
+};
+bool paged_attention_plan(PagedAttnParams& p, uint32_t cus);   // false: too large a grid of tiles
+size_t paged_attention_workspace(const PagedAttnParams& p);
+void paged_attention_set_workspace(PagedAttnParams& p, void* ws);
+hipError_t paged_attention_launch(const PagedAttnParams& p, hipStream_t s);
+
+// Drafted tokens against the target's probabilities (verify_drafts.hip).
+struct VerifyParams {
+    uint32_t* out_tokens;
+    uint32_t* accepted;
+    uint32_t* new_counts;
+    const void* target;
+    const void* draft;
+    const uint32_t* tokens;
+    const float* uniform;
+    const float* temperature;
+    const uint32_t* start;
+    const uint32_t* counts;
+    uint32_t sequences, rows, vocab, target_stride, draft_stride;
+    int target_dtype, draft_dtype;
+    void* workspace;
+};
+size_t verify_workspace(const VerifyParams& p);
+hipError_t verify_launch(const VerifyParams& p, hipStream_t s);
+
 // Linear over 8-bit weights (linear_i8.hip).
 struct LinearI8Params {
     void* out;

@@ -1,0 +1,232 @@
+// paged_attention.hip -- attention of a ragged batch over a KV cache in pages:
+// the fp32 kernel for any head dim, page size and dtype, the merge of partial
+// results, and which kernel a call takes.
+//
+// The fp32 kernel: v_mfma_f32_16x16x4_f32 throughout, operands from memory to
+// registers. S^T = K Q^T over 16 keys x 16 query rows: lane (c16, g) reads 4
+// neighbouring values of key c16 at a time, which are its k's of four steps, and
+// gets the scores of row c16 with keys 4 g ..+3. Those are, as they stand, the
+// lane's P^T operands of O^T += V^T P^T when step r of it takes key 4 g + r. No
+// value moves between lanes but for the row's maximum and sum.
+#include "paged_plan.h"
+
+#include "launch_once.h"
+
+namespace vai_dev {
+
+template <int DP, typename T>
+__global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParams p)
+{
+    using namespace pg;
+    constexpr int KB = DP / 16, RB = 16;
+    extern __shared__ float4v paged_lds[];
+    __shared__ uint32_t pre[KvPages::MAX_SEQUENCES + 1];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t c16 = lane & 15, g = lane >> 4, D = p.head_dim, group = p.hq / p.hkv;
+    const KvPages& pgs = p.pages;
+    const float sl2 = p.scale * 1.4426950408889634f;   // scores in log2 units
+    plan_line(p, RB, pre);
+    walk<RB>(p, pre, [&](const Piece& u) {
+        const uint32_t rows = u.q.n * group, row = min(u.rb * RB + c16, rows - 1);
+        const uint32_t tok = row / group, pos = u.q.held + tok;
+        const uint32_t kbeg = first_key(p, pos), kend = p.causal ? min(pos + 1, u.q.live) : u.q.live;
+        const size_t qat = (size_t)(u.q.first + tok) * p.q_stride + (size_t)(u.hk * group + row % group) * D;
+        float4v qf[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t d = 16 * b + 4 * g + i;
+                qf[b][i] = d < D ? ld(p.q, p.q_dtype, qat + d) : 0.f;
+            }
+        float m[1] = {-__builtin_inff()}, l[1] = {0.f};
+        float4v o[1][KB];
+#pragma unroll
+        for (int d = 0; d < KB; ++d) o[0][d] = (float4v)0.f;
+        const uint32_t see = first_key(p, u.q.held);     // no row sees a position before it
+        for (uint32_t t = u.t0 + wave; t < u.t1; t += NW)
+            for (uint32_t j0 = t * KT; j0 < (t + 1) * KT; j0 += 16) {
+                // the lane's key: where its K and V start, if it is there
+                const uint32_t j = j0 + c16, i = j / pgs.page_size;
+                int64_t at = -1;
+                if (j >= see && j < u.q.live) {
+                    const uint32_t page = pgs.table[(size_t)u.s * pgs.max_pages + i];
+                    if (page < pgs.num_pages)
+                        at = (int64_t)(page * pgs.stride + ((uint64_t)u.hk * pgs.page_size + (j - i * pgs.page_size)) * D);
+                }
+                if (!__any(at >= 0)) continue;
+                float4v sa = (float4v)0.f;
+                const T* k = (const T*)pgs.k + (at < 0 ? 0 : at);
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    const uint32_t d = 16 * b + 4 * g;
+                    const float4v x = some4<false>(k + d, at >= 0 && d < D ? min(4u, D - d) : 0u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sa = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], qf[b][e], sa, 0, 0, 0);
+                }
+                // scores of the lane's row with keys 4 g + r
+                float v[4], top = -__builtin_inff();
+                int64_t vat[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t key = j0 + 4 * g + r;
+                    vat[r] = __shfl(at, 4 * g + r);
+                    const bool seen = key >= kbeg && key < kend && vat[r] >= 0;
+                    v[r] = seen ? sa[r] * sl2 : -__builtin_inff();
+                    top = fmaxf(top, v[r]);
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float mnew = fmaxf(m[0], top), ref = mnew == -__builtin_inff() ? 0.f : mnew;
+                const float alpha = __builtin_amdgcn_exp2f(m[0] - ref);
+                m[0] = mnew;
+                float e[4], sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    e[r] = __builtin_amdgcn_exp2f(v[r] - ref);
+                    sum += e[r];
+                }
+                sum += __shfl_xor(sum, 16);
+                sum += __shfl_xor(sum, 32);
+                l[0] = l[0] * alpha + sum;
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    const uint32_t d = 16 * b + c16;
+                    float x[4];
+                    bool odd = false;       // a value that is not finite: 0 times it would reach rows that do not see it
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[r] = vat[r] >= 0 && d < D ? (float)((const T*)pgs.v)[vat[r] + d] : 0.f;
+                        odd = odd || !(__builtin_fabsf(x[r]) < __builtin_inff());
+                    }
+                    o[0][b] *= alpha;
+                    if (__any(odd)) {
+                        float4v bad = (float4v)0.f;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool is = !(__builtin_fabsf(x[r]) < __builtin_inff());
+                            bad = __builtin_amdgcn_mfma_f32_16x16x4f32(is ? 1.f : 0.f, v[r] != -__builtin_inff() ? 1.f : 0.f, bad, 0, 0, 0);
+                            x[r] = is ? 0.f : x[r];
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[0][b][r] = bad[r] > 0.f ? __builtin_nanf("") : o[0][b][r];
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[0][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], e[r], o[0][b], 0, 0, 0);
+                }
+            }
+        finish_piece<DP, 1>(p, u, (char*)paged_lds, m, l, o);
+    });
+}
+
+// Joins the partial results of the units that a cut of the line runs through:
+// O = sum_u 2^(m_u - M) O_u / sum_u 2^(m_u - M) l_u. Grid: (cuts, rows); the first
+// cut inside a unit takes it.
+template <int DP>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p, uint32_t rb)
+{
+    constexpr uint32_t C4 = DP / 4, UG = 256 / C4;     // lanes to a part's row; parts read at a time
+    __shared__ float4v part[256];
+    __shared__ float psum[256], pmax[4];
+    const uint32_t n = p.pages.sequences, share = p.ws_plan[n + 1], total = p.ws_plan[n];
+    const uint64_t cut = (uint64_t)(blockIdx.x + 1) * share;
+    if (cut >= total) return;
+    const uint32_t s = wave_last_le(p.ws_plan, n, (uint32_t)cut);
+    const Sequence q = sequence_of(p.pages, s, p.tokens);
+    const pg::Span r = pg::span_of(p, q, rb);
+    const uint32_t tiles = r.te - r.tb, off = (uint32_t)cut - p.ws_plan[s], unit = off / tiles;
+    const uint32_t a = p.ws_plan[s] + unit * tiles;
+    if (s == n || unit >= r.blocks * p.hkv) return;    // (starts that do not increase)
+    if (a == cut || a < cut - share) return;           // cut between two units; an earlier cut's unit
+    const uint32_t g0 = a / share, g1 = (a + tiles - 1) / share, parts = g1 - g0 + 1;
+    const uint32_t hk = unit / r.blocks, blk = unit - hk * r.blocks, group = p.hq / p.hkv;
+    const uint32_t rows = min(rb, q.n * group - blk * rb), t = threadIdx.x, c = t % C4, ug = t / C4;
+    const auto slot = [&](uint32_t i) { return 2 * (g0 + i) + (i == 0 && a != g0 * share ? 1u : 0u); };
+    for (uint32_t row = blockIdx.y; row < rows; row += gridDim.y) {
+        float M = -__builtin_inff();
+        for (uint32_t i = t; i < parts; i += 256) M = fmaxf(M, p.ws_ml[2 * ((size_t)slot(i) * rb + row)]);
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+        if ((t & 63) == 0) pmax[t >> 6] = M;
+        __syncthreads();
+        M = fmaxf(fmaxf(pmax[0], pmax[1]), fmaxf(pmax[2], pmax[3]));
+        const float ref = M == -__builtin_inff() ? 0.f : M;
+        float4v acc = (float4v)0.f;
+        float sum = 0.f;
+        for (uint32_t i = ug; i < parts; i += UG) {
+            const size_t at = (size_t)slot(i) * rb + row;
+            const float w = __builtin_amdgcn_exp2f(p.ws_ml[2 * at] - ref);
+            acc += w * *(const float4v*)(p.ws_o + at * DP + 4 * c);
+            sum += w * p.ws_ml[2 * at + 1];
+        }
+        part[t] = acc;
+        psum[t] = sum;
+        __syncthreads();
+        if (t < C4 && 4 * c < p.head_dim) {
+            for (uint32_t i = 1; i < UG; ++i) {
+                acc += part[i * C4 + c];
+                sum += psum[i * C4 + c];
+            }
+            pg::put_row(p, q.first, hk, blk * rb + row, 4 * c, acc, sum);
+        }
+        __syncthreads();
+    }
+}
+
+hipError_t paged_merge_launch(const PagedAttnParams& p, uint32_t rb, hipStream_t s)
+{
+    if (p.wgs == 1) return hipSuccess;
+    const dim3 grid(p.wgs - 1, rb);
+    if (p.dp == 64) hipLaunchKernelGGL(paged_merge_kernel<64>, grid, dim3(256), 0, s, p, rb);
+    else if (p.dp == 128) hipLaunchKernelGGL(paged_merge_kernel<128>, grid, dim3(256), 0, s, p, rb);
+    else hipLaunchKernelGGL(paged_merge_kernel<256>, grid, dim3(256), 0, s, p, rb);
+    return hipGetLastError();
+}
+
+bool paged_attention_plan(PagedAttnParams& p, uint32_t cus)
+{
+    p.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
+    // the line's length stays below 2^32
+    const uint64_t blocks = (uint64_t)p.tokens * (p.hq / p.hkv) / 16 + std::min(p.tokens, p.pages.sequences);
+    const uint64_t tiles = ((uint64_t)p.pages.max_pages * p.pages.page_size + pg::KT - 1) / pg::KT + 1;
+    if (blocks * p.hkv > 0xffffffffull / tiles) return false;
+    p.wgs = (uint32_t)std::min<uint64_t>(2 * cus, std::max<uint64_t>(1, (blocks * p.hkv * tiles + pg::MIN_SHARE - 1) / pg::MIN_SHARE));
+    return true;
+}
+
+static size_t plan_bytes(const PagedAttnParams& p) { return ((size_t)p.pages.sequences + 2 + 3) / 4 * 16; }
+
+size_t paged_attention_workspace(const PagedAttnParams& p)
+{
+    return plan_bytes(p) + (size_t)2 * p.wgs * 16 * (p.dp + 2) * sizeof(float);
+}
+
+void paged_attention_set_workspace(PagedAttnParams& p, void* ws)
+{
+    p.ws_plan = (uint32_t*)ws;
+    p.ws_o = (float*)((char*)ws + plan_bytes(p));
+    p.ws_ml = p.ws_o + (size_t)2 * p.wgs * 16 * p.dp;
+}
+
+template <int DP, typename T>
+static hipError_t any_launch(const PagedAttnParams& p, hipStream_t s)
+{
+    constexpr int bytes = pg::finish_bytes<DP, 1>();
+    static PerDevice once;
+    const hipError_t e = set_max_lds(once, (const void*)paged_attention_any_kernel<DP, T>, bytes);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((paged_attention_any_kernel<DP, T>), dim3(p.wgs), dim3(256), bytes, s, p);
+    return hipGetLastError();
+}
+
+hipError_t paged_attention_launch(const PagedAttnParams& p, hipStream_t s)
+{
+    const auto go = [&](auto t) {
+        typedef decltype(t) T;
+        return p.dp == 64 ? any_launch<64, T>(p, s) : p.dp == 128 ? any_launch<128, T>(p, s) : any_launch<256, T>(p, s);
+    };
+    const hipError_t e = p.pages.dtype == DT_F16 ? go(half_t{}) : go(float{});
+    return e != hipSuccess ? e : paged_merge_launch(p, 16, s);
+}
+
+}   // namespace vai_dev

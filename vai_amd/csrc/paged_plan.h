@@ -1,0 +1,205 @@
+// paged_plan.h -- how the attention kernels over pages deal their work out, and
+// what they share at the end of a piece of it.
+//
+// A unit is RB query rows (token-major: row r is token r / g, head r % g of the KV
+// head's g) of one sequence and KV head. Its keys are the 32-position tiles that
+// some row of the sequence sees. All units' tiles form one line, sequence by
+// sequence, which the workgroups cut into equal shares: however different the
+// lengths, each walks as many tiles as the next, and the host, which does not know
+// the lengths, need not. A unit that a cut runs through leaves partial results
+// (its rows' maximum, sum and weighted values, fp32) in the workspace, at most two
+// a workgroup, which paged_merge_kernel joins in a fixed order.
+#pragma once
+#include <algorithm>
+
+#include "head_rows.h"
+#include "pages.h"
+
+namespace vai_dev {
+namespace pg {
+
+constexpr int NW = 4, KT = 32;         // waves a workgroup; positions a tile
+constexpr uint32_t MIN_SHARE = NW;     // tiles
+
+// The tiles [tb, te) that a sequence's rows see (at least one), and its blocks of rows.
+struct Span {
+    uint32_t tb, te, blocks;
+};
+__device__ __forceinline__ uint32_t first_key(const PagedAttnParams& p, uint32_t pos)
+{
+    return p.span && pos + 1 > p.span ? pos + 1 - p.span : 0u;
+}
+__device__ __forceinline__ Span span_of(const PagedAttnParams& p, const Sequence& q, uint32_t rb)
+{
+    Span r;
+    r.tb = first_key(p, q.held) / KT;
+    r.te = std::max(r.tb + 1, (q.live + KT - 1) / KT);
+    r.blocks = (q.n * (p.hq / p.hkv) + rb - 1) / rb;
+    return r;
+}
+
+// pre[s] = the line's tiles before sequence s, pre[sequences] all. LDS; every
+// thread of the 256 calls.
+__device__ __forceinline__ void plan_line(const PagedAttnParams& p, uint32_t rb, uint32_t* pre)
+{
+    __shared__ uint32_t wave_sum_[NW];
+    const uint32_t n = p.pages.sequences, per = (n + 255) / 256, lane = threadIdx.x & 63;
+    const uint32_t s0 = std::min(threadIdx.x * per, n), s1 = std::min(s0 + per, n);
+    uint32_t sum = 0;
+    for (uint32_t s = s0; s < s1; ++s) {
+        const Sequence q = sequence_of(p.pages, s, p.tokens);
+        uint32_t w = 0;
+        if (q.n) {
+            const Span r = span_of(p, q, rb);
+            w = (r.te - r.tb) * r.blocks * p.hkv;
+        }
+        pre[s] = w;
+        sum += w;
+    }
+    uint32_t scan = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = __shfl_up(scan, o);
+        if (lane >= (uint32_t)o) scan += x;
+    }
+    if (lane == 63) wave_sum_[threadIdx.x >> 6] = scan;
+    __syncthreads();
+    uint32_t at = scan - sum;
+    for (uint32_t w = 0; w < threadIdx.x >> 6; ++w) at += wave_sum_[w];
+    for (uint32_t s = s0; s < s1; ++s) {
+        const uint32_t w = pre[s];
+        pre[s] = at;
+        at += w;
+    }
+    if (s1 == n && (s0 < n || threadIdx.x == 0)) pre[n] = at;   // (thread 0 where there is none: n >= 1)
+    __syncthreads();
+}
+
+// The sequence that position f of the line is in.
+__device__ __forceinline__ uint32_t line_sequence(const uint32_t* pre, uint32_t n, uint32_t f)
+{
+    uint32_t lo = 0, hi = n;           // pre[lo] <= f < pre[hi]
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (pre[mid] <= f) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// A share's piece of a unit.
+struct Piece {
+    Sequence q;
+    uint32_t s, hk, rb;        // sequence, KV head, block of rows
+    uint32_t t0, t1;           // tiles
+    bool whole;
+    uint32_t slot;             // of the partial results
+};
+
+// Rows of a unit as partial results or output: acc / sum of 4 values from value d on.
+__device__ __forceinline__ void put_row(const PagedAttnParams& p, uint32_t first, uint32_t hk, uint32_t row, uint32_t d,
+                                        float4v acc, float sum)
+{
+    const uint32_t group = p.hq / p.hkv, token = first + row / group, h = hk * group + row % group;
+    acc *= sum != 0.f ? 1.0f / sum : 0.f;     // (a NaN sum divides)
+    const size_t at = ((size_t)token * p.hq + h) * p.head_dim + d;
+    const uint32_t n = std::min(4u, p.head_dim - d);
+    if (p.o_dtype == DT_F16) put4<false>((half_t*)p.out + at, n, acc);
+    else put4<false>((float*)p.out + at, n, acc);
+}
+
+template <int DP> constexpr int orow() { return DP * 4 + 16; }   // bytes of an fp32 row in LDS
+template <int DP, int NQ> constexpr int finish_bytes() { return NW * NQ * 16 * (orow<DP>() + 8); }
+
+// The waves' sums meet in LDS (`lds`, finish_bytes(); what it held is done with
+// once every wave is here) and leave as rows or partial results. Lane (c16, g) of
+// a wave holds row c16 of each 16: m (log2 units), l, and values 16 d + 4 g ..+3.
+template <int DP, int NQ>
+__device__ __forceinline__ void finish_piece(const PagedAttnParams& p, const Piece& u, char* lds, const float (&m)[NQ],
+                                             const float (&l)[NQ], const float4v (&o)[NQ][DP / 16])
+{
+    constexpr int RB = NQ * 16, C4 = DP / 4;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g = lane >> 4;
+    float* ml = (float*)(lds + NW * RB * orow<DP>());
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const uint32_t r = wave * RB + q * 16 + c16;
+        if (g == 0) {
+            ml[2 * r] = m[q];
+            ml[2 * r + 1] = l[q];
+        }
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) *(float4v*)(lds + r * orow<DP>() + (16 * d + 4 * g) * 4) = o[q][d];
+    }
+    __syncthreads();
+    const uint32_t rows = std::min<uint32_t>(RB, u.q.n * (p.hq / p.hkv) - u.rb * RB);
+    for (uint32_t e = threadIdx.x; e < rows * C4; e += 256) {
+        const uint32_t r = e / C4, d = 4 * (e % C4);
+        float mw[NW], M = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            mw[w] = ml[2 * (w * RB + r)];
+            M = fmaxf(M, mw[w]);
+        }
+        const float ref = M == -__builtin_inff() ? 0.f : M;
+        float4v acc = (float4v)0.f;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float a = __builtin_amdgcn_exp2f(mw[w] - ref);
+            acc += a * *(const float4v*)(lds + (w * RB + r) * orow<DP>() + d * 4);
+            sum += a * ml[2 * (w * RB + r) + 1];
+        }
+        if (u.whole) {
+            if (d < p.head_dim) put_row(p, u.q.first, u.hk, u.rb * RB + r, d, acc, sum);
+        } else {
+            const size_t at = (size_t)u.slot * RB + r;
+            *(float4v*)(p.ws_o + at * DP + d) = acc;
+            if (d == 0) {
+                p.ws_ml[2 * at] = M;
+                p.ws_ml[2 * at + 1] = sum;
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// Calls f for each piece of this workgroup's share; pre: plan_line's. Workgroup 0
+// leaves the line for the merge.
+template <int RB, class F>
+__device__ __forceinline__ void walk(const PagedAttnParams& p, const uint32_t* pre, F&& f)
+{
+    const uint32_t n = p.pages.sequences, total = pre[n];
+    const uint32_t share = std::max(MIN_SHARE, (total + p.wgs - 1) / p.wgs), wg = blockIdx.x;
+    if (wg == 0) {
+        for (uint32_t i = threadIdx.x; i <= n; i += 256) p.ws_plan[i] = pre[i];
+        if (threadIdx.x == 0) p.ws_plan[n + 1] = share;
+    }
+    const uint64_t begin = (uint64_t)wg * share;
+    if (begin >= total) return;
+    const uint32_t end = (uint32_t)std::min<uint64_t>(begin + share, total);
+    for (uint32_t at = (uint32_t)begin; at < end;) {
+        Piece u;
+        u.s = __builtin_amdgcn_readfirstlane(line_sequence(pre, n, at));
+        u.q = sequence_of(p.pages, u.s, p.tokens);
+        const Span r = span_of(p, u.q, RB);
+        const uint32_t tiles = r.te - r.tb, off = at - __builtin_amdgcn_readfirstlane(pre[u.s]), unit = off / tiles, t = off - unit * tiles;
+        const uint32_t take = std::min(tiles - t, end - at);
+        if (unit >= r.blocks * p.hkv) break;   // (starts that do not increase)
+        u.hk = unit / r.blocks;
+        u.rb = unit - u.hk * r.blocks;
+        u.t0 = r.tb + t;
+        u.t1 = u.t0 + take;
+        u.whole = take == tiles;
+        u.slot = 2 * wg + (at == begin ? 0u : 1u);
+        f(u);
+        at += take;
+    }
+}
+
+}   // namespace pg
+
+hipError_t paged_merge_launch(const PagedAttnParams& p, uint32_t rb, hipStream_t s);
+
+}   // namespace vai_dev
