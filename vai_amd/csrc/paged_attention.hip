@@ -18,14 +18,14 @@ template <int DP, typename T>
 __global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParams p)
 {
     using namespace pg;
-    constexpr int KB = DP / 16, RB = 16;
+    constexpr int KB = DP / 16, RB = 16, NW = 4;
     extern __shared__ float4v paged_lds[];
     __shared__ uint32_t pre[KvPages::MAX_SEQUENCES + 1];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c16 = lane & 15, g = lane >> 4, D = p.head_dim, group = p.hq / p.hkv;
     const KvPages& pgs = p.pages;
     const float sl2 = p.scale * 1.4426950408889634f;   // scores in log2 units
-    plan_line(p, RB, pre);
+    plan_line<NW>(p, RB, pre);
     walk<RB>(p, pre, [&](const Piece& u) {
         const uint32_t rows = u.q.n * group, row = min(u.rb * RB + c16, rows - 1);
         const uint32_t tok = row / group, pos = u.q.held + tok;
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParam
                     for (int r = 0; r < 4; ++r) o[0][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], e[r], o[0][b], 0, 0, 0);
                 }
             }
-        finish_piece<DP, 1>(p, u, (char*)paged_lds, m, l, o);
+        finish_piece<DP, 1, NW>(p, u, (char*)paged_lds, m, l, o);
     });
 }
 
@@ -190,7 +190,12 @@ bool paged_attention_plan(PagedAttnParams& p, uint32_t cus)
     const uint64_t blocks = (uint64_t)p.tokens * (p.hq / p.hkv) / 16 + std::min(p.tokens, p.pages.sequences);
     const uint64_t tiles = ((uint64_t)p.pages.max_pages * p.pages.page_size + pg::KT - 1) / pg::KT + 1;
     if (blocks * p.hkv > 0xffffffffull / tiles) return false;
-    p.wgs = (uint32_t)std::min<uint64_t>(2 * cus, std::max<uint64_t>(1, (blocks * p.hkv * tiles + pg::MIN_SHARE - 1) / pg::MIN_SHARE));
+    uint32_t resident = 2;
+    p.rb = 16;
+    p.min_share = 4;
+    p.decode = paged_decode_ok(p);
+    if (p.decode) paged_decode_plan(p, &resident);
+    p.wgs = (uint32_t)std::min<uint64_t>((uint64_t)resident * cus, (blocks * p.hkv * tiles + p.min_share - 1) / p.min_share);
     return true;
 }
 
@@ -198,20 +203,20 @@ static size_t plan_bytes(const PagedAttnParams& p) { return ((size_t)p.pages.seq
 
 size_t paged_attention_workspace(const PagedAttnParams& p)
 {
-    return plan_bytes(p) + (size_t)2 * p.wgs * 16 * (p.dp + 2) * sizeof(float);
+    return plan_bytes(p) + (size_t)2 * p.wgs * p.rb * (p.dp + 2) * sizeof(float);
 }
 
 void paged_attention_set_workspace(PagedAttnParams& p, void* ws)
 {
     p.ws_plan = (uint32_t*)ws;
     p.ws_o = (float*)((char*)ws + plan_bytes(p));
-    p.ws_ml = p.ws_o + (size_t)2 * p.wgs * 16 * p.dp;
+    p.ws_ml = p.ws_o + (size_t)2 * p.wgs * p.rb * p.dp;
 }
 
 template <int DP, typename T>
 static hipError_t any_launch(const PagedAttnParams& p, hipStream_t s)
 {
-    constexpr int bytes = pg::finish_bytes<DP, 1>();
+    constexpr int bytes = pg::finish_bytes<DP, 1, 4>();
     static PerDevice once;
     const hipError_t e = set_max_lds(once, (const void*)paged_attention_any_kernel<DP, T>, bytes);
     if (e != hipSuccess) return e;
@@ -225,8 +230,8 @@ hipError_t paged_attention_launch(const PagedAttnParams& p, hipStream_t s)
         typedef decltype(t) T;
         return p.dp == 64 ? any_launch<64, T>(p, s) : p.dp == 128 ? any_launch<128, T>(p, s) : any_launch<256, T>(p, s);
     };
-    const hipError_t e = p.pages.dtype == DT_F16 ? go(half_t{}) : go(float{});
-    return e != hipSuccess ? e : paged_merge_launch(p, 16, s);
+    const hipError_t e = p.decode ? paged_decode_launch(p, s) : p.pages.dtype == DT_F16 ? go(half_t{}) : go(float{});
+    return e != hipSuccess ? e : paged_merge_launch(p, p.rb, s);
 }
 
 }   // namespace vai_dev

@@ -18,8 +18,7 @@
 namespace vai_dev {
 namespace pg {
 
-constexpr int NW = 4, KT = 32;         // waves a workgroup; positions a tile
-constexpr uint32_t MIN_SHARE = NW;     // tiles
+constexpr int KT = 32;                 // positions a tile
 
 // The tiles [tb, te) that a sequence's rows see (at least one), and its blocks of rows.
 struct Span {
@@ -39,11 +38,12 @@ __device__ __forceinline__ Span span_of(const PagedAttnParams& p, const Sequence
 }
 
 // pre[s] = the line's tiles before sequence s, pre[sequences] all. LDS; every
-// thread of the 256 calls.
+// thread of the workgroup's NW waves calls.
+template <int NW>
 __device__ __forceinline__ void plan_line(const PagedAttnParams& p, uint32_t rb, uint32_t* pre)
 {
     __shared__ uint32_t wave_sum_[NW];
-    const uint32_t n = p.pages.sequences, per = (n + 255) / 256, lane = threadIdx.x & 63;
+    const uint32_t n = p.pages.sequences, per = (n + 64 * NW - 1) / (64 * NW), lane = threadIdx.x & 63;
     const uint32_t s0 = std::min(threadIdx.x * per, n), s1 = std::min(s0 + per, n);
     uint32_t sum = 0;
     for (uint32_t s = s0; s < s1; ++s) {
@@ -109,12 +109,12 @@ __device__ __forceinline__ void put_row(const PagedAttnParams& p, uint32_t first
 }
 
 template <int DP> constexpr int orow() { return DP * 4 + 16; }   // bytes of an fp32 row in LDS
-template <int DP, int NQ> constexpr int finish_bytes() { return NW * NQ * 16 * (orow<DP>() + 8); }
+template <int DP, int NQ, int NW> constexpr int finish_bytes() { return NW * NQ * 16 * (orow<DP>() + 8); }
 
 // The waves' sums meet in LDS (`lds`, finish_bytes(); what it held is done with
 // once every wave is here) and leave as rows or partial results. Lane (c16, g) of
 // a wave holds row c16 of each 16: m (log2 units), l, and values 16 d + 4 g ..+3.
-template <int DP, int NQ>
+template <int DP, int NQ, int NW>
 __device__ __forceinline__ void finish_piece(const PagedAttnParams& p, const Piece& u, char* lds, const float (&m)[NQ],
                                              const float (&l)[NQ], const float4v (&o)[NQ][DP / 16])
 {
@@ -134,7 +134,7 @@ __device__ __forceinline__ void finish_piece(const PagedAttnParams& p, const Pie
     }
     __syncthreads();
     const uint32_t rows = std::min<uint32_t>(RB, u.q.n * (p.hq / p.hkv) - u.rb * RB);
-    for (uint32_t e = threadIdx.x; e < rows * C4; e += 256) {
+    for (uint32_t e = threadIdx.x; e < rows * C4; e += 64 * NW) {
         const uint32_t r = e / C4, d = 4 * (e % C4);
         float mw[NW], M = -__builtin_inff();
 #pragma unroll
@@ -171,9 +171,9 @@ template <int RB, class F>
 __device__ __forceinline__ void walk(const PagedAttnParams& p, const uint32_t* pre, F&& f)
 {
     const uint32_t n = p.pages.sequences, total = pre[n];
-    const uint32_t share = std::max(MIN_SHARE, (total + p.wgs - 1) / p.wgs), wg = blockIdx.x;
+    const uint32_t share = std::max(p.min_share, (total + p.wgs - 1) / p.wgs), wg = blockIdx.x;
     if (wg == 0) {
-        for (uint32_t i = threadIdx.x; i <= n; i += 256) p.ws_plan[i] = pre[i];
+        for (uint32_t i = threadIdx.x; i <= n; i += blockDim.x) p.ws_plan[i] = pre[i];
         if (threadIdx.x == 0) p.ws_plan[n + 1] = share;
     }
     const uint64_t begin = (uint64_t)wg * share;
