@@ -351,11 +351,12 @@ struct PagedAttnParams {
     uint32_t tokens, max_new, hq, hkv, head_dim, q_stride;
     float scale;
     uint32_t causal, span;
-    // set by the plan: the padded head dim, query rows of a unit, workgroups and the
-    // fewest tiles of a share; partial results in the workspace
-    uint32_t dp, rb, wgs, min_share;
+    // set by the plan: the padded head dim, query rows of a unit, workgroups, the fewest
+    // tiles of a share and those before each unit; partial results in the workspace
+    static constexpr uint32_t MAX_WGS = 1024;
+    uint32_t dp, rb, wgs, min_share, lead;
     bool decode;                  // paged_decode.hip
-    uint32_t* ws_plan;            // [sequences + 2]
+    uint32_t* ws_plan;            // a Joint a workgroup
     float* ws_o;                  // [2 wgs][rb][dp]
     float* ws_ml;                 // [2 wgs][rb][2]
 };
@@ -365,7 +366,7 @@ void paged_attention_set_workspace(PagedAttnParams& p, void* ws);
 hipError_t paged_attention_launch(const PagedAttnParams& p, hipStream_t s);
 // fp16 pages of whole 16 positions, head dims of whole 8s (paged_decode.hip)
 bool paged_decode_ok(const PagedAttnParams& p);
-void paged_decode_plan(PagedAttnParams& p, uint32_t* resident);   // rb, min_share; workgroups a CU
+void paged_decode_plan(PagedAttnParams& p, uint32_t* resident);   // rb, min_share, lead; workgroups a CU
 hipError_t paged_decode_launch(const PagedAttnParams& p, hipStream_t s);
 
 // Drafted tokens against the target's probabilities (verify_drafts.hip).

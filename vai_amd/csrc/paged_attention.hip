@@ -120,66 +120,85 @@ __global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParam
 }
 
 // Joins the partial results of the units that a cut of the line runs through:
-// O = sum_u 2^(m_u - M) O_u / sum_u 2^(m_u - M) l_u. Grid: (cuts, rows); the first
-// cut inside a unit takes it.
+// O = sum_u 2^(m_u - M) O_u / sum_u 2^(m_u - M) l_u. Grid: (cuts, rows), a Joint a cut.
 template <int DP>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p, uint32_t rb)
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p)
 {
-    constexpr uint32_t C4 = DP / 4, UG = 256 / C4;     // lanes to a part's row; parts read at a time
+    constexpr uint32_t C4 = DP / 4, UG = 256 / C4, AHEAD = 8;     // lanes to a part's row; parts at a time; loads in flight
+    constexpr uint32_t MAXP = PagedAttnParams::MAX_WGS;
+    __shared__ float wgt[MAXP];
     __shared__ float4v part[256];
-    __shared__ float psum[256], pmax[4];
-    const uint32_t n = p.pages.sequences, share = p.ws_plan[n + 1], total = p.ws_plan[n];
-    const uint64_t cut = (uint64_t)(blockIdx.x + 1) * share;
-    if (cut >= total) return;
-    const uint32_t s = wave_last_le(p.ws_plan, n, (uint32_t)cut);
-    const Sequence q = sequence_of(p.pages, s, p.tokens);
-    const pg::Span r = pg::span_of(p, q, rb);
-    const uint32_t tiles = r.te - r.tb, off = (uint32_t)cut - p.ws_plan[s], unit = off / tiles;
-    const uint32_t a = p.ws_plan[s] + unit * tiles;
-    if (s == n || unit >= r.blocks * p.hkv) return;    // (starts that do not increase)
-    if (a == cut || a < cut - share) return;           // cut between two units; an earlier cut's unit
-    const uint32_t g0 = a / share, g1 = (a + tiles - 1) / share, parts = g1 - g0 + 1;
-    const uint32_t hk = unit / r.blocks, blk = unit - hk * r.blocks, group = p.hq / p.hkv;
-    const uint32_t rows = min(rb, q.n * group - blk * rb), t = threadIdx.x, c = t % C4, ug = t / C4;
-    const auto slot = [&](uint32_t i) { return 2 * (g0 + i) + (i == 0 && a != g0 * share ? 1u : 0u); };
-    for (uint32_t row = blockIdx.y; row < rows; row += gridDim.y) {
-        float M = -__builtin_inff();
-        for (uint32_t i = t; i < parts; i += 256) M = fmaxf(M, p.ws_ml[2 * ((size_t)slot(i) * rb + row)]);
+    __shared__ float red[8];
+    const pg::Joint x = ((const pg::Joint*)p.ws_plan)[blockIdx.x + 1];
+    if (x.parts == 0) return;
+    const uint32_t t = threadIdx.x, c = t % C4, ug = t / C4;
+    const auto at = [&](uint32_t i, uint32_t row) { return (size_t)(2 * (x.wg + i) + (i == 0 ? 1u : 0u)) * p.rb + row; };
+    for (uint32_t row = blockIdx.y; row < x.rows; row += gridDim.y) {
+        // the first loads of values are in flight while the weights are made
+        float4v v[AHEAD];
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i)
+            v[i] = *(const float4v*)(p.ws_o + at(min(ug + i * UG, x.parts - 1), row) * DP + 4 * c);
+        float m[MAXP / 256], l[MAXP / 256], M = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < MAXP / 256; ++i) {
+            m[i] = -__builtin_inff();
+            l[i] = 0.f;
+            if (t + 256 * i < x.parts) {
+                const float* ml = p.ws_ml + 2 * at(t + 256 * i, row);
+                m[i] = ml[0];
+                l[i] = ml[1];
+            }
+            M = fmaxf(M, m[i]);
+        }
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-        if ((t & 63) == 0) pmax[t >> 6] = M;
+        if ((t & 63) == 0) red[t >> 6] = M;
         __syncthreads();
-        M = fmaxf(fmaxf(pmax[0], pmax[1]), fmaxf(pmax[2], pmax[3]));
+        M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         const float ref = M == -__builtin_inff() ? 0.f : M;
+#pragma unroll
+        for (uint32_t i = 0; i < MAXP / 256; ++i) {
+            const float w = __builtin_amdgcn_exp2f(m[i] - ref);
+            wgt[t + 256 * i] = w;
+            sum += w * l[i];
+        }
+        sum = wave_sum(sum);
+        if ((t & 63) == 0) red[4 + (t >> 6)] = sum;
+        __syncthreads();
         float4v acc = (float4v)0.f;
-        float sum = 0.f;
-        for (uint32_t i = ug; i < parts; i += UG) {
-            const size_t at = (size_t)slot(i) * rb + row;
-            const float w = __builtin_amdgcn_exp2f(p.ws_ml[2 * at] - ref);
-            acc += w * *(const float4v*)(p.ws_o + at * DP + 4 * c);
-            sum += w * p.ws_ml[2 * at + 1];
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i)
+            if (ug + i * UG < x.parts) acc += wgt[ug + i * UG] * v[i];
+        for (uint32_t u = ug + AHEAD * UG; u < x.parts; u += AHEAD * UG) {
+#pragma unroll
+            for (uint32_t i = 0; i < AHEAD; ++i)
+                v[i] = *(const float4v*)(p.ws_o + at(min(u + i * UG, x.parts - 1), row) * DP + 4 * c);
+#pragma unroll
+            for (uint32_t i = 0; i < AHEAD; ++i)
+                if (u + i * UG < x.parts) acc += wgt[u + i * UG] * v[i];
         }
         part[t] = acc;
-        psum[t] = sum;
         __syncthreads();
         if (t < C4 && 4 * c < p.head_dim) {
-            for (uint32_t i = 1; i < UG; ++i) {
-                acc += part[i * C4 + c];
-                sum += psum[i * C4 + c];
-            }
-            pg::put_row(p, q.first, hk, blk * rb + row, 4 * c, acc, sum);
+#pragma unroll
+            for (uint32_t i = 1; i < UG; ++i) acc += part[i * C4 + c];
+            sum = (red[4] + red[5]) + (red[6] + red[7]);
+            pg::put_row(p, x.first, x.hk, x.row0 + row, 4 * c, acc, sum);
         }
         __syncthreads();
     }
 }
 
-hipError_t paged_merge_launch(const PagedAttnParams& p, uint32_t rb, hipStream_t s)
+hipError_t paged_merge_launch(const PagedAttnParams& p, hipStream_t s)
 {
     if (p.wgs == 1) return hipSuccess;
-    const dim3 grid(p.wgs - 1, rb);
-    if (p.dp == 64) hipLaunchKernelGGL(paged_merge_kernel<64>, grid, dim3(256), 0, s, p, rb);
-    else if (p.dp == 128) hipLaunchKernelGGL(paged_merge_kernel<128>, grid, dim3(256), 0, s, p, rb);
-    else hipLaunchKernelGGL(paged_merge_kernel<256>, grid, dim3(256), 0, s, p, rb);
+    // (a unit's rows, as far as the hint knows: more take turns)
+    const uint32_t rows = (uint32_t)std::min<uint64_t>(p.rb, (uint64_t)p.max_new * (p.hq / p.hkv));
+    const dim3 grid(p.wgs - 1, rows);
+    if (p.dp == 64) hipLaunchKernelGGL(paged_merge_kernel<64>, grid, dim3(256), 0, s, p);
+    else if (p.dp == 128) hipLaunchKernelGGL(paged_merge_kernel<128>, grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(paged_merge_kernel<256>, grid, dim3(256), 0, s, p);
     return hipGetLastError();
 }
 
@@ -189,17 +208,20 @@ bool paged_attention_plan(PagedAttnParams& p, uint32_t cus)
     // the line's length stays below 2^32
     const uint64_t blocks = (uint64_t)p.tokens * (p.hq / p.hkv) / 16 + std::min(p.tokens, p.pages.sequences);
     const uint64_t tiles = ((uint64_t)p.pages.max_pages * p.pages.page_size + pg::KT - 1) / pg::KT + 1;
-    if (blocks * p.hkv > 0xffffffffull / tiles) return false;
     uint32_t resident = 2;
     p.rb = 16;
     p.min_share = 4;
+    p.lead = 2;
     p.decode = paged_decode_ok(p);
     if (p.decode) paged_decode_plan(p, &resident);
-    p.wgs = (uint32_t)std::min<uint64_t>((uint64_t)resident * cus, (blocks * p.hkv * tiles + p.min_share - 1) / p.min_share);
+    const uint64_t unit = tiles + p.lead;
+    if (blocks * p.hkv > 0xffffffffull / unit) return false;
+    p.wgs = (uint32_t)std::min<uint64_t>({(uint64_t)resident * cus, (blocks * p.hkv * unit + p.min_share - 1) / p.min_share,
+                                          (uint64_t)PagedAttnParams::MAX_WGS});
     return true;
 }
 
-static size_t plan_bytes(const PagedAttnParams& p) { return ((size_t)p.pages.sequences + 2 + 3) / 4 * 16; }
+static size_t plan_bytes(const PagedAttnParams& p) { return p.wgs * sizeof(pg::Joint); }
 
 size_t paged_attention_workspace(const PagedAttnParams& p)
 {
@@ -231,7 +253,7 @@ hipError_t paged_attention_launch(const PagedAttnParams& p, hipStream_t s)
         return p.dp == 64 ? any_launch<64, T>(p, s) : p.dp == 128 ? any_launch<128, T>(p, s) : any_launch<256, T>(p, s);
     };
     const hipError_t e = p.decode ? paged_decode_launch(p, s) : p.pages.dtype == DT_F16 ? go(half_t{}) : go(float{});
-    return e != hipSuccess ? e : paged_merge_launch(p, p.rb, s);
+    return e != hipSuccess ? e : paged_merge_launch(p, s);
 }
 
 }   // namespace vai_dev

@@ -375,6 +375,7 @@ void paged_decode_plan(PagedAttnParams& p, uint32_t* resident)
     // (32 rows of 256-wide heads would spill)
     p.rb = p.dp == 256 || (uint64_t)p.max_new * (p.hq / p.hkv) <= 16 ? 16 : 32;
     p.min_share = p.dp == 64 ? Ring<64>::NW : Ring<128>::NW;
+    p.lead = p.dp == 64 ? 10 : 6;
     *resident = p.dp == 256 ? Ring<256>::RES : Ring<128>::RES;
 }
 

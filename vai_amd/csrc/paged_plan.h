@@ -6,9 +6,12 @@
 // some row of the sequence sees. All units' tiles form one line, sequence by
 // sequence, which the workgroups cut into equal shares: however different the
 // lengths, each walks as many tiles as the next, and the host, which does not know
-// the lengths, need not. A unit that a cut runs through leaves partial results
-// (its rows' maximum, sum and weighted values, fp32) in the workspace, at most two
-// a workgroup, which paged_merge_kernel joins in a fixed order.
+// the lengths, need not. Beginning and ending a unit takes as long as `lead` tiles,
+// which therefore stand before its own in the line (64 sequences of 64 to 8192
+// positions, where a share without them could hold 25 short units: 123 us, with
+// them 87). A unit that a cut runs through leaves partial results (its rows'
+// maximum, sum and weighted values, fp32) in the workspace, at most two a
+// workgroup, which paged_merge_kernel joins in a fixed order.
 #pragma once
 #include <algorithm>
 
@@ -51,7 +54,7 @@ __device__ __forceinline__ void plan_line(const PagedAttnParams& p, uint32_t rb,
         uint32_t w = 0;
         if (q.n) {
             const Span r = span_of(p, q, rb);
-            w = (r.te - r.tb) * r.blocks * p.hkv;
+            w = (r.te - r.tb + p.lead) * r.blocks * p.hkv;
         }
         pre[s] = w;
         sum += w;
@@ -93,7 +96,15 @@ struct Piece {
     uint32_t s, hk, rb;        // sequence, KV head, block of rows
     uint32_t t0, t1;           // tiles
     bool whole;
-    uint32_t slot;             // of the partial results
+    uint32_t slot;             // of the partial results: 2 w for a unit that an earlier
+};                             // workgroup began, 2 w + 1 for one that a later one ends
+
+// A unit to merge, left in ws_plan by the second of the workgroups that share it.
+struct Joint {
+    uint32_t parts;            // 0: none
+    uint32_t wg;               // the first part's workgroup
+    uint32_t first, hk, row0, rows;   // the sequence's first row; rows row0 .. + rows - 1 of the KV head
+    uint32_t pad[2];
 };
 
 // Rows of a unit as partial results or output: acc / sum of 4 values from value d on.
@@ -165,41 +176,46 @@ __device__ __forceinline__ void finish_piece(const PagedAttnParams& p, const Pie
     __syncthreads();
 }
 
-// Calls f for each piece of this workgroup's share; pre: plan_line's. Workgroup 0
-// leaves the line for the merge.
+// Calls f for each piece of this workgroup's share; pre: plan_line's.
 template <int RB, class F>
 __device__ __forceinline__ void walk(const PagedAttnParams& p, const uint32_t* pre, F&& f)
 {
-    const uint32_t n = p.pages.sequences, total = pre[n];
-    const uint32_t share = std::max(p.min_share, (total + p.wgs - 1) / p.wgs), wg = blockIdx.x;
-    if (wg == 0) {
-        for (uint32_t i = threadIdx.x; i <= n; i += blockDim.x) p.ws_plan[i] = pre[i];
-        if (threadIdx.x == 0) p.ws_plan[n + 1] = share;
-    }
+    const uint32_t n = p.pages.sequences, total = __builtin_amdgcn_readfirstlane(pre[n]), wg = blockIdx.x;
+    const uint32_t share = std::max(p.min_share, (total + p.wgs - 1) / p.wgs);
     const uint64_t begin = (uint64_t)wg * share;
-    if (begin >= total) return;
+    Joint joint{};
     const uint32_t end = (uint32_t)std::min<uint64_t>(begin + share, total);
-    for (uint32_t at = (uint32_t)begin; at < end;) {
+    for (uint32_t at = (uint32_t)std::min<uint64_t>(begin, total); at < end;) {
         Piece u;
         u.s = __builtin_amdgcn_readfirstlane(line_sequence(pre, n, at));
         u.q = sequence_of(p.pages, u.s, p.tokens);
         const Span r = span_of(p, u.q, RB);
-        const uint32_t tiles = r.te - r.tb, off = at - __builtin_amdgcn_readfirstlane(pre[u.s]), unit = off / tiles, t = off - unit * tiles;
-        const uint32_t take = std::min(tiles - t, end - at);
+        const uint32_t tiles = r.te - r.tb, len = tiles + p.lead;
+        const uint32_t off = at - __builtin_amdgcn_readfirstlane(pre[u.s]), unit = off / len, o0 = off - unit * len;
+        const uint32_t o1 = std::min(len, o0 + (end - at));
         if (unit >= r.blocks * p.hkv) break;   // (starts that do not increase)
         u.hk = unit / r.blocks;
         u.rb = unit - u.hk * r.blocks;
-        u.t0 = r.tb + t;
-        u.t1 = u.t0 + take;
-        u.whole = take == tiles;
-        u.slot = 2 * wg + (at == begin ? 0u : 1u);
+        const uint32_t t0 = o0 > p.lead ? o0 - p.lead : 0u, t1 = o1 > p.lead ? o1 - p.lead : 0u;
+        if (at == begin && t0 > 0) {
+            const uint32_t a = at - o0 + p.lead, wg0 = a / share;    // (the unit's first tile)
+            if (wg0 + 1 == wg)
+                joint = Joint{(a + tiles - 1) / share - wg0 + 1, wg0, u.q.first, u.hk, u.rb * RB,
+                              std::min<uint32_t>(RB, u.q.n * (p.hq / p.hkv) - u.rb * RB), {0, 0}};
+        }
+        at += o1 - o0;
+        if (t1 == t0) continue;
+        u.t0 = r.tb + t0;
+        u.t1 = r.tb + t1;
+        u.whole = t1 - t0 == tiles;
+        u.slot = 2 * wg + (t0 == 0 ? 1u : 0u);
         f(u);
-        at += take;
     }
+    if (threadIdx.x == 0) ((Joint*)p.ws_plan)[wg] = joint;
 }
 
 }   // namespace pg
 
-hipError_t paged_merge_launch(const PagedAttnParams& p, uint32_t rb, hipStream_t s);
+hipError_t paged_merge_launch(const PagedAttnParams& p, hipStream_t s);
 
 }   // namespace vai_dev
