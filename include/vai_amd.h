@@ -507,7 +507,8 @@ vai_status vai_paged_append_launch(const vai_paged_append_args* args, vai_stream
  *   for fp16 out they are rounded to one. fp32 pages, head dims of no whole 8s
  *   and pages of no whole 16s are attended in fp32 throughout.
  *   What hidden positions hold does not matter. A value of V that is not finite
- *   makes its column NaN for the queries that see it.
+ *   makes its column so for the queries that see it; their other columns may be
+ *   NaN too.
  * Calls that overlap in time need a workspace each (vai_paged_attention_
  * workspace_size() bytes, 16-byte aligned). The result does not depend on what
  * it held. */

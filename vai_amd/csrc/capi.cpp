@@ -722,13 +722,13 @@ vai_status vai_paged_append_launch(const vai_paged_append_args* a, vai_stream_t 
     return hip_status(paged_append_launch(p, a->theta, (hipStream_t)stream));
 }
 
-static vai_status paged_attention_params(const vai_paged_attention_args* a, PagedAttnParams& p)
+static vai_status paged_attention_params(const vai_paged_attention_args* a, PagedAttnPlan& plan)
 {
     if (!a || !a->out || !a->q) return VAI_ERR_INVALID_ARG;
     if (!dtype_ok(a->q_dtype) || !dtype_ok(a->o_dtype)) return VAI_ERR_DTYPE;
     if (a->tokens == 0 || a->hq == 0 || a->hkv == 0 || a->head_dim == 0 || a->hq % a->hkv != 0) return VAI_ERR_SHAPE;
     if (a->head_dim > 256 || (uint64_t)a->tokens * a->hq >= 1ull << 31) return VAI_ERR_UNSUPPORTED;
-    p = PagedAttnParams{};
+    PagedAttnParams p{};
     if (vai_status st = kv_pages_params(a->pages, a->hkv, a->head_dim, p.pages); st != VAI_OK) return st;
     if ((uint64_t)a->hq * a->head_dim > UINT32_MAX || (a->q_stride && a->q_stride < a->hq * a->head_dim)) return VAI_ERR_SHAPE;
     if (a->causal > 1 || a->scale != a->scale) return VAI_ERR_INVALID_ARG;
@@ -739,23 +739,22 @@ static vai_status paged_attention_params(const vai_paged_attention_args* a, Page
     p.q_stride = a->q_stride ? a->q_stride : a->hq * a->head_dim;
     p.scale = a->scale != 0.f ? a->scale : 1.0f / std::sqrt((float)a->head_dim);
     p.causal = a->causal; p.span = a->span;
-    return paged_attention_plan(p, plan_cus()) ? VAI_OK : VAI_ERR_UNSUPPORTED;
+    return paged_attention_plan(p, plan, plan_cus()) ? VAI_OK : VAI_ERR_UNSUPPORTED;
 }
 
 size_t vai_paged_attention_workspace_size(const vai_paged_attention_args* a)
 {
-    PagedAttnParams p;
+    PagedAttnPlan p;
     return paged_attention_params(a, p) == VAI_OK ? paged_attention_workspace(p) : 0;
 }
 
 vai_status vai_paged_attention_launch(const vai_paged_attention_args* a, vai_stream_t stream)
 {
-    PagedAttnParams p;
+    PagedAttnPlan p;
     if (vai_status st = paged_attention_params(a, p); st != VAI_OK) return st;
     if (!a->workspace || a->workspace_bytes < paged_attention_workspace(p)) return VAI_ERR_WORKSPACE;
     if ((uintptr_t)a->workspace % 16 != 0) return VAI_ERR_INVALID_ARG;
-    paged_attention_set_workspace(p, a->workspace);
-    return hip_status(paged_attention_launch(p, (hipStream_t)stream));
+    return hip_status(paged_attention_launch(p, a->workspace, (hipStream_t)stream));
 }
 
 static vai_status verify_params(const vai_verify_drafts_args* a, VerifyParams& p)

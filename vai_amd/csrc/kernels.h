@@ -355,19 +355,28 @@ struct PagedAttnParams {
     // tiles of a share and those before each unit; partial results in the workspace
     static constexpr uint32_t MAX_WGS = 1024;
     uint32_t dp, rb, wgs, min_share, lead;
-    bool decode;                  // paged_decode.hip
+    // sequences of more rows a KV head than few_rows are paged_prefill.hip's, the others
+    // paged_decode.hip's (decode) or the fp32 kernel's
+    uint32_t few_rows;
+    bool decode;
     uint32_t* ws_plan;            // a Joint a workgroup
     float* ws_o;                  // [2 wgs][rb][dp]
     float* ws_ml;                 // [2 wgs][rb][2]
 };
-bool paged_attention_plan(PagedAttnParams& p, uint32_t cus);   // false: too large a grid of tiles
-size_t paged_attention_workspace(const PagedAttnParams& p);
-void paged_attention_set_workspace(PagedAttnParams& p, void* ws);
-hipError_t paged_attention_launch(const PagedAttnParams& p, hipStream_t s);
+// The launches of a call: few rows a sequence, and many (many.wgs = 0: none).
+struct PagedAttnPlan {
+    PagedAttnParams few, many;
+};
+bool paged_attention_plan(const PagedAttnParams& p, PagedAttnPlan& plan, uint32_t cus);   // false: too large a grid of tiles
+size_t paged_attention_workspace(const PagedAttnPlan& plan);
+hipError_t paged_attention_launch(PagedAttnPlan& plan, void* ws, hipStream_t s);
 // fp16 pages of whole 16 positions, head dims of whole 8s (paged_decode.hip)
 bool paged_decode_ok(const PagedAttnParams& p);
 void paged_decode_plan(PagedAttnParams& p, uint32_t* resident);   // rb, min_share, lead; workgroups a CU
 hipError_t paged_decode_launch(const PagedAttnParams& p, hipStream_t s);
+// the same pages, many rows a sequence (paged_prefill.hip)
+void paged_prefill_plan(PagedAttnParams& p, uint32_t cus);
+hipError_t paged_prefill_launch(const PagedAttnParams& p, hipStream_t s);
 
 // Drafted tokens against the target's probabilities (verify_drafts.hip).
 struct VerifyParams {

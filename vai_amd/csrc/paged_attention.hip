@@ -14,6 +14,8 @@
 
 namespace vai_dev {
 
+constexpr uint32_t FEW_ROWS = 64;      // rows a KV head
+
 template <int DP, typename T>
 __global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParams p)
 {
@@ -202,36 +204,46 @@ hipError_t paged_merge_launch(const PagedAttnParams& p, hipStream_t s)
     return hipGetLastError();
 }
 
-bool paged_attention_plan(PagedAttnParams& p, uint32_t cus)
+bool paged_attention_plan(const PagedAttnParams& call, PagedAttnPlan& plan, uint32_t cus)
 {
+    PagedAttnParams& p = plan.few;
+    p = call;
     p.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
-    // the line's length stays below 2^32
-    const uint64_t blocks = (uint64_t)p.tokens * (p.hq / p.hkv) / 16 + std::min(p.tokens, p.pages.sequences);
+    const uint32_t group = p.hq / p.hkv;
+    // the lines' lengths stay below 2^32
+    const uint64_t blocks = (uint64_t)p.tokens * group / 16 + std::min(p.tokens, p.pages.sequences);
     const uint64_t tiles = ((uint64_t)p.pages.max_pages * p.pages.page_size + pg::KT - 1) / pg::KT + 1;
     uint32_t resident = 2;
     p.rb = 16;
     p.min_share = 4;
     p.lead = 2;
+    p.few_rows = 0xffffffffu;
     p.decode = paged_decode_ok(p);
     if (p.decode) paged_decode_plan(p, &resident);
     const uint64_t unit = tiles + p.lead;
     if (blocks * p.hkv > 0xffffffffull / unit) return false;
     p.wgs = (uint32_t)std::min<uint64_t>({(uint64_t)resident * cus, (blocks * p.hkv * unit + p.min_share - 1) / p.min_share,
                                           (uint64_t)PagedAttnParams::MAX_WGS});
+    plan.many = p;
+    plan.many.wgs = 0;
+    if (p.decode && (uint64_t)p.max_new * group > FEW_ROWS) {
+        p.few_rows = plan.many.few_rows = FEW_ROWS;
+        paged_prefill_plan(plan.many, cus);
+    }
     return true;
 }
 
-static size_t plan_bytes(const PagedAttnParams& p) { return p.wgs * sizeof(pg::Joint); }
-
-size_t paged_attention_workspace(const PagedAttnParams& p)
+static size_t part_bytes(const PagedAttnParams& p)
 {
-    return plan_bytes(p) + (size_t)2 * p.wgs * p.rb * (p.dp + 2) * sizeof(float);
+    return p.wgs * (sizeof(pg::Joint) + (size_t)2 * p.rb * (p.dp + 2) * sizeof(float));
 }
 
-void paged_attention_set_workspace(PagedAttnParams& p, void* ws)
+size_t paged_attention_workspace(const PagedAttnPlan& plan) { return part_bytes(plan.few) + part_bytes(plan.many); }
+
+static void set_workspace(PagedAttnParams& p, char* ws)
 {
     p.ws_plan = (uint32_t*)ws;
-    p.ws_o = (float*)((char*)ws + plan_bytes(p));
+    p.ws_o = (float*)(ws + p.wgs * sizeof(pg::Joint));
     p.ws_ml = p.ws_o + (size_t)2 * p.wgs * p.rb * p.dp;
 }
 
@@ -246,13 +258,18 @@ static hipError_t any_launch(const PagedAttnParams& p, hipStream_t s)
     return hipGetLastError();
 }
 
-hipError_t paged_attention_launch(const PagedAttnParams& p, hipStream_t s)
+hipError_t paged_attention_launch(PagedAttnPlan& plan, void* ws, hipStream_t s)
 {
+    set_workspace(plan.few, (char*)ws);
+    set_workspace(plan.many, (char*)ws + part_bytes(plan.few));
+    const PagedAttnParams& p = plan.few;
     const auto go = [&](auto t) {
         typedef decltype(t) T;
         return p.dp == 64 ? any_launch<64, T>(p, s) : p.dp == 128 ? any_launch<128, T>(p, s) : any_launch<256, T>(p, s);
     };
-    const hipError_t e = p.decode ? paged_decode_launch(p, s) : p.pages.dtype == DT_F16 ? go(half_t{}) : go(float{});
+    hipError_t e = plan.many.wgs ? paged_prefill_launch(plan.many, s) : hipSuccess;
+    if (e != hipSuccess) return e;
+    e = p.decode ? paged_decode_launch(p, s) : p.pages.dtype == DT_F16 ? go(half_t{}) : go(float{});
     return e != hipSuccess ? e : paged_merge_launch(p, s);
 }
 

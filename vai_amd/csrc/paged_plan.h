@@ -52,7 +52,7 @@ __device__ __forceinline__ void plan_line(const PagedAttnParams& p, uint32_t rb,
     for (uint32_t s = s0; s < s1; ++s) {
         const Sequence q = sequence_of(p.pages, s, p.tokens);
         uint32_t w = 0;
-        if (q.n) {
+        if (q.n && q.n * (p.hq / p.hkv) <= p.few_rows) {
             const Span r = span_of(p, q, rb);
             w = (r.te - r.tb + p.lead) * r.blocks * p.hkv;
         }
