@@ -14,7 +14,12 @@
 
 namespace vai_dev {
 
-constexpr uint32_t FEW_ROWS = 64;      // rows a KV head
+// Rows a KV head up to which a sequence is paged_decode.hip's, whose units of 32 (D =
+// 256: 16) rows read the keys once each. 8 sequences of 4000 positions, 32 heads over
+// 8 of 128, us there / in paged_prefill.hip: 32 rows 40 / 55, 48 rows 61 / 55, 64 rows
+// 63 / 55, where one sequence of 16000 takes 28 / 52, 35 / 52, 35 / 53; of 64, 64 rows
+// 40 / 30; of 256 (16 over 4), 32 rows 56 / 53, 64 rows 93 / 54.
+static uint32_t few_most(uint32_t dp) { return dp == 128 ? 64 : 32; }
 
 template <int DP, typename T>
 __global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParams p)
@@ -226,9 +231,17 @@ bool paged_attention_plan(const PagedAttnParams& call, PagedAttnPlan& plan, uint
                                           (uint64_t)PagedAttnParams::MAX_WGS});
     plan.many = p;
     plan.many.wgs = 0;
-    if (p.decode && (uint64_t)p.max_new * group > FEW_ROWS) {
-        p.few_rows = plan.many.few_rows = FEW_ROWS;
+    if (p.decode && (uint64_t)p.max_new * group > few_most(p.dp)) {
+        p.few_rows = plan.many.few_rows = few_most(p.dp);
         paged_prefill_plan(plan.many, cus);
+        // One launch takes them all where the units of the sequences with few rows are not
+        // many: it fills 4 of 128 rows then, but is bound by memory like the other, whose
+        // launch and merge are saved. A chunk of 512 tokens beside 8, 32, 64 and 128 single
+        // ones, 8 KV heads: 112, 147, 195, 276 us so, 134, 161, 215, 274 apart.
+        if ((uint64_t)p.pages.sequences * p.hkv <= plan.many.wgs * 3 / 2) {
+            plan.many.few_rows = 0;
+            p.wgs = 0;
+        }
     }
     return true;
 }
@@ -268,7 +281,7 @@ hipError_t paged_attention_launch(PagedAttnPlan& plan, void* ws, hipStream_t s)
         return p.dp == 64 ? any_launch<64, T>(p, s) : p.dp == 128 ? any_launch<128, T>(p, s) : any_launch<256, T>(p, s);
     };
     hipError_t e = plan.many.wgs ? paged_prefill_launch(plan.many, s) : hipSuccess;
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || p.wgs == 0) return e;
     e = p.decode ? paged_decode_launch(p, s) : p.pages.dtype == DT_F16 ? go(half_t{}) : go(float{});
     return e != hipSuccess ? e : paged_merge_launch(p, s);
 }

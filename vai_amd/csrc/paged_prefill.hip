@@ -8,7 +8,10 @@
 // LDS while the tile before is multiplied, each wave one page's 16 positions of
 // them (attention.hip's tile and fragment order: S^T = K Q^T and O^T += V^T P^T on
 // v_mfma_f32_32x32x16_f16, the scores of a row in a lane and its partner). Two
-// groups of four waves take the tiles in turn (D = 256: one group, by registers).
+// workgroups a CU (D = 256: one, by registers): one's softmax, and its beginning
+// and end of a unit, under the other's products. (One of two groups of waves that
+// take the tiles in turn halves the partial results, but 8192 tokens of a prompt
+// took 823 us so where two workgroups take 700.)
 // All units' tiles form a line that the workgroups cut into equal shares, head by
 // head on one XCD, as paged_plan.h does for few rows; a unit's tiles are those its
 // own rows see. An fp32 q enters as two fp16 numbers (Q2), and so do the
@@ -180,26 +183,23 @@ __device__ __forceinline__ half8 vfrag_now(const uint32_t (&vaddr)[2])
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-template <int D> constexpr int groups() { return D == 256 ? 1 : 2; }
 __device__ __forceinline__ bool finite(half_t x) { return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) != 0x7c00u; }
 
 }   // namespace pp
 
 template <int D, bool Q2, bool P2>
-__global__ __launch_bounds__(256 * pp::groups<D>(), pp::groups<D>()) void paged_prefill_kernel(PagedAttnParams p, uint32_t tiles_at)
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(PagedAttnParams p, uint32_t tiles_at)
 {
     using namespace fa;
     using pp::Piece;
     using pp::RB;
     using L = Lds<D>;
-    constexpr int KG = pp::groups<D>(), KS = D / 16, DF = D / 32, CR = D / 4;
+    constexpr int KS = D / 16, DF = D / 32, CR = D / 4;
     constexpr float SLACK = 8.f, LIFT = 7.f;     // P stays below 2^15
     extern __shared__ __attribute__((aligned(1024))) float4v paged_prefill_lds[];
     uint32_t* pre = (uint32_t*)paged_prefill_lds;
-    const uint32_t lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t wave = KG == 1 ? wid : wid & 3, kg = KG == 1 ? 0u : wid >> 2;   // rows of the unit; key group
-    LDS_AS char* all = (LDS_AS char*)(LDS_AS void*)paged_prefill_lds + tiles_at;
-    LDS_AS char* lds = all + kg * L::BYTES;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    LDS_AS char* lds = (LDS_AS char*)(LDS_AS void*)paged_prefill_lds + tiles_at;
     const int ql = lane & 31, hf = lane >> 5;
     const uint32_t HD = p.head_dim, group = p.hq / p.hkv;
     const KvPages& pgs = p.pages;
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(256 * pp::groups<D>(), pp::groups<D>()) void paged_
         vaddr[j] = lds0 + (vkey + vrow) * L::ROWB + ((4 * j + (vcol >> 3)) ^ swz_f((vkey + vrow) & 7)) * 16 +
                   (vcol & 7) * 2;
 
-    pp::plan_line<4 * KG>(p, pre);
+    pp::plan_line<NW>(p, pre);
     pp::walk(p, pre, fa_xcd_block(blockIdx.x, gridDim.x), [&](const Piece& u) __attribute__((always_inline)) {
         const uint32_t rows = u.q.n * group, row = min(u.rb * RB + wave * QW + ql, rows - 1);
         const uint32_t tok = row / group, pos = u.q.held + tok;
@@ -271,14 +271,12 @@ __global__ __launch_bounds__(256 * pp::groups<D>(), pp::groups<D>()) void paged_
             }
         }
 
-        // this group's tiles are t0 + kg, + KG, ..; where the 16 of a batch lie, four blocks of
-        // 16 positions each: lane 4 i + b holds tile i's block b
-        const uint32_t first = u.t0 + kg;
-        const int mine = first < u.t1 ? (int)((u.t1 - first + KG - 1) / KG) : 0;
-        const int most = (int)((u.t1 - u.t0 + KG - 1) / KG);      // (group 0's, the barriers' count)
+        // where the 16 tiles of a batch lie, four blocks of 16 positions each: lane 4 i + b holds
+        // tile i's block b
+        const int mine = (int)(u.t1 - u.t0);
         uint32_t entry, start, entry2 = 0xffffffffu, start2 = 0;
         const auto look_up = [&](int t, uint32_t& e, uint32_t& st) __attribute__((always_inline)) {
-            const uint64_t at = (uint64_t)(first + (uint32_t)(t + (int)(lane >> 2)) * KG) * pp::KT + 16 * (lane & 3);
+            const uint64_t at = (uint64_t)(u.t0 + (uint32_t)(t + (int)(lane >> 2))) * pp::KT + 16 * (lane & 3);
             e = 0xffffffffu;
             st = 0;
             if (at < u.q.live) {
@@ -291,181 +289,179 @@ __global__ __launch_bounds__(256 * pp::groups<D>(), pp::groups<D>()) void paged_
         const auto rsrc = [&](int t, const void* pool) __attribute__((always_inline)) {
             const int l = 4 * (t & 15) + (int)wave;
             const uint32_t e = __builtin_amdgcn_readlane(entry, l), at = __builtin_amdgcn_readlane(start, l);
-            const uint32_t ps = (first + (uint32_t)t * KG) * pp::KT + 16 * wave;
+            const uint32_t ps = (u.t0 + (uint32_t)t) * pp::KT + 16 * wave;
             // positions that are not there, and rows past the last one, read as zeros
             const uint32_t n = t < mine && e < pgs.num_pages && ps < u.q.live ? min(16u, u.q.live - ps) * HD * 2 : 0u;
             const size_t byte = n ? (e * pgs.stride + (uint64_t)u.hk * pgs.page_size * HD) * 2 + at : 0u;
             return __builtin_amdgcn_make_buffer_rsrc((void*)(uniform_ptr((char*)pool) + byte), (short)0, (int)n, 0x00020000);
         };
-        if (mine > 0) fa_issue<D>(rsrc(0, pgs.k), rsrc(0, pgs.v), lds, coff, 0, wave);
+        fa_issue<D>(rsrc(0, pgs.k), rsrc(0, pgs.v), lds, coff, 0, wave);
 
         float m = -__builtin_inff(), l = 0.f;
         float16v o[DF];
 #pragma unroll
         for (int d = 0; d < DF; ++d) o[d] = (float16v)0.f;
 
-        for (int t = 0; t < most; ++t) {
+        for (int t = 0; t < mine; ++t) {
             // tile t is in stage t % 2; the next one's copies go out during its S^T products
             fa_wait_vmcnt<0>();
             __builtin_amdgcn_s_barrier();
-            if (t < mine) {
-                const uint32_t blocks = (uint32_t)(__ballot(entry < pgs.num_pages) >> (4 * (t & 15))) & 15u;
-                if ((t & 15) == 14) look_up(t + 2, entry2, start2);
-                if ((t & 15) == 15) {
-                    entry = entry2;
-                    start = start2;
-                }
-                const int j0 = (int)((first + (uint32_t)t * KG) * pp::KT);
+            const uint32_t blocks = (uint32_t)(__ballot(entry < pgs.num_pages) >> (4 * (t & 15))) & 15u;
+            if ((t & 15) == 14) look_up(t + 2, entry2, start2);
+            if ((t & 15) == 15) {
+                entry = entry2;
+                start = start2;
+            }
+            const int j0 = (int)((u.t0 + (uint32_t)t) * pp::KT);
 
-                // step i of the 2 KS products is key block i % 2, head-dim step i / 2; K fragments are
-                // read G at a time, the next group's behind this one's products
-                constexpr int NS = 2 * KS, G = D == 64 ? 8 : 4;
-                constexpr int OPG = 2 * L::COPIES / (NS / G);
-                static_assert(OPG * (NS / G) == 2 * L::COPIES, "copies spread evenly over the groups");
-                const bool next = t + 1 < mine;
-                const __amdgpu_buffer_rsrc_t rkn = rsrc(t + 1, pgs.k), rvn = rsrc(t + 1, pgs.v);
-                LDS_AS char* nst = lds + ((t + 1) & 1) * L::STAGE + wave * L::COPIES * 1024;
-                float16v sacc[2] = {(float16v)0.f, (float16v)0.f};
-                half8 ka[2][G];
-                static_for<G>([&](auto I) __attribute__((always_inline)) { ka[0][I] = fa_kfrag<D, I>(kaddr); });
-                static_for<NS / G>([&](auto GI) __attribute__((always_inline)) {
-                    constexpr int gi = GI, cur = gi & 1;
-                    if constexpr (gi + 1 < NS / G) {
-                        static_for<G>([&](auto I) __attribute__((always_inline)) {
-                            ka[cur ^ 1][I] = fa_kfrag<D, (gi + 1) * G + I>(kaddr);
+            // step i of the 2 KS products is key block i % 2, head-dim step i / 2; K fragments are
+            // read G at a time, the next group's behind this one's products
+            constexpr int NS = 2 * KS, G = D == 64 ? 8 : 4;
+            constexpr int OPG = 2 * L::COPIES / (NS / G);
+            static_assert(OPG * (NS / G) == 2 * L::COPIES, "copies spread evenly over the groups");
+            const bool next = t + 1 < mine;
+            const __amdgpu_buffer_rsrc_t rkn = rsrc(t + 1, pgs.k), rvn = rsrc(t + 1, pgs.v);
+            LDS_AS char* nst = lds + ((t + 1) & 1) * L::STAGE + wave * L::COPIES * 1024;
+            float16v sacc[2] = {(float16v)0.f, (float16v)0.f};
+            half8 ka[2][G];
+            static_for<G>([&](auto I) __attribute__((always_inline)) { ka[0][I] = fa_kfrag<D, I>(kaddr); });
+            static_for<NS / G>([&](auto GI) __attribute__((always_inline)) {
+                constexpr int gi = GI, cur = gi & 1;
+                if constexpr (gi + 1 < NS / G) {
+                    static_for<G>([&](auto I) __attribute__((always_inline)) {
+                        ka[cur ^ 1][I] = fa_kfrag<D, (gi + 1) * G + I>(kaddr);
+                    });
+                    fa_lgkm_wait<G>();
+                } else {
+                    fa_lgkm_wait<0>();
+                }
+#pragma unroll
+                for (int i = 0; i < G; ++i) fa_pin(ka[cur][i]);
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    const int idx = gi * G + i;
+                    sacc[idx & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[cur][i], qf[idx >> 1], sacc[idx & 1], 0, 0, 0);
+                    if constexpr (Q2)
+                        sacc[idx & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[cur][i], q2[idx >> 1], sacc[idx & 1], 0, 0, 0);
+                }
+                if (next) {
+                    static_for<OPG>([&](auto I) __attribute__((always_inline)) {
+                        constexpr int op = gi * OPG + I;   // K copies, then V copies
+                        constexpr int j = op % L::COPIES;
+                        if constexpr (op < L::COPIES)
+                            __builtin_amdgcn_raw_ptr_buffer_load_lds(rkn, (LDS_AS void*)(nst + j * 1024), 16, (int)coff[j], 0, 0, 0);
+                        else
+                            __builtin_amdgcn_raw_ptr_buffer_load_lds(rvn, (LDS_AS void*)(nst + L::TILE + j * 1024), 16,
+                                                                     (int)coff[j], 0, 0, 0);
+                    });
+                }
+            });
+
+            // Softmax in log2 units. Keys of the tile: kb*32 + 8 (rr / 4) + 4 hf + rr % 4. Where every
+            // row of the wave sees the whole tile: the maximum over the raw scores, then 2^(fma(s, scale, -m)).
+            const int lo = kbeg - j0, hi = kend - j0;
+            const bool edge = !(__all(lo <= 0 && hi >= pp::KT) && blocks == 15u);
+            const bool fast = !edge && sc >= 0.f;     // (the scale's sign is every lane's)
+            // A position whose V holds a value that is not finite must not reach rows that do not
+            // see it through 0 times that value: its V is 0 here and its score NaN, which the mask
+            // replaces. Bit 8 kk + i of a lane is the position of its probability i of step kk.
+            bool odd = false;
+            if (edge) {
+                uint32_t bad = 0;
+                static_for<4>([&](auto KK) __attribute__((always_inline)) {
+                    static_for<DF>([&](auto DD) __attribute__((always_inline)) {
+                        const half8 v = pp::vfrag_now<D, KK, DD>(vaddr);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) bad |= pp::finite(v[i]) ? 0u : 1u << (8 * KK + i);
+                    });
+                });
+                odd = __any(bad != 0);
+                if (__builtin_expect(odd, 0)) {
+#pragma unroll
+                    for (int x = 1; x < 32; x <<= 1) bad |= __shfl_xor(bad, x);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (bad >> i & 1u) sacc[i >> 4][i & 15] = __builtin_nanf("");
+                }
+            }
+            if (!fast) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int rr = 0; rr < 16; ++rr) {
+                        const int kl = kb * 32 + 8 * (rr >> 2) + 4 * hf + (rr & 3);
+                        sacc[kb][rr] = kl < hi && kl >= lo ? sacc[kb][rr] * sc : -__builtin_inff();
+                    }
+                if (blocks != 15u) {
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        if (!(blocks >> b & 1u))
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) sacc[b >> 1][8 * (b & 1) + i] = -__builtin_inff();
+                }
+            }
+            float tm[10];
+#pragma unroll
+            for (int i = 0, j = 0; i < 10; ++i, j += 3)
+                tm[i] = fa_max3(sacc[j >> 4][j & 15], sacc[(j + 1) >> 4][(j + 1) & 15], sacc[(j + 2) >> 4][(j + 2) & 15]);
+            float tmax = fa_max3(fa_max3(tm[0], tm[1], tm[2]), fa_max3(tm[3], tm[4], tm[5]),
+                                 fa_max3(fa_max3(tm[6], tm[7], tm[8]), tm[9], fa_max3(sacc[1][14], sacc[1][15], sacc[1][15])));
+            if (fast) tmax *= sc;
+            tmax = swap_max32(tmax);
+            // the row's reference moves only when the maximum exceeds it by more than SLACK, for the
+            // whole wave at once
+            if (__builtin_expect(__any(tmax > m + SLACK), 0)) {
+                const float mnew = fmaxf(m, tmax);
+                const float alpha = __builtin_amdgcn_exp2f(m - (mnew == -__builtin_inff() ? 0.f : mnew));
+                l *= alpha;
+                m = mnew;
+                if (t > 0) {
+#pragma unroll
+                    for (int d = 0; d < DF; ++d) o[d] *= alpha;
+                }
+            }
+            const float ref = (m == -__builtin_inff() ? 0.f : m) - LIFT;    // (l and o carry 2^LIFT alike)
+            half8 pb[4], p2[P2 ? 4 : 1];
+            const float esc = fast ? sc : 1.f;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                float8v e;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kk >> 1][8 * (kk & 1) + i], esc, -ref));
+                pb[kk] = __builtin_convertvector(e, half8);
+                if constexpr (P2) p2[kk] = __builtin_convertvector(e - __builtin_convertvector(pb[kk], float8v), half8);
+                l += ((e[0] + e[4]) + (e[1] + e[5])) + ((e[2] + e[6]) + (e[3] + e[7]));   // (the lane's positions)
+            }
+
+            {
+                // O^T += V^T P^T, the next step's V^T fragments in flight behind this one's products
+                half8 vb[2][DF];
+                static_for<DF>([&](auto DD) __attribute__((always_inline)) { vb[0][DD] = fa_vfrag<D, 0, DD>(vaddr); });
+                static_for<4>([&](auto KK) __attribute__((always_inline)) {
+                    constexpr int kk = KK, cur = kk & 1;
+                    if constexpr (kk + 1 < 4) {
+                        static_for<DF>([&](auto DD) __attribute__((always_inline)) {
+                            vb[cur ^ 1][DD] = fa_vfrag<D, kk + 1, DD>(vaddr);
                         });
-                        fa_lgkm_wait<G>();
+                        fa_lgkm_wait<(2 * DF < 15 ? 2 * DF : 15)>();
                     } else {
                         fa_lgkm_wait<0>();
                     }
 #pragma unroll
-                    for (int i = 0; i < G; ++i) fa_pin(ka[cur][i]);
-#pragma unroll
-                    for (int i = 0; i < G; ++i) {
-                        const int idx = gi * G + i;
-                        sacc[idx & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[cur][i], qf[idx >> 1], sacc[idx & 1], 0, 0, 0);
-                        if constexpr (Q2)
-                            sacc[idx & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[cur][i], q2[idx >> 1], sacc[idx & 1], 0, 0, 0);
-                    }
-                    if (next) {
-                        static_for<OPG>([&](auto I) __attribute__((always_inline)) {
-                            constexpr int op = gi * OPG + I;   // K copies, then V copies
-                            constexpr int j = op % L::COPIES;
-                            if constexpr (op < L::COPIES)
-                                __builtin_amdgcn_raw_ptr_buffer_load_lds(rkn, (LDS_AS void*)(nst + j * 1024), 16, (int)coff[j], 0, 0, 0);
-                            else
-                                __builtin_amdgcn_raw_ptr_buffer_load_lds(rvn, (LDS_AS void*)(nst + L::TILE + j * 1024), 16,
-                                                                         (int)coff[j], 0, 0, 0);
-                        });
-                    }
-                });
-
-                // Softmax in log2 units. Keys of the tile: kb*32 + 8 (rr / 4) + 4 hf + rr % 4. Where every
-                // row of the wave sees the whole tile: the maximum over the raw scores, then 2^(fma(s, scale, -m)).
-                const int lo = kbeg - j0, hi = kend - j0;
-                const bool edge = !(__all(lo <= 0 && hi >= pp::KT) && blocks == 15u);
-                const bool fast = !edge && sc >= 0.f;     // (the scale's sign is every lane's)
-                // A position whose V holds a value that is not finite must not reach rows that do not
-                // see it through 0 times that value: its V is 0 here and its score NaN, which the mask
-                // replaces. Bit 8 kk + i of a lane is the position of its probability i of step kk.
-                bool odd = false;
-                if (edge) {
-                    uint32_t bad = 0;
-                    static_for<4>([&](auto KK) __attribute__((always_inline)) {
-                        static_for<DF>([&](auto DD) __attribute__((always_inline)) {
-                            const half8 v = pp::vfrag_now<D, KK, DD>(vaddr);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) bad |= pp::finite(v[i]) ? 0u : 1u << (8 * KK + i);
-                        });
-                    });
-                    odd = __any(bad != 0);
+                    for (int d = 0; d < DF; ++d) fa_pin(vb[cur][d]);
                     if (__builtin_expect(odd, 0)) {
 #pragma unroll
-                        for (int x = 1; x < 32; x <<= 1) bad |= __shfl_xor(bad, x);
+                        for (int d = 0; d < DF; ++d)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (bad >> i & 1u) sacc[i >> 4][i & 15] = __builtin_nanf("");
+                            for (int i = 0; i < 8; ++i) vb[cur][d][i] = pp::finite(vb[cur][d][i]) ? vb[cur][d][i] : (half_t)0.f;
                     }
-                }
-                if (!fast) {
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                        for (int rr = 0; rr < 16; ++rr) {
-                            const int kl = kb * 32 + 8 * (rr >> 2) + 4 * hf + (rr & 3);
-                            sacc[kb][rr] = kl < hi && kl >= lo ? sacc[kb][rr] * sc : -__builtin_inff();
-                        }
-                    if (blocks != 15u) {
-#pragma unroll
-                        for (int b = 0; b < 4; ++b)
-                            if (!(blocks >> b & 1u))
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) sacc[b >> 1][8 * (b & 1) + i] = -__builtin_inff();
+                    for (int d = 0; d < DF; ++d) {
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[cur][d], pb[kk], o[d], 0, 0, 0);
+                        if constexpr (P2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[cur][d], p2[kk], o[d], 0, 0, 0);
                     }
-                }
-                float tm[10];
-#pragma unroll
-                for (int i = 0, j = 0; i < 10; ++i, j += 3)
-                    tm[i] = fa_max3(sacc[j >> 4][j & 15], sacc[(j + 1) >> 4][(j + 1) & 15], sacc[(j + 2) >> 4][(j + 2) & 15]);
-                float tmax = fa_max3(fa_max3(tm[0], tm[1], tm[2]), fa_max3(tm[3], tm[4], tm[5]),
-                                     fa_max3(fa_max3(tm[6], tm[7], tm[8]), tm[9], fa_max3(sacc[1][14], sacc[1][15], sacc[1][15])));
-                if (fast) tmax *= sc;
-                tmax = swap_max32(tmax);
-                // the row's reference moves only when the maximum exceeds it by more than SLACK, for the
-                // whole wave at once
-                if (__builtin_expect(__any(tmax > m + SLACK), 0)) {
-                    const float mnew = fmaxf(m, tmax);
-                    const float alpha = __builtin_amdgcn_exp2f(m - (mnew == -__builtin_inff() ? 0.f : mnew));
-                    l *= alpha;
-                    m = mnew;
-                    if (t > 0) {
-#pragma unroll
-                        for (int d = 0; d < DF; ++d) o[d] *= alpha;
-                    }
-                }
-                const float ref = (m == -__builtin_inff() ? 0.f : m) - LIFT;    // (l and o carry 2^LIFT alike)
-                half8 pb[4], p2[P2 ? 4 : 1];
-                const float esc = fast ? sc : 1.f;
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    float8v e;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kk >> 1][8 * (kk & 1) + i], esc, -ref));
-                    pb[kk] = __builtin_convertvector(e, half8);
-                    if constexpr (P2) p2[kk] = __builtin_convertvector(e - __builtin_convertvector(pb[kk], float8v), half8);
-                    l += ((e[0] + e[4]) + (e[1] + e[5])) + ((e[2] + e[6]) + (e[3] + e[7]));   // (the lane's positions)
-                }
-
-                {
-                    // O^T += V^T P^T, the next step's V^T fragments in flight behind this one's products
-                    half8 vb[2][DF];
-                    static_for<DF>([&](auto DD) __attribute__((always_inline)) { vb[0][DD] = fa_vfrag<D, 0, DD>(vaddr); });
-                    static_for<4>([&](auto KK) __attribute__((always_inline)) {
-                        constexpr int kk = KK, cur = kk & 1;
-                        if constexpr (kk + 1 < 4) {
-                            static_for<DF>([&](auto DD) __attribute__((always_inline)) {
-                                vb[cur ^ 1][DD] = fa_vfrag<D, kk + 1, DD>(vaddr);
-                            });
-                            fa_lgkm_wait<(2 * DF < 15 ? 2 * DF : 15)>();
-                        } else {
-                            fa_lgkm_wait<0>();
-                        }
-#pragma unroll
-                        for (int d = 0; d < DF; ++d) fa_pin(vb[cur][d]);
-                        if (__builtin_expect(odd, 0)) {
-#pragma unroll
-                            for (int d = 0; d < DF; ++d)
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) vb[cur][d][i] = pp::finite(vb[cur][d][i]) ? vb[cur][d][i] : (half_t)0.f;
-                        }
-#pragma unroll
-                        for (int d = 0; d < DF; ++d) {
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[cur][d], pb[kk], o[d], 0, 0, 0);
-                            if constexpr (P2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[cur][d], p2[kk], o[d], 0, 0, 0);
-                        }
-                    });
-                }
+                });
             }
             const int32_t flip = t & 1 ? -L::STAGE : L::STAGE;    // the other stage
 #pragma unroll
@@ -477,81 +473,49 @@ __global__ __launch_bounds__(256 * pp::groups<D>(), pp::groups<D>()) void paged_
             __builtin_amdgcn_s_barrier();
         }
 
-        if (most & 1) {
+        if (mine & 1) {
 #pragma unroll
             for (int j = 0; j < NK; ++j) kaddr[j] -= L::STAGE;
 #pragma unroll
             for (int j = 0; j < 2; ++j) vaddr[j] -= L::STAGE;
         }
 
-        if constexpr (KG == 2) {
-            // the second group's sums, by register image
-            typedef float float2v __attribute__((ext_vector_type(2)));
-            LDS_AS float4v* po = (LDS_AS float4v*)(all + L::BYTES + wave * (QW * D * 4)) + lane;
-            LDS_AS float2v* pm = (LDS_AS float2v*)(all + wave * (QW * D * 4)) + lane;
-            if (kg == 1) {
-                *pm = float2v{m, l};
+        // The wave's rows go out through LDS (chunk c of row r at slot c ^ (r % 16)), as
+        // partial results or as rows of the output. Fragment d: values 32 d + 8 q4 + 4 hf ..+3.
+        l = swap_sum<32>(l, l);
+        const float inv = u.whole ? (l != 0.f ? 1.0f / l : 0.f) : 1.0f;
+        LDS_AS float4v* ob = (LDS_AS float4v*)(lds + wave * QW * D * 4);
 #pragma unroll
-                for (int d = 0; d < DF; ++d)
+        for (int d = 0; d < DF; ++d)
 #pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4)
-                        po[(d * 4 + q4) * 64] = float4v{o[d][4 * q4], o[d][4 * q4 + 1], o[d][4 * q4 + 2], o[d][4 * q4 + 3]};
-            }
-            __syncthreads();
-            if (kg == 0) {
-                const float2v ml = *pm;
-                const float mm = fmaxf(m, ml[0]), mr = mm == -__builtin_inff() ? 0.f : mm;
-                const float a0 = __builtin_amdgcn_exp2f(m - mr), a1 = __builtin_amdgcn_exp2f(ml[0] - mr);
-                l = l * a0 + ml[1] * a1;
-                m = mm;
-#pragma unroll
-                for (int d = 0; d < DF; ++d)
-#pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4) {
-                        const float4v v = po[(d * 4 + q4) * 64];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[d][4 * q4 + e] = o[d][4 * q4 + e] * a0 + v[e] * a1;
-                    }
-            }
-        }
-        if (kg == 0) {
-            // The wave's rows go out through LDS (chunk c of row r at slot c ^ (r % 16)), as
-            // partial results or as rows of the output. Fragment d: values 32 d + 8 q4 + 4 hf ..+3.
-            l = swap_sum<32>(l, l);
-            const float inv = u.whole ? (l != 0.f ? 1.0f / l : 0.f) : 1.0f;
-            LDS_AS float4v* ob = (LDS_AS float4v*)(all + wave * QW * D * 4);
-#pragma unroll
-            for (int d = 0; d < DF; ++d)
-#pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4)
-                    ob[ql * CR + ((8 * d + 2 * q4 + hf) ^ (ql & 15))] = float4v{o[d][4 * q4] * inv, o[d][4 * q4 + 1] * inv,
-                                                                              o[d][4 * q4 + 2] * inv, o[d][4 * q4 + 3] * inv};
-            constexpr int NJ = QW * CR / 64;
-            if (u.whole) {
-                const uint32_t row0 = u.rb * RB + wave * QW;
+            for (int q4 = 0; q4 < 4; ++q4)
+                ob[ql * CR + ((8 * d + 2 * q4 + hf) ^ (ql & 15))] = float4v{o[d][4 * q4] * inv, o[d][4 * q4 + 1] * inv,
+                                                                          o[d][4 * q4 + 2] * inv, o[d][4 * q4 + 3] * inv};
+        constexpr int NJ = QW * CR / 64;
+        if (u.whole) {
+            const uint32_t row0 = u.rb * RB + wave * QW;
 #pragma unroll 4
-                for (int j = 0; j < NJ; ++j) {
-                    const uint32_t e = j * 64 + lane, r = e / CR, c = e % CR, rr = row0 + r;
-                    const float4v v = ob[r * CR + (c ^ (r & 15))];
-                    if (rr < rows && 4 * c < HD) {
-                        const uint32_t tk = rr / group;
-                        const size_t at = ((size_t)(u.q.first + tk) * p.hq + u.hk * group + (rr - tk * group)) * HD + 4 * c;
-                        if (p.o_dtype == DT_F16) put4<true>((half_t*)p.out + at, 4, v);
-                        else put4<true>((float*)p.out + at, 4, v);
-                    }
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t e = j * 64 + lane, r = e / CR, c = e % CR, rr = row0 + r;
+                const float4v v = ob[r * CR + (c ^ (r & 15))];
+                if (rr < rows && 4 * c < HD) {
+                    const uint32_t tk = rr / group;
+                    const size_t at = ((size_t)(u.q.first + tk) * p.hq + u.hk * group + (rr - tk * group)) * HD + 4 * c;
+                    if (p.o_dtype == DT_F16) put4<true>((half_t*)p.out + at, 4, v);
+                    else put4<true>((float*)p.out + at, 4, v);
                 }
-            } else {
-                const size_t at = (size_t)u.slot * RB + wave * QW;
-                if (hf == 0) {
-                    p.ws_ml[2 * (at + ql)] = m;
-                    p.ws_ml[2 * (at + ql) + 1] = l;
-                }
-                float* dst = uniform_ptr(p.ws_o + at * D);
+            }
+        } else {
+            const size_t at = (size_t)u.slot * RB + wave * QW;
+            if (hf == 0) {
+                p.ws_ml[2 * (at + ql)] = m;
+                p.ws_ml[2 * (at + ql) + 1] = l;
+            }
+            float* dst = uniform_ptr(p.ws_o + at * D);
 #pragma unroll 4
-                for (int j = 0; j < NJ; ++j) {
-                    const uint32_t e = j * 64 + lane, r = e / CR, c = e % CR;
-                    *(float4v*)(dst + r * D + 4 * c) = ob[r * CR + (c ^ (r & 15))];
-                }
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t e = j * 64 + lane, r = e / CR, c = e % CR;
+                *(float4v*)(dst + r * D + 4 * c) = ob[r * CR + (c ^ (r & 15))];
             }
         }
         __syncthreads();     // the next piece's copies go where these were
@@ -563,21 +527,36 @@ __global__ __launch_bounds__(256 * pp::groups<D>(), pp::groups<D>()) void paged_
 template <int D>
 __global__ __launch_bounds__(256) void paged_merge_rows_kernel(PagedAttnParams p)
 {
-    constexpr uint32_t C4 = D / 4;
+    constexpr uint32_t C4 = D / 4, AHEAD = 8;
     const pg::Joint x = ((const pg::Joint*)p.ws_plan)[blockIdx.x + 1];
     const uint32_t e = blockIdx.y * 256 + threadIdx.x, row = e / C4, c = e % C4;
     if (x.parts == 0 || row >= x.rows || 4 * c >= p.head_dim) return;
     const auto at = [&](uint32_t i) { return (size_t)(2 * (x.wg + i) + (i == 0 ? 1u : 0u)) * pp::RB + row; };
-    float M = -__builtin_inff();
-    for (uint32_t i = 0; i < x.parts; ++i) M = fmaxf(M, p.ws_ml[2 * at(i)]);
-    const float ref = M == -__builtin_inff() ? 0.f : M;
+    float M = -__builtin_inff(), sum = 0.f;
     float4v acc = (float4v)0.f;
-    float sum = 0.f;
-    for (uint32_t i = 0; i < x.parts; ++i) {
-        const size_t a = at(i);
-        const float w = __builtin_amdgcn_exp2f(p.ws_ml[2 * a] - ref);
-        acc += w * *(const float4v*)(p.ws_o + a * D + 4 * c);
-        sum += w * p.ws_ml[2 * a + 1];
+    for (uint32_t i = 0; i < x.parts; i += AHEAD) {      // (all their loads in flight)
+        float m[AHEAD], l[AHEAD], top = M;
+        float4v v[AHEAD];
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) {
+            const size_t a = at(min(i + k, x.parts - 1));
+            m[k] = p.ws_ml[2 * a];
+            l[k] = p.ws_ml[2 * a + 1];
+            v[k] = *(const float4v*)(p.ws_o + a * D + 4 * c);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) top = fmaxf(top, m[k]);
+        const float ref = top == -__builtin_inff() ? 0.f : top, w0 = __builtin_amdgcn_exp2f(M - ref);
+        acc *= w0;
+        sum *= w0;
+        M = top;
+#pragma unroll
+        for (uint32_t k = 0; k < AHEAD; ++k) {
+            if (i + k >= x.parts) break;
+            const float w = __builtin_amdgcn_exp2f(m[k] - ref);
+            acc += w * v[k];
+            sum += w * l[k];
+        }
     }
     pg::put_row(p, x.first, x.hk, x.row0 + row, 4 * c, acc, sum);
 }
@@ -585,20 +564,20 @@ __global__ __launch_bounds__(256) void paged_merge_rows_kernel(PagedAttnParams p
 void paged_prefill_plan(PagedAttnParams& p, uint32_t cus)
 {
     p.rb = pp::RB;
-    p.lead = 2;
+    p.lead = 6;
     p.min_share = 4;
-    p.wgs = std::min<uint32_t>(cus, PagedAttnParams::MAX_WGS);
+    p.wgs = std::min<uint32_t>(p.dp == 256 ? cus : 2 * cus, PagedAttnParams::MAX_WGS);
 }
 
 template <int D, bool Q2, bool P2>
 static hipError_t prefill_launch(const PagedAttnParams& p, hipStream_t s)
 {
-    constexpr int KG = pp::groups<D>(), bytes = KG * fa::Lds<D>::BYTES;
+    constexpr int bytes = fa::Lds<D>::BYTES;
     const uint32_t at = ((p.pages.sequences + 1) * 4 + 1023) / 1024 * 1024;
     static PerDevice once;
     const hipError_t e = set_max_lds(once, (const void*)paged_prefill_kernel<D, Q2, P2>, bytes + KvPages::MAX_SEQUENCES * 4 + 1024);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_prefill_kernel<D, Q2, P2>), dim3(p.wgs), dim3(256 * KG), at + bytes, s, p, at);
+    hipLaunchKernelGGL((paged_prefill_kernel<D, Q2, P2>), dim3(p.wgs), dim3(256), at + bytes, s, p, at);
     return hipGetLastError();
 }
 
