@@ -393,9 +393,10 @@ struct VerifyParams {
     uint32_t sequences, rows, vocab, target_stride, draft_stride;
     int target_dtype, draft_dtype;
     void* workspace;
+    double powers[32];            // set by the launch: 2^(i / 32)
 };
 size_t verify_workspace(const VerifyParams& p);
-hipError_t verify_launch(const VerifyParams& p, hipStream_t s);
+hipError_t verify_launch(VerifyParams p, hipStream_t s);
 
 // Linear over 8-bit weights (linear_i8.hip).
 struct LinearI8Params {

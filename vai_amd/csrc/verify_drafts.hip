@@ -12,6 +12,8 @@
 // by reading the logits, the others by latency: loads that do not wait for the
 // judgement are issued before it.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "pages.h"
 
@@ -19,11 +21,12 @@ namespace vai_dev {
 
 namespace {
 
-constexpr uint32_t CH = 4096, NT = 256, PT = CH / NT;   // logits a workgroup, threads, logits a thread
+constexpr uint32_t CH = 4096;                           // logits a workgroup
+constexpr uint32_t NT = 256, PT = CH / NT;              // threads of the first pass, logits a thread
 constexpr uint32_t NO_TOKEN = 0xffffffffu;
 
-// A part of a row: its largest logit (NaN: one that is NaN or +infinity is there),
-// where that is first, and the sum of exp((x - largest) / T).
+// A part of a row: its largest logit (infinity: one that is NaN or +infinity is
+// there), where that is first (T = 0), and the sum of exp((x - largest) / T).
 struct Stat {
     float top;
     uint32_t at;
@@ -35,8 +38,7 @@ __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 // e^y for y <= 0, within 2e-14 of it: 2^n e^r, n = y / ln 2 rounded and |r| <= ln 2 / 2
 // (ln 2 in two parts, the first short enough that n times it is exact), e^r its power
 // series up to r^11 (the next term is below 7e-15). Below -800, and where the logit
-// is -infinity, nothing is left. Sixteen fp64 operations: 46 M logits take 19 us of
-// them where they take 36 to read; the library's exp takes three times as many.
+// is -infinity, nothing is left.
 __device__ __forceinline__ double power(double y)
 {
     y = fmax(y, -800.0);
@@ -56,8 +58,60 @@ __device__ __forceinline__ double power(double y)
     p = fma(p, r, 1.0);
     return ldexp(p, (int)n);
 }
+// The same for the first pass, where every logit needs one: n = 32 y / ln 2 rounded,
+// |r| <= ln 2 / 64, the power series up to r^5 (the next term is below 3e-15) and
+// 2^(n % 32 / 32) from `table`, whose 32 entries lie in as many pairs of LDS banks. A
+// third fewer operations: 46 M logits, 184 MB, took 51 us with the long series.
+__device__ __forceinline__ double power(double y, const double* table)
+{
+    y = fmax(y, -800.0);
+    const double n = rint(y * 46.16624130844682904);
+    const double r = fma(-n, 0x1.9ef35793c7673p-46, fma(-n, 0x1.62e42fefa2p-6, y));
+    double p = 1.0 / 120;
+    p = fma(p, r, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    const int i = (int)n;
+    return ldexp(p * table[i & 31], i >> 5);
+}
 // exp((x - top) / T)
 __device__ __forceinline__ double power(float x, float top, double inv_t) { return power(((double)x - (double)top) * inv_t); }
+
+// Which logits a thread of N takes as its 8: neighbouring ones of fp16, two times 4 of
+// fp32, 16 bytes a lane and load
+template <uint32_t N>
+__device__ __forceinline__ uint32_t nth(int dt, uint32_t t, uint32_t i)
+{
+    return dt == DT_F16 ? 8 * t + i : (i >> 2) * (4 * N) + 4 * t + (i & 3);
+}
+template <uint32_t N>
+__device__ __forceinline__ void logits8_apart(const void* rows, int dt, size_t row, uint32_t j, uint32_t t, uint32_t vocab, float (&x)[8])
+{
+    if (j + 8 * N <= vocab) {
+        if (dt == DT_F16) {
+            typedef half8 half8u __attribute__((aligned(2)));
+            const half8 v = *(const half8u*)((const half_t*)rows + row + j + 8 * t);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+        } else {
+            const float* at = (const float*)rows + row + j + 4 * t;
+            const float4v a = load4f(at), b = load4f(at + 4 * N);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = a[i];
+                x[4 + i] = b[i];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t k = j + nth<N>(dt, t, i);
+            x[i] = k < vocab ? ld(rows, dt, row + k) : -__builtin_inff();
+        }
+    }
+}
 
 // 8 logits of a row from j on, -infinity past its end
 __device__ __forceinline__ void logits8(const void* rows, int dt, size_t row, uint32_t j, uint32_t vocab, float (&x)[8])
@@ -82,27 +136,34 @@ __device__ __forceinline__ void logits8(const void* rows, int dt, size_t row, ui
     }
 }
 
-__device__ __forceinline__ double wave_sum64(double v)
+// op over the wave's lanes: within rows of 16 lanes by DPP, the four rows' by reading
+// their first lanes. The order is fixed.
+template <class T, class Op>
+__device__ __forceinline__ T wave_reduce(T v, Op op)
 {
+    constexpr int N = sizeof(T) / 4;
+    struct Words { int w[N]; };
+    const auto moved = [](T x, auto ctrl) __attribute__((always_inline)) {
+        Words a = __builtin_bit_cast(Words, x);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-// the larger top (NaN above all), the lower place among equals
-__device__ __forceinline__ void take_larger(float& top, uint32_t& at, float top2, uint32_t at2)
-{
-    const bool nan = top != top, nan2 = top2 != top2;
-    if (nan2 ? !nan || at2 < at : !nan && (top2 > top || (top2 == top && at2 < at))) {
-        top = top2;
-        at = at2;
-    }
-}
-__device__ __forceinline__ void wave_larger(float& top, uint32_t& at)
-{
+        for (int i = 0; i < N; ++i) a.w[i] = __builtin_amdgcn_update_dpp(0, a.w[i], decltype(ctrl)::value, 0xf, 0xf, true);
+        return __builtin_bit_cast(T, a);
+    };
+    const auto lane = [](T x, int l) __attribute__((always_inline)) {
+        Words a = __builtin_bit_cast(Words, x);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) take_larger(top, at, __shfl_xor(top, o), __shfl_xor(at, o));
+        for (int i = 0; i < N; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], l);
+        return __builtin_bit_cast(T, a);
+    };
+    v = op(v, moved(v, std::integral_constant<int, 0xB1>{}));     // lane ^ 1
+    v = op(v, moved(v, std::integral_constant<int, 0x4E>{}));     // lane ^ 2
+    v = op(v, moved(v, std::integral_constant<int, 0x141>{}));    // the other 4 of 8 (mirrored)
+    v = op(v, moved(v, std::integral_constant<int, 0x140>{}));    // the other 8 of 16
+    return op(op(lane(v, 0), lane(v, 16)), op(lane(v, 32), lane(v, 48)));
 }
+__device__ __forceinline__ double wave_sum64(double v) { return wave_reduce(v, [](double a, double b) { return a + b; }); }
+__device__ __forceinline__ float wave_max(float v) { return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) { return wave_reduce(v, [](uint32_t a, uint32_t b) { return min(a, b); }); }
 
 __device__ __forceinline__ uint32_t parts_of(uint32_t vocab) { return (vocab + CH - 1) / CH; }
 __device__ __forceinline__ Stat* stats_of(const VerifyParams& p, uint32_t which, uint32_t row)
@@ -134,13 +195,16 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyParams p)
     __shared__ uint32_t ats[4];
     __shared__ double sums[4];
     const uint32_t parts = parts_of(p.vocab), row = blockIdx.x / parts, part = blockIdx.x - row * parts;
-    const uint32_t which = blockIdx.y, t = threadIdx.x, j0 = part * CH + 8 * t;
+    const uint32_t which = blockIdx.y, t = threadIdx.x;
+    const int dt = which ? p.draft_dtype : p.target_dtype;
+    __shared__ double table[32];
+    if (t < 32) table[t] = p.powers[t];
     float x[PT / 8][8];
     const auto read = [&] {
 #pragma unroll
         for (uint32_t k = 0; k < PT / 8; ++k)
-            logits8(which ? p.draft : p.target, which ? p.draft_dtype : p.target_dtype,
-                    (size_t)row * (which ? p.draft_stride : p.target_stride), j0 + k * NT * 8, p.vocab, x[k]);
+            logits8_apart<NT>(which ? p.draft : p.target, dt, (size_t)row * (which ? p.draft_stride : p.target_stride),
+                              part * CH + k * NT * 8, t, p.vocab, x[k]);
     };
     if (!which) read();          // (a row of no sequence in vain: the loads do not wait for the search)
     const uint32_t s = wave_last_le(p.start, p.sequences, row);
@@ -160,8 +224,7 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyParams p)
             odd = odd || !(x[k][i] < __builtin_inff());
         }
     if (odd) top = __builtin_inff();
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    top = wave_max(top);
     if ((t & 63) == 0) tops[t >> 6] = top;
     __syncthreads();
     top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
@@ -173,7 +236,7 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyParams p)
 #pragma unroll
             for (uint32_t k = 0; k < PT / 8; ++k)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += power(x[k][i], top, inv_t);
+                for (int i = 0; i < 8; ++i) sum += power(((double)x[k][i] - (double)top) * inv_t, table);
             sum = wave_sum64(sum);
         } else {
             // the lowest index of the largest
@@ -181,9 +244,8 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyParams p)
             for (uint32_t k = 0; k < PT / 8; ++k)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (x[k][i] == top) at = min(at, j0 + k * NT * 8 + i);
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
+                    if (x[k][i] == top) at = min(at, part * CH + k * NT * 8 + nth<NT>(dt, t, i));
+            at = wave_min(at);
         }
     }
     if ((t & 63) == 0) {
@@ -192,7 +254,6 @@ __global__ __launch_bounds__(NT) void verify_rows_kernel(VerifyParams p)
     }
     __syncthreads();
     if (t != 0) return;
-    if (top == __builtin_inff()) top = __builtin_nanf("");
     stats_of(p, which, row)[part] = Stat{top, min(min(ats[0], ats[1]), min(ats[2], ats[3])), (sums[0] + sums[1]) + (sums[2] + sums[3])};
 }
 
@@ -200,9 +261,10 @@ namespace {
 
 // A whole row, from its parts' (a wave).
 struct Row {
-    float top;         // NaN or -infinity: no distribution
+    float top;         // infinite: no distribution
     uint32_t at;
     double sum;
+    __device__ bool good() const { return top < __builtin_inff() && top > neg_inf(); }
 };
 __device__ __forceinline__ Row row_of(const VerifyParams& p, uint32_t which, uint32_t row, float T)
 {
@@ -211,14 +273,20 @@ __device__ __forceinline__ Row row_of(const VerifyParams& p, uint32_t which, uin
     const uint32_t parts = parts_of(p.vocab), lane = threadIdx.x & 63;
     Row r{neg_inf(), 0xffffffffu, 0.0};
     const Stat mine = lane < parts ? st[lane] : Stat{neg_inf(), 0xffffffffu, 0.0};
-    take_larger(r.top, r.at, mine.top, mine.at);
-    for (uint32_t i = lane + 64; i < parts; i += 64) take_larger(r.top, r.at, st[i].top, st[i].at);
-    wave_larger(r.top, r.at);
-    if (T > 0.f && r.top > neg_inf()) {
+    r.top = mine.top;
+    for (uint32_t i = lane + 64; i < parts; i += 64) r.top = fmaxf(r.top, st[i].top);
+    r.top = wave_max(r.top);
+    if (!r.good()) return r;
+    if (T > 0.f) {
         if (mine.top > neg_inf()) r.sum = mine.sum * power(mine.top, r.top, inv_t);
         for (uint32_t i = lane + 64; i < parts; i += 64)
             if (st[i].top > neg_inf()) r.sum += st[i].sum * power(st[i].top, r.top, inv_t);
         r.sum = wave_sum64(r.sum);
+    } else {
+        if (mine.top == r.top) r.at = mine.at;
+        for (uint32_t i = lane + 64; i < parts; i += 64)
+            if (st[i].top == r.top) r.at = min(r.at, st[i].at);
+        r.at = wave_min(r.at);
     }
     return r;
 }
@@ -244,7 +312,7 @@ __device__ __forceinline__ uint32_t judge_row(const VerifyParams& p, uint32_t r,
     a = row_of(p, 0, r, T);
     b = Row{0.f, 0, 1.0};
     if (p.draft && draft_follows) b = row_of(p, 1, r, T);
-    if (!(a.top > neg_inf()) || !(b.top > neg_inf())) return 3;
+    if (!a.good() || !b.good()) return 3;
     if (!draft_follows) return T > 0.f ? 1 : 4;
     double px, qx;
     if (T > 0.f) {
@@ -322,31 +390,43 @@ __device__ __forceinline__ Verdict* verdict_of(const VerifyParams& p, uint32_t s
 
 }   // namespace
 
-// Grid: (parts, sequences): the judged row's max(p - q, 0), summed over the part.
+// Grid: (shares of the parts, sequences): the judged row's max(p - q, 0), summed over
+// each part. (Every workgroup judges for itself: with one a part, 32 sequences of 32
+// parts, that took 22 us.)
 __global__ __launch_bounds__(512) void verify_weights_kernel(VerifyParams p)
 {
-    __shared__ double sums[8];
-    const uint32_t part = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
+    __shared__ double sums[2][8];
+    const uint32_t s = blockIdx.y, t = threadIdx.x, parts = parts_of(p.vocab);
     const Verdict v = judge<8>(p, s);
-    if (part == 0 && t == 0) *verdict_of(p, s) = v;
+    if (blockIdx.x == 0 && t == 0) *verdict_of(p, s) = v;
     if (v.mode != 1) return;
-    double w[8], sum = 0;
-    weights8(p, v, true, inverse_of(v.T), part * CH + 8 * t, w);
+    uint32_t turn = 0;
+    for (uint32_t part = blockIdx.x; part < parts; part += gridDim.x, turn ^= 1) {
+        double sum = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += w[i];
-    sum = wave_sum64(sum);
-    if ((t & 63) == 0) sums[t >> 6] = sum;
-    __syncthreads();
-    if (t == 0)
-        weights_of(p, s)[part] = ((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7]));
+        for (uint32_t k = 0; k < CH / 4096; ++k) {
+            double w[8];
+            weights8(p, v, true, inverse_of(v.T), part * CH + k * 4096 + 8 * t, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += w[i];
+        }
+        sum = wave_sum64(sum);
+        double* all = sums[turn];    // (the other turn's may still be read)
+        if ((t & 63) == 0) all[t >> 6] = sum;
+        __syncthreads();
+        if (t == 0) weights_of(p, s)[part] = ((all[0] + all[1]) + (all[2] + all[3])) + ((all[4] + all[5]) + (all[6] + all[7]));
+    }
 }
 
 namespace {
 
+constexpr uint32_t DT = 512;       // threads of the last pass, 8 logits each
+static_assert(DT * 8 == CH);
+
 // The sum of the values of the threads before this one, and the whole sum.
 __device__ __forceinline__ double before_me(double v, double& whole)
 {
-    __shared__ double sums[4];
+    __shared__ double sums[DT / 64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double scan = v;
 #pragma unroll
@@ -358,25 +438,29 @@ __device__ __forceinline__ double before_me(double v, double& whole)
     if (lane == 63) sums[wave] = scan;
     __syncthreads();
     double at = scan - v;
-    for (uint32_t w = 0; w < wave; ++w) at += sums[w];
-    whole = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    whole = 0;
+    for (uint32_t w = 0; w < DT / 64; ++w) {
+        if (w < wave) at += sums[w];
+        whole += sums[w];
+    }
     return at;
 }
 __device__ __forceinline__ uint32_t smallest(uint32_t v)
 {
-    __shared__ uint32_t all[4];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
+    __shared__ uint32_t all[DT / 64];
+    v = wave_min(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) all[threadIdx.x >> 6] = v;
     __syncthreads();
-    return min(min(all[0], all[1]), min(all[2], all[3]));
+    v = all[0];
+    for (uint32_t w = 1; w < DT / 64; ++w) v = min(v, all[w]);
+    return v;
 }
 
 }   // namespace
 
 // One workgroup a sequence: the last token, and what is reported.
-__global__ __launch_bounds__(NT) void verify_draw_kernel(VerifyParams p)
+__global__ __launch_bounds__(DT) void verify_draw_kernel(VerifyParams p)
 {
     const uint32_t s = blockIdx.x, t = threadIdx.x;
     const Verdict v = *verdict_of(p, s);
@@ -390,7 +474,7 @@ __global__ __launch_bounds__(NT) void verify_draw_kernel(VerifyParams p)
     uint32_t token = v.mode == 3 ? v.p.at : NO_TOKEN;
     if (v.mode < 2) {
         const double inv_t = inverse_of(v.T), u = (double)p.uniform[v.last];
-        const uint32_t parts = parts_of(p.vocab), per = (parts + NT - 1) / NT;
+        const uint32_t parts = parts_of(p.vocab), per = (parts + DT - 1) / DT;
         const uint32_t i0 = min(t * per, parts), i1 = min(i0 + per, parts);
         bool rest = v.mode == 1;
         const auto part_sum = [&](uint32_t i) {
@@ -432,24 +516,17 @@ __global__ __launch_bounds__(NT) void verify_draw_kernel(VerifyParams p)
         }
         __syncthreads();
         const double goal = u * whole - before;
-        // the same inside the part: thread t has PT neighbouring logits
-        const uint32_t j0 = part * CH + t * PT;
-        double w[PT];
+        // the same inside the part: thread t has 8 neighbouring logits
+        const uint32_t j0 = part * CH + t * 8;
+        double w[8];
+        weights8(p, v, rest, inv_t, j0, w);
         own = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < PT; k += 8) {
-            double y[8];
-            weights8(p, v, rest, inv_t, j0 + k, y);
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                w[k + i] = y[i];
-                own += y[i];
-            }
-        }
+        for (uint32_t i = 0; i < 8; ++i) own += w[i];
         run = before_me(own, whole);
         uint32_t found = 0xffffffffu, last = 0xffffffffu;
 #pragma unroll
-        for (uint32_t i = 0; i < PT; ++i) {
+        for (uint32_t i = 0; i < 8; ++i) {
             run += w[i];
             if (w[i] > 0) last = j0 + i;
             if (found == 0xffffffffu && w[i] > 0 && run > goal) found = j0 + i;
@@ -458,7 +535,7 @@ __global__ __launch_bounds__(NT) void verify_draw_kernel(VerifyParams p)
         if (token == 0xffffffffu) token = ~smallest(last == 0xffffffffu ? last : ~last);
     }
     const uint32_t kept = v.stop - v.first;
-    for (uint32_t r = v.first + t; r <= v.last; r += NT)
+    for (uint32_t r = v.first + t; r <= v.last; r += DT)
         p.out_tokens[r] = r < v.stop ? p.tokens[r + 1] : r == v.stop ? token : NO_TOKEN;
     if (t == 0) {
         p.accepted[s] = kept;
@@ -472,12 +549,14 @@ size_t verify_workspace(const VerifyParams& p)
     return (size_t)(p.draft ? 2 : 1) * p.rows * parts * sizeof(Stat) + (size_t)p.sequences * (parts * sizeof(double) + sizeof(Verdict));
 }
 
-hipError_t verify_launch(const VerifyParams& p, hipStream_t s)
+hipError_t verify_launch(VerifyParams p, hipStream_t s)
 {
+    for (int i = 0; i < 32; ++i) p.powers[i] = std::exp2(i / 32.0);
     const uint32_t parts = (p.vocab + CH - 1) / CH;
     hipLaunchKernelGGL(verify_rows_kernel, dim3(parts * p.rows, p.draft ? 2 : 1), dim3(NT), 0, s, p);
-    hipLaunchKernelGGL(verify_weights_kernel, dim3(parts, p.sequences), dim3(512), 0, s, p);
-    hipLaunchKernelGGL(verify_draw_kernel, dim3(p.sequences), dim3(NT), 0, s, p);
+    const uint32_t shares = std::max(1u, std::min(parts, 256 / p.sequences));
+    hipLaunchKernelGGL(verify_weights_kernel, dim3(shares, p.sequences), dim3(512), 0, s, p);
+    hipLaunchKernelGGL(verify_draw_kernel, dim3(p.sequences), dim3(DT), 0, s, p);
     return hipGetLastError();
 }
 
