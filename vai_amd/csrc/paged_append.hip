@@ -27,13 +27,15 @@ __device__ __forceinline__ Place place_of(const PagedAppendParams& p, uint32_t t
 {
     Place r{0, -1, false};
     const KvPages& g = p.pages;
+    // (the same in every lane: scalar registers)
+    const auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane(x); };
     const uint32_t s = wave_last_le(g.start, g.sequences, token);
-    if (s == g.sequences || token >= g.start[s + 1]) return r;
+    if (s == g.sequences || token >= uniform(g.start[s + 1])) return r;
     r.row = true;
-    const uint64_t pos = (uint64_t)g.counts[s] + (token - g.start[s]);
+    const uint64_t pos = (uint64_t)uniform(g.counts[s]) + (token - uniform(g.start[s]));
     r.pos = (uint32_t)pos;
     if (pos < (uint64_t)g.max_pages * g.page_size) {
-        const uint32_t i = r.pos / g.page_size, page = g.table[(size_t)s * g.max_pages + i];
+        const uint32_t i = r.pos / g.page_size, page = uniform(g.table[(size_t)s * g.max_pages + i]);
         if (page < g.num_pages) r.slot = (int64_t)(page * g.stride + (uint64_t)(r.pos - i * g.page_size) * p.head_dim);
     }
     return r;
@@ -111,9 +113,12 @@ __global__ __launch_bounds__(64) void paged_append_any_kernel(PagedAppendParams 
 // Head dims up to 512, as qk_norm_rope_kernel cuts them: L lanes share a head, 8
 // values each, so that a lane holds both values of its four pairs (FULL: of all
 // its groups of four). A wave takes a token's heads 64 / L at a time, its share of
-// them (blockIdx.y of `shares`).
+// them (blockIdx.y of `shares`), the next heads' values in flight. 4098 tokens in
+// three sequences, 32 + 8 + 8 fp16 heads of 128: 24 us, 4.2 TB/s (with one step's
+// loads at a time and the weights in registers, four waves a SIMD, 33); a single
+// token's 5 us are latency.
 template <typename TI, int L, bool FULL>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p, uint32_t shares, uint32_t steps)
+__global__ __launch_bounds__(256, 5) void paged_append_kernel(PagedAppendParams p, uint32_t shares, uint32_t steps)
 {
     constexpr int HPW = 64 / L;
     const uint32_t D = p.head_dim, heads = p.hq + 2 * p.hkv, nk = p.hq + p.hkv, lane = threadIdx.x & 63;
@@ -126,15 +131,18 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p, 
     const uint32_t na = oa < lim ? min(4u, lim - oa) : 0u, nb = split ? na : ob < D ? min(4u, D - ob) : 0u;
     const bool on = na != 0;   // (a lane past the head's last value loads its first ones where FULL, and drops them)
     const float inv_d = 1.0f / (float)D;
-    float4v wq[2] = {(float4v)1.0f, (float4v)1.0f}, wk[2] = {(float4v)1.0f, (float4v)1.0f};
+    // a lane's weights wait in LDS, not in registers: six waves a SIMD instead of four
+    __shared__ float4v weights[4][4][64];
+    float4v w4[4] = {(float4v)1.0f, (float4v)1.0f, (float4v)1.0f, (float4v)1.0f};
     if (p.q_weight) {
-        wq[0] = weight4(p.q_weight, p.w_dtype, oa, na) + p.weight_offset;
-        wq[1] = weight4(p.q_weight, p.w_dtype, ob, nb) + p.weight_offset;
+        w4[0] = weight4(p.q_weight, p.w_dtype, oa, na);
+        w4[1] = weight4(p.q_weight, p.w_dtype, ob, nb);
     }
     if (p.k_weight) {
-        wk[0] = weight4(p.k_weight, p.w_dtype, oa, na) + p.weight_offset;
-        wk[1] = weight4(p.k_weight, p.w_dtype, ob, nb) + p.weight_offset;
+        w4[2] = weight4(p.k_weight, p.w_dtype, oa, na);
+        w4[3] = weight4(p.k_weight, p.w_dtype, ob, nb);
     }
+    bool kept = false;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t s0 = steps * blockIdx.y / shares, s1 = steps * (blockIdx.y + 1) / shares;
     for (uint32_t token = blockIdx.x * 4 + wave; token < p.tokens; token += gridDim.x * 4) {
@@ -142,13 +150,37 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p, 
         Place at{};
         float c[4], s[4];
         bool angles = false;
+        typedef TI t4 __attribute__((ext_vector_type(4)));
+        typedef t4 t4u __attribute__((aligned(sizeof(TI))));
+        t4 ra, rb;               // (FULL: the next step's values, as they are)
+        const auto read = [&](uint32_t it) __attribute__((always_inline)) {
+            const TI* src = row + (size_t)min(h0 + it * HPW + sub, heads - 1) * D;
+            ra = *(const t4u*)(src + (on ? oa : 0u));
+            rb = *(const t4u*)(src + (on ? ob : 0u));
+        };
+        if constexpr (FULL) read(s0);
         for (uint32_t it = s0; it < s1; ++it) {
-            const uint32_t h = h0 + it * HPW + sub, hc = min(h, heads - 1);
-            const float4v xa = some4<FULL>(row + (size_t)hc * D + (FULL && !on ? 0u : oa), na);
-            const float4v xb = some4<FULL>(row + (size_t)hc * D + (FULL && !on ? 0u : ob), nb);
+            const uint32_t h = h0 + it * HPW + sub;
+            float4v xa, xb;
+            if constexpr (FULL) {
+                xa = __builtin_convertvector(ra, float4v);
+                xb = __builtin_convertvector(rb, float4v);
+                if (it + 1 < s1) read(it + 1);
+            } else {
+                const TI* src = row + (size_t)min(h, heads - 1) * D;
+                xa = some4<false>(src + oa, na);
+                xb = some4<false>(src + ob, nb);
+            }
             if (!angles) {   // (under the first loads)
                 angles = true;
                 at = place_of(p, token);
+                if (!kept) {
+                    kept = true;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        weights[wave][i][lane] = w4[i] + ((i < 2 ? p.q_weight : p.k_weight) ? p.weight_offset : 0.f);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     c[i] = 1.f;
@@ -185,8 +217,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p, 
                     v = sum * inv_d + ldexpf(p.eps, -2 * e2);
                 }
                 const float inv = inv_root(v);
+                const float4v wa = weights[wave][is_q ? 0 : 2][lane], wb = weights[wave][is_q ? 1 : 3][lane];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] *= inv * (is_q ? wq[e >> 2][e & 3] : wk[e >> 2][e & 3]);
+                for (int e = 0; e < 8; ++e) y[e] *= inv * (e < 4 ? wa[e & 3] : wb[e & 3]);
             }
             if (turned && !is_v) {
                 const auto turn = [&](float& a, float& e, int i) __attribute__((always_inline)) {
@@ -218,10 +251,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p, 
 template <typename TI, int L, bool FULL>
 static hipError_t launch_vec(const PagedAppendParams& p, hipStream_t s)
 {
-    // tokens whose waves alone fill the chip are not shared out: each share takes
-    // the place and the angles again
+    // tokens whose waves alone fill the chip are not shared out: each share takes the
+    // place and the angles again, as long as one and a half of its steps (32 + 8 + 8
+    // heads of 128, 12 steps; tokens: us with 1, 2, 4, 12 shares: 64: 12.8, 9.0, 7.3, 6.4;
+    // 1000: 15.1, 11.8, 11.7, 18.6; 2500: 19.3, 17.5; 3000: 19.6, 23.6)
     const uint32_t steps = ((p.q_out ? p.hq : 0u) + 2 * p.hkv + 64 / L - 1) / (64 / L);
-    const uint32_t shares = std::min(steps, std::max(1u, 4096 / p.tokens));
+    const uint32_t shares = std::min(steps, std::max(1u, (3800 + p.tokens / 2) / p.tokens));
     hipLaunchKernelGGL((paged_append_kernel<TI, L, FULL>), dim3(std::min((p.tokens + 3) / 4, 1u << 20), shares), dim3(256), 0,
                        s, p, shares, steps);
     return hipGetLastError();
