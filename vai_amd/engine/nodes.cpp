@@ -644,4 +644,202 @@ void QkNormRope::run(CommandStream& cmd)
     check(vai_qk_norm_rope_launch(&a, (vai_stream_t)cmd.stream()), "QkNormRope");
 }
 
+// ----------------------------------------- PagedAppend, PagedAttention ----
+
+PagedAppend::PagedAppend(Config config) : config_(config)
+{
+    if (config_.numKVHeads == 0) config_.numKVHeads = config_.numQHeads;
+    require(config_.numQHeads > 0 && config_.headDim > 0, "PagedAppend: heads and headDim must be positive");
+    if (config_.rotDim == 0) config_.rotDim = config_.headDim;
+    require(config_.pairs == Pairs::None || (config_.rotDim <= config_.headDim && config_.rotDim % 2 == 0),
+            "PagedAppend: rotDim must be even and at most headDim");
+    addSlot("in0", NodeSlot::input);
+    addSlot("Q", NodeSlot::output);
+    addSlot("q_weight", NodeSlot::persistent);
+    addSlot("k_weight", NodeSlot::persistent);
+    addSlot("inv_freq", NodeSlot::persistent);
+}
+
+void PagedAppend::setPages(const vai_kv_pages& pages)
+{
+    pages_ = pages;
+    if (ownedNet_) ownedNet_->invalidateCommandBuffer();
+}
+
+void PagedAppend::prepare()
+{
+    const Tensor& in = (*this)["in0"];
+    const auto& s = in.shape();
+    const uint32_t hq = config_.numQHeads, hkv = config_.numKVHeads, d = config_.headDim;
+    require(s.size() >= 2 && s.back() == (hq + 2 * hkv) * d,
+            "PagedAppend: in0 must be [..., (numQHeads + 2 numKVHeads) headDim]");
+    Dtype weights = Dtype::None;
+    for (const char* name : {"q_weight", "k_weight"}) {
+        const Tensor& w = (*this)[name];
+        if (!w.validShape()) continue;
+        require(config_.norm, "PagedAppend: weights without norm");
+        require(w.isShapeOf({d}), "PagedAppend: weights must be [headDim]");
+        require(weights == Dtype::None || weights == w.dtype(), "PagedAppend: the weights must share a dtype");
+        weights = w.dtype();
+    }
+    const Tensor& f = (*this)["inv_freq"];
+    require(!f.validShape() || (f.isShapeOf({config_.rotDim / 2}) && f.dtype() == Dtype::Fp32),
+            "PagedAppend: inv_freq must be [rotDim / 2] fp32");
+    require(pages_.k_pages != nullptr, "PagedAppend: setPages comes before a forward");
+    tokens_ = outerSize(s, 1);
+    std::vector<uint32_t> os(s.begin(), s.end() - 1);
+    os.insert(os.end(), {hq, d});
+    (*this)["Q"] = Tensor(os, outputDtype());
+}
+
+void PagedAppend::run(CommandStream& cmd)
+{
+    vai_paged_append_args a{};
+    const Tensor &qw = (*this)["q_weight"], &kw = (*this)["k_weight"];
+    a.qkv = (*this)["in0"].devicePtr();
+    a.q_out = (*this)["Q"].devicePtr();
+    a.q_weight = ptrOrNull(qw);
+    a.k_weight = ptrOrNull(kw);
+    a.inv_freq = static_cast<const float*>(ptrOrNull((*this)["inv_freq"]));
+    a.pages = pages_;
+    a.tokens = tokens_;
+    a.hq = config_.numQHeads;
+    a.hkv = config_.numKVHeads;
+    a.head_dim = config_.headDim;
+    a.i_dtype = code((*this)["in0"].dtype());
+    a.o_dtype = code(outputDtype());
+    a.w_dtype = qw.validShape() ? code(qw.dtype()) : code(kw.dtype());
+    a.norm = config_.norm ? 1 : 0;
+    a.eps = config_.eps;
+    a.weight_offset = config_.weightOffset;
+    a.rope = uint32_t(config_.pairs);
+    a.rot_dim = config_.rotDim;
+    a.theta = config_.theta;
+    check(vai_paged_append_launch(&a, (vai_stream_t)cmd.stream()), "PagedAppend");
+}
+
+PagedAttention::PagedAttention(Config config) : config_(config)
+{
+    if (config_.numKVHeads == 0) config_.numKVHeads = config_.numQHeads;
+    require(config_.numQHeads > 0 && config_.headDim > 0, "PagedAttention: heads and headDim must be positive");
+    require(config_.numQHeads % config_.numKVHeads == 0, "PagedAttention: numQHeads must be a multiple of numKVHeads");
+    require(config_.headDim <= 256, "PagedAttention: headDim must be at most 256");
+    addSlot("out0", NodeSlot::output);
+    addSlot("Q", NodeSlot::input);
+    addSlot("partialO", NodeSlot::temporary);
+}
+
+void PagedAttention::setPages(const vai_kv_pages& pages)
+{
+    pages_ = pages;
+    if (ownedNet_) ownedNet_->invalidateCommandBuffer();
+}
+
+// The launch without its buffers: the size query needs no more.
+vai_paged_attention_args PagedAttention::args() const
+{
+    vai_paged_attention_args a{};
+    alignas(16) static char dummy[16];
+    a.out = dummy;
+    a.q = dummy;
+    a.pages = pages_;
+    a.tokens = tokens_;
+    a.max_new = config_.maxNew;
+    a.hq = config_.numQHeads;
+    a.hkv = config_.numKVHeads;
+    a.head_dim = config_.headDim;
+    a.o_dtype = code(outputDtype());
+    a.q_dtype = code((*this)["Q"].dtype());
+    a.scale = config_.scale;
+    a.causal = config_.causal ? 1 : 0;
+    a.span = config_.span;
+    return a;
+}
+
+void PagedAttention::prepare()
+{
+    const Tensor& q = (*this)["Q"];
+    const auto& s = q.shape();
+    require(s.size() >= 3 && s.back() == config_.headDim && s[s.size() - 2] == config_.numQHeads,
+            "PagedAttention: Q must be [..., numQHeads, headDim]");
+    require(pages_.k_pages != nullptr, "PagedAttention: setPages comes before a forward");
+    tokens_ = outerSize(s, 2);
+    (*this)["out0"] = Tensor(s, outputDtype());
+    const vai_paged_attention_args a = args();
+    const size_t ws = vai_paged_attention_workspace_size(&a);
+    (*this)["partialO"] = ws ? Tensor({uint32_t((ws + 3) / 4)}, Dtype::Fp32) : Tensor();   // (0: the launch says why)
+}
+
+void PagedAttention::run(CommandStream& cmd)
+{
+    vai_paged_attention_args a = args();
+    const Tensor& part = (*this)["partialO"];
+    a.out = (*this)["out0"].devicePtr();
+    a.q = (*this)["Q"].devicePtr();
+    a.workspace = ptrOrNull(part);
+    a.workspace_bytes = part.validShape() ? part.numBytes() : 0;
+    check(vai_paged_attention_launch(&a, (vai_stream_t)cmd.stream()), "PagedAttention");
+}
+
+// ---------------------------------------------------------- VerifyDrafts ----
+
+VerifyDrafts::VerifyDrafts()
+{
+    addSlot("target", NodeSlot::input);
+    addSlot("draft", NodeSlot::input);
+    addSlot("partials", NodeSlot::temporary);
+}
+
+void VerifyDrafts::setBatch(const Batch& batch)
+{
+    batch_ = batch;
+    if (ownedNet_) ownedNet_->invalidateCommandBuffer();
+}
+
+// The launch without its buffers: the size query needs no more.
+vai_verify_drafts_args VerifyDrafts::args() const
+{
+    const Tensor &target = (*this)["target"], &draft = (*this)["draft"];
+    vai_verify_drafts_args a{};
+    alignas(16) static char dummy[16];
+    a.target = dummy;
+    a.draft = draft.validShape() ? dummy : nullptr;
+    a.out_tokens = batch_.outTokens;
+    a.accepted = batch_.accepted;
+    a.new_counts = batch_.newCounts;
+    a.tokens = batch_.tokens;
+    a.uniform = batch_.uniform;
+    a.temperature = batch_.temperature;
+    a.seq_start = batch_.seqStart;
+    a.counts = batch_.counts;
+    a.sequences = batch_.sequences;
+    a.rows = outerSize(target.shape(), 1);
+    a.vocab = target.shape().back();
+    a.target_dtype = code(target.dtype());
+    a.draft_dtype = draft.validShape() ? code(draft.dtype()) : VAI_DTYPE_NONE;
+    return a;
+}
+
+void VerifyDrafts::prepare()
+{
+    const Tensor &target = (*this)["target"], &draft = (*this)["draft"];
+    require(target.shape().size() >= 2, "VerifyDrafts: target must be [..., rows, vocab]");
+    require(!draft.validShape() || draft.shape() == target.shape(), "VerifyDrafts: target and draft must share a shape");
+    require(batch_.outTokens != nullptr, "VerifyDrafts: setBatch comes before a forward");
+    const vai_verify_drafts_args a = args();
+    const size_t ws = vai_verify_drafts_workspace_size(&a);
+    (*this)["partials"] = ws ? Tensor({uint32_t((ws + 3) / 4)}, Dtype::Fp32) : Tensor();   // (0: the launch says why)
+}
+
+void VerifyDrafts::run(CommandStream& cmd)
+{
+    vai_verify_drafts_args a = args();
+    const Tensor &part = (*this)["partials"], &draft = (*this)["draft"];
+    a.target = (*this)["target"].devicePtr();
+    a.draft = ptrOrNull(draft);
+    a.workspace = ptrOrNull(part);
+    a.workspace_bytes = part.validShape() ? part.numBytes() : 0;
+    check(vai_verify_drafts_launch(&a, (vai_stream_t)cmd.stream()), "VerifyDrafts");
+}
+
 }   // namespace vai::node

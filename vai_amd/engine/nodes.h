@@ -271,5 +271,92 @@ private:
     uint32_t batch_ = 1, tokens_ = 0;
 };
 
+// Many sequences in one forward over a KV cache in pages (vai_kv_pages; not the
+// reference's). The pages, the table, the rows' starts and the counts are device
+// memory of the model's; a net's PagedAppend and PagedAttention of one layer take the
+// same ones. They are read when the kernels run, so a recorded forward follows what
+// the model (or VerifyDrafts) writes there; other pointers or sizes re-record.
+//
+// PagedAppend: in0 [..., (numQHeads + 2 numKVHeads) headDim], the tokens' fused
+// projections in fp32 or fp16; keys and values go to their pages, "Q" [..., numQHeads,
+// headDim] to the node's output dtype. Norm, weights and rotation as QkNormRope's
+// (theirs is the same Config), at the tokens' positions (vai_paged_append_launch).
+class PagedAppend : public Node
+{
+public:
+    using Pairs = QkNormRope::Pairs;
+    using Config = QkNormRope::Config;
+    Config config_;
+
+    explicit PagedAppend(Config config);
+    void prepare() override;
+    void run(CommandStream& cmd) override;
+    const char* kind() const override { return "PagedAppend"; }
+    void setPages(const vai_kv_pages& pages);
+
+private:
+    vai_kv_pages pages_{};
+    uint32_t tokens_ = 0;
+};
+
+// PagedAttention: "Q" [..., numQHeads, headDim] (PagedAppend's, whose wire also orders
+// the two), out0 the same shape in the node's output dtype (vai_paged_attention_launch).
+class PagedAttention : public Node
+{
+public:
+    struct Config {
+        uint32_t headDim;
+        uint32_t numQHeads;
+        uint32_t numKVHeads = 0;              // 0: numQHeads
+        bool causal = true;
+        uint32_t span = 0;                    // sliding window; 0: none
+        float scale = 0.0f;                   // 0: 1/sqrt(headDim)
+        uint32_t maxNew = 0;                  // no sequence brings more tokens (chooses kernels); 0: all of the rows
+    } config_;
+
+    explicit PagedAttention(Config config);
+    void prepare() override;
+    void run(CommandStream& cmd) override;
+    const char* kind() const override { return "PagedAttention"; }
+    void setPages(const vai_kv_pages& pages);
+
+private:
+    vai_paged_attention_args args() const;
+    vai_kv_pages pages_{};
+    uint32_t tokens_ = 0;
+};
+
+// Drafted tokens against the target's logits, "target" [rows, vocab] (and "draft"
+// [rows, vocab], left unwired for drafts without probabilities), fp32 or fp16
+// (vai_verify_drafts_launch). It has no output slot: tokens and counts are whole
+// numbers, in device memory of the model's. With newCounts the counts that the next
+// forward's PagedAppend reads, a recorded forward advances them by itself (after the
+// layers that read them: the logits come from these).
+class VerifyDrafts : public Node
+{
+public:
+    struct Batch {
+        uint32_t sequences = 0;
+        const uint32_t* seqStart = nullptr;   // [sequences + 1]
+        const uint32_t* tokens = nullptr;     // [rows]
+        const float* uniform = nullptr;       // [rows]
+        const float* temperature = nullptr;   // [sequences]; null: 1
+        const uint32_t* counts = nullptr;     // [sequences]; needed with newCounts
+        uint32_t* outTokens = nullptr;        // [rows]
+        uint32_t* accepted = nullptr;         // [sequences]
+        uint32_t* newCounts = nullptr;        // [sequences], or null
+    };
+
+    VerifyDrafts();
+    void prepare() override;
+    void run(CommandStream& cmd) override;
+    const char* kind() const override { return "VerifyDrafts"; }
+    void setBatch(const Batch& batch);
+
+private:
+    vai_verify_drafts_args args() const;
+    Batch batch_;
+};
+
 }   // namespace node
 }   // namespace vai

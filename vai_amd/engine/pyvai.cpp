@@ -92,6 +92,28 @@ static vai::node::CausalBlockEnd block_ends(const std::vector<uint32_t>& ends)
     return e;
 }
 
+// (device addresses and sizes, as vai_kv_pages has them)
+template <class N>
+static void set_pages(N& n, uintptr_t k_pages, uintptr_t v_pages, uintptr_t page_table, uintptr_t seq_start, uintptr_t counts,
+                      uint32_t sequences, uint32_t num_pages, uint32_t page_size, uint32_t max_pages, Dtype dtype,
+                      uint64_t page_stride)
+{
+    if (dtype == Dtype::Q4) throw std::invalid_argument("pages are F32 or F16");
+    vai_kv_pages p{};
+    p.k_pages = reinterpret_cast<void*>(k_pages);
+    p.v_pages = reinterpret_cast<void*>(v_pages);
+    p.page_table = reinterpret_cast<const uint32_t*>(page_table);
+    p.seq_start = reinterpret_cast<const uint32_t*>(seq_start);
+    p.counts = reinterpret_cast<const uint32_t*>(counts);
+    p.page_stride = page_stride;
+    p.sequences = sequences;
+    p.num_pages = num_pages;
+    p.page_size = page_size;
+    p.max_pages = max_pages;
+    p.page_dtype = dtype == Dtype::Fp16 ? VAI_DTYPE_F16 : VAI_DTYPE_F32;
+    n.setPages(p);
+}
+
 PYBIND11_MODULE(_pyvai, m)
 {
     m.doc() = "vai_amd engine: NeuralNet / Tensor / nodes on MI355X kernels";
@@ -197,6 +219,43 @@ PYBIND11_MODULE(_pyvai, m)
         .def("set_position_counter", [](node::QkNormRope& n, uintptr_t ptr) {
                  n.setPositionCounter(reinterpret_cast<const uint32_t*>(ptr));
              }, py::arg("device_ptr"));
+    py::class_<node::PagedAppend, Node>(nodes, "PagedAppendNode")
+        .def(py::init([](uint32_t num_q_heads, uint32_t head_dim, uint32_t num_kv_heads, bool norm, float eps,
+                         float weight_offset, node::QkNormRope::Pairs pairs, uint32_t rot_dim, float theta) {
+                 node::PagedAppend::Config c{.headDim = head_dim, .numQHeads = num_q_heads, .numKVHeads = num_kv_heads,
+                                             .norm = norm, .eps = eps, .weightOffset = weight_offset, .pairs = pairs,
+                                             .rotDim = rot_dim, .theta = theta};
+                 return std::make_unique<node::PagedAppend>(c);
+             }),
+             py::arg("num_q_heads"), py::arg("head_dim"), py::arg("num_kv_heads") = 0, py::arg("norm") = true,
+             py::arg("eps") = 1e-6f, py::arg("weight_offset") = 0.0f, py::arg("pairs") = node::QkNormRope::Pairs::Halves,
+             py::arg("rot_dim") = 0, py::arg("theta") = 10000.0f)
+        .def("set_pages", &set_pages<node::PagedAppend>, py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"),
+             py::arg("seq_start"), py::arg("counts"), py::arg("sequences"), py::arg("num_pages"), py::arg("page_size"),
+             py::arg("max_pages"), py::arg("dtype"), py::arg("page_stride") = 0);
+    py::class_<node::PagedAttention, Node>(nodes, "PagedAttentionNode")
+        .def(py::init([](uint32_t num_q_heads, uint32_t head_dim, uint32_t num_kv_heads, bool causal, uint32_t span,
+                         float scale, uint32_t max_new) {
+                 return std::make_unique<node::PagedAttention>(node::PagedAttention::Config{
+                     .headDim = head_dim, .numQHeads = num_q_heads, .numKVHeads = num_kv_heads, .causal = causal,
+                     .span = span, .scale = scale, .maxNew = max_new});
+             }),
+             py::arg("num_q_heads"), py::arg("head_dim"), py::arg("num_kv_heads") = 0, py::arg("causal") = true,
+             py::arg("span") = 0, py::arg("scale") = 0.0f, py::arg("max_new") = 0)
+        .def("set_pages", &set_pages<node::PagedAttention>, py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"),
+             py::arg("seq_start"), py::arg("counts"), py::arg("sequences"), py::arg("num_pages"), py::arg("page_size"),
+             py::arg("max_pages"), py::arg("dtype"), py::arg("page_stride") = 0);
+    py::class_<node::VerifyDrafts, Node>(nodes, "VerifyDraftsNode")
+        .def(py::init<>())
+        .def("set_batch", [](node::VerifyDrafts& n, uint32_t sequences, uintptr_t seq_start, uintptr_t tokens, uintptr_t uniform,
+                             uintptr_t out_tokens, uintptr_t accepted, uintptr_t temperature, uintptr_t counts, uintptr_t new_counts) {
+                 const auto u32 = [](uintptr_t x) { return reinterpret_cast<uint32_t*>(x); };
+                 n.setBatch({.sequences = sequences, .seqStart = u32(seq_start), .tokens = u32(tokens),
+                             .uniform = reinterpret_cast<const float*>(uniform),
+                             .temperature = reinterpret_cast<const float*>(temperature), .counts = u32(counts),
+                             .outTokens = u32(out_tokens), .accepted = u32(accepted), .newCounts = u32(new_counts)});
+             }, py::arg("sequences"), py::arg("seq_start"), py::arg("tokens"), py::arg("uniform"), py::arg("out_tokens"),
+             py::arg("accepted"), py::arg("temperature") = 0, py::arg("counts") = 0, py::arg("new_counts") = 0);
     py::class_<node::GatedMul, Node>(nodes, "GatedMulNode")
         .def(py::init([](Epilogue activation) {
                  return std::make_unique<node::GatedMul>(node::GatedMul::Config{activation});
