@@ -6,8 +6,13 @@
 // registers. S^T = K Q^T over 16 keys x 16 query rows: lane (c16, g) reads 4
 // neighbouring values of key c16 at a time, which are its k's of four steps, and
 // gets the scores of row c16 with keys 4 g ..+3. Those are, as they stand, the
-// lane's P^T operands of O^T += V^T P^T when step r of it takes key 4 g + r. No
-// value moves between lanes but for the row's maximum and sum.
+// lane's P^T operands of O^T += V^T P^T when step r of it takes key 4 g + r; of that
+// key's V the lane reads DP / 16 neighbouring values, one for each output block (so
+// that O^T's row i of block b is value i DP / 16 + b). No value moves between lanes
+// but for where the keys lie and the row's maximum and sum. Where the next 16 keys'
+// K and V lie is looked up, and what the next ones hold is read, while 16 are
+// multiplied: 64 sequences of up to 8192 positions of fp32 pages, 8 heads of 128,
+// take 205 us (409 with one load after the other).
 #include "paged_plan.h"
 
 #include "launch_once.h"
@@ -21,23 +26,93 @@ namespace vai_dev {
 // 40 / 30; of 256 (16 over 4), 32 rows 56 / 53, 64 rows 93 / 54.
 static uint32_t few_most(uint32_t dp) { return dp == 128 ? 64 : 32; }
 
-template <int DP, typename T>
-__global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParams p)
+// Values d ..+3 of a row of D, as they are, zeros past its end or where there is no row
+// (any row that is), W at a time: D is a multiple of W (1, 2 or 4). Without branches:
+// what is not wanted is read from the row's own values.
+template <int W, typename T>
+__device__ __forceinline__ auto raw4(const T* row, uint32_t d, uint32_t D, bool there)
+{
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    if constexpr (W == 4) {
+        typedef t4 t4u __attribute__((aligned(sizeof(T))));
+        const t4 v = *(const t4u*)(row + (d < D ? d : 0u));
+        return there && d < D ? v : (t4)(T)0;
+    } else if constexpr (W == 2) {
+        typedef t2 t2u __attribute__((aligned(sizeof(T))));
+        t2 a = *(const t2u*)(row + (d < D ? d : 0u)), b = *(const t2u*)(row + (d + 2 < D ? d + 2 : 0u));
+        a = there && d < D ? a : (t2)(T)0;
+        b = there && d + 2 < D ? b : (t2)(T)0;
+        return (t4)__builtin_shufflevector(a, b, 0, 1, 2, 3);
+    } else {
+        t4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const T x = row[min(d + e, D - 1)];
+            v[e] = there && d + e < D ? x : (T)0;
+        }
+        return v;
+    }
+}
+
+template <int DP, typename T, int W>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void paged_attention_any_kernel(PagedAttnParams p)
 {
     using namespace pg;
     constexpr int KB = DP / 16, RB = 16, NW = 4;
+    constexpr bool AHEAD = DP < 256;       // (of 256-wide heads two steps' values would not fit the registers)
     extern __shared__ float4v paged_lds[];
     __shared__ uint32_t pre[KvPages::MAX_SEQUENCES + 1];
+    __shared__ Sequence kept[KEPT];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c16 = lane & 15, g = lane >> 4, D = p.head_dim, group = p.hq / p.hkv;
     const KvPages& pgs = p.pages;
     const float sl2 = p.scale * 1.4426950408889634f;   // scores in log2 units
-    plan_line<NW>(p, RB, pre);
-    walk<RB>(p, pre, [&](const Piece& u) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    struct Step {                          // 16 keys
+        t4 k[KB], v[4][KB / 4];            // key c16's values 16 b + 4 g ..+3; keys 4 g + r's values c16 KB ..
+        uint32_t there;                    // bit r: key 4 g + r is there
+    };
+    plan_line<NW>(p, RB, pre, kept);
+    walk<RB>(p, pre, kept, [&](const Piece& u) {
         const uint32_t rows = u.q.n * group, row = min(u.rb * RB + c16, rows - 1);
         const uint32_t tok = row / group, pos = u.q.held + tok;
         const uint32_t kbeg = first_key(p, pos), kend = p.causal ? min(pos + 1, u.q.live) : u.q.live;
         const size_t qat = (size_t)(u.q.first + tok) * p.q_stride + (size_t)(u.hk * group + row % group) * D;
+        const uint32_t see = first_key(p, u.q.held);     // no row sees a position before it
+        const uint32_t first = u.t0 + wave;
+        const int steps = first < u.t1 ? 2 * (int)((u.t1 - first + NW - 1) / NW) : 0;
+        const auto j0_of = [&](int i) __attribute__((always_inline)) { return (first + (uint32_t)(i >> 1) * NW) * KT + 16 * (i & 1); };
+        // where the lane's key of step i starts (in both pools), -1: it is not there
+        const auto locate = [&](int i) __attribute__((always_inline)) {
+            const uint32_t j = j0_of(i) + c16, n = j / pgs.page_size;
+            if (i >= steps || j < see || j >= u.q.live) return (int64_t)-1;
+            const uint32_t page = pgs.table[(size_t)u.s * pgs.max_pages + n];
+            if (page >= pgs.num_pages) return (int64_t)-1;
+            return (int64_t)(page * pgs.stride + ((uint64_t)u.hk * pgs.page_size + (j - n * pgs.page_size)) * D);
+        };
+        const auto load = [&](int64_t at, Step& x) __attribute__((always_inline)) {
+            const T* k = (const T*)pgs.k + (at < 0 ? 0 : at);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                x.k[b] = raw4<W>(k, 16 * b + 4 * g, D, at >= 0);
+            }
+            x.there = 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t vat = __shfl(at, 4 * g + r);
+                x.there |= vat >= 0 ? 1u << r : 0u;
+                const T* v = (const T*)pgs.v + (vat < 0 ? 0 : vat);
+#pragma unroll
+                for (int b = 0; b < KB / 4; ++b) x.v[r][b] = raw4<W>(v, c16 * KB + 4 * b, D, vat >= 0);
+            }
+        };
+        Step cur, nxt;
+        int64_t at = locate(0);
+        if constexpr (AHEAD) {
+            load(at, cur);
+            at = locate(1);
+        }
         float4v qf[KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b)
@@ -50,36 +125,27 @@ __global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParam
         float4v o[1][KB];
 #pragma unroll
         for (int d = 0; d < KB; ++d) o[0][d] = (float4v)0.f;
-        const uint32_t see = first_key(p, u.q.held);     // no row sees a position before it
-        for (uint32_t t = u.t0 + wave; t < u.t1; t += NW)
-            for (uint32_t j0 = t * KT; j0 < (t + 1) * KT; j0 += 16) {
-                // the lane's key: where its K and V start, if it is there
-                const uint32_t j = j0 + c16, i = j / pgs.page_size;
-                int64_t at = -1;
-                if (j >= see && j < u.q.live) {
-                    const uint32_t page = pgs.table[(size_t)u.s * pgs.max_pages + i];
-                    if (page < pgs.num_pages)
-                        at = (int64_t)(page * pgs.stride + ((uint64_t)u.hk * pgs.page_size + (j - i * pgs.page_size)) * D);
-                }
-                if (!__any(at >= 0)) continue;
+        for (int i = 0; i < steps; ++i) {
+            if constexpr (AHEAD) {
+                load(at, nxt);
+                at = locate(i + 2);
+            } else {
+                load(at, cur);
+                at = locate(i + 1);
+            }
+            if (__any(cur.there != 0)) {
+                const uint32_t j0 = j0_of(i);
                 float4v sa = (float4v)0.f;
-                const T* k = (const T*)pgs.k + (at < 0 ? 0 : at);
 #pragma unroll
-                for (int b = 0; b < KB; ++b) {
-                    const uint32_t d = 16 * b + 4 * g;
-                    const float4v x = some4<false>(k + d, at >= 0 && d < D ? min(4u, D - d) : 0u);
+                for (int b = 0; b < KB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sa = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], qf[b][e], sa, 0, 0, 0);
-                }
+                    for (int e = 0; e < 4; ++e) sa = __builtin_amdgcn_mfma_f32_16x16x4f32((float)cur.k[b][e], qf[b][e], sa, 0, 0, 0);
                 // scores of the lane's row with keys 4 g + r
                 float v[4], top = -__builtin_inff();
-                int64_t vat[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const uint32_t key = j0 + 4 * g + r;
-                    vat[r] = __shfl(at, 4 * g + r);
-                    const bool seen = key >= kbeg && key < kend && vat[r] >= 0;
-                    v[r] = seen ? sa[r] * sl2 : -__builtin_inff();
+                    v[r] = key >= kbeg && key < kend && (cur.there >> r & 1u) ? sa[r] * sl2 : -__builtin_inff();
                     top = fmaxf(top, v[r]);
                 }
                 top = fmaxf(top, __shfl_xor(top, 16));
@@ -87,27 +153,21 @@ __global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParam
                 const float mnew = fmaxf(m[0], top), ref = mnew == -__builtin_inff() ? 0.f : mnew;
                 const float alpha = __builtin_amdgcn_exp2f(m[0] - ref);
                 m[0] = mnew;
-                float e[4], sum = 0.f;
+                float e[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    e[r] = __builtin_amdgcn_exp2f(v[r] - ref);
-                    sum += e[r];
-                }
-                sum += __shfl_xor(sum, 16);
-                sum += __shfl_xor(sum, 32);
-                l[0] = l[0] * alpha + sum;
+                for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(v[r] - ref);
+                l[0] = l[0] * alpha + ((e[0] + e[1]) + (e[2] + e[3]));    // (the lane's keys)
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
-                    const uint32_t d = 16 * b + c16;
                     float x[4];
                     bool odd = false;       // a value that is not finite: 0 times it would reach rows that do not see it
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        x[r] = vat[r] >= 0 && d < D ? (float)((const T*)pgs.v)[vat[r] + d] : 0.f;
+                        x[r] = (float)cur.v[r][b >> 2][b & 3];
                         odd = odd || !(__builtin_fabsf(x[r]) < __builtin_inff());
                     }
                     o[0][b] *= alpha;
-                    if (__any(odd)) {
+                    if (__builtin_expect(__any(odd), 0)) {
                         float4v bad = (float4v)0.f;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -122,7 +182,11 @@ __global__ __launch_bounds__(256) void paged_attention_any_kernel(PagedAttnParam
                     for (int r = 0; r < 4; ++r) o[0][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], e[r], o[0][b], 0, 0, 0);
                 }
             }
-        finish_piece<DP, 1, NW>(p, u, (char*)paged_lds, m, l, o);
+            if constexpr (AHEAD) cur = nxt;
+        }
+        l[0] += __shfl_xor(l[0], 16);
+        l[0] += __shfl_xor(l[0], 32);
+        finish_piece<DP, 1, NW, true>(p, u, (char*)paged_lds, m, l, o);
     });
 }
 
@@ -260,15 +324,21 @@ static void set_workspace(PagedAttnParams& p, char* ws)
     p.ws_ml = p.ws_o + (size_t)2 * p.wgs * p.rb * p.dp;
 }
 
-template <int DP, typename T>
+template <int DP, typename T, int W>
 static hipError_t any_launch(const PagedAttnParams& p, hipStream_t s)
 {
     constexpr int bytes = pg::finish_bytes<DP, 1, 4>();
     static PerDevice once;
-    const hipError_t e = set_max_lds(once, (const void*)paged_attention_any_kernel<DP, T>, bytes);
+    const hipError_t e = set_max_lds(once, (const void*)paged_attention_any_kernel<DP, T, W>, bytes);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_attention_any_kernel<DP, T>), dim3(p.wgs), dim3(256), bytes, s, p);
+    hipLaunchKernelGGL((paged_attention_any_kernel<DP, T, W>), dim3(p.wgs), dim3(256), bytes, s, p);
     return hipGetLastError();
+}
+
+template <typename T, int W>
+static hipError_t any_launch_d(const PagedAttnParams& p, hipStream_t s)
+{
+    return p.dp == 64 ? any_launch<64, T, W>(p, s) : p.dp == 128 ? any_launch<128, T, W>(p, s) : any_launch<256, T, W>(p, s);
 }
 
 hipError_t paged_attention_launch(PagedAttnPlan& plan, void* ws, hipStream_t s)
@@ -278,7 +348,7 @@ hipError_t paged_attention_launch(PagedAttnPlan& plan, void* ws, hipStream_t s)
     const PagedAttnParams& p = plan.few;
     const auto go = [&](auto t) {
         typedef decltype(t) T;
-        return p.dp == 64 ? any_launch<64, T>(p, s) : p.dp == 128 ? any_launch<128, T>(p, s) : any_launch<256, T>(p, s);
+        return p.head_dim % 4 == 0 ? any_launch_d<T, 4>(p, s) : p.head_dim % 2 == 0 ? any_launch_d<T, 2>(p, s) : any_launch_d<T, 1>(p, s);
     };
     hipError_t e = plan.many.wgs ? paged_prefill_launch(plan.many, s) : hipSuccess;
     if (e != hipSuccess || p.wgs == 0) return e;

@@ -126,8 +126,9 @@ __global__ __launch_bounds__(64 * Ring<DP>::NW, Ring<DP>::RES) void paged_decode
     const uint32_t vrow = 4 * g + (c16 >> 2);
     const uint32_t vread = 2 * R::BLOCK + vrow * R::ROWB + ((((c16 >> 1) & 1u) ^ (uint32_t)swz_row<DP>(vrow)) << 4) + (c16 & 1) * 8;
 
-    plan_line<NW>(p, RB, pre);
-    walk<RB>(p, pre, [&](const Piece& u) __attribute__((always_inline)) {
+    __shared__ Sequence kept[KEPT];
+    plan_line<NW>(p, RB, pre, kept);
+    walk<RB>(p, pre, kept, [&](const Piece& u) __attribute__((always_inline)) {
         const uint32_t rows = u.q.n * group, row0 = u.rb * RB, rend = min(row0 + RB, rows);
         typedef typename std::conditional<Q32, float, half_t>::type qt;
         typedef qt q8 __attribute__((ext_vector_type(8)));

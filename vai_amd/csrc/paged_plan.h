@@ -40,10 +40,13 @@ __device__ __forceinline__ Span span_of(const PagedAttnParams& p, const Sequence
     return r;
 }
 
-// pre[s] = the line's tiles before sequence s, pre[sequences] all. LDS; every
-// thread of the workgroup's NW waves calls.
+// The first sequences of a batch, kept in LDS by plan_line: walk need not load them again.
+constexpr uint32_t KEPT = 128;
+
+// pre[s] = the line's tiles before sequence s, pre[sequences] all. LDS, as `kept`
+// [KEPT]; every thread of the workgroup's NW waves calls.
 template <int NW>
-__device__ __forceinline__ void plan_line(const PagedAttnParams& p, uint32_t rb, uint32_t* pre)
+__device__ __forceinline__ void plan_line(const PagedAttnParams& p, uint32_t rb, uint32_t* pre, Sequence* kept)
 {
     __shared__ uint32_t wave_sum_[NW];
     const uint32_t n = p.pages.sequences, per = (n + 64 * NW - 1) / (64 * NW), lane = threadIdx.x & 63;
@@ -51,6 +54,7 @@ __device__ __forceinline__ void plan_line(const PagedAttnParams& p, uint32_t rb,
     uint32_t sum = 0;
     for (uint32_t s = s0; s < s1; ++s) {
         const Sequence q = sequence_of(p.pages, s, p.tokens);
+        if (s < KEPT) kept[s] = q;
         uint32_t w = 0;
         if (q.n && q.n * (p.hq / p.hkv) <= p.few_rows) {
             const Span r = span_of(p, q, rb);
@@ -124,8 +128,9 @@ template <int DP, int NQ, int NW> constexpr int finish_bytes() { return NW * NQ 
 
 // The waves' sums meet in LDS (`lds`, finish_bytes(); what it held is done with
 // once every wave is here) and leave as rows or partial results. Lane (c16, g) of
-// a wave holds row c16 of each 16: m (log2 units), l, and values 16 d + 4 g ..+3.
-template <int DP, int NQ, int NW>
+// a wave holds row c16 of each 16: m (log2 units), l, and in o[d][r] value 16 d + 4 g
+// + r (ACROSS: (4 g + r) DP / 16 + d).
+template <int DP, int NQ, int NW, bool ACROSS = false>
 __device__ __forceinline__ void finish_piece(const PagedAttnParams& p, const Piece& u, char* lds, const float (&m)[NQ],
                                              const float (&l)[NQ], const float4v (&o)[NQ][DP / 16])
 {
@@ -140,8 +145,17 @@ __device__ __forceinline__ void finish_piece(const PagedAttnParams& p, const Pie
             ml[2 * r] = m[q];
             ml[2 * r + 1] = l[q];
         }
+        if constexpr (ACROSS) {
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) *(float4v*)(lds + r * orow<DP>() + (16 * d + 4 * g) * 4) = o[q][d];
+            for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+                for (int d = 0; d < DP / 16; d += 4)
+                    *(float4v*)(lds + r * orow<DP>() + ((4 * g + rr) * (DP / 16) + d) * 4) =
+                        float4v{o[q][d][rr], o[q][d + 1][rr], o[q][d + 2][rr], o[q][d + 3][rr]};
+        } else {
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) *(float4v*)(lds + r * orow<DP>() + (16 * d + 4 * g) * 4) = o[q][d];
+        }
     }
     __syncthreads();
     const uint32_t rows = std::min<uint32_t>(RB, u.q.n * (p.hq / p.hkv) - u.rb * RB);
@@ -178,7 +192,7 @@ __device__ __forceinline__ void finish_piece(const PagedAttnParams& p, const Pie
 
 // Calls f for each piece of this workgroup's share; pre: plan_line's.
 template <int RB, class F>
-__device__ __forceinline__ void walk(const PagedAttnParams& p, const uint32_t* pre, F&& f)
+__device__ __forceinline__ void walk(const PagedAttnParams& p, const uint32_t* pre, const Sequence* kept, F&& f)
 {
     const uint32_t n = p.pages.sequences, total = __builtin_amdgcn_readfirstlane(pre[n]), wg = blockIdx.x;
     const uint32_t share = std::max(p.min_share, (total + p.wgs - 1) / p.wgs);
@@ -188,7 +202,7 @@ __device__ __forceinline__ void walk(const PagedAttnParams& p, const uint32_t* p
     for (uint32_t at = (uint32_t)std::min<uint64_t>(begin, total); at < end;) {
         Piece u;
         u.s = __builtin_amdgcn_readfirstlane(line_sequence(pre, n, at));
-        u.q = sequence_of(p.pages, u.s, p.tokens);
+        u.q = uniform(u.s < KEPT ? kept[u.s] : sequence_of(p.pages, u.s, p.tokens));
         const Span r = span_of(p, u.q, RB);
         const uint32_t tiles = r.te - r.tb, len = tiles + p.lead;
         const uint32_t off = at - __builtin_amdgcn_readfirstlane(pre[u.s]), unit = off / len, o0 = off - unit * len;

@@ -40,4 +40,14 @@ __device__ __forceinline__ Sequence sequence_of(const KvPages& p, uint32_t s, ui
     return q;
 }
 
+// The same in every lane, in scalar registers.
+__device__ __forceinline__ Sequence uniform(Sequence q)
+{
+    q.first = __builtin_amdgcn_readfirstlane(q.first);
+    q.n = __builtin_amdgcn_readfirstlane(q.n);
+    q.held = __builtin_amdgcn_readfirstlane(q.held);
+    q.live = __builtin_amdgcn_readfirstlane(q.live);
+    return q;
+}
+
 }   // namespace vai_dev
