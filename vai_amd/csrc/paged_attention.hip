@@ -12,7 +12,7 @@
 // but for where the keys lie and the row's maximum and sum. Where the next 16 keys'
 // K and V lie is looked up, and what the next ones hold is read, while 16 are
 // multiplied: 64 sequences of up to 8192 positions of fp32 pages, 8 heads of 128,
-// take 205 us (409 with one load after the other).
+// take 182 us (409 with one load after the other).
 #include "paged_plan.h"
 
 #include "launch_once.h"
@@ -285,7 +285,10 @@ bool paged_attention_plan(const PagedAttnParams& call, PagedAttnPlan& plan, uint
     uint32_t resident = 2;
     p.rb = 16;
     p.min_share = 4;
-    p.lead = 2;
+    // the fp32 kernel's: fp32 pages, 64 sequences of up to 8192 positions, 8 heads of 128,
+    // 64 and 50 (fp16) with 2, 4, 6, 10: 204, 185, 182, 185 us; 109, 96, 99, 102; 120, 106,
+    // 100, 104; 4 heads of 256 257, 261, 279, 284
+    p.lead = p.dp == 256 ? 2 : 5;
     p.few_rows = 0xffffffffu;
     p.decode = paged_decode_ok(p);
     if (p.decode) paged_decode_plan(p, &resident);
