@@ -499,7 +499,8 @@ vai_status vai_paged_append_launch(const vai_paged_append_args* args, vai_stream
  * positions after the query's own; span > 0 those up to its own - span. A query
  * that sees none (or only scores of -infinity) gives zeros.
  *   q [tokens] rows of q_stride elements (0: hq * head_dim) of hq heads in
- *   q_dtype; out [tokens, hq, head_dim] in o_dtype. head_dim <= 256.
+ *   q_dtype; out [tokens, hq, head_dim] in o_dtype, disjoint from q. head_dim <=
+ *   256.
  *   max_new: no sequence brings more tokens (0: tokens). It only chooses kernels
  *   and their workspace: sequences that bring more are attended too.
  *   Statistics and sums are fp32. Over fp16 pages an fp32 q enters the matrix
@@ -548,8 +549,8 @@ size_t vai_paged_attention_workspace_size(const vai_paged_attention_args* args);
  *   target, draft: [rows] rows of target_stride / draft_stride elements (0:
  *   vocab); draft's row of a sequence's last token is not read. tokens [rows]
  *   uint32, uniform [rows] fp32 in [0, 1); a token >= vocab has no probability.
- *   out_tokens [rows]: row seq_start[s] + i the token at place i, VAI_NO_TOKEN
- *   past the last; accepted [sequences]: drafts kept. new_counts (may be NULL, or
+ *   out_tokens [rows], another array than tokens: row seq_start[s] + i the token at
+ *   place i, VAI_NO_TOKEN past the last; accepted [sequences]: drafts kept. new_counts (may be NULL, or
  *   counts itself): counts[s] + accepted + 1, the positions of the cache that
  *   hold. A sequence without rows: accepted 0, its count unchanged. The arrays are
  *   read when the kernels run. sequences <= 4096, rows and vocab < 2^24.

@@ -106,6 +106,11 @@ CASES = [
     ([300, 2], [333, 600], 4, 1, 128, 64, F16, F32, F32, 0), ([200, 100], [50, 0], 6, 2, 80, 32, F16, F16, F16, 64),
     ([70, 1, 33], [20, 900, 0], 16, 2, 256, 16, F16, F16, F16, 0), ([64], [4], 4, 4, 64, 8, F16, F16, F16, 0),
     ([50, 3], [7, 200], 3, 3, 33, 16, F16, F32, F32, 0), ([61], [0], 8, 4, 72, 16, F32, F32, F32, 9),
+    ([2, 1], [30, 600], 4, 2, 8, 16, F16, F16, F16, 0), ([2, 40], [30, 600], 4, 2, 16, 16, F16, F32, F32, 0),
+    ([3, 70], [100, 9], 6, 3, 40, 48, F16, F16, F32, 20), ([1, 33], [100, 300], 4, 2, 248, 16, F16, F16, F16, 0),
+    ([1, 2], [1000, 70], 128, 1, 64, 16, F16, F16, F16, 0), ([3, 200], [900, 70], 4, 1, 128, 4096, F16, F16, F16, 0),
+    ([1, 5], [3000, 0], 4, 2, 128, 1, F16, F16, F16, 0), ([7, 1], [2100, 90], 8, 2, 192, 64, F16, F32, F32, 0),
+    ([2100, 1], [10, 70], 4, 1, 64, 16, F16, F16, F16, 0), ([700], [10], 8, 1, 32, 16, F32, F32, F32, 0),
     ([513], [1030], 8, 8, 64, 128, F16, F16, F16, 0), ([1] * 40, [37 * i for i in range(40)], 8, 2, 64, 16, F16, F16, F16, 0),
 ]
 
@@ -119,7 +124,7 @@ def test_attention(gpu, case):
     b.upload()
     q = draw((b.rows, hq, d), rng, qdt)
     q[:1] = np.nan
-    for hint in (max(new), 0):
+    for hint in (max(new), 0, 1):          # (a hint that sequences exceed is only slower)
         print(f"paged attention {case} max_new={hint}", flush=True)
         got = call(gpu, b, q, odt, span=span, max_new=hint)
         check(b, q, got, odt, span)
@@ -255,19 +260,40 @@ def test_sequences_may_share_pages(gpu, new):
     check(b, q, call(gpu, b, q, F16), F16)
 
 
-@pytest.mark.parametrize("d, pdt", [(64, F16), (50, F32)])
-def test_many_sequences(gpu, d, pdt):
-    """As many as a call takes, most of one position, with gaps."""
+@pytest.mark.parametrize("d, pdt, most", [(64, F16, 1), (64, F16, 0), (256, F16, 0), (50, F32, 1)])
+def test_many_sequences(gpu, d, pdt, most):
+    """As many as a call takes, most of one position, with gaps (and, without a hint, one of a whole prompt)."""
     rng = np.random.default_rng(9)
     n = 4096
     new = [int(i % 3 != 1) for i in range(n)]
+    new[2000] = 1 if most else 150
     held = [int(x) for x in rng.integers(0, 40, n)]
     b = Batch(gpu, rng, new, held, 1, d, 16, pdt)
     b.fill(rng)
     b.upload()
     q = draw((b.rows, 2, d), rng, F16)
     print(f"paged attention of {n}", flush=True)
-    check(b, q, call(gpu, b, q, F32, max_new=1), F32)
+    check(b, q, call(gpu, b, q, F32, max_new=most), F32)
+
+
+@pytest.mark.parametrize("d, page, pdt", [(64, 16, F16), (128, 16, F16), (50, 12, F32)])
+@pytest.mark.parametrize("new", [[3, 1], [80, 1]])
+def test_a_query_of_nan_is_alone(gpu, d, page, pdt, new):
+    rng = np.random.default_rng(d)
+    b = Batch(gpu, rng, new, [70, 33], 2, d, page, pdt)
+    b.fill(rng)
+    b.upload()
+    for qdt in (F16, F32):
+        q = draw((b.rows, 4, d), rng, qdt)
+        bad = q.copy()
+        bad[1, 2, 3] = np.nan
+        bad[0, 1] = np.inf
+        print(f"paged attention nan query d={d} new={new}", flush=True)
+        got = call(gpu, b, bad, F32)
+        assert np.isnan(got[1, 2]).all() and not np.isfinite(got[0, 1]).any()
+        good = call(gpu, b, q, F32)
+        got[1, 2], got[0, 1] = good[1, 2], good[0, 1]
+        check(b, q, got, F32)
 
 
 @pytest.mark.parametrize("d, hq, pdt, qdt", [(64, 8, F16, F16), (128, 4, F16, F32), (50, 4, F32, F32)])

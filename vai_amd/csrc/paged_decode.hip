@@ -368,7 +368,8 @@ __global__ __launch_bounds__(64 * Ring<DP>::NW, Ring<DP>::RES) void paged_decode
 bool paged_decode_ok(const PagedAttnParams& p)
 {
     return p.pages.dtype == DT_F16 && p.head_dim % 8 == 0 && p.pages.page_size % 16 == 0 && p.pages.stride % 8 == 0 &&
-           (uintptr_t)p.pages.k % 16 == 0 && (uintptr_t)p.pages.v % 16 == 0;
+           (uintptr_t)p.pages.k % 16 == 0 && (uintptr_t)p.pages.v % 16 == 0 &&
+           (uint64_t)p.pages.page_size * p.head_dim * 2 < 1ull << 32;   // (offsets in a head's part of a page)
 }
 
 void paged_decode_plan(PagedAttnParams& p, uint32_t* resident)
