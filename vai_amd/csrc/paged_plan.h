@@ -214,7 +214,7 @@ __device__ __forceinline__ void walk(const PagedAttnParams& p, const uint32_t* p
         if (at == begin && t0 > 0) {
             const uint32_t a = at - o0 + p.lead, wg0 = a / share;    // (the unit's first tile)
             if (wg0 + 1 == wg)
-                joint = Joint{(a + tiles - 1) / share - wg0 + 1, wg0, u.q.first, u.hk, u.rb * RB,
+                joint = Joint{std::min((a + tiles - 1) / share + 1, p.wgs) - wg0, wg0, u.q.first, u.hk, u.rb * RB,
                               std::min<uint32_t>(RB, u.q.n * (p.hq / p.hkv) - u.rb * RB), {0, 0}};
         }
         at += o1 - o0;
