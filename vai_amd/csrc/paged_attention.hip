@@ -192,7 +192,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void paged_attention_any_ke
 
 // Joins the partial results of the units that a cut of the line runs through:
 // O = sum_u 2^(m_u - M) O_u / sum_u 2^(m_u - M) l_u. Grid: (cuts, rows), a Joint a cut.
-template <int DP>
+// WAVES: (cuts, rows / 4), a row a wave where a unit has up to 64 parts, which needs
+// neither barriers nor, for the cuts without a Joint, as many workgroups.
+template <int DP, bool WAVES>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p)
 {
     constexpr uint32_t C4 = DP / 4, UG = 256 / C4, AHEAD = 8;     // lanes to a part's row; parts at a time; loads in flight
@@ -204,6 +206,44 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p)
     if (x.parts == 0) return;
     const uint32_t t = threadIdx.x, c = t % C4, ug = t / C4;
     const auto at = [&](uint32_t i, uint32_t row) { return (size_t)(2 * (x.wg + i) + (i == 0 ? 1u : 0u)) * p.rb + row; };
+    if (WAVES && x.parts <= 64) {
+        // a row a wave: lane i makes part i's weight
+        constexpr uint32_t WG = 64 / C4;
+        const uint32_t lane = t & 63, wu = lane / C4;
+        for (uint32_t row = 4 * blockIdx.y + (t >> 6); row < x.rows; row += 4 * gridDim.y) {
+            float4v v[AHEAD];
+#pragma unroll
+            for (uint32_t i = 0; i < AHEAD; ++i)
+                v[i] = *(const float4v*)(p.ws_o + at(min(wu + i * WG, x.parts - 1), row) * DP + 4 * c);
+            const float* ml = p.ws_ml + 2 * at(min(lane, x.parts - 1), row);
+            const float m = lane < x.parts ? ml[0] : -__builtin_inff(), l = ml[1];
+            float M = m;
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+            const float w = lane < x.parts ? __builtin_amdgcn_exp2f(m - (M == -__builtin_inff() ? 0.f : M)) : 0.f;
+            const float sum = wave_sum(lane < x.parts ? w * l : 0.f);
+            float4v acc = (float4v)0.f;
+            for (uint32_t u = 0; u < x.parts; u += AHEAD * WG) {
+                if (u > 0) {
+#pragma unroll
+                    for (uint32_t i = 0; i < AHEAD; ++i)
+                        v[i] = *(const float4v*)(p.ws_o + at(min(u + wu + i * WG, x.parts - 1), row) * DP + 4 * c);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < AHEAD; ++i) {
+                    const uint32_t k = u + wu + i * WG;
+                    const float wk = __shfl(w, k & 63);
+                    if (k < x.parts) acc += wk * v[i];
+                }
+            }
+#pragma unroll
+            for (uint32_t o = C4; o < 64; o <<= 1)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
+            if (lane < C4 && 4 * c < p.head_dim) pg::put_row(p, x.first, x.hk, x.row0 + row, 4 * c, acc, sum);
+        }
+        return;
+    }
     for (uint32_t row = blockIdx.y; row < x.rows; row += gridDim.y) {
         // the first loads of values are in flight while the weights are made
         float4v v[AHEAD];
@@ -261,16 +301,24 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnParams p)
     }
 }
 
+template <int DP>
+static hipError_t merge_launch(const PagedAttnParams& p, hipStream_t s)
+{
+    // (a unit's rows, as far as the hint knows: more take turns)
+    const uint32_t rows = (uint32_t)std::min<uint64_t>(p.rb, (uint64_t)p.max_new * (p.hq / p.hkv));
+    // Rows a wave where there are rows and, on average, at most 32 parts to a unit: 7
+    // sequences of 30 rows 17.9 us so (with the attention), 20.2 with a workgroup a row;
+    // 64 of 12 rows 49, 52; but one of 16 over 60000 positions, 4 heads of 256, 65, 62.
+    if (rows < 8 || (uint64_t)p.pages.sequences * p.hkv * 32 < p.wgs)
+        hipLaunchKernelGGL((paged_merge_kernel<DP, false>), dim3(p.wgs - 1, rows), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((paged_merge_kernel<DP, true>), dim3(p.wgs - 1, (rows + 3) / 4), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
 hipError_t paged_merge_launch(const PagedAttnParams& p, hipStream_t s)
 {
     if (p.wgs == 1) return hipSuccess;
-    // (a unit's rows, as far as the hint knows: more take turns)
-    const uint32_t rows = (uint32_t)std::min<uint64_t>(p.rb, (uint64_t)p.max_new * (p.hq / p.hkv));
-    const dim3 grid(p.wgs - 1, rows);
-    if (p.dp == 64) hipLaunchKernelGGL(paged_merge_kernel<64>, grid, dim3(256), 0, s, p);
-    else if (p.dp == 128) hipLaunchKernelGGL(paged_merge_kernel<128>, grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL(paged_merge_kernel<256>, grid, dim3(256), 0, s, p);
-    return hipGetLastError();
+    return p.dp == 64 ? merge_launch<64>(p, s) : p.dp == 128 ? merge_launch<128>(p, s) : merge_launch<256>(p, s);
 }
 
 bool paged_attention_plan(const PagedAttnParams& call, PagedAttnPlan& plan, uint32_t cus)
@@ -303,9 +351,11 @@ bool paged_attention_plan(const PagedAttnParams& call, PagedAttnPlan& plan, uint
         paged_prefill_plan(plan.many, cus);
         // One launch takes them all where the units of the sequences with few rows are not
         // many: it fills 4 of 128 rows then, but is bound by memory like the other, whose
-        // launch and merge are saved. A chunk of 512 tokens beside 8, 32, 64 and 128 single
-        // ones, 8 KV heads: 112, 147, 195, 276 us so, 134, 161, 215, 274 apart.
-        if ((uint64_t)p.pages.sequences * p.hkv <= plan.many.wgs * 3 / 2) {
+        // launch and merge are saved. A chunk of 512 tokens beside 8, 32, 64, 128 (and of
+        // half the length 256) single ones, 8 KV heads: 107, 134, 188, 248, 201 us so, 118,
+        // 156, 203, 270, 219 apart; beside 512 shorter ones 217 and 219. (128 with an fp32 q
+        // 217 and 199, with head dims of 64 164 and 159.)
+        if ((uint64_t)p.pages.sequences * p.hkv <= plan.many.wgs * 3) {
             plan.many.few_rows = 0;
             p.wgs = 0;
         }

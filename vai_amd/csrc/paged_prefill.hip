@@ -11,7 +11,7 @@
 // workgroups a CU (D = 256: one, by registers): one's softmax, and its beginning
 // and end of a unit, under the other's products. (One of two groups of waves that
 // take the tiles in turn halves the partial results, but 8192 tokens of a prompt
-// took 823 us so where two workgroups take 700.)
+// took 823 us so where two workgroups took 700; 665 by now.)
 // All units' tiles form a line that the workgroups cut into equal shares, head by
 // head on one XCD, as paged_plan.h does for few rows; a unit's tiles are those its
 // own rows see. An fp32 q enters as two fp16 numbers (Q2), and so do the
@@ -158,7 +158,7 @@ __device__ __forceinline__ void walk(const PagedAttnParams& p, const uint32_t* p
         if (at == begin && t0 > 0) {
             const uint32_t a = at - o0 + p.lead, wg0 = a / share;    // (the unit's first tile)
             if (wg0 + 1 == me)
-                joint = pg::Joint{(a + tiles - 1) / share - wg0 + 1, wg0, u.q.first, u.hk, u.rb * RB,
+                joint = pg::Joint{min((a + tiles - 1) / share + 1, p.wgs) - wg0, wg0, u.q.first, u.hk, u.rb * RB,
                                   min((uint32_t)RB, rows - u.rb * RB), {0, 0}};
         }
         at += o1 - o0;
@@ -302,7 +302,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
 #pragma unroll
         for (int d = 0; d < DF; ++d) o[d] = (float16v)0.f;
 
-        for (int t = 0; t < mine; ++t) {
+        // A wave without rows (a sequence's last unit, one of few rows) only copies: a chunk
+        // of 512 tokens beside 32 single ones takes 134 us, 147 where it multiplies too.
+        const bool idle = u.rb * RB + wave * QW >= rows;
+        if (idle) {
+            for (int t = 0; t < mine; ++t) {
+                fa_wait_vmcnt<0>();
+                __builtin_amdgcn_s_barrier();
+                if ((t & 15) == 14) look_up(t + 2, entry2, start2);
+                if ((t & 15) == 15) {
+                    entry = entry2;
+                    start = start2;
+                }
+                if (t + 1 < mine) fa_issue<D>(rsrc(t + 1, pgs.k), rsrc(t + 1, pgs.v), lds, coff, (t + 1) & 1, wave);
+                __builtin_amdgcn_s_barrier();
+            }
+        }
+        for (int t = 0; t < mine && !idle; ++t) {
             // tile t is in stage t % 2; the next one's copies go out during its S^T products
             fa_wait_vmcnt<0>();
             __builtin_amdgcn_s_barrier();
@@ -473,7 +489,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
             __builtin_amdgcn_s_barrier();
         }
 
-        if (mine & 1) {
+        if ((mine & 1) && !idle) {
 #pragma unroll
             for (int j = 0; j < NK; ++j) kaddr[j] -= L::STAGE;
 #pragma unroll
@@ -492,7 +508,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
                 ob[ql * CR + ((8 * d + 2 * q4 + hf) ^ (ql & 15))] = float4v{o[d][4 * q4] * inv, o[d][4 * q4 + 1] * inv,
                                                                           o[d][4 * q4 + 2] * inv, o[d][4 * q4 + 3] * inv};
         constexpr int NJ = QW * CR / 64;
-        if (u.whole) {
+        if (idle) {
+        } else if (u.whole) {
             const uint32_t row0 = u.rb * RB + wave * QW;
 #pragma unroll 4
             for (int j = 0; j < NJ; ++j) {
@@ -515,7 +532,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
 #pragma unroll 4
             for (int j = 0; j < NJ; ++j) {
                 const uint32_t e = j * 64 + lane, r = e / CR, c = e % CR;
-                *(float4v*)(dst + r * D + 4 * c) = ob[r * CR + (c ^ (r & 15))];
+                const float4v v = ob[r * CR + (c ^ (r & 15))];
+                if (u.rb * RB + wave * QW + r < rows) *(float4v*)(dst + r * D + 4 * c) = v;
             }
         }
         __syncthreads();     // the next piece's copies go where these were
