@@ -503,10 +503,9 @@ vai_status vai_paged_append_launch(const vai_paged_append_args* args, vai_stream
  *   256.
  *   max_new: no sequence brings more tokens (0: tokens). It only chooses kernels
  *   and their workspace: sequences that bring more are attended too.
- *   Statistics and sums are fp32. Over fp16 pages an fp32 q enters the matrix
- *   cores as two fp16 numbers, and so do the probabilities where out is fp32;
- *   for fp16 out they may be rounded to one. fp32 pages, head dims of no whole 8s
- *   and pages of no whole 16s are attended in fp32 throughout.
+ *   Statistics and sums are fp32. Over fp16 pages an fp32 q and the probabilities
+ *   enter the matrix cores as two fp16 numbers each. fp32 pages, head dims of no
+ *   whole 8s and pages of no whole 16s are attended in fp32 throughout.
  *   What hidden positions hold does not matter. A value of V that is not finite
  *   makes its column so for the queries that see it; their other columns may be
  *   NaN too.

@@ -15,7 +15,10 @@
 // All units' tiles form a line that the workgroups cut into equal shares, head by
 // head on one XCD, as paged_plan.h does for few rows; a unit's tiles are those its
 // own rows see. An fp32 q enters as two fp16 numbers (Q2), and so do the
-// probabilities where the output is fp32 (P2).
+// probabilities, whatever the output's type: one number alone leaves 2^-11 of sum p
+// |v| in the result, as much as an fp16 output's own rounding, and would give a
+// sequence's single token other bits where a prompt joins its batch. (A chunk of 512
+// beside 8 single tokens, 32 heads over 8 of 128: 128 us, with one number 106.)
 #include "attention_tile.h"
 #include "paged_plan.h"
 
@@ -187,7 +190,7 @@ __device__ __forceinline__ bool finite(half_t x) { return (__builtin_bit_cast(ui
 
 }   // namespace pp
 
-template <int D, bool Q2, bool P2>
+template <int D, bool Q2>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(PagedAttnParams p, uint32_t tiles_at)
 {
     using namespace fa;
@@ -437,7 +440,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
                 }
             }
             const float ref = (m == -__builtin_inff() ? 0.f : m) - LIFT;    // (l and o carry 2^LIFT alike)
-            half8 pb[4], p2[P2 ? 4 : 1];
+            half8 pb[4], p2[4];
             const float esc = fast ? sc : 1.f;
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
@@ -446,7 +449,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
                 for (int i = 0; i < 8; ++i)
                     e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[kk >> 1][8 * (kk & 1) + i], esc, -ref));
                 pb[kk] = __builtin_convertvector(e, half8);
-                if constexpr (P2) p2[kk] = __builtin_convertvector(e - __builtin_convertvector(pb[kk], float8v), half8);
+                p2[kk] = __builtin_convertvector(e - __builtin_convertvector(pb[kk], float8v), half8);
                 l += ((e[0] + e[4]) + (e[1] + e[5])) + ((e[2] + e[6]) + (e[3] + e[7]));   // (the lane's positions)
             }
 
@@ -475,7 +478,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
 #pragma unroll
                     for (int d = 0; d < DF; ++d) {
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[cur][d], pb[kk], o[d], 0, 0, 0);
-                        if constexpr (P2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[cur][d], p2[kk], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[cur][d], p2[kk], o[d], 0, 0, 0);
                     }
                 });
             }
@@ -587,24 +590,22 @@ void paged_prefill_plan(PagedAttnParams& p, uint32_t cus)
     p.wgs = std::min<uint32_t>(p.dp == 256 ? cus : 2 * cus, PagedAttnParams::MAX_WGS);
 }
 
-template <int D, bool Q2, bool P2>
+template <int D, bool Q2>
 static hipError_t prefill_launch(const PagedAttnParams& p, hipStream_t s)
 {
     constexpr int bytes = fa::Lds<D>::BYTES;
     const uint32_t at = ((p.pages.sequences + 1) * 4 + 1023) / 1024 * 1024;
     static PerDevice once;
-    const hipError_t e = set_max_lds(once, (const void*)paged_prefill_kernel<D, Q2, P2>, bytes + KvPages::MAX_SEQUENCES * 4 + 1024);
+    const hipError_t e = set_max_lds(once, (const void*)paged_prefill_kernel<D, Q2>, bytes + KvPages::MAX_SEQUENCES * 4 + 1024);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_prefill_kernel<D, Q2, P2>), dim3(p.wgs), dim3(256), at + bytes, s, p, at);
+    hipLaunchKernelGGL((paged_prefill_kernel<D, Q2>), dim3(p.wgs), dim3(256), at + bytes, s, p, at);
     return hipGetLastError();
 }
 
 template <int D>
 static hipError_t prefill_launch_d(const PagedAttnParams& p, hipStream_t s)
 {
-    const bool q2 = p.q_dtype == DT_F32, p2 = p.o_dtype == DT_F32;
-    const hipError_t e = q2 ? p2 ? prefill_launch<D, true, true>(p, s) : prefill_launch<D, true, false>(p, s)
-                            : p2 ? prefill_launch<D, false, true>(p, s) : prefill_launch<D, false, false>(p, s);
+    const hipError_t e = p.q_dtype == DT_F32 ? prefill_launch<D, true>(p, s) : prefill_launch<D, false>(p, s);
     if (e != hipSuccess || p.wgs == 1) return e;
     hipLaunchKernelGGL(paged_merge_rows_kernel<D>, dim3(p.wgs - 1, pp::RB * (D / 4) / 256), dim3(256), 0, s, p);
     return hipGetLastError();
