@@ -29,3 +29,27 @@ def test_probabilities_keep_their_bits(gpu, d, page, new, held):
             at = int(b.starts[s])
             want, tol = att.attend(q[at:at + n], b.K[s], b.V[s], att.visible(h, n, 0), F16, F32)
             att.near(got[at:at + n], want, tol + np.abs(want) * 2.0 ** -11 + 2.0 ** -25, f"sequence {s}")
+
+
+@pytest.mark.parametrize("d, page, pdt", [(64, 16, F16), (128, 32, F16), (256, 16, F16), (50, 12, F32)])
+@pytest.mark.parametrize("new, held", [([1, 3], [400, 300]), ([80, 40], [400, 300])])
+@pytest.mark.parametrize("at", [0, 299])
+def test_probabilities_far_below_the_largest(gpu, d, page, pdt, new, held, at):
+    """One position whose score is 16.5 above all others' and whose value is 0: the output is what the others, at
+    probabilities of e^-16.5, make of it. (Two fp16 numbers after 2^14 hold them to 2^-25 of 2^-9.8, a tenth of the
+    tolerance that a score of 16.5 has by itself.)"""
+    rng = np.random.default_rng(d)
+    b = Batch(gpu, rng, new, held, 2, d, page, pdt)
+    b.fill(rng, loud=False)
+    for s in range(len(new)):
+        b.K[s][:, :, 0] = 0
+        b.K[s][at, :, 0] = 16.5 * d ** 0.5
+        b.V[s][:] = np.abs(b.V[s]) + 1
+        b.V[s][at] = 0
+        b.store(s, b.K[s], b.V[s])
+    b.upload()
+    for qdt in (F16, F32):
+        q = np.zeros((b.rows, 8, d), qdt)
+        q[:, :, 0] = 1
+        print(f"paged precision far below d={d} new={new} at={at}", flush=True)
+        att.check(b, q, att.call(gpu, b, q, F32, max_new=max(new)), F32)

@@ -198,7 +198,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
     using pp::RB;
     using L = Lds<D>;
     constexpr int KS = D / 16, DF = D / 32, CR = D / 4;
-    constexpr float SLACK = 8.f, LIFT = 7.f;     // P stays below 2^15
+    // P stays below 2^15, and of those far below the row's largest two fp16 numbers hold
+    // what lies above 2^-25, which is 2^-39 of the largest. (8 and 7, with fewer changes of
+    // the reference, take 125 us of a chunk's 128, and hold 2^-32 of it.)
+    constexpr float SLACK = 1.f, LIFT = 14.f;
     extern __shared__ __attribute__((aligned(1024))) float4v paged_prefill_lds[];
     uint32_t* pre = (uint32_t*)paged_prefill_lds;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
