@@ -76,10 +76,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void paged_attention_any_ke
     plan_line<NW>(p, RB, pre, kept);
     walk<RB>(p, pre, kept, [&](const Piece& u) {
         const uint32_t rows = u.q.n * group, row = min(u.rb * RB + c16, rows - 1);
-        const uint32_t tok = row / group, pos = u.q.held + tok;
-        const uint32_t kbeg = first_key(p, pos), kend = p.causal ? min(pos + 1, u.q.live) : u.q.live;
+        const uint32_t tok = row / group;
+        const uint32_t kbeg = first_key(p, u.q.held, tok), kend = end_key(p, u.q.held, u.q.live, tok);
         const size_t qat = (size_t)(u.q.first + tok) * p.q_stride + (size_t)(u.hk * group + row % group) * D;
-        const uint32_t see = first_key(p, u.q.held);     // no row sees a position before it
+        const uint32_t see = first_key(p, u.q.held, 0);     // no row sees a position before it
         const uint32_t first = u.t0 + wave;
         const int steps = first < u.t1 ? 2 * (int)((u.t1 - first + NW - 1) / NW) : 0;
         const auto j0_of = [&](int i) __attribute__((always_inline)) { return (first + (uint32_t)(i >> 1) * NW) * KT + 16 * (i & 1); };

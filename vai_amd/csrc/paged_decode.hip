@@ -137,9 +137,9 @@ __global__ __launch_bounds__(64 * Ring<DP>::NW, Ring<DP>::RES) void paged_decode
         int kbeg[NQ], kend[NQ];
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-            const uint32_t r = min(row0 + q * 16 + c16, rend - 1), tok = r / group, pos = u.q.held + tok;
-            kbeg[q] = (int)first_key(p, pos);
-            kend[q] = (int)(p.causal ? min(pos + 1, u.q.live) : u.q.live);
+            const uint32_t r = min(row0 + q * 16 + c16, rend - 1), tok = r / group;
+            kbeg[q] = (int)first_key(p, u.q.held, tok);
+            kend[q] = (int)end_key(p, u.q.held, u.q.live, tok);
             const qt* src = (const qt*)p.q + (size_t)(u.q.first + tok) * p.q_stride + (size_t)(u.hk * group + r % group) * HD;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -150,8 +150,8 @@ __global__ __launch_bounds__(64 * Ring<DP>::NW, Ring<DP>::RES) void paged_decode
         }
         // what every row of the block sees
         const uint32_t tok0 = row0 / group, tok1 = (rend - 1) / group;
-        const int all_beg = (int)first_key(p, u.q.held + tok1);
-        const int all_end = (int)(p.causal ? min(u.q.held + tok0 + 1, u.q.live) : u.q.live);
+        const int all_beg = (int)first_key(p, u.q.held, tok1);
+        const int all_end = (int)end_key(p, u.q.held, u.q.live, tok0);
 
         const uint32_t first = u.t0 + wave;
         const int mine = first < u.t1 ? (int)((u.t1 - first + NW - 1) / NW) : 0;

@@ -27,14 +27,22 @@ constexpr int KT = 32;                 // positions a tile
 struct Span {
     uint32_t tb, te, blocks;
 };
-__device__ __forceinline__ uint32_t first_key(const PagedAttnParams& p, uint32_t pos)
+// The positions [first_key, end_key) that row t of a sequence sees: held + t itself may
+// lie past what the table holds, and past 32 bits, and its window with it (2^30 then:
+// no position).
+__device__ __forceinline__ uint32_t first_key(const PagedAttnParams& p, uint32_t held, uint32_t t)
 {
-    return p.span && pos + 1 > p.span ? pos + 1 - p.span : 0u;
+    const uint64_t end = (uint64_t)held + t + 1;
+    return p.span && end > p.span ? (uint32_t)std::min<uint64_t>(end - p.span, KvPages::MAX_POSITIONS) : 0u;
+}
+__device__ __forceinline__ uint32_t end_key(const PagedAttnParams& p, uint32_t held, uint32_t live, uint32_t t)
+{
+    return p.causal && held < live ? std::min(held + t + 1, live) : live;
 }
 __device__ __forceinline__ Span span_of(const PagedAttnParams& p, const Sequence& q, uint32_t rb)
 {
     Span r;
-    r.tb = first_key(p, q.held) / KT;
+    r.tb = first_key(p, q.held, 0) / KT;
     r.te = std::max(r.tb + 1, (q.live + KT - 1) / KT);
     r.blocks = (q.n * (p.hq / p.hkv) + rb - 1) / rb;
     return r;

@@ -36,9 +36,9 @@ struct Tiles {
 __device__ __forceinline__ Tiles tiles_of(const PagedAttnParams& p, uint32_t held, uint32_t live, uint32_t rows, uint32_t rb)
 {
     const uint32_t group = p.hq / p.hkv, tok0 = rb * RB / group, tok1 = (min((rb + 1) * RB, rows) - 1) / group;
-    const uint32_t end = p.causal ? min(held + tok1 + 1, live) : live;
+    const uint32_t end = pg::end_key(p, held, live, tok1);
     Tiles t;
-    t.tb = pg::first_key(p, held + tok0) / KT;
+    t.tb = pg::first_key(p, held, tok0) / KT;
     t.te = max(t.tb + 1, (end + KT - 1) / KT);
     return t;
 }
@@ -236,8 +236,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
     pp::plan_line<NW>(p, pre);
     pp::walk(p, pre, fa_xcd_block(blockIdx.x, gridDim.x), [&](const Piece& u) __attribute__((always_inline)) {
         const uint32_t rows = u.q.n * group, row = min(u.rb * RB + wave * QW + ql, rows - 1);
-        const uint32_t tok = row / group, pos = u.q.held + tok;
-        const int kbeg = (int)pg::first_key(p, pos), kend = (int)(p.causal ? min(pos + 1, u.q.live) : u.q.live);
+        const uint32_t tok = row / group;
+        const int kbeg = (int)pg::first_key(p, u.q.held, tok), kend = (int)pg::end_key(p, u.q.held, u.q.live, tok);
 
         // query rows: lane l holds query l % 32, values 16 s + 8 (l / 32) ..+7
         half8 qf[KS], q2[Q2 ? KS : 1];

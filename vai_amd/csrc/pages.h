@@ -1,6 +1,8 @@
 // pages.h -- which sequence a row of a ragged batch belongs to, and where a
 // position lies in the pages.
 #pragma once
+#include <algorithm>
+
 #include "device_common.h"
 #include "kernels.h"
 
@@ -26,7 +28,8 @@ __device__ __forceinline__ uint32_t wave_last_le(const uint32_t* a, uint32_t n, 
 // A sequence of a ragged batch: its rows, and the positions held before them.
 struct Sequence {
     uint32_t first, n;        // rows first .. first + n - 1
-    uint32_t held, live;      // positions before the call, and with its rows (as far as pages can hold)
+    uint32_t held;            // positions before the call, as counts has them: row t is at held + t
+    uint32_t live;            // positions with its rows, as far as the table can hold them
 };
 __device__ __forceinline__ Sequence sequence_of(const KvPages& p, uint32_t s, uint32_t rows)
 {
@@ -35,8 +38,8 @@ __device__ __forceinline__ Sequence sequence_of(const KvPages& p, uint32_t s, ui
     const uint32_t room = p.max_pages * p.page_size;      // (at most 2^30)
     q.first = a;
     q.n = b > a ? b - a : 0u;
-    q.held = min(p.counts[s], room);
-    q.live = min(q.held + q.n, room);                     // (rows are below 2^31)
+    q.held = p.counts[s];
+    q.live = (uint32_t)std::min<uint64_t>((uint64_t)q.held + q.n, room);
     return q;
 }
 
