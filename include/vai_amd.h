@@ -552,7 +552,8 @@ size_t vai_paged_attention_workspace_size(const vai_paged_attention_args* args);
  *   place i, VAI_NO_TOKEN past the last; accepted [sequences]: drafts kept. new_counts (may be NULL, or
  *   counts itself): counts[s] + accepted + 1, the positions of the cache that
  *   hold. A sequence without rows: accepted 0, its count unchanged. The arrays are
- *   read when the kernels run. sequences <= 4096, rows and vocab < 2^24.
+ *   read when the kernels run. sequences <= 4096, rows and vocab < 2^24, and rows
+ *   times the 4096s of vocab, rounded up, < 2^24.
  * The workspace (16-byte aligned) as for vai_paged_attention_launch.
  * ------------------------------------------------------------------------- */
 #define VAI_NO_TOKEN 0xffffffffu

@@ -767,7 +767,8 @@ static vai_status verify_params(const vai_verify_drafts_args* a, VerifyParams& p
     if ((a->target_stride && a->target_stride < a->vocab) || (a->draft && a->draft_stride && a->draft_stride < a->vocab))
         return VAI_ERR_SHAPE;
     if (a->sequences > KvPages::MAX_SEQUENCES || a->rows >= 1u << 24 || a->vocab >= 1u << 24) return VAI_ERR_UNSUPPORTED;
-    if ((uint64_t)a->rows * ((a->vocab + 4095) / 4096) >= 1u << 31) return VAI_ERR_UNSUPPORTED;   // (the grid)
+    // (the first pass: 256 threads for each 4096 logits of a row, fewer than 2^32 in a launch)
+    if ((uint64_t)a->rows * ((a->vocab + 4095) / 4096) >= 1u << 24) return VAI_ERR_UNSUPPORTED;
     p = VerifyParams{};
     p.out_tokens = a->out_tokens; p.accepted = a->accepted; p.new_counts = a->new_counts;
     p.target = a->target; p.draft = a->draft; p.tokens = a->tokens; p.uniform = a->uniform;

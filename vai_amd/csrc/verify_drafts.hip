@@ -554,6 +554,8 @@ hipError_t verify_launch(VerifyParams p, hipStream_t s)
     for (int i = 0; i < 32; ++i) p.powers[i] = std::exp2(i / 32.0);
     const uint32_t parts = (p.vocab + CH - 1) / CH;
     hipLaunchKernelGGL(verify_rows_kernel, dim3(parts * p.rows, p.draft ? 2 : 1), dim3(NT), 0, s, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;      // (the others would judge by what the workspace held)
     const uint32_t shares = std::max(1u, std::min(parts, 512 / p.sequences));
     hipLaunchKernelGGL(verify_weights_kernel, dim3(shares, p.sequences), dim3(512), 0, s, p);
     hipLaunchKernelGGL(verify_draw_kernel, dim3(p.sequences), dim3(DT), 0, s, p);
