@@ -98,7 +98,7 @@ static void set_pages(N& n, uintptr_t k_pages, uintptr_t v_pages, uintptr_t page
                       uint32_t sequences, uint32_t num_pages, uint32_t page_size, uint32_t max_pages, Dtype dtype,
                       uint64_t page_stride)
 {
-    if (dtype == Dtype::Q4) throw std::invalid_argument("pages are F32 or F16");
+    if (dtype != Dtype::Fp32 && dtype != Dtype::Fp16) throw std::invalid_argument("pages are F32 or F16");
     vai_kv_pages p{};
     p.k_pages = reinterpret_cast<void*>(k_pages);
     p.v_pages = reinterpret_cast<void*>(v_pages);
