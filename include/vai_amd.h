@@ -506,6 +506,9 @@ vai_status vai_paged_append_launch(const vai_paged_append_args* args, vai_stream
  *   Statistics and sums are fp32. Over fp16 pages an fp32 q and the probabilities
  *   enter the matrix cores as two fp16 numbers each. fp32 pages, head dims of no
  *   whole 8s and pages of no whole 16s are attended in fp32 throughout.
+ *   A table so long that sequences * hkv * max_pages * page_size comes near 2^37, or
+ *   tokens * hq * max_pages * page_size near 2^41 (2^45 for prompts on the fast
+ *   kernels), is refused: VAI_ERR_UNSUPPORTED.
  *   What hidden positions hold does not matter. A value of V that is not finite
  *   makes its column so for the queries that see it; their other columns may be
  *   NaN too.

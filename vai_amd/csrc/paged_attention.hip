@@ -327,7 +327,6 @@ bool paged_attention_plan(const PagedAttnParams& call, PagedAttnPlan& plan, uint
     p = call;
     p.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
     const uint32_t group = p.hq / p.hkv;
-    // the lines' lengths stay below 2^32
     const uint64_t blocks = (uint64_t)p.tokens * group / 16 + std::min(p.tokens, p.pages.sequences);
     const uint64_t tiles = ((uint64_t)p.pages.max_pages * p.pages.page_size + pg::KT - 1) / pg::KT + 1;
     uint32_t resident = 2;
@@ -341,7 +340,6 @@ bool paged_attention_plan(const PagedAttnParams& call, PagedAttnPlan& plan, uint
     p.decode = paged_decode_ok(p);
     if (p.decode) paged_decode_plan(p, &resident);
     const uint64_t unit = tiles + p.lead;
-    if (blocks * p.hkv > 0xffffffffull / unit) return false;
     p.wgs = (uint32_t)std::min<uint64_t>({(uint64_t)resident * cus, (blocks * p.hkv * unit + p.min_share - 1) / p.min_share,
                                           (uint64_t)PagedAttnParams::MAX_WGS});
     plan.many = p;
@@ -360,7 +358,12 @@ bool paged_attention_plan(const PagedAttnParams& call, PagedAttnPlan& plan, uint
             p.wgs = 0;
         }
     }
-    return true;
+    // a line's length, and the shares' sum rounded up, stay below 2^32
+    const uint64_t seqs = std::min(p.tokens, p.pages.sequences), rows = (uint64_t)p.tokens * group;
+    const uint64_t most = 0xffffffffull - PagedAttnParams::MAX_WGS;
+    const uint64_t few = std::min(rows / p.rb + seqs, seqs * ((p.few_rows + (uint64_t)p.rb - 1) / p.rb));
+    if (p.wgs && few * p.hkv > most / unit) return false;
+    return !plan.many.wgs || (rows / plan.many.rb + seqs) * p.hkv <= most / (tiles / 2 + 2 + plan.many.lead);
 }
 
 static size_t part_bytes(const PagedAttnParams& p)
