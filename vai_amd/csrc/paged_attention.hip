@@ -21,10 +21,10 @@ namespace vai_dev {
 
 // Rows a KV head up to which a sequence is paged_decode.hip's, whose units of 32 (D =
 // 256: 16) rows read the keys once each. 8 sequences of 4000 positions, 32 heads over
-// 8 of 128, us there / in paged_prefill.hip: 32 rows 40 / 55, 48 rows 61 / 55, 64 rows
-// 63 / 55, where one sequence of 16000 takes 28 / 52, 35 / 52, 35 / 53; of 64, 64 rows
-// 40 / 30; of 256 (16 over 4), 32 rows 56 / 53, 64 rows 93 / 54.
-static uint32_t few_most(uint32_t dp) { return dp == 128 ? 64 : 32; }
+// 8 of 128, us there / in paged_prefill.hip: 32 rows 37 / 42, 64 rows 55 / 48, where one
+// sequence of 16000 takes 28 / 47, 35 / 50; of 64, 64 rows 33 / 32, one 23 / 38; of 256
+// (16 over 4), 32 rows 55 / 52, one 35 / 47, 64 rows 90 / 55, one 50 / 51.
+static uint32_t few_most(uint32_t dp) { return dp <= 128 ? 64 : 32; }
 
 // Values d ..+3 of a row of D, as they are, zeros past its end or where there is no row
 // (any row that is), W at a time: D is a multiple of W (1, 2 or 4). Without branches:
@@ -350,10 +350,11 @@ bool paged_attention_plan(const PagedAttnParams& call, PagedAttnPlan& plan, uint
         // One launch takes them all where the units of the sequences with few rows are not
         // many: it fills 4 of 128 rows then, but is bound by memory like the other, whose
         // launch and merge are saved. A chunk of 512 tokens beside 8, 32, 64, 128 (and of
-        // half the length 256) single ones, 8 KV heads: 107, 134, 188, 248, 201 us so, 118,
-        // 156, 203, 270, 219 apart; beside 512 shorter ones 217 and 219. (128 with an fp32 q
-        // 217 and 199, with head dims of 64 164 and 159.)
-        if ((uint64_t)p.pages.sequences * p.hkv <= plan.many.wgs * 3) {
+        // half the length 256) single ones, 32 heads over 8 of 128: 136, 175, 223, 308, 238
+        // us so, 146, 182, 221, 292, 230 apart. Beside 32, 64, 128: with an fp32 q 220, 280,
+        // 386 and 220, 264, 339; 16 over 2 85, 97, 121 and 96, 112, 135; 16 over 4 of 256
+        // 197, 271, 335 and 199, 239, 310.
+        if ((uint64_t)p.pages.sequences * p.hkv <= plan.many.wgs) {
             plan.many.few_rows = 0;
             p.wgs = 0;
         }
