@@ -544,10 +544,11 @@ size_t vai_paged_attention_workspace_size(const vai_paged_attention_args* args);
  *     sum_{i <= j} w_i > uniform[last row] * sum_i w_i,  w = max(p_r - q_r, 0)
  *   (w = p_r if that is 0 everywhere); where all are kept, the token after the
  *   last row is drawn so with w = p of the last row.
- * T = temperature[s] (NULL: 1). T = 0: p and q are 1 at the lowest index of the
- * largest logit. Everything is computed in 64 bits. Logits of -infinity have no
- * probability. A row that is needed and holds a NaN or +infinity, or nothing
- * above -infinity, ends its sequence with the token VAI_NO_TOKEN.
+ * T = temperature[s] (NULL: 1). T = 0, or any that is not above 0: p and q are 1 at
+ * the lowest index of the largest logit. Everything is computed in 64 bits. Logits
+ * of -infinity have no probability. A row that is needed and holds a NaN or
+ * +infinity, or nothing above -infinity, ends its sequence with the token
+ * VAI_NO_TOKEN.
  *   target, draft: [rows] rows of target_stride / draft_stride elements (0:
  *   vocab); draft's row of a sequence's last token is not read. tokens [rows]
  *   uint32, uniform [rows] fp32 in [0, 1); a token >= vocab has no probability.

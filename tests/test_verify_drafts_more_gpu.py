@@ -44,3 +44,13 @@ def test_greedy_with_a_draft_model(gpu, dt):
         for u in (0.0, 0.5, 0.99999994):
             out, acc = ver.check(gpu, target, draft, [5] + drafts, [u] * rows, [0, rows], [0.0])
             assert acc[0] == kept and out[kept] == choice[kept]
+
+
+def test_temperatures_that_are_not_above_zero(gpu):
+    """They are 0: greedy. An infinite one makes every logit above -infinity equally likely."""
+    rng = np.random.default_rng(4)
+    temps = [-1.0, np.nan, -0.0, -np.inf, np.inf, 1e-45]
+    args = ver.batch(rng, 5000, [3, 3, 3, 3, 3, 3], F32, True, [0.0] * 4 + [1e30, 0.0])
+    args[0][:, 40:50] = -np.inf
+    print("verify temperatures", flush=True)
+    ver.check(gpu, *args, temps)
