@@ -131,7 +131,8 @@ __global__ __launch_bounds__(256, 5) void paged_append_kernel(PagedAppendParams 
     const uint32_t na = oa < lim ? min(4u, lim - oa) : 0u, nb = split ? na : ob < D ? min(4u, D - ob) : 0u;
     const bool on = na != 0;   // (a lane past the head's last value loads its first ones where FULL, and drops them)
     const float inv_d = 1.0f / (float)D;
-    // a lane's weights wait in LDS, not in registers: six waves a SIMD instead of four
+    // a lane's weights wait in LDS, not in registers: five waves a SIMD instead of four (for
+    // which 8 to 32 lanes a head of whole groups still keep 4 or 5 registers in scratch)
     __shared__ float4v weights[4][4][64];
     float4v w4[4] = {(float4v)1.0f, (float4v)1.0f, (float4v)1.0f, (float4v)1.0f};
     if (p.q_weight) {
@@ -254,7 +255,8 @@ static hipError_t launch_vec(const PagedAppendParams& p, hipStream_t s)
     // tokens whose waves alone fill the chip are not shared out: each share takes the
     // place and the angles again, as long as one and a half of its steps (32 + 8 + 8
     // heads of 128, 12 steps; tokens: us with 1, 2, 4, 12 shares: 64: 12.8, 9.0, 7.3, 6.4;
-    // 1000: 15.1, 11.8, 11.7, 18.6; 2500: 19.3, 17.5; 3000: 19.6, 23.6)
+    // 1000: 15.1, 11.8, 11.7, 18.6; 2500: 19.3, 17.5; 3000: 19.6, 23.6. Other numbers of
+    // steps take the line that these draw.)
     const uint32_t steps = ((p.q_out ? p.hq : 0u) + 2 * p.hkv + 64 / L - 1) / (64 / L);
     const uint32_t shares = std::min(steps, std::max(1u, (3800 + p.tokens / 2) / p.tokens));
     hipLaunchKernelGGL((paged_append_kernel<TI, L, FULL>), dim3(std::min((p.tokens + 3) / 4, 1u << 20), shares), dim3(256), 0,

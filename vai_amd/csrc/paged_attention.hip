@@ -27,8 +27,10 @@ namespace vai_dev {
 static uint32_t few_most(uint32_t dp) { return dp <= 128 ? 64 : 32; }
 
 // Values d ..+3 of a row of D, as they are, zeros past its end or where there is no row
-// (any row that is), W at a time: D is a multiple of W (1, 2 or 4). Without branches:
-// what is not wanted is read from the row's own values.
+// (any row that is), W at a time: D is a multiple of W (1, 2 or 4). Without branches,
+// what is not wanted is read from the row's own values. That is not for speed alone: a
+// form whose loads stood behind divergent branches gave wrong scores for head dims up
+// to 48, for a reason that was not found.
 template <int W, typename T>
 __device__ __forceinline__ auto raw4(const T* row, uint32_t d, uint32_t D, bool there)
 {

@@ -6,8 +6,9 @@
 // through a ring of D tiles in LDS of its own: the copies (K and V as they lie, 16
 // positions of one page at a time, 16-byte chunks XOR-swizzled by row) of the next
 // tiles are in flight during a tile, and no wave waits for another until the piece
-// of the share ends. Where a position's page lies is looked up 32 tiles ahead, a
-// lane for each 16 positions.
+// of the share ends. Where their pages lie is looked up for a wave's next 32 tiles
+// at once, a lane for each 16 positions; the wave waits for that, and for the copies
+// before it, once in 32 tiles.
 //
 // S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32_f16, the query rows of a KV
 // head the columns: lane (c16, g) gets row c16's scores of keys 16 k + 4 g ..+3,

@@ -11,7 +11,8 @@
 // workgroups a CU (D = 256: one, by registers): one's softmax, and its beginning
 // and end of a unit, under the other's products. (One of two groups of waves that
 // take the tiles in turn halves the partial results, but 8192 tokens of a prompt
-// took 823 us so where two workgroups took 700; 665 by now.)
+// took 823 us so where two workgroups took 700, with probabilities in one number
+// each; 888 by now, with two.)
 // All units' tiles form a line that the workgroups cut into equal shares, head by
 // head on one XCD, as paged_plan.h does for few rows; a unit's tiles are those its
 // own rows see. An fp32 q enters as two fp16 numbers (Q2), and so do the
@@ -19,6 +20,10 @@
 // |v| in the result, as much as an fp16 output's own rounding, and would give a
 // sequence's single token other bits where a prompt joins its batch. (A chunk of 512
 // beside 8 single tokens, 32 heads over 8 of 128: 128 us, with one number 106.)
+// Registers are short: heads of 128 keep 43 of a lane's in scratch (an fp32 q 85),
+// heads of 256 25 (80). With an fp16 q they come back once a piece, or where V is not
+// finite; with an fp32 q in the tile loop, behind the copies in flight (the chunk
+// 161 us; 512 beside 8 with heads of 256 263 and 547).
 #include "attention_tile.h"
 #include "paged_plan.h"
 
@@ -309,7 +314,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prefill_kernel(Pa
         for (int d = 0; d < DF; ++d) o[d] = (float16v)0.f;
 
         // A wave without rows (a sequence's last unit, one of few rows) only copies: a chunk
-        // of 512 tokens beside 32 single ones takes 134 us, 147 where it multiplies too.
+        // of 512 tokens beside 32 single ones takes 165 us, 178 where it multiplies too.
         const bool idle = u.rb * RB + wave * QW >= rows;
         if (idle) {
             for (int t = 0; t < mine; ++t) {

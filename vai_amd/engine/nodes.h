@@ -311,7 +311,10 @@ public:
         bool causal = true;
         uint32_t span = 0;                    // sliding window; 0: none
         float scale = 0.0f;                   // 0: 1/sqrt(headDim)
-        uint32_t maxNew = 0;                  // no sequence brings more tokens (chooses kernels); 0: all of the rows
+        // No sequence brings more tokens (chooses kernels); 0: all of the rows may be one's, which
+        // sends a batch of single tokens to the kernels for prompts (64 of up to 8192 positions, 32
+        // heads over 8 of 128: 88 us with 1, 106 with 0).
+        uint32_t maxNew = 0;
     } config_;
 
     explicit PagedAttention(Config config);
