@@ -17,8 +17,8 @@
 // head on one XCD, as paged_plan.h does for few rows; a unit's tiles are those its
 // own rows see. An fp32 q enters as two fp16 numbers (Q2), and so do the
 // probabilities, whatever the output's type: one number alone leaves 2^-11 of sum p
-// |v| in the result, as much as an fp16 output's own rounding, and would give a
-// sequence's single token other bits where a prompt joins its batch. (A chunk of 512
+// |v| in the result, as much as an fp16 output's own rounding, and would cost a
+// sequence's single token bits where a prompt joins its batch. (A chunk of 512
 // beside 8 single tokens, 32 heads over 8 of 128: 128 us, with one number 106.)
 // Registers are short: heads of 128 keep 43 of a lane's in scratch (an fp32 q 85),
 // heads of 256 25 (80). With an fp16 q they come back once a piece, or where V is not
